@@ -72,6 +72,11 @@ EXPORTED_SYMBOLS = (
     "dsa_indexer_kl_loss_grad_state",
     "dsa_indexer_kl_loss_grad_apply",
     "dsa_topk_index_mask",
+    "dsa_latent_mla_fwd",
+    "dsa_latent_mla_expanded_fwd",
+    "dsa_latent_mla_bwd_workspace_size",
+    "dsa_latent_mla_bwd",
+    "dsa_latent_mla_expanded_bwd",
     "dsa_stage_timing",
     "dsa_stage_times",
 )
@@ -156,6 +161,12 @@ _SIGNATURES = {
                                        + [_f32, _i32, _c_void_p]),
     "dsa_topk_index_mask": (_i32, [_c_void_p, _i32, _i64, _c_void_p, _i64, _i64, _i64, _i64, _i64,
                                    _f32, _f32, _i32, _c_void_p]),
+    "dsa_latent_mla_fwd": (_i32, [_c_void_p] * 6 + [_i64] * 7 + [_f32, _i32, _c_void_p]),
+    "dsa_latent_mla_expanded_fwd": (_i32, [_c_void_p] * 8 + [_i64] * 7 + [ctypes.POINTER(_i64), _f32, _i32, _c_void_p]),
+    "dsa_latent_mla_bwd_workspace_size": (_size_t, [_i64] * 7 + [_i32]),
+    "dsa_latent_mla_bwd": (_i32, [_c_void_p] * 10 + [_size_t] + [_i64] * 7 + [_f32, _i32, _c_void_p]),
+    "dsa_latent_mla_expanded_bwd": (_i32, [_c_void_p] * 14 + [_size_t] + [_i64] * 7
+                                    + [ctypes.POINTER(_i64), _f32, _i32, _c_void_p]),
     "dsa_stage_timing": (_i32, [_i32]),
     "dsa_stage_times": (_i32, [_i32, ctypes.POINTER(ctypes.c_float), _i32]),
 }

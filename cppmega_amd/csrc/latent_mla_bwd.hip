@@ -1,0 +1,638 @@
+// Dense latent attention backward on gfx950 MFMA (bf16).  With p = 2^(sl2 q.k - lse2),
+// delta = out . dO and ds = p (dO . v - delta) scale:
+//   dq = sum_keys ds k     dk = sum_rows ds q     dv = sum_rows p dO
+// (absorbed: dkv = dk + [dv, 0], summed over the group's heads, which are rows).
+//
+//   latent_bwd_q_kernel    row-major, as the forward: a wave keeps RT * 32 rows of Q
+//     and dO, S^T = K Q^T and dP^T = V dO^T leave one row per lane, dQ^T[d][row] +=
+//     K^T dS^T.  It also leaves every row's lse2, delta * scale and window, and the
+//     windows' spans per 32 rows, for the next kernel.
+//   latent_bwd_kv_kernel   key-major: a wave keeps CT * 32 keys of K (and V) and streams
+//     LDS tiles of 64 rows of Q and dO: S = Q K^T and dP = dO V^T leave one key per
+//     lane, dK^T[d][key] += Q^T dS, dV^T[d][key] += dO^T P (absorbed: into the same
+//     accumulators).  Row tiles that no key of the workgroup is admitted by are passed
+//     over.  Where (batch, group, key block) triples leave the GPU idle, the rows are
+//     split over nsplit workgroups, whose fp32 partial sums
+//   latent_bwd_reduce_kernel adds in split order (and k_pe's over the heads).
+// No float atomics: the order of every sum follows from the shapes, so results repeat
+// bit for bit.  P and dS are rounded to bf16 (nearest even) for the matrix products;
+// sums are fp32.  Both kernels form S and dP (the reading and the rounding of a stored
+// P and dS, 4 bytes a pair, would take longer than the two products).
+#include "latent_mla.hpp"
+
+namespace dsa {
+
+constexpr float kNoRow = 1.0e30f;  // lse2 of a row without keys: 2^(x - it) = 0
+
+template <int DK, int DN, int DV, int RT, int NW>
+struct LatentBwdQ {
+  static constexpr bool SHARED = DN == DK;
+  static constexpr int KP = DK / 64, NP = DN / 64, VP = DV / 64;
+  static constexpr int K_BYTES = 2 * KP * 4096, V_BYTES = SHARED ? 0 : 2 * VP * 4096;
+  static constexpr int BUF = K_BYTES + V_BYTES;
+  static constexpr int ROWS = NW * RT * 32;
+  static constexpr int OFF_SPAN = 2 * BUF;
+  static constexpr int BYTES = OFF_SPAN + NW * 16 + 16;
+};
+
+template <int DK, int DN, int DV, int RT, int NW>
+__global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParams p) {
+  using C = LatentBwdQ<DK, DN, DV, RT, NW>;
+  constexpr int KS = DK / 16, VS = DV / 16, NDT = DK / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
+  const int nblk = (int)((p.rows + C::ROWS - 1) / C::ROWS);
+  const int64_t item = xcd_remap(blockIdx.x, gridDim.x);
+  const int64_t bg = item / nblk, b = bg / p.G, g = bg - b * p.G;
+  const int blk = nblk - 1 - (int)(item - bg * nblk);
+  int *span_lds = reinterpret_cast<int *>(smem + C::OFF_SPAN);
+
+  int lo[RT], hi[RT];
+  int64_t orow[RT];
+  i32x4 q[RT][KS], dO[RT][VS];
+  float lse[RT], delta[RT];  // delta * scale
+  RowSpan span = no_rows();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int64_t row = (int64_t)blk * C::ROWS + (w * RT + rt) * 32 + l32;
+    lo[rt] = hi[rt] = 0;
+    orow[rt] = -1;
+    RowSpan mine = no_rows();
+    if (row < p.rows) {
+      const int64_t t = (int64_t)((uint32_t)row / (uint32_t)p.hpg);
+      orow[rt] = (b * p.S + t) * p.H + g * p.hpg + (row - t * p.hpg);
+      latent_window(p, b, t, lo[rt], hi[rt]);
+      span_add(mine, lo[rt], hi[rt]);
+      span_add(span, lo[rt], hi[rt]);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      q[rt][ks] = i32x4{0, 0, 0, 0};
+      if (orow[rt] >= 0) q[rt][ks] = ld_global_16(p.q + (orow[rt] * DK + 16 * ks + 8 * g32) * 2);
+    }
+    float dl = 0.0f;
+#pragma unroll
+    for (int vs = 0; vs < VS; ++vs) {
+      dO[rt][vs] = i32x4{0, 0, 0, 0};
+      if (orow[rt] >= 0) {
+        dO[rt][vs] = ld_global_16(p.dO + (orow[rt] * DV + 16 * vs + 8 * g32) * 2);
+        const i32x4 ov = ld_global_16(p.o + (orow[rt] * DV + 16 * vs + 8 * g32) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = (uint32_t)ov[e], c = (uint32_t)dO[rt][vs][e];
+          dl = fmaf(__uint_as_float(a << 16), __uint_as_float(c << 16), dl);
+          dl = fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(c & 0xffff0000u), dl);
+        }
+      }
+    }
+    const bool any = hi[rt] > lo[rt];
+    delta[rt] = any ? sum_halves(dl) * p.scale : 0.0f;
+    lse[rt] = any ? p.lse_in[orow[rt]] : kNoRow;
+    // what the key-major kernel needs of these rows
+    const int64_t r32 = (int64_t)blk * (C::ROWS / 32) + w * RT + rt, t64 = r32 >> 1;
+    if (t64 < p.nt64) {
+      const RowSpan s = span_wave(mine);
+      float *st = p.stat + (bg * p.nt64 + t64) * 256 + (r32 & 1) * 32 + l32;
+      if (g32 == 0) {
+        st[0] = lse[rt];
+        st[64] = delta[rt];
+      } else {
+        st[128] = __int_as_float(lo[rt]);
+        st[192] = __int_as_float(hi[rt]);
+      }
+      if (lane == 0) *reinterpret_cast<i32x4 *>(p.info + (bg * p.nt64 * 2 + r32) * 4) = i32x4{s.lo, s.hi, s.lo_max, s.hi_min};
+    }
+  }
+  span = span_wave(span);
+  if (lane == 0) {
+    span_lds[2 * w] = span.lo;
+    span_lds[2 * w + 1] = span.hi;
+  }
+  __syncthreads();
+  int klo = kNoLo, khi = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    klo = min(klo, span_lds[2 * i]);
+    khi = max(khi, span_lds[2 * i + 1]);
+  }
+  klo = __builtin_amdgcn_readfirstlane(klo);
+  khi = __builtin_amdgcn_readfirstlane(khi);
+  const int t0 = khi > klo ? klo / kKeyTile : 0, t1 = khi > klo ? (khi + kKeyTile - 1) / kKeyTile : 0;
+
+  const uint32_t lds0 = lds_address(smem);
+  const unsigned char *kb = p.k + b * p.k_b + g * p.k_g;
+  auto fetch = [&](int tile, int buf) {
+    const int64_t k0 = (int64_t)tile * kKeyTile;
+    const int n = (int)(p.S_kv - k0 < kKeyTile ? p.S_kv - k0 : kKeyTile);
+    const uint32_t at = lds0 + (uint32_t)(buf * C::BUF);
+    const uint32_t kt = (uint32_t)p.k_t;
+    tile_fetch<C::KP, 0, C::NP, NW>(at, tile_rsrc(kb + k0 * p.k_t), w,
+                                    [&](int r) { return r < n ? (uint32_t)r * kt : kMaskedOff; });
+    if constexpr (!C::SHARED) {
+      const uint32_t pt = (uint32_t)p.pe_t, vt = (uint32_t)p.v_t;
+      tile_fetch<C::KP, C::NP, C::KP - C::NP, NW>(at, tile_rsrc(p.kpe + b * p.pe_b + k0 * p.pe_t), w,
+                                                  [&](int r) { return r < n ? (uint32_t)r * pt : kMaskedOff; });
+      tile_fetch<C::VP, 0, C::VP, NW>(at + C::K_BYTES, tile_rsrc(p.v + b * p.v_b + g * p.v_g + k0 * p.v_t), w,
+                                      [&](int r) { return r < n ? (uint32_t)r * vt : kMaskedOff; });
+    }
+  };
+
+  const RowRead row_read;
+  const ColRead col_read;
+  f32x16 acc[RT][NDT];
+  for (int careful = 0; careful < 2; ++careful) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) acc[rt][dt] = zero16();
+    if (t0 < t1) fetch(t0, 0);
+    for (int tile = t0; tile < t1; ++tile) {
+      const int buf = (tile - t0) & 1, k0 = tile * kKeyTile;
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's share of the tile
+      __syncthreads();
+      if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
+      const unsigned char *Kt = smem + buf * C::BUF, *Vt = C::SHARED ? Kt : Kt + C::K_BYTES;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int ks0 = k0 + 32 * s;
+        if (ks0 >= span.hi || ks0 + 32 <= span.lo) continue;
+        const bool whole = span.lo_max <= ks0 && span.hi_min >= ks0 + 32;
+        const unsigned char *Ks = Kt + s * C::KP * 4096, *Vs = Vt + s * (C::SHARED ? C::KP : C::VP) * 4096;
+        f32x16 sc[RT], dp[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt] = dp[rt] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const i32x4 a = row_read(Ks, ks);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            sc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(q[rt][ks]), sc[rt], 0, 0, 0);
+            if constexpr (C::SHARED)
+              if (ks < VS)
+                dp[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(dO[rt][ks < VS ? ks : 0]), dp[rt], 0, 0, 0);
+          }
+        }
+        if constexpr (!C::SHARED) {
+#pragma unroll
+          for (int vs = 0; vs < VS; ++vs) {
+            const i32x4 a = row_read(Vs, vs);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              dp[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(dO[rt][vs]), dp[rt], 0, 0, 0);
+          }
+        }
+        i32x4 db[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sc[rt][i] = exp2_fast(fmaf(sc[rt][i], p.sl2, -lse[rt])) * fmaf(dp[rt][i], p.scale, -delta[rt]);
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int key = ks0 + acc_row(i, g32);
+              sc[rt][i] = key >= lo[rt] && key < hi[rt] ? sc[rt][i] : 0.0f;
+            }
+          }
+          pack_operand(sc[rt], db[rt]);
+        }
+        if (!careful || whole) {
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const i32x4 a = col_read(Ks, dt, u);
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                acc[rt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(db[rt][u]), acc[rt][dt], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            careful_product<NDT>(acc[rt], sc[rt], Ks, [&](int r) { return ks0 + r >= lo[rt] && ks0 + r < hi[rt]; });
+        }
+      }
+    }
+    __syncthreads();
+    if (careful) break;
+    bool bad = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bad |= not_finite(acc[rt][dt][i]);
+    if (__syncthreads_or(bad) == 0) break;  // a masked Inf or NaN may have reached a row: once more, without it
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+    if (orow[rt] >= 0) {
+      const bool empty = hi[rt] <= lo[rt];
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const f32x16 &x = acc[rt][dt];
+          const i32x2 v{(int)pack_bf16x2(x[4 * m], x[4 * m + 1]), (int)pack_bf16x2(x[4 * m + 2], x[4 * m + 3])};
+          *reinterpret_cast<i32x2 *>(p.dq + orow[rt] * DK + acc_col(dt, 4 * m, g32)) = empty ? i32x2{0, 0} : v;
+        }
+    }
+}
+
+template <int DK, int DN, int DV, int CT, int NW>
+struct LatentBwdKv {
+  static constexpr bool SHARED = DN == DK;
+  static constexpr int KP = DK / 64, VP = DV / 64;
+  static constexpr int Q_BYTES = 2 * KP * 4096, D_BYTES = 2 * VP * 4096;
+  static constexpr int OFF_STAT = Q_BYTES + D_BYTES;
+  static constexpr int BUF = OFF_STAT + 1024;
+  static constexpr int KEYS = NW * CT * 32;
+  static constexpr int BYTES = 2 * BUF;
+  // columns of a partial row: absorbed DK; expanded, split: [k_nope, k_pe, v]; expanded, unsplit: k_pe
+  static constexpr int WIDE = SHARED ? DK : DK + DV;
+};
+
+template <int DK, int DN, int DV, int CT, int NW>
+__global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentParams p) {
+  using C = LatentBwdKv<DK, DN, DV, CT, NW>;
+  constexpr int KS = DK / 16, VS = DV / 16, NDK = DK / 32, NDV = DV / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
+  int64_t item = xcd_remap(blockIdx.x, gridDim.x);
+  const int kblk = (int)(item % p.nkb);
+  item /= p.nkb;
+  const int split = (int)(item % p.nsplit);
+  const int64_t bg = item / p.nsplit, b = bg / p.G, g = bg - b * p.G;
+  const int key_lo = kblk * C::KEYS, key_hi = key_lo + C::KEYS < p.S_kv ? key_lo + C::KEYS : (int)p.S_kv;
+  const int wkey = key_lo + w * CT * 32;  // this wave's first key
+
+  int key[CT];
+  i32x4 kr[CT][KS], vr[C::SHARED ? 1 : CT][VS];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    key[ct] = wkey + ct * 32 + l32;
+    const bool in = key[ct] < p.S_kv;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kr[ct][ks] = i32x4{0, 0, 0, 0};
+      if (in) {
+        const int64_t kk = key[ct];
+        kr[ct][ks] = ks < DN / 16 ? ld_global_16(p.k + b * p.k_b + kk * p.k_t + g * p.k_g + (16 * ks + 8 * g32) * 2)
+                                  : ld_global_16(p.kpe + b * p.pe_b + kk * p.pe_t + (16 * (ks - DN / 16) + 8 * g32) * 2);
+      }
+    }
+    if constexpr (!C::SHARED) {
+#pragma unroll
+      for (int vs = 0; vs < VS; ++vs) {
+        vr[ct][vs] = i32x4{0, 0, 0, 0};
+        if (in) vr[ct][vs] = ld_global_16(p.v + b * p.v_b + (int64_t)key[ct] * p.v_t + g * p.v_g + (16 * vs + 8 * g32) * 2);
+      }
+    }
+  }
+
+  // the next row tile at or after t (below c1) that a key of this workgroup is admitted by
+  const int32_t *info = p.info + bg * p.nt64 * 8;
+  const int c0 = split * p.tiles_per_split;
+  const int c1 = c0 + p.tiles_per_split < p.nt64 ? c0 + p.tiles_per_split : (int)p.nt64;
+  auto next = [&](int t) {
+    for (; t < c1; t += 64) {
+      bool hit = false;
+      if (t + lane < c1) {
+        const i32x4 a = *reinterpret_cast<const i32x4 *>(info + (int64_t)(t + lane) * 8);
+        const i32x4 c = *reinterpret_cast<const i32x4 *>(info + (int64_t)(t + lane) * 8 + 4);
+        hit = (a[0] < key_hi && a[1] > key_lo) || (c[0] < key_hi && c[1] > key_lo);
+      }
+      const uint64_t m = wv::ballot(hit);
+      if (m != 0ull) return t + __builtin_ctzll(m);
+    }
+    return c1;
+  };
+
+  const uint32_t lds0 = lds_address(smem);
+  const uint32_t hpg = (uint32_t)p.hpg;
+  auto fetch = [&](int tile, int buf) {
+    const uint32_t at = lds0 + (uint32_t)(buf * C::BUF);
+    const int64_t r0 = (int64_t)tile * 64, tok0 = (int64_t)((uint32_t)r0 / hpg);
+    const uint32_t h0 = (uint32_t)(r0 - tok0 * p.hpg);
+    const int n = (int)(p.rows - r0 < 64 ? p.rows - r0 : 64);
+    const int64_t base = (b * p.S + tok0) * p.H + g * p.hpg;  // row (token tok0, first head)
+    const uint32_t H = (uint32_t)p.H;
+    auto at_row = [&](int r) {  // rows from base: tokens tok0 ..
+      const uint32_t x = h0 + (uint32_t)r, dt = x / hpg;
+      return dt * H + (x - dt * hpg);
+    };
+    tile_fetch<C::KP, 0, C::KP, NW>(at, tile_rsrc(p.q + base * DK * 2), w,
+                                    [&](int r) { return r < n ? at_row(r) * (DK * 2) : kMaskedOff; });
+    tile_fetch<C::VP, 0, C::VP, NW>(at + C::Q_BYTES, tile_rsrc(p.dO + base * DV * 2), w,
+                                    [&](int r) { return r < n ? at_row(r) * (DV * 2) : kMaskedOff; });
+    if (w == 0)
+      lds_dma_16(at + C::OFF_STAT, (uint32_t)lane * 16, tile_rsrc(reinterpret_cast<const unsigned char *>(p.stat + (bg * p.nt64 + tile) * 256)), 0);
+  };
+
+  const RowRead row_read;
+  const ColRead col_read;
+  f32x16 dk[CT][NDK], dv[C::SHARED ? 1 : CT][NDV];
+  const int first = __builtin_amdgcn_readfirstlane(next(c0));
+  for (int careful = 0; careful < 2; ++careful) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+      for (int dt = 0; dt < NDK; ++dt) dk[ct][dt] = zero16();
+      if constexpr (!C::SHARED) {
+#pragma unroll
+        for (int dt = 0; dt < NDV; ++dt) dv[ct][dt] = zero16();
+      }
+    }
+    int tile = first, buf = 0;
+    if (tile < c1) fetch(tile, 0);
+    while (tile < c1) {
+      const int nxt = __builtin_amdgcn_readfirstlane(next(tile + 1));
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's share of the tile
+      __syncthreads();
+      if (nxt < c1) fetch(nxt, buf ^ 1);
+      const unsigned char *Qt = smem + buf * C::BUF, *Dt = Qt + C::Q_BYTES;
+      const float *st = reinterpret_cast<const float *>(Qt + C::OFF_STAT);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const i32x4 in = *reinterpret_cast<const i32x4 *>(info + ((int64_t)tile * 2 + s) * 4);
+        if (in[0] >= wkey + CT * 32 || in[1] <= wkey) continue;  // wave-uniform
+        const bool whole = in[2] <= wkey && in[3] >= wkey + CT * 32;
+        const unsigned char *Qs = Qt + s * C::KP * 4096, *Ds = Dt + s * C::VP * 4096;
+        f32x16 sc[CT], dp[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) sc[ct] = dp[ct] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const i32x4 a = row_read(Qs, ks);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            sc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(kr[ct][ks]), sc[ct], 0, 0, 0);
+        }
+#pragma unroll
+        for (int vs = 0; vs < VS; ++vs) {
+          const i32x4 a = row_read(Ds, vs);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            const i32x4 &bv = C::SHARED ? kr[ct][vs] : vr[C::SHARED ? 0 : ct][vs];
+            dp[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(bv), dp[ct], 0, 0, 0);
+          }
+        }
+        i32x4 pb[CT][2], db[CT][2];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int r = 32 * s + 8 * m + 4 * g32;  // registers 4 m .. are rows r ..
+          const f32x4 ls = *reinterpret_cast<const f32x4 *>(st + r), de = *reinterpret_cast<const f32x4 *>(st + 64 + r);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 4 * m + e;
+              sc[ct][i] = exp2_fast(fmaf(sc[ct][i], p.sl2, -ls[e]));
+              dp[ct][i] = sc[ct][i] * fmaf(dp[ct][i], p.scale, -de[e]);
+            }
+          if (!whole) {
+            const i32x4 lo = *reinterpret_cast<const i32x4 *>(st + 128 + r), hi = *reinterpret_cast<const i32x4 *>(st + 192 + r);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const bool ok = key[ct] >= lo[e] && key[ct] < hi[e];
+                sc[ct][4 * m + e] = ok ? sc[ct][4 * m + e] : 0.0f;
+                dp[ct][4 * m + e] = ok ? dp[ct][4 * m + e] : 0.0f;
+              }
+          }
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          pack_operand(sc[ct], pb[ct]);
+          pack_operand(dp[ct], db[ct]);
+        }
+        if (!careful || whole) {
+#pragma unroll
+          for (int dt = 0; dt < NDV; ++dt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const i32x4 a = col_read(Ds, dt, u);
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct) {
+                f32x16 &t = C::SHARED ? dk[ct][dt] : dv[C::SHARED ? 0 : ct][dt];
+                t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(pb[ct][u]), t, 0, 0, 0);
+              }
+            }
+#pragma unroll
+          for (int dt = 0; dt < NDK; ++dt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const i32x4 a = col_read(Qs, dt, u);
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct)
+                dk[ct][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(db[ct][u]), dk[ct][dt], 0, 0, 0);
+            }
+        } else {
+          const int *sti = reinterpret_cast<const int *>(st);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            auto admit = [&](int r) { return key[ct] >= sti[128 + 32 * s + r] && key[ct] < sti[192 + 32 * s + r]; };
+            if constexpr (C::SHARED) {
+              f32x16 part[NDV];
+#pragma unroll
+              for (int dt = 0; dt < NDV; ++dt) part[dt] = dk[ct][dt];
+              careful_product<NDV>(part, sc[ct], Ds, admit);
+#pragma unroll
+              for (int dt = 0; dt < NDV; ++dt) dk[ct][dt] = part[dt];
+            } else {
+              careful_product<NDV>(dv[C::SHARED ? 0 : ct], sc[ct], Ds, admit);
+            }
+            careful_product<NDK>(dk[ct], dp[ct], Qs, admit);
+          }
+        }
+      }
+      tile = nxt;
+      buf ^= 1;
+    }
+    __syncthreads();
+    if (careful) break;
+    bool bad = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+      for (int dt = 0; dt < NDK; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bad |= not_finite(dk[ct][dt][i]);
+      if constexpr (!C::SHARED) {
+#pragma unroll
+        for (int dt = 0; dt < NDV; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) bad |= not_finite(dv[ct][dt][i]);
+      }
+    }
+    if (__syncthreads_or(bad) == 0) break;
+  }
+
+  const int64_t bgs = p.B * p.G;
+  const bool split_rows = p.nsplit > 1;
+  if (split_rows && threadIdx.x == 0) p.used[((int64_t)split * bgs + bg) * p.nkb + kblk] = first < c1;
+  if (split_rows && first >= c1) return;
+  const int width = split_rows ? C::WIDE : 64;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (key[ct] >= p.S_kv) continue;
+    float *row = p.part + (((int64_t)split * bgs + bg) * p.S_kv + key[ct]) * width;
+    auto put = [&](const f32x16 &x, int dt, uint16_t *out, float *part) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int col = acc_col(dt, 4 * m, g32);
+        if (out != nullptr)
+          *reinterpret_cast<i32x2 *>(out + col) =
+              i32x2{(int)pack_bf16x2(x[4 * m], x[4 * m + 1]), (int)pack_bf16x2(x[4 * m + 2], x[4 * m + 3])};
+        else
+          *reinterpret_cast<f32x4 *>(part + col) = f32x4{x[4 * m], x[4 * m + 1], x[4 * m + 2], x[4 * m + 3]};
+      }
+    };
+    const int64_t orow = (b * p.S_kv + key[ct]) * p.G + g;
+#pragma unroll
+    for (int dt = 0; dt < NDK; ++dt) {
+      if (dt * 32 < DN)
+        put(dk[ct][dt], dt, split_rows ? nullptr : p.dk + orow * DN, row);
+      else  // k_pe: summed over the heads by the reduction
+        put(dk[ct][dt], dt, nullptr, split_rows ? row : row - DN);
+    }
+    if constexpr (!C::SHARED) {
+#pragma unroll
+      for (int dt = 0; dt < NDV; ++dt) put(dv[ct][dt], dt, split_rows ? nullptr : p.dv + orow * DV, row + DK);
+    }
+  }
+}
+
+// One thread per 4 columns: partial rows added in split order (k_pe: group by group,
+// each group's splits in order) and rounded once.
+struct LatentReduce {
+  const float *part;
+  const int32_t *used;
+  uint16_t *dk, *dkpe, *dv;
+  int64_t S_kv, B, G;
+  int nsplit, nkb, keys, width, dn, dr, dvw;  // width of a partial row: dn + dr + dvw, or dr
+};
+__global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentReduce r) {
+  const int64_t bgs = r.B * r.G;
+  const int own = (r.width - r.dr) / 4;  // columns of the group's own rows
+  const int64_t n_own = bgs * r.S_kv * own, n_pe = r.B * r.S_kv * (r.dr / 4);
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= n_own + n_pe) return;
+  f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](int64_t bg, int64_t key, int col) {
+    const int64_t kb = key / r.keys;
+    for (int s = 0; s < r.nsplit; ++s) {
+      if (r.used != nullptr && r.used[(s * bgs + bg) * r.nkb + kb] == 0) continue;
+      sum += *reinterpret_cast<const f32x4 *>(r.part + ((s * bgs + bg) * r.S_kv + key) * r.width + col);
+    }
+  };
+  uint16_t *dst;
+  if (id < n_own) {
+    const int64_t row = id / own, bg = row / r.S_kv, key = row - bg * r.S_kv;
+    const int c = (int)(id - row * own) * 4;
+    const int64_t b = bg / r.G, orow = (b * r.S_kv + key) * r.G + (bg - b * r.G);
+    const bool is_k = c < r.dn;
+    add(bg, key, is_k ? c : c + r.dr);
+    dst = is_k ? r.dk + orow * r.dn + c : r.dv + orow * r.dvw + (c - r.dn);
+  } else {
+    const int64_t x = id - n_own, row = x / (r.dr / 4), b = row / r.S_kv, key = row - b * r.S_kv;
+    const int c = (int)(x - row * (r.dr / 4)) * 4;
+    for (int64_t g = 0; g < r.G; ++g) add(b * r.G + g, key, (r.width == r.dr ? 0 : r.dn) + c);
+    dst = r.dkpe + (b * r.S_kv + key) * r.dr + c;
+  }
+  *reinterpret_cast<i32x2 *>(dst) = i32x2{(int)pack_bf16x2(sum[0], sum[1]), (int)pack_bf16x2(sum[2], sum[3])};
+}
+
+struct BwdKvPlan {
+  int keys, nkb, nsplit, tiles_per_split, width;
+};
+// Row splits: enough workgroups for four rounds of two a compute unit under a causal mask, which
+// leaves half of them without work, and at least 8 row tiles each.
+static BwdKvPlan kv_plan(int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t d_qk, int64_t d_v, bool expanded) {
+  BwdKvPlan r;
+  r.keys = 4 * 32;
+  r.nkb = (int)((S_kv + r.keys - 1) / r.keys);
+  const int64_t tiles = (S * (H / G) + 63) / 64, wgs = B * G * r.nkb;
+  int64_t n = wgs > 0 ? (2048 + wgs - 1) / wgs : 1;
+  if (n > (tiles + 7) / 8) n = (tiles + 7) / 8;
+  if (n > 64) n = 64;
+  if (n < 1) n = 1;
+  r.tiles_per_split = tiles > 0 ? (int)((tiles + n - 1) / n) : 1;
+  r.nsplit = tiles > 0 ? (int)((tiles + r.tiles_per_split - 1) / r.tiles_per_split) : 1;
+  r.width = expanded ? (r.nsplit > 1 ? (int)(d_qk + d_v) : 64) : (int)d_qk;
+  return r;
+}
+
+static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+struct BwdSections {
+  size_t stat, info, used, part, total;
+};
+static BwdSections bwd_sections(const BwdKvPlan &k, int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, bool expanded) {
+  const size_t nt64 = (size_t)((S * (H / G) + 63) / 64), bgs = (size_t)(B * G);
+  BwdSections s;
+  s.stat = 0;
+  s.info = s.stat + bgs * nt64 * 1024;
+  s.used = s.info + up256(bgs * nt64 * 32);
+  s.part = s.used + (k.nsplit > 1 ? up256((size_t)k.nsplit * bgs * (size_t)k.nkb * 4) : 0);
+  s.total = s.part + (k.nsplit > 1 || expanded ? (size_t)k.nsplit * bgs * (size_t)S_kv * (size_t)k.width * 4 : 0);
+  return s;
+}
+size_t latent_bwd_workspace(int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t d_qk, int64_t d_v, bool expanded) {
+  return bwd_sections(kv_plan(B, S, S_kv, H, G, d_qk, d_v, expanded), B, S, S_kv, H, G, expanded).total;
+}
+
+template <int DK, int DN, int DV, int RT, int CT, int NW>
+static int launch(LatentParams p, unsigned char *ws, hipStream_t st) {
+  using Q = LatentBwdQ<DK, DN, DV, RT, NW>;
+  using K = LatentBwdKv<DK, DN, DV, CT, NW>;
+  constexpr bool expanded = DN != DK;
+  const BwdKvPlan k = kv_plan(p.B, p.S, p.S_kv, p.H, p.G, DK, DV, expanded);
+  const BwdSections s = bwd_sections(k, p.B, p.S, p.S_kv, p.H, p.G, expanded);
+  p.nt64 = (p.rows + 63) / 64;
+  p.stat = reinterpret_cast<float *>(ws + s.stat);
+  p.info = reinterpret_cast<int32_t *>(ws + s.info);
+  p.used = reinterpret_cast<int32_t *>(ws + s.used);
+  p.part = reinterpret_cast<float *>(ws + s.part);
+  p.nsplit = k.nsplit;
+  p.tiles_per_split = k.tiles_per_split;
+  p.nkb = k.nkb;
+  const auto qk = latent_bwd_q_kernel<DK, DN, DV, RT, NW>;
+  const auto kk = latent_bwd_kv_kernel<DK, DN, DV, CT, NW>;
+  hipError_t e = hipFuncSetAttribute((const void *)qk, hipFuncAttributeMaxDynamicSharedMemorySize, Q::BYTES);
+  if (e == hipSuccess) e = hipFuncSetAttribute((const void *)kk, hipFuncAttributeMaxDynamicSharedMemorySize, K::BYTES);
+  if (e != hipSuccess) return set_error(DSA_ERR_HIP, "dsa_latent_mla_bwd: LDS attribute: %s", hipGetErrorString(e));
+  const int64_t bgs = p.B * p.G;
+  const int64_t nq = (p.rows + Q::ROWS - 1) / Q::ROWS * bgs, nk = (int64_t)k.nkb * k.nsplit * bgs;
+  DSA_REQUIRE(nq < (1ll << 31) && nk < (1ll << 31), "dsa_latent_mla_bwd: grid too large");
+  int rc = DSA_OK;
+  if (nq > 0) {  // no rows: the key gradients below are zeros
+    hipLaunchKernelGGL(qk, dim3((unsigned)nq), dim3(64 * NW), Q::BYTES, st, p);
+    rc = check_launch("dsa_latent_mla_bwd (rows)");
+  }
+  if (rc || nk == 0) return rc;
+  hipLaunchKernelGGL(kk, dim3((unsigned)nk), dim3(64 * NW), K::BYTES, st, p);
+  rc = check_launch("dsa_latent_mla_bwd (keys)");
+  if (rc || (!expanded && k.nsplit == 1)) return rc;
+  LatentReduce r{p.part, k.nsplit > 1 ? p.used : nullptr, p.dk, p.dkpe, p.dv, p.S_kv, p.B, p.G, k.nsplit, k.nkb, k.keys,
+                 k.width, DN, DK - DN, expanded ? DV : 0};
+  const int64_t n = bgs * p.S_kv * ((r.width - r.dr) / 4) + p.B * p.S_kv * (r.dr / 4), wgs = (n + 255) / 256;
+  DSA_REQUIRE(wgs < (1ll << 31), "dsa_latent_mla_bwd: grid too large");
+  hipLaunchKernelGGL(latent_bwd_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, r);
+  return check_launch("dsa_latent_mla_bwd (reduction)");
+}
+
+int launch_latent_bwd(const LatentParams &p, int64_t d_qk, int64_t d_v, bool expanded, unsigned char *ws, hipStream_t st) {
+  if (!expanded) {
+    if (d_qk == 128 && d_v == 64) return launch<128, 128, 64, 1, 1, 4>(p, ws, st);
+    if (d_qk == 128 && d_v == 128) return launch<128, 128, 128, 1, 1, 4>(p, ws, st);
+    if (d_qk == 192 && d_v == 128) return launch<192, 192, 128, 1, 1, 4>(p, ws, st);
+  } else {
+    if (d_qk == 192 && d_v == 128) return launch<192, 128, 128, 1, 1, 4>(p, ws, st);
+    if (d_qk == 128 && d_v == 64) return launch<128, 64, 64, 1, 1, 4>(p, ws, st);
+  }
+  return set_error(DSA_ERR_UNSUPPORTED, "dsa_latent_mla_bwd: no %s kernel for d_qk=%lld d_v=%lld",
+                   expanded ? "expanded" : "absorbed", (long long)d_qk, (long long)d_v);
+}
+
+}  // namespace dsa

@@ -600,6 +600,52 @@ int dsa_topk_index_mask(const void *topk_indices, int topk_dtype, int64_t topk,
                         int fill_rows, void *stream);
 
 /*
+ * Dense latent attention: every key of a row's window instead of a top-k of them
+ * (the attention of the DSA warm-up, and of layers without an indexer; bf16).
+ *
+ * Absorbed: q [B, S, H, D_qk], kv [B, S_kv, G, D_qk], V = kv[..., :D_v]; head h
+ *   reads kv group h / (H / G).  (D_qk, D_v) in {(128, 64), (128, 128), (192, 128)}.
+ * Expanded: q [B, S, H, D_nope + D_pe], k_nope [B, S_kv, H, D_nope], k_pe
+ *   [B, S_kv, D_pe] shared by the heads, v [B, S_kv, H, D_v]; D_pe = 64 and
+ *   (D_nope, D_v) in {(128, 128), (64, 64)}.  strides: in elements, of
+ *   (k_nope: batch, token, head; k_pe: batch, token; v: batch, token, head), multiples
+ *   of 8 (0 broadcasts), token strides below 2^23; the last axes are dense.
+ * Row t sees the keys [starts[b, t], ends[b, t]) clipped to [0, S_kv) where the int32
+ *   [B, S] windows are given (both or neither, causal 0); else, with causal, the keys up
+ *   to position t + S_kv - S; else all.  A row without keys: out 0, lse2 -inf, no gradient.
+ *   Keys outside a row's window reach neither its results nor its gradients, whatever
+ *   they hold.
+ *   out [B, S, H, D_v] bf16, lse2 [B, S, H] f32 (log2 units); sm_scale > 0.
+ *
+ * Backward, from the forward's out (o) and lse2 and the upstream gradient dO:
+ *   dq, and dkv (absorbed) or dk_nope, dk_pe (summed over the heads), dv (expanded),
+ *   all dense bf16.  No float atomics: repeated calls give the same bits.  workspace:
+ *   dsa_latent_mla_bwd_workspace_size() bytes, 256-byte aligned (expanded: G = H,
+ *   D_qk = D_nope + D_pe, expanded = 1; 0 where the sizes are refused).
+ * Device pointers are 16-byte aligned.  Outputs and workspace overlap no input.
+ */
+int dsa_latent_mla_fwd(const void *q, const void *kv, const int32_t *starts, const int32_t *ends,
+                       void *out, float *lse2, int64_t B, int64_t S, int64_t S_kv, int64_t H,
+                       int64_t G, int64_t D_qk, int64_t D_v, float sm_scale, int causal, void *stream);
+int dsa_latent_mla_expanded_fwd(const void *q, const void *k_nope, const void *k_pe, const void *v,
+                                const int32_t *starts, const int32_t *ends, void *out, float *lse2,
+                                int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t D_nope,
+                                int64_t D_pe, int64_t D_v, const int64_t *strides, float sm_scale,
+                                int causal, void *stream);
+size_t dsa_latent_mla_bwd_workspace_size(int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G,
+                                         int64_t D_qk, int64_t D_v, int expanded);
+int dsa_latent_mla_bwd(const void *q, const void *kv, const void *o, const void *dO, const float *lse2,
+                       const int32_t *starts, const int32_t *ends, void *dq, void *dkv, void *workspace,
+                       size_t workspace_bytes, int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G,
+                       int64_t D_qk, int64_t D_v, float sm_scale, int causal, void *stream);
+int dsa_latent_mla_expanded_bwd(const void *q, const void *k_nope, const void *k_pe, const void *v,
+                                const void *o, const void *dO, const float *lse2, const int32_t *starts,
+                                const int32_t *ends, void *dq, void *dk_nope, void *dk_pe, void *dv,
+                                void *workspace, size_t workspace_bytes, int64_t B, int64_t S,
+                                int64_t S_kv, int64_t H, int64_t D_nope, int64_t D_pe, int64_t D_v,
+                                const int64_t *strides, float sm_scale, int causal, void *stream);
+
+/*
  * Stage timing (measurement aid; no counterpart in the reference, which
  * times whole calls with CUDA events in its benchmark scripts).  With
  * dsa_stage_timing(1) on a thread, every later dsa_sparse_mla_bwd call on
