@@ -26,6 +26,7 @@ DTYPE_F32 = 2
 DTYPE_I32 = 3
 DTYPE_I64 = 4
 DTYPE_MXFP8 = 5
+DTYPE_MXFP4 = 6
 
 BWD_FP32_PARTIALS = 1
 
@@ -77,6 +78,12 @@ EXPORTED_SYMBOLS = (
     "dsa_latent_mla_bwd_workspace_size",
     "dsa_latent_mla_bwd",
     "dsa_latent_mla_expanded_bwd",
+    "dsa_latent_cache_row_bytes",
+    "dsa_latent_cache_append",
+    "dsa_latent_cache_gather",
+    "dsa_latent_plan_step",
+    "dsa_paged_latent_mla_workspace_size",
+    "dsa_paged_latent_mla_fwd",
     "dsa_stage_timing",
     "dsa_stage_times",
 )
@@ -167,6 +174,13 @@ _SIGNATURES = {
     "dsa_latent_mla_bwd": (_i32, [_c_void_p] * 10 + [_size_t] + [_i64] * 7 + [_f32, _i32, _c_void_p]),
     "dsa_latent_mla_expanded_bwd": (_i32, [_c_void_p] * 14 + [_size_t] + [_i64] * 7
                                     + [ctypes.POINTER(_i64), _f32, _i32, _c_void_p]),
+    "dsa_latent_cache_row_bytes": (_i64, [_i64, _i64, _i32]),
+    "dsa_latent_cache_append": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p] + [_i64] * 5
+                                + [_i32, _c_void_p]),
+    "dsa_latent_cache_gather": (_i32, [_c_void_p] * 3 + [_i64] * 5 + [_i32, _c_void_p]),
+    "dsa_latent_plan_step": (_i32, [_c_void_p] * 14 + [_i64] * 5 + [_c_void_p]),
+    "dsa_paged_latent_mla_workspace_size": (_size_t, [_i64] * 7),
+    "dsa_paged_latent_mla_fwd": (_i32, [_c_void_p] * 8 + [_size_t] + [_i64] * 8 + [_i32, _f32, _c_void_p]),
     "dsa_stage_timing": (_i32, [_i32]),
     "dsa_stage_times": (_i32, [_i32, ctypes.POINTER(ctypes.c_float), _i32]),
 }

@@ -7,6 +7,15 @@ same (out, lse) results, every admitted key instead of a top-k.  Every entry poi
 launches the HIP kernels of libdsa_hip.so; importing this package does not load the
 library.
 """
+from .latent_cache import (
+    LatentCache,
+    LatentStepPlan,
+    latent_cache_append,
+    latent_cache_gather,
+    latent_cache_row_bytes,
+    paged_latent_mla_fwd,
+    plan_latent_step,
+)
 from .latent_mla import (
     LatentMLA,
     LatentMLAExpanded,
@@ -17,10 +26,17 @@ from .latent_mla import (
 )
 
 __all__ = [
+    "LatentCache",
     "LatentMLA",
     "LatentMLAExpanded",
+    "LatentStepPlan",
+    "latent_cache_append",
+    "latent_cache_gather",
+    "latent_cache_row_bytes",
     "latent_mla_bwd",
     "latent_mla_expanded_bwd",
     "latent_mla_expanded_fwd",
     "latent_mla_fwd_interface",
+    "paged_latent_mla_fwd",
+    "plan_latent_step",
 ]

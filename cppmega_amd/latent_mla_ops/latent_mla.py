@@ -206,10 +206,13 @@ class LatentMLA(torch.autograd.Function):
         out, lse = latent_mla_fwd_interface(q, kv, d_v=q.shape[-1] if d_v is None else d_v, starts=starts, ends=ends, **ctx.args)
         ctx.save_for_backward(q, kv, out, lse, starts, ends)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     def backward(ctx, grad_output, grad_lse):
+        if grad_output is None:
+            return (None,) * 7
         q, kv, out, lse, starts, ends = ctx.saved_tensors
         dq, dkv = latent_mla_bwd(q, kv, out, grad_output.contiguous(), lse, starts=starts, ends=ends, **ctx.args)
         return dq, dkv, None, None, None, None, None
@@ -226,10 +229,13 @@ class LatentMLAExpanded(torch.autograd.Function):
         out, lse = latent_mla_expanded_fwd(q, k_nope, k_pe, v, starts=starts, ends=ends, **ctx.args)
         ctx.save_for_backward(q, k_nope, k_pe, v, out, lse, starts, ends)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     def backward(ctx, grad_output, grad_lse):
+        if grad_output is None:
+            return (None,) * 8
         q, k_nope, k_pe, v, out, lse, starts, ends = ctx.saved_tensors
         grads = latent_mla_expanded_bwd(q, k_nope, k_pe, v, out, grad_output.contiguous(), lse, starts=starts, ends=ends, **ctx.args)
         return (*grads, None, None, None, None)

@@ -40,7 +40,8 @@ enum dsa_dtype {
   DSA_DTYPE_F32 = 2,         /* float32                                      */
   DSA_DTYPE_I32 = 3,         /* int32 (index tensors)                        */
   DSA_DTYPE_I64 = 4,         /* int64 (index tensors)                        */
-  DSA_DTYPE_MXFP8 = 5        /* e4m3 with one f32 scale per 32 channels      */
+  DSA_DTYPE_MXFP8 = 5,       /* e4m3 with one f32 scale per 32 channels      */
+  DSA_DTYPE_MXFP4 = 6        /* latent cache rows: e2m1, one exponent byte per 32 channels */
 };
 
 /* Per-thread message for the last non-zero status returned on this thread. */
@@ -644,6 +645,67 @@ int dsa_latent_mla_expanded_bwd(const void *q, const void *k_nope, const void *k
                                 void *workspace, size_t workspace_bytes, int64_t B, int64_t S,
                                 int64_t S_kv, int64_t H, int64_t D_nope, int64_t D_pe, int64_t D_v,
                                 const int64_t *strides, float sm_scale, int causal, void *stream);
+
+/*
+ * Paged cache of latent rows: [num_blocks][block_size] rows of D_qk channels, the
+ * latent's D_v and then the rope part; (D_qk, D_v) in {(576, 512), (128, 64)}.
+ *   DSA_DTYPE_BF16   D_qk bf16
+ *   DSA_DTYPE_MXFP4  D_v / 2 bytes of e2m1 codes (channel 2 i in the low half of byte
+ *                    i), the rope part in bf16, D_v / 32 exponent bytes e (scale
+ *                    2^(e - 127), 255: NaN), zero or more bytes up to a multiple of 16
+ * A slot is page * block_size + offset.  dsa_latent_cache_row_bytes: bytes of a row (0
+ * where the sizes are refused).
+ * append: token t's latent (row stride latent_stride elements) and rope to slots[t];
+ *   slots outside the cache are skipped; a slot may be given once.  MXFP4: scale
+ *   2^(floor(log2 amax) - 2) of each 32 channels, its exponent held to +-125 (all zeros:
+ *   2^0), codes to nearest even, saturating at 6; a block with Inf or NaN gets 255.
+ * gather: out [T, D_qk] bf16 of slots (zeros outside the cache), exact.
+ * Pointers of rows are 16-byte aligned, row strides multiples of 8 elements.
+ */
+int64_t dsa_latent_cache_row_bytes(int64_t D_qk, int64_t D_v, int dtype);
+int dsa_latent_cache_append(void *cache, const void *latent, int64_t latent_stride, const void *rope,
+                            int64_t rope_stride, const int64_t *slots, int64_t T, int64_t num_blocks,
+                            int64_t block_size, int64_t D_qk, int64_t D_v, int dtype, void *stream);
+int dsa_latent_cache_gather(const void *cache, const int64_t *slots, void *out, int64_t T,
+                            int64_t num_blocks, int64_t block_size, int64_t D_qk, int64_t D_v, int dtype,
+                            void *stream);
+
+/*
+ * Plan of a serving step, one launch: from context_lens [R] (cached tokens), query_lens
+ * [R] (new tokens; negative: the request is done), block_table [R, W], free_blocks [F]
+ * and free_count [1] (how many of its first entries are free), all int32 on the device,
+ *   block_table_out [R, W]; slots int64 [T], positions [T] of the token batch (-1: none);
+ *   query_starts [R + 1]; kv_lens [R] (context + new tokens, 0 where not granted);
+ *   context_lens_out [R]; granted [R]; free_blocks_out [F], free_count_out [1].
+ * New pages are taken from the end of the free list in request order; a request is
+ * granted its tokens where they lie within T and W pages and the pages needed up to and
+ * with it are free (or it needs none).  Pages of done requests are appended to what is
+ * left.  Lengths and counts are clipped to their ranges.  No output may be an input.
+ */
+int dsa_latent_plan_step(const int32_t *context_lens, const int32_t *query_lens, const int32_t *block_table,
+                         const int32_t *free_blocks, const int32_t *free_count, int32_t *block_table_out,
+                         int64_t *slots, int32_t *positions, int32_t *query_starts, int32_t *kv_lens,
+                         int32_t *context_lens_out, int32_t *granted, int32_t *free_blocks_out,
+                         int32_t *free_count_out, int64_t R, int64_t W, int64_t F, int64_t T,
+                         int64_t block_size, void *stream);
+
+/*
+ * Latent attention over the paged cache (absorbed form): q [T, H, D_qk] bf16, request
+ * r's tokens query_starts[r] .. query_starts[r + 1] (ascending; NULL: token r alone) are
+ * the last of its kv_lens[r] positions; a token sees the positions up to its own.
+ * block_table [R, W] int32: an entry outside [0, num_blocks) hides its keys; lengths
+ * past W * block_size are cut.  out [T, H, D_v] bf16, lse2 [T, H] f32; a token without
+ * keys: 0 and -inf; tokens of no request are not written.  Keys that a token does not
+ * see do not reach it, whatever they hold.  workspace:
+ * dsa_paged_latent_mla_workspace_size() bytes, 256-byte aligned.
+ */
+size_t dsa_paged_latent_mla_workspace_size(int64_t T, int64_t R, int64_t W, int64_t block_size, int64_t H,
+                                           int64_t D_qk, int64_t D_v);
+int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const int32_t *block_table,
+                             const int32_t *query_starts, const int32_t *kv_lens, void *out, float *lse2,
+                             void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t W,
+                             int64_t H, int64_t D_qk, int64_t D_v, int64_t num_blocks, int64_t block_size,
+                             int dtype, float sm_scale, void *stream);
 
 /*
  * Stage timing (measurement aid; no counterpart in the reference, which
