@@ -26,12 +26,13 @@ struct LatentParams {
   const unsigned char *o, *dO;
   const float *lse_in;
   uint16_t *dq, *dk, *dkpe, *dv;       // absorbed: dk = dkv [B, S_kv, G, DK]
-  float *stat;                         // [B * G][nt64][4][64]: lse2, delta * scale, lo, hi (int bits) of a row
+  float *stat;                         // [B * G][nt64][4][64]: -lse2 / sl2, -delta, lo, hi (int bits) of a row
   int32_t *info;                       // [B * G][2 nt64][4]: least lo, largest hi, largest lo, least hi of 32 rows
   int64_t nt64;                        // 64-row tiles of a (batch, group)
   float *part;                         // [nsplit][B * G][S_kv][width] partial sums of the key gradients
   int32_t *used;                       // [nsplit][B * G][key blocks]: a partial was written
   int nsplit, tiles_per_split, nkb;
+  int64_t items;                       // key-major workgroups of a (batch, group)
 };
 
 constexpr int kKeyTile = 64;           // keys (or, in the key-major kernel, rows) of an LDS tile
@@ -53,6 +54,20 @@ __device__ __forceinline__ void latent_window(const LatentParams &p, int64_t b, 
     hi = e < 0 ? 0 : (e < sk ? (int)e : sk);
   }
   if (hi <= lo) lo = hi = 0;
+}
+
+// Workgroups reach the XCDs in turn (blockIdx % 8).  Of n groups with `per` items each, item id's group and index:
+// where the groups divide among the XCDs, a group's items stay on one (they share its tensors in that L2), group after
+// group; else index after index, so that every XCD gets long and short ones alike.
+__device__ __forceinline__ void spread_items(int64_t id, int64_t n, int64_t per, int64_t &group, int64_t &index) {
+  if (n % 8 == 0) {
+    const int64_t j = id >> 3, round = j / per;
+    group = round * 8 + (id & 7);
+    index = j - round * per;
+  } else {
+    index = id / n;
+    group = id - index * n;
+  }
 }
 
 // What a set of rows admits: the union [lo, hi) of their windows and the keys
@@ -145,6 +160,39 @@ __device__ __forceinline__ void pack_operand(const f32x16 &x, i32x4 (&b)[2]) {
                  (int)pack_bf16x2(x[8 * u + 4], x[8 * u + 5]), (int)pack_bf16x2(x[8 * u + 6], x[8 * u + 7])};
 }
 
+// Keeps a wave-uniform branch a branch: what it holds is then not computed, and selected from, where it is not taken.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
+// The operands of N products read from LDS, kGroup at a time, a group ahead of its use:
+// use(i, operand) for i in order.  The first group was loaded by the caller (while
+// something else ran); the barriers keep the compiler from sinking a load to its use.
+constexpr int kGroup = 4;
+struct Operands {
+  i32x4 x[kGroup];
+};
+template <int N, class Load>
+__device__ __forceinline__ void load_group(Operands &o, int g, Load load) {
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i)
+    if (g * kGroup + i < N) o.x[i] = load(g * kGroup + i);
+}
+template <int N, class Load, class Use>
+__device__ __forceinline__ void stream_operands(const Operands &first, Load load, Use use) {
+  constexpr int NG = (N + kGroup - 1) / kGroup;
+  Operands cur = first;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    Operands nxt;
+    if (g + 1 < NG) load_group<N>(nxt, g + 1, load);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i)
+      if (g * kGroup + i < N) use(g * kGroup + i, cur.x[i]);
+    __builtin_amdgcn_sched_barrier(0);
+    if (g + 1 < NG) cur = nxt;
+  }
+}
+
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
@@ -161,8 +209,10 @@ __device__ __forceinline__ f32x16 zero16() {
 template <int NDT, class Admit>
 __device__ __forceinline__ void careful_product(f32x16 (&acc)[NDT], const f32x16 &x, const unsigned char *sub, Admit admit) {
   const int g32 = lane_id() >> 5;
+#pragma unroll 1
   for (int i = 0; i < 16; ++i) {
     const float mine = x[i], other = xor32(mine);
+#pragma unroll 1
     for (int hf = 0; hf < 2; ++hf) {
       const int r = 8 * (i >> 2) + 4 * hf + (i & 3);
       const float xv = g32 == hf ? mine : other;
@@ -176,6 +226,7 @@ __device__ __forceinline__ void careful_product(f32x16 (&acc)[NDT], const f32x16
               *reinterpret_cast<const uint16_t *>(sub + (col >> 6) * 4096 + tile_byte(r, (col & 63) >> 3) + (col & 7) * 2);
           const float t = fmaf(xv, bf16_bits_to_f32(raw), acc[dt][a]);
           acc[dt][a] = ok ? t : acc[dt][a];
+          if ((a & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // few loads in flight: the registers are the fast path's
         }
     }
   }
@@ -186,6 +237,6 @@ __device__ __forceinline__ i32x4 tile_rsrc(const unsigned char *base) { return m
 
 int launch_latent_fwd(const LatentParams &p, int64_t d_qk, int64_t d_v, bool expanded, hipStream_t st);
 int launch_latent_bwd(const LatentParams &p, int64_t d_qk, int64_t d_v, bool expanded, unsigned char *ws, hipStream_t st);
-size_t latent_bwd_workspace(int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t d_qk, int64_t d_v, bool expanded);
+size_t latent_bwd_workspace(LatentParams p, int64_t d_qk, int64_t d_v, bool expanded);  // (the sizes of p)
 
 }  // namespace dsa

@@ -124,7 +124,7 @@ extern "C" size_t dsa_latent_mla_bwd_workspace_size(int64_t B, int64_t S, int64_
                                                     int64_t D_v, int expanded) {
   if (check_common("dsa_latent_mla_bwd_workspace_size", B, S, S_kv, H, G, 1.0f, 0, nullptr, nullptr)) return 0;
   if (check_shape("dsa_latent_mla_bwd_workspace_size", D_qk, D_v, expanded != 0)) return 0;
-  return latent_bwd_workspace(B, S, S_kv, H, G, D_qk, D_v, expanded != 0);
+  return latent_bwd_workspace(common_params(nullptr, nullptr, nullptr, B, S, S_kv, H, G, 1.0f, 0), D_qk, D_v, expanded != 0);
 }
 
 static int backward(const char *who, LatentParams &p, const void *o, const void *dO, const float *lse2, void *dq, int64_t d_qk,
@@ -132,7 +132,7 @@ static int backward(const char *who, LatentParams &p, const void *o, const void 
   const int64_t n = p.B * p.S;
   DSA_REQUIRE(given(p.q, n) && given(o, n) && given(dO, n) && given(dq, n) && (n == 0 || lse2 != nullptr),
               "%s: null or misaligned pointer", who);
-  const size_t need = latent_bwd_workspace(p.B, p.S, p.S_kv, p.H, p.G, d_qk, d_v, expanded);
+  const size_t need = latent_bwd_workspace(p, d_qk, d_v, expanded);
   if (need > 0 && (ws == nullptr || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u)))
     return set_error(DSA_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", who, need, ws_bytes);
   p.o = (const unsigned char *)o;

@@ -18,6 +18,8 @@
 // bit for bit.  P and dS are rounded to bf16 (nearest even) for the matrix products;
 // sums are fp32.  Both kernels form S and dP (the reading and the rounding of a stored
 // P and dS, 4 bytes a pair, would take longer than the two products).
+#include <type_traits>
+
 #include "latent_mla.hpp"
 
 namespace dsa {
@@ -35,16 +37,17 @@ struct LatentBwdQ {
   static constexpr int BYTES = OFF_SPAN + NW * 16 + 16;
 };
 
-template <int DK, int DN, int DV, int RT, int NW>
-__global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParams p) {
+template <int DK, int DN, int DV, int RT, int NW, int OCC>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) latent_bwd_q_kernel(const LatentParams p) {
   using C = LatentBwdQ<DK, DN, DV, RT, NW>;
   constexpr int KS = DK / 16, VS = DV / 16, NDT = DK / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const int nblk = (int)((p.rows + C::ROWS - 1) / C::ROWS);
-  const int64_t item = xcd_remap(blockIdx.x, gridDim.x);
-  const int64_t bg = item / nblk, b = bg / p.G, g = bg - b * p.G;
-  const int blk = nblk - 1 - (int)(item - bg * nblk);
+  int64_t bg, index;
+  spread_items(blockIdx.x, p.B * p.G, nblk, bg, index);
+  const int64_t b = bg / p.G, g = bg - b * p.G;
+  const int blk = nblk - 1 - (int)index;
   int *span_lds = reinterpret_cast<int *>(smem + C::OFF_SPAN);
 
   int lo[RT], hi[RT];
@@ -86,7 +89,8 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
       }
     }
     const bool any = hi[rt] > lo[rt];
-    delta[rt] = any ? sum_halves(dl) * p.scale : 0.0f;
+    dl = sum_halves(dl);
+    delta[rt] = any ? dl * p.scale : 0.0f;
     lse[rt] = any ? p.lse_in[orow[rt]] : kNoRow;
     // what the key-major kernel needs of these rows
     const int64_t r32 = (int64_t)blk * (C::ROWS / 32) + w * RT + rt, t64 = r32 >> 1;
@@ -94,8 +98,8 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
       const RowSpan s = span_wave(mine);
       float *st = p.stat + (bg * p.nt64 + t64) * 256 + (r32 & 1) * 32 + l32;
       if (g32 == 0) {
-        st[0] = lse[rt];
-        st[64] = delta[rt];
+        st[0] = -lse[rt] / p.sl2;
+        st[64] = any ? -dl : 0.0f;
       } else {
         st[128] = __int_as_float(lo[rt]);
         st[192] = __int_as_float(hi[rt]);
@@ -140,7 +144,8 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
   const RowRead row_read;
   const ColRead col_read;
   f32x16 acc[RT][NDT];
-  for (int careful = 0; careful < 2; ++careful) {
+  auto pass = [&](auto careful_t) {
+    constexpr bool careful = decltype(careful_t)::value;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -152,35 +157,38 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
       __syncthreads();
       if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
       const unsigned char *Kt = smem + buf * C::BUF, *Vt = C::SHARED ? Kt : Kt + C::K_BYTES;
+if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
+      // operands 0 .. KS - 1: K; absorbed: the first VS of them V too; expanded: V after them
+      constexpr int NR = C::SHARED ? KS : KS + VS;
+      auto rows_of = [&](int sub) {
+        return [=](int i) { return i < KS ? row_read(Kt + sub * C::KP * 4096, i) : row_read(Vt + sub * C::VP * 4096, i - KS); };
+      };
+      Operands ka;
+      load_group<NR>(ka, 0, rows_of(0));
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int ks0 = k0 + 32 * s;
-        if (ks0 >= span.hi || ks0 + 32 <= span.lo) continue;
         const bool whole = span.lo_max <= ks0 && span.hi_min >= ks0 + 32;
-        const unsigned char *Ks = Kt + s * C::KP * 4096, *Vs = Vt + s * (C::SHARED ? C::KP : C::VP) * 4096;
+        const unsigned char *Ks = Kt + s * C::KP * 4096;
+        auto cols = [&](int i) { return col_read(Ks, i >> 1, i & 1); };
         f32x16 sc[RT], dp[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) sc[rt] = dp[rt] = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const i32x4 a = row_read(Ks, ks);
+        stream_operands<NR>(ka, rows_of(s), [&](int i, i32x4 a) {
+          const int vs = C::SHARED ? i : i - KS;
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            sc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(q[rt][ks]), sc[rt], 0, 0, 0);
-            if constexpr (C::SHARED)
-              if (ks < VS)
-                dp[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(dO[rt][ks < VS ? ks : 0]), dp[rt], 0, 0, 0);
+            if (i < KS)
+              sc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(q[rt][i < KS ? i : 0]), sc[rt], 0, 0, 0);
+            if (vs >= 0 && vs < VS)
+              dp[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(dO[rt][vs >= 0 && vs < VS ? vs : 0]), dp[rt], 0, 0, 0);
           }
-        }
-        if constexpr (!C::SHARED) {
-#pragma unroll
-          for (int vs = 0; vs < VS; ++vs) {
-            const i32x4 a = row_read(Vs, vs);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              dp[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(dO[rt][vs]), dp[rt], 0, 0, 0);
-          }
-        }
+        });
+        // in flight beside the softmax: the first operands of its product with K, and of the next keys
+        Operands ca;
+        load_group<2 * NDT>(ca, 0, cols);
+        if (s == 0) load_group<NR>(ka, 0, rows_of(1));
+        __builtin_amdgcn_sched_barrier(0);
         i32x4 db[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -188,6 +196,7 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
           for (int i = 0; i < 16; ++i)
             sc[rt][i] = exp2_fast(fmaf(sc[rt][i], p.sl2, -lse[rt])) * fmaf(dp[rt][i], p.scale, -delta[rt]);
           if (!whole) {
+            keep_branch();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int key = ks0 + acc_row(i, g32);
@@ -197,15 +206,12 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
           pack_operand(sc[rt], db[rt]);
         }
         if (!careful || whole) {
+          stream_operands<2 * NDT>(ca, cols, [&](int i, i32x4 a) {
 #pragma unroll
-          for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const i32x4 a = col_read(Ks, dt, u);
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt)
-                acc[rt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(db[rt][u]), acc[rt][dt], 0, 0, 0);
-            }
+            for (int rt = 0; rt < RT; ++rt)
+              acc[rt][i >> 1] =
+                  __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(db[rt][i & 1]), acc[rt][i >> 1], 0, 0, 0);
+          });
         } else {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
@@ -213,17 +219,17 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
         }
       }
     }
-    __syncthreads();
-    if (careful) break;
-    bool bad = false;
+    __syncthreads();  // the buffers are free again
+  };
+  pass(std::false_type{});
+  bool bad = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
+    for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) bad |= not_finite(acc[rt][dt][i]);
-    if (__syncthreads_or(bad) == 0) break;  // a masked Inf or NaN may have reached a row: once more, without it
-  }
+      for (int i = 0; i < 16; ++i) bad |= not_finite(acc[rt][dt][i]);
+  if (__syncthreads_or(bad)) pass(std::true_type{});  // a masked Inf or NaN may have reached a row: once more, without it
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
     if (orow[rt] >= 0) {
@@ -239,6 +245,15 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_q_kernel(const LatentParam
     }
 }
 
+// Key blocks that the rows of a split reach: all, or up to its last token's under the causal mask.
+__host__ __device__ inline int split_blocks(const LatentParams &p, int split, int keys) {
+  if (!p.causal || p.nsplit == 1) return p.nkb;  // unsplit: every key block is written, if with zeros
+  const int64_t row1 = (int64_t)(split + 1) * p.tiles_per_split * 64, end = row1 < p.rows ? row1 : p.rows;
+  const int64_t key1 = (end + p.hpg - 1) / p.hpg + p.S_kv - p.S;  // one past the last key
+  const int64_t n = key1 <= 0 ? 0 : (key1 + keys - 1) / keys;
+  return (int)(n < p.nkb ? n : p.nkb);
+}
+
 template <int DK, int DN, int DV, int CT, int NW>
 struct LatentBwdKv {
   static constexpr bool SHARED = DN == DK;
@@ -252,17 +267,22 @@ struct LatentBwdKv {
   static constexpr int WIDE = SHARED ? DK : DK + DV;
 };
 
-template <int DK, int DN, int DV, int CT, int NW>
-__global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentParams p) {
+template <int DK, int DN, int DV, int CT, int NW, int OCC>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) latent_bwd_kv_kernel(const LatentParams p) {
   using C = LatentBwdKv<DK, DN, DV, CT, NW>;
   constexpr int KS = DK / 16, VS = DV / 16, NDK = DK / 32, NDV = DV / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
-  int64_t item = xcd_remap(blockIdx.x, gridDim.x);
-  const int kblk = (int)(item % p.nkb);
-  item /= p.nkb;
-  const int split = (int)(item % p.nsplit);
-  const int64_t bg = item / p.nsplit, b = bg / p.G, g = bg - b * p.G;
+  // item -> (batch and group, row split, key block): the splits from the last (the causal mask's with most key blocks),
+  // each with the key blocks that its rows reach; consecutive items, which share rows, on one XCD
+  const int64_t item = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int64_t bg = item / p.items, b = bg / p.G, g = bg - b * p.G;
+  if (bg >= p.B * p.G) return;
+  int kblk = (int)(item - bg * p.items), split = p.nsplit - 1;
+  for (int n = split_blocks(p, split, C::KEYS); kblk >= n; n = split_blocks(p, split, C::KEYS)) {
+    kblk -= n;
+    --split;
+  }
   const int key_lo = kblk * C::KEYS, key_hi = key_lo + C::KEYS < p.S_kv ? key_lo + C::KEYS : (int)p.S_kv;
   const int wkey = key_lo + w * CT * 32;  // this wave's first key
 
@@ -294,18 +314,34 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
   const int32_t *info = p.info + bg * p.nt64 * 8;
   const int c0 = split * p.tiles_per_split;
   const int c1 = c0 + p.tiles_per_split < p.nt64 ? c0 + p.tiles_per_split : (int)p.nt64;
-  auto next = [&](int t) {
-    for (; t < c1; t += 64) {
-      bool hit = false;
-      if (t + lane < c1) {
-        const i32x4 a = *reinterpret_cast<const i32x4 *>(info + (int64_t)(t + lane) * 8);
-        const i32x4 c = *reinterpret_cast<const i32x4 *>(info + (int64_t)(t + lane) * 8 + 4);
-        hit = (a[0] < key_hi && a[1] > key_lo) || (c[0] < key_hi && c[1] > key_lo);
-      }
-      const uint64_t m = wv::ballot(hit);
-      if (m != 0ull) return t + __builtin_ctzll(m);
+  int hits_at = 0;       // tiles hits_at .. + 63 that do: bit by bit
+  uint64_t hits = 0;
+  auto scan = [&](int t) {
+    bool hit = false;
+    if (t + lane < c1) {
+      const i32x4 a = *reinterpret_cast<const i32x4 *>(info + (int64_t)(t + lane) * 8);
+      const i32x4 c = *reinterpret_cast<const i32x4 *>(info + (int64_t)(t + lane) * 8 + 4);
+      hit = (a[0] < key_hi && a[1] > key_lo) || (c[0] < key_hi && c[1] > key_lo);
+    }
+    hits_at = t;
+    hits = wv::ballot(hit);
+  };
+  auto next = [&](int t) {  // t in [hits_at, hits_at + 64]
+    while (t < c1) {
+      if (t >= hits_at + 64) scan(t);
+      const uint64_t m = hits >> (t - hits_at);
+      if (m != 0ull) return t + (int)__builtin_ctzll(m);
+      t = hits_at + 64;
     }
     return c1;
+  };
+  // the two spans of a row tile, read a tile ahead
+  struct Spans {
+    i32x4 s[2];
+  };
+  auto spans = [&](int t) {
+    const int tt = t < c1 ? t : c1 - 1;  // (a tile there is: c0 < c1 wherever this is asked)
+    return Spans{*reinterpret_cast<const i32x4 *>(info + (int64_t)tt * 8), *reinterpret_cast<const i32x4 *>(info + (int64_t)tt * 8 + 4)};
   };
 
   const uint32_t lds0 = lds_address(smem);
@@ -317,8 +353,11 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
     const int n = (int)(p.rows - r0 < 64 ? p.rows - r0 : 64);
     const int64_t base = (b * p.S + tok0) * p.H + g * p.hpg;  // row (token tok0, first head)
     const uint32_t H = (uint32_t)p.H;
-    auto at_row = [&](int r) {  // rows from base: tokens tok0 ..
-      const uint32_t x = h0 + (uint32_t)r, dt = x / hpg;
+    auto at_row = [&](int r) {  // rows from base: tokens tok0 .. (one group: they lie together; one head a group: a token apart)
+      const uint32_t x = h0 + (uint32_t)r;
+      if (hpg == H) return x;
+      if (hpg == 1) return x * H;
+      const uint32_t dt = x / hpg;
       return dt * H + (x - dt * hpg);
     };
     tile_fetch<C::KP, 0, C::KP, NW>(at, tile_rsrc(p.q + base * DK * 2), w,
@@ -332,8 +371,10 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
   const RowRead row_read;
   const ColRead col_read;
   f32x16 dk[CT][NDK], dv[C::SHARED ? 1 : CT][NDV];
-  const int first = __builtin_amdgcn_readfirstlane(next(c0));
-  for (int careful = 0; careful < 2; ++careful) {
+  scan(c0);
+  const int first = next(c0);
+  auto pass = [&](auto careful_t) {
+    constexpr bool careful = decltype(careful_t)::value;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
@@ -344,53 +385,79 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
       }
     }
     int tile = first, buf = 0;
-    if (tile < c1) fetch(tile, 0);
+    Spans now{}, then{};
+    if (careful) scan(c0);
+    if (tile < c1) {
+      fetch(tile, 0);
+      now = spans(tile);
+    }
     while (tile < c1) {
-      const int nxt = __builtin_amdgcn_readfirstlane(next(tile + 1));
+      const int nxt = next(tile + 1);
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's share of the tile
       __syncthreads();
       if (nxt < c1) fetch(nxt, buf ^ 1);
+      then = spans(nxt);
       const unsigned char *Qt = smem + buf * C::BUF, *Dt = Qt + C::Q_BYTES;
       const float *st = reinterpret_cast<const float *>(Qt + C::OFF_STAT);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const i32x4 in = *reinterpret_cast<const i32x4 *>(info + ((int64_t)tile * 2 + s) * 4);
-        if (in[0] >= wkey + CT * 32 || in[1] <= wkey) continue;  // wave-uniform
-        const bool whole = in[2] <= wkey && in[3] >= wkey + CT * 32;
-        const unsigned char *Qs = Qt + s * C::KP * 4096, *Ds = Dt + s * C::VP * 4096;
-        f32x16 sc[CT], dp[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) sc[ct] = dp[ct] = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const i32x4 a = row_read(Qs, ks);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            sc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(kr[ct][ks]), sc[ct], 0, 0, 0);
-        }
-#pragma unroll
-        for (int vs = 0; vs < VS; ++vs) {
-          const i32x4 a = row_read(Ds, vs);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            const i32x4 &bv = C::SHARED ? kr[ct][vs] : vr[C::SHARED ? 0 : ct][vs];
-            dp[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(bv), dp[ct], 0, 0, 0);
-          }
-        }
-        i32x4 pb[CT][2], db[CT][2];
+// operands 0 .. KS - 1: Q, then the VS of dO
+      auto rows_of = [&](int sub) {
+        return [=](int i) { return i < KS ? row_read(Qt + sub * C::KP * 4096, i) : row_read(Dt + sub * C::VP * 4096, i - KS); };
+      };
+      // the accumulators begin at -lse2 / sl2 and -delta of their rows
+      f32x16 sc[CT], dp[CT];
+      auto begin = [&](int sub) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const int r = 32 * s + 8 * m + 4 * g32;  // registers 4 m .. are rows r ..
+          const int r = 32 * sub + 8 * m + 4 * g32;  // registers 4 m .. are rows r ..
           const f32x4 ls = *reinterpret_cast<const f32x4 *>(st + r), de = *reinterpret_cast<const f32x4 *>(st + 64 + r);
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int i = 4 * m + e;
-              sc[ct][i] = exp2_fast(fmaf(sc[ct][i], p.sl2, -ls[e]));
-              dp[ct][i] = sc[ct][i] * fmaf(dp[ct][i], p.scale, -de[e]);
+              sc[ct][4 * m + e] = ls[e];
+              dp[ct][4 * m + e] = de[e];
             }
-          if (!whole) {
+        }
+      };
+      Operands qa;
+      load_group<KS + VS>(qa, 0, rows_of(0));
+      begin(0);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const bool whole = __builtin_amdgcn_readfirstlane(now.s[s][2]) <= wkey &&
+                           __builtin_amdgcn_readfirstlane(now.s[s][3]) >= wkey + CT * 32;
+        const unsigned char *Qs = Qt + s * C::KP * 4096, *Ds = Dt + s * C::VP * 4096;
+        // operands 0 .. 2 NDV - 1: dO^T, then the 2 NDK of Q^T
+        auto cols = [&](int i) { return i < 2 * NDV ? col_read(Ds, i >> 1, i & 1) : col_read(Qs, (i - 2 * NDV) >> 1, i & 1); };
+        stream_operands<KS + VS>(qa, rows_of(s), [&](int i, i32x4 a) {
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            if (i < KS) {
+              sc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(kr[ct][i < KS ? i : 0]), sc[ct], 0, 0, 0);
+            } else {
+              const i32x4 &bv = C::SHARED ? kr[ct][i < KS ? 0 : i - KS] : vr[C::SHARED ? 0 : ct][i < KS ? 0 : i - KS];
+              dp[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(bv), dp[ct], 0, 0, 0);
+            }
+          }
+        });
+        // in flight beside the softmax: the first operands of its products, and of the next rows
+        Operands ca;
+        load_group<2 * NDV + 2 * NDK>(ca, 0, cols);
+        if (s == 0) load_group<KS + VS>(qa, 0, rows_of(1));
+        __builtin_amdgcn_sched_barrier(0);
+        i32x4 pb[CT][2], db[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sc[ct][i] = exp2_fast(sc[ct][i] * p.sl2);
+            dp[ct][i] *= sc[ct][i] * p.scale;
+          }
+        if (!whole) {
+          keep_branch();
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const int r = 32 * s + 8 * m + 4 * g32;
             const i32x4 lo = *reinterpret_cast<const i32x4 *>(st + 128 + r), hi = *reinterpret_cast<const i32x4 *>(st + 192 + r);
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)
@@ -408,26 +475,19 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
           pack_operand(dp[ct], db[ct]);
         }
         if (!careful || whole) {
+          if (s == 0) begin(1);
+          stream_operands<2 * NDV + 2 * NDK>(ca, cols, [&](int i, i32x4 a) {
 #pragma unroll
-          for (int dt = 0; dt < NDV; ++dt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const i32x4 a = col_read(Ds, dt, u);
-#pragma unroll
-              for (int ct = 0; ct < CT; ++ct) {
-                f32x16 &t = C::SHARED ? dk[ct][dt] : dv[C::SHARED ? 0 : ct][dt];
-                t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(pb[ct][u]), t, 0, 0, 0);
+            for (int ct = 0; ct < CT; ++ct) {
+              const int j = i < 2 * NDV ? 0 : (i - 2 * NDV) >> 1, jv = i < 2 * NDV ? i >> 1 : 0;
+              if (i < 2 * NDV) {
+                f32x16 &t = C::SHARED ? dk[ct][jv] : dv[C::SHARED ? 0 : ct][jv];
+                t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(pb[ct][i & 1]), t, 0, 0, 0);
+              } else {
+                dk[ct][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(db[ct][i & 1]), dk[ct][j], 0, 0, 0);
               }
             }
-#pragma unroll
-          for (int dt = 0; dt < NDK; ++dt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const i32x4 a = col_read(Qs, dt, u);
-#pragma unroll
-              for (int ct = 0; ct < CT; ++ct)
-                dk[ct][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(db[ct][u]), dk[ct][dt], 0, 0, 0);
-            }
+          });
         } else {
           const int *sti = reinterpret_cast<const int *>(st);
 #pragma unroll
@@ -445,14 +505,18 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
             }
             careful_product<NDK>(dk[ct], dp[ct], Qs, admit);
           }
+          if (s == 0) begin(1);
         }
       }
       tile = nxt;
+      now = then;
       buf ^= 1;
     }
     __syncthreads();
-    if (careful) break;
-    bool bad = false;
+  };
+  pass(std::false_type{});
+  bool bad = false;
+  {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
@@ -466,8 +530,8 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
           for (int i = 0; i < 16; ++i) bad |= not_finite(dv[ct][dt][i]);
       }
     }
-    if (__syncthreads_or(bad) == 0) break;
   }
+  if (__syncthreads_or(bad)) pass(std::true_type{});
 
   const int64_t bgs = p.B * p.G;
   const bool split_rows = p.nsplit > 1;
@@ -507,59 +571,69 @@ __global__ void __launch_bounds__(64 * NW) latent_bwd_kv_kernel(const LatentPara
 // One thread per 4 columns: partial rows added in split order (k_pe: group by group,
 // each group's splits in order) and rounded once.
 struct LatentReduce {
-  const float *part;
-  const int32_t *used;
-  uint16_t *dk, *dkpe, *dv;
-  int64_t S_kv, B, G;
-  int nsplit, nkb, keys, width, dn, dr, dvw;  // width of a partial row: dn + dr + dvw, or dr
+  int keys, width, dn, dr, dvw;  // keys of a block; width of a partial row: dn + dr + dvw, or dr
 };
-__global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentReduce r) {
-  const int64_t bgs = r.B * r.G;
+__global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentParams p, const LatentReduce r) {
+  const int64_t bgs = p.B * p.G;
   const int own = (r.width - r.dr) / 4;  // columns of the group's own rows
-  const int64_t n_own = bgs * r.S_kv * own, n_pe = r.B * r.S_kv * (r.dr / 4);
+  const int64_t n_own = bgs * p.S_kv * own, n_pe = p.B * p.S_kv * (r.dr / 4);
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= n_own + n_pe) return;
   f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
   auto add = [&](int64_t bg, int64_t key, int col) {
-    const int64_t kb = key / r.keys;
-    for (int s = 0; s < r.nsplit; ++s) {
-      if (r.used != nullptr && r.used[(s * bgs + bg) * r.nkb + kb] == 0) continue;
-      sum += *reinterpret_cast<const f32x4 *>(r.part + ((s * bgs + bg) * r.S_kv + key) * r.width + col);
+    const int kb = (int)((uint32_t)key / (uint32_t)r.keys);
+    for (int s = 0; s < p.nsplit; ++s) {
+      if (p.nsplit > 1 && (kb >= split_blocks(p, s, r.keys) || p.used[(s * bgs + bg) * p.nkb + kb] == 0)) continue;
+      sum += *reinterpret_cast<const f32x4 *>(p.part + ((s * bgs + bg) * p.S_kv + key) * r.width + col);
     }
   };
   uint16_t *dst;
   if (id < n_own) {
-    const int64_t row = id / own, bg = row / r.S_kv, key = row - bg * r.S_kv;
+    const int64_t row = id / own, bg = row / p.S_kv, key = row - bg * p.S_kv;
     const int c = (int)(id - row * own) * 4;
-    const int64_t b = bg / r.G, orow = (b * r.S_kv + key) * r.G + (bg - b * r.G);
+    const int64_t b = bg / p.G, orow = (b * p.S_kv + key) * p.G + (bg - b * p.G);
     const bool is_k = c < r.dn;
     add(bg, key, is_k ? c : c + r.dr);
-    dst = is_k ? r.dk + orow * r.dn + c : r.dv + orow * r.dvw + (c - r.dn);
+    dst = is_k ? p.dk + orow * r.dn + c : p.dv + orow * r.dvw + (c - r.dn);
   } else {
-    const int64_t x = id - n_own, row = x / (r.dr / 4), b = row / r.S_kv, key = row - b * r.S_kv;
+    const int64_t x = id - n_own, row = x / (r.dr / 4), b = row / p.S_kv, key = row - b * p.S_kv;
     const int c = (int)(x - row * (r.dr / 4)) * 4;
-    for (int64_t g = 0; g < r.G; ++g) add(b * r.G + g, key, (r.width == r.dr ? 0 : r.dn) + c);
-    dst = r.dkpe + (b * r.S_kv + key) * r.dr + c;
+    for (int64_t g = 0; g < p.G; ++g) add(b * p.G + g, key, (r.width == r.dr ? 0 : r.dn) + c);
+    dst = p.dkpe + (b * p.S_kv + key) * r.dr + c;
   }
   *reinterpret_cast<i32x2 *>(dst) = i32x2{(int)pack_bf16x2(sum[0], sum[1]), (int)pack_bf16x2(sum[2], sum[3])};
 }
 
+// Waves per SIMD of the key-major kernel: two where its 32 keys a wave and their gradients leave the registers for it.
+constexpr int kv_waves(int64_t d_qk, int64_t d_v, bool expanded) { return !expanded && d_qk == 128 ? 2 : 1; }
+
+// Row splits of the key-major kernel: what takes least of the rounds of its workgroups on the card (1.3 us a row tile,
+// 8 tiles' time for a workgroup's beginning and end) and of the partial sums' way to memory and back.
 struct BwdKvPlan {
   int keys, nkb, nsplit, tiles_per_split, width;
+  int64_t items;  // workgroups of a (batch, group)
 };
-// Row splits: enough workgroups for four rounds of two a compute unit under a causal mask, which
-// leaves half of them without work, and at least 8 row tiles each.
-static BwdKvPlan kv_plan(int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t d_qk, int64_t d_v, bool expanded) {
-  BwdKvPlan r;
+static BwdKvPlan kv_plan(LatentParams p, int64_t d_qk, int64_t d_v, bool expanded) {
+  BwdKvPlan r{};
   r.keys = 4 * 32;
-  r.nkb = (int)((S_kv + r.keys - 1) / r.keys);
-  const int64_t tiles = (S * (H / G) + 63) / 64, wgs = B * G * r.nkb;
-  int64_t n = wgs > 0 ? (2048 + wgs - 1) / wgs : 1;
-  if (n > (tiles + 7) / 8) n = (tiles + 7) / 8;
-  if (n > 64) n = 64;
-  if (n < 1) n = 1;
-  r.tiles_per_split = tiles > 0 ? (int)((tiles + n - 1) / n) : 1;
-  r.nsplit = tiles > 0 ? (int)((tiles + r.tiles_per_split - 1) / r.tiles_per_split) : 1;
+  p.nkb = r.nkb = (int)((p.S_kv + r.keys - 1) / r.keys);
+  const int64_t tiles = (p.rows + 63) / 64, bgs = p.B * p.G, slots = kv_waves(d_qk, d_v, expanded) * 256;
+  const double row_us = (double)(bgs * p.S_kv * (expanded ? d_qk + d_v : d_qk)) * 8 / 4.9e6 * (p.causal ? 0.5 : 1.0);
+  double least = 0;
+  for (int64_t n = 1; n <= 64 && (n == 1 || n * 4 <= tiles); ++n) {
+    p.tiles_per_split = tiles > 0 ? (int)((tiles + n - 1) / n) : 1;
+    p.nsplit = tiles > 0 ? (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
+    int64_t items = 0;
+    for (int s = 0; s < p.nsplit; ++s) items += split_blocks(p, s, r.keys);
+    const double us = (double)((bgs * items + slots - 1) / slots) * 1.3 * (double)(p.tiles_per_split + 8) +
+                      (p.nsplit > 1 ? 6.0 + row_us * (double)p.nsplit : 0.0);
+    if (n == 1 || us < least) {
+      least = us;
+      r.nsplit = p.nsplit;
+      r.tiles_per_split = p.tiles_per_split;
+      r.items = items;
+    }
+  }
   r.width = expanded ? (r.nsplit > 1 ? (int)(d_qk + d_v) : 64) : (int)d_qk;
   return r;
 }
@@ -568,27 +642,34 @@ static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 struct BwdSections {
   size_t stat, info, used, part, total;
 };
-static BwdSections bwd_sections(const BwdKvPlan &k, int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, bool expanded) {
-  const size_t nt64 = (size_t)((S * (H / G) + 63) / 64), bgs = (size_t)(B * G);
+static BwdSections bwd_sections(const BwdKvPlan &k, const LatentParams &p, bool expanded) {
+  const size_t nt64 = (size_t)((p.rows + 63) / 64), bgs = (size_t)(p.B * p.G);
   BwdSections s;
   s.stat = 0;
   s.info = s.stat + bgs * nt64 * 1024;
   s.used = s.info + up256(bgs * nt64 * 32);
   s.part = s.used + (k.nsplit > 1 ? up256((size_t)k.nsplit * bgs * (size_t)k.nkb * 4) : 0);
-  s.total = s.part + (k.nsplit > 1 || expanded ? (size_t)k.nsplit * bgs * (size_t)S_kv * (size_t)k.width * 4 : 0);
+  s.total = s.part + (k.nsplit > 1 || expanded ? (size_t)k.nsplit * bgs * (size_t)p.S_kv * (size_t)k.width * 4 : 0);
   return s;
 }
-size_t latent_bwd_workspace(int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t d_qk, int64_t d_v, bool expanded) {
-  return bwd_sections(kv_plan(B, S, S_kv, H, G, d_qk, d_v, expanded), B, S, S_kv, H, G, expanded).total;
+size_t latent_bwd_workspace(LatentParams p, int64_t d_qk, int64_t d_v, bool expanded) {
+  // the larger of the two masks' plans: the query does not know the mask
+  size_t most = 0;
+  for (p.causal = 0; p.causal < 2; ++p.causal) {
+    const size_t n = bwd_sections(kv_plan(p, d_qk, d_v, expanded), p, expanded).total;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
-template <int DK, int DN, int DV, int RT, int CT, int NW>
+template <int DK, int DN, int DV, int RT, int OQ>
 static int launch(LatentParams p, unsigned char *ws, hipStream_t st) {
+  constexpr int NW = 4, CT = 1, OK = kv_waves(DK, DV, DN != DK);
   using Q = LatentBwdQ<DK, DN, DV, RT, NW>;
   using K = LatentBwdKv<DK, DN, DV, CT, NW>;
   constexpr bool expanded = DN != DK;
-  const BwdKvPlan k = kv_plan(p.B, p.S, p.S_kv, p.H, p.G, DK, DV, expanded);
-  const BwdSections s = bwd_sections(k, p.B, p.S, p.S_kv, p.H, p.G, expanded);
+  const BwdKvPlan k = kv_plan(p, DK, DV, expanded);
+  const BwdSections s = bwd_sections(k, p, expanded);
   p.nt64 = (p.rows + 63) / 64;
   p.stat = reinterpret_cast<float *>(ws + s.stat);
   p.info = reinterpret_cast<int32_t *>(ws + s.info);
@@ -597,13 +678,14 @@ static int launch(LatentParams p, unsigned char *ws, hipStream_t st) {
   p.nsplit = k.nsplit;
   p.tiles_per_split = k.tiles_per_split;
   p.nkb = k.nkb;
-  const auto qk = latent_bwd_q_kernel<DK, DN, DV, RT, NW>;
-  const auto kk = latent_bwd_kv_kernel<DK, DN, DV, CT, NW>;
+  p.items = k.items;
+  const auto qk = latent_bwd_q_kernel<DK, DN, DV, RT, NW, OQ>;
+  const auto kk = latent_bwd_kv_kernel<DK, DN, DV, CT, NW, OK>;
   hipError_t e = hipFuncSetAttribute((const void *)qk, hipFuncAttributeMaxDynamicSharedMemorySize, Q::BYTES);
   if (e == hipSuccess) e = hipFuncSetAttribute((const void *)kk, hipFuncAttributeMaxDynamicSharedMemorySize, K::BYTES);
   if (e != hipSuccess) return set_error(DSA_ERR_HIP, "dsa_latent_mla_bwd: LDS attribute: %s", hipGetErrorString(e));
   const int64_t bgs = p.B * p.G;
-  const int64_t nq = (p.rows + Q::ROWS - 1) / Q::ROWS * bgs, nk = (int64_t)k.nkb * k.nsplit * bgs;
+  const int64_t nq = (p.rows + Q::ROWS - 1) / Q::ROWS * bgs, nk = (k.items * bgs + 7) / 8 * 8;
   DSA_REQUIRE(nq < (1ll << 31) && nk < (1ll << 31), "dsa_latent_mla_bwd: grid too large");
   int rc = DSA_OK;
   if (nq > 0) {  // no rows: the key gradients below are zeros
@@ -614,22 +696,21 @@ static int launch(LatentParams p, unsigned char *ws, hipStream_t st) {
   hipLaunchKernelGGL(kk, dim3((unsigned)nk), dim3(64 * NW), K::BYTES, st, p);
   rc = check_launch("dsa_latent_mla_bwd (keys)");
   if (rc || (!expanded && k.nsplit == 1)) return rc;
-  LatentReduce r{p.part, k.nsplit > 1 ? p.used : nullptr, p.dk, p.dkpe, p.dv, p.S_kv, p.B, p.G, k.nsplit, k.nkb, k.keys,
-                 k.width, DN, DK - DN, expanded ? DV : 0};
+  const LatentReduce r{k.keys, k.width, DN, DK - DN, expanded ? DV : 0};
   const int64_t n = bgs * p.S_kv * ((r.width - r.dr) / 4) + p.B * p.S_kv * (r.dr / 4), wgs = (n + 255) / 256;
   DSA_REQUIRE(wgs < (1ll << 31), "dsa_latent_mla_bwd: grid too large");
-  hipLaunchKernelGGL(latent_bwd_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, r);
+  hipLaunchKernelGGL(latent_bwd_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, p, r);
   return check_launch("dsa_latent_mla_bwd (reduction)");
 }
 
 int launch_latent_bwd(const LatentParams &p, int64_t d_qk, int64_t d_v, bool expanded, unsigned char *ws, hipStream_t st) {
   if (!expanded) {
-    if (d_qk == 128 && d_v == 64) return launch<128, 128, 64, 1, 1, 4>(p, ws, st);
-    if (d_qk == 128 && d_v == 128) return launch<128, 128, 128, 1, 1, 4>(p, ws, st);
-    if (d_qk == 192 && d_v == 128) return launch<192, 192, 128, 1, 1, 4>(p, ws, st);
+    if (d_qk == 128 && d_v == 64) return launch<128, 128, 64, 1, 2>(p, ws, st);
+    if (d_qk == 128 && d_v == 128) return launch<128, 128, 128, 1, 2>(p, ws, st);
+    if (d_qk == 192 && d_v == 128) return launch<192, 192, 128, 1, 1>(p, ws, st);
   } else {
-    if (d_qk == 192 && d_v == 128) return launch<192, 128, 128, 1, 1, 4>(p, ws, st);
-    if (d_qk == 128 && d_v == 64) return launch<128, 64, 64, 1, 1, 4>(p, ws, st);
+    if (d_qk == 192 && d_v == 128) return launch<192, 128, 128, 1, 1>(p, ws, st);
+    if (d_qk == 128 && d_v == 64) return launch<128, 64, 64, 1, 2>(p, ws, st);
   }
   return set_error(DSA_ERR_UNSUPPORTED, "dsa_latent_mla_bwd: no %s kernel for d_qk=%lld d_v=%lld",
                    expanded ? "expanded" : "absorbed", (long long)d_qk, (long long)d_v);

@@ -12,6 +12,8 @@
 //                               they stand, V^T by transposed LDS reads)
 // Sums, statistics and O are fp32.  P is rounded to nearest even for the matrix
 // product; l sums the weights before that rounding.
+#include <type_traits>
+
 #include "latent_mla.hpp"
 
 namespace dsa {
@@ -27,16 +29,17 @@ struct LatentFwd {
   static constexpr int BYTES = OFF_SPAN + NW * 16 + 16;
 };
 
-template <int DK, int DN, int DV, int RT, int NW>
-__global__ void __launch_bounds__(64 * NW) latent_fwd_kernel(const LatentParams p) {
+template <int DK, int DN, int DV, int RT, int NW, int OCC>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) latent_fwd_kernel(const LatentParams p) {
   using C = LatentFwd<DK, DN, DV, RT, NW>;
   constexpr int KS = DK / 16, NDT = DV / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const int nblk = (int)((p.rows + C::ROWS - 1) / C::ROWS);
-  const int64_t item = xcd_remap(blockIdx.x, gridDim.x);
-  const int64_t bg = item / nblk, b = bg / p.G, g = bg - b * p.G;
-  const int blk = nblk - 1 - (int)(item - bg * nblk);  // the causal mask's longest first
+  int64_t bg, index;
+  spread_items(blockIdx.x, p.B * p.G, nblk, bg, index);
+  const int64_t b = bg / p.G, g = bg - b * p.G;
+  const int blk = nblk - 1 - (int)index;  // the causal mask's longest first
   int *span_lds = reinterpret_cast<int *>(smem + C::OFF_SPAN);
 
   // this lane's rows
@@ -100,7 +103,8 @@ __global__ void __launch_bounds__(64 * NW) latent_fwd_kernel(const LatentParams 
   float m_run[RT], l_run[RT];
   f32x16 o[RT][NDT];
 
-  for (int careful = 0; careful < 2; ++careful) {
+  auto pass = [&](auto careful_t) {
+    constexpr bool careful = decltype(careful_t)::value;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       m_run[rt] = kNegBig;
@@ -115,23 +119,31 @@ __global__ void __launch_bounds__(64 * NW) latent_fwd_kernel(const LatentParams 
       __syncthreads();                     // the tile is whole; the other buffer is consumed
       if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
       const unsigned char *Kt = smem + buf * C::BUF, *Vt = C::SHARED ? Kt : Kt + C::K_BYTES;
+if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
+      auto rows_of = [&](int sub) { return [=](int ks) { return row_read(Kt + sub * C::KP * 4096, ks); }; };
+      Operands ka;
+      load_group<KS>(ka, 0, rows_of(0));
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int ks0 = k0 + 32 * s;
-        if (ks0 >= span.hi || ks0 + 32 <= span.lo) continue;  // wave-uniform
         const bool whole = span.lo_max <= ks0 && span.hi_min >= ks0 + 32;
-        const unsigned char *Ks = Kt + s * C::KP * 4096, *Vs = Vt + s * (C::SHARED ? C::KP : C::VP) * 4096;
+        const unsigned char *Vs = Vt + s * (C::SHARED ? C::KP : C::VP) * 4096;
+        auto cols = [&](int i) { return col_read(Vs, i >> 1, i & 1); };
         f32x16 acc[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt] = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const i32x4 a = row_read(Ks, ks);
+        stream_operands<KS>(ka, rows_of(s), [&](int ks, i32x4 a) {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
             acc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(q[rt][ks]), acc[rt], 0, 0, 0);
-        }
+        });
+        // in flight beside the softmax: the first operands of its product with V, and of the next keys
+        Operands va;
+        load_group<2 * NDT>(va, 0, cols);
+        if (s == 0) load_group<KS>(ka, 0, rows_of(1));
+        __builtin_amdgcn_sched_barrier(0);
         if (!whole) {
+          keep_branch();
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -164,15 +176,12 @@ __global__ void __launch_bounds__(64 * NW) latent_fwd_kernel(const LatentParams 
           pack_operand(acc[rt], pb[rt]);
         }
         if (!careful || whole) {
+          stream_operands<2 * NDT>(va, cols, [&](int i, i32x4 a) {
 #pragma unroll
-          for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const i32x4 a = col_read(Vs, dt, u);
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt)
-                o[rt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(pb[rt][u]), o[rt][dt], 0, 0, 0);
-            }
+            for (int rt = 0; rt < RT; ++rt)
+              o[rt][i >> 1] =
+                  __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(pb[rt][i & 1]), o[rt][i >> 1], 0, 0, 0);
+          });
         } else {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
@@ -180,17 +189,17 @@ __global__ void __launch_bounds__(64 * NW) latent_fwd_kernel(const LatentParams 
         }
       }
     }
-    __syncthreads();  // the buffers (and the flag) are free again
-    if (careful) break;
-    bool bad = false;
+    __syncthreads();  // the buffers are free again
+  };
+  pass(std::false_type{});
+  bool bad = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
+    for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) bad |= not_finite(o[rt][dt][i]);
-    if (__syncthreads_or(bad) == 0) break;  // a masked Inf or NaN may have reached a row: once more, without it
-  }
+      for (int i = 0; i < 16; ++i) bad |= not_finite(o[rt][dt][i]);
+  if (__syncthreads_or(bad)) pass(std::true_type{});  // a masked Inf or NaN may have reached a row: once more, without it
 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -214,10 +223,10 @@ __global__ void __launch_bounds__(64 * NW) latent_fwd_kernel(const LatentParams 
   }
 }
 
-template <int DK, int DN, int DV, int RT, int NW>
+template <int DK, int DN, int DV, int RT, int NW, int OCC>
 static int launch(const LatentParams &p, hipStream_t st) {
   using C = LatentFwd<DK, DN, DV, RT, NW>;
-  const auto kernel = latent_fwd_kernel<DK, DN, DV, RT, NW>;
+  const auto kernel = latent_fwd_kernel<DK, DN, DV, RT, NW, OCC>;
   const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
   if (e != hipSuccess) return set_error(DSA_ERR_HIP, "dsa_latent_mla_fwd: LDS attribute: %s", hipGetErrorString(e));
   const int64_t n = (p.rows + C::ROWS - 1) / C::ROWS * p.B * p.G;
@@ -228,12 +237,12 @@ static int launch(const LatentParams &p, hipStream_t st) {
 
 int launch_latent_fwd(const LatentParams &p, int64_t d_qk, int64_t d_v, bool expanded, hipStream_t st) {
   if (!expanded) {
-    if (d_qk == 128 && d_v == 64) return launch<128, 128, 64, 2, 4>(p, st);
-    if (d_qk == 128 && d_v == 128) return launch<128, 128, 128, 2, 4>(p, st);
-    if (d_qk == 192 && d_v == 128) return launch<192, 192, 128, 2, 4>(p, st);
+    if (d_qk == 128 && d_v == 64) return launch<128, 128, 64, 1, 4, 3>(p, st);
+    if (d_qk == 128 && d_v == 128) return launch<128, 128, 128, 1, 4, 2>(p, st);
+    if (d_qk == 192 && d_v == 128) return launch<192, 192, 128, 1, 4, 2>(p, st);
   } else {
-    if (d_qk == 192 && d_v == 128) return launch<192, 128, 128, 2, 4>(p, st);
-    if (d_qk == 128 && d_v == 64) return launch<128, 64, 64, 2, 4>(p, st);
+    if (d_qk == 192 && d_v == 128) return launch<192, 128, 128, 1, 4, 2>(p, st);
+    if (d_qk == 128 && d_v == 64) return launch<128, 64, 64, 1, 4, 3>(p, st);
   }
   return set_error(DSA_ERR_UNSUPPORTED, "dsa_latent_mla_fwd: no %s kernel for d_qk=%lld d_v=%lld",
                    expanded ? "expanded" : "absorbed", (long long)d_qk, (long long)d_v);
