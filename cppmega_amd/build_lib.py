@@ -52,6 +52,7 @@ FILE_FLAGS = {
     "latent_mla_fwd.hip": _MFMA_VGPR + ["-fno-honor-nans", "-mno-amdgpu-ieee"],
     "latent_mla_bwd.hip": _MFMA_VGPR,
     "latent_paged.hip": _MFMA_VGPR,
+    "latent_paged_few.hip": _MFMA_VGPR,
 }
 
 

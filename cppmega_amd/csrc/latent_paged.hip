@@ -21,30 +21,6 @@
 
 namespace dsa {
 
-__device__ const i32x4 kZeroRow[80] = {};  // a masked key's row
-
-struct PagedUnit {
-  int req, first;       // request and first row of the unit within it
-  int rows, n, kv;      // rows of the request, its new tokens, its length
-  int64_t row0;         // row of q of the request's first
-};
-
-__device__ __forceinline__ int request_start(const PagedParams &p, int r) {
-  return p.query_starts == nullptr ? r : min(max(p.query_starts[r], 0), (int)p.T);
-}
-// new tokens of request r (within q's rows)
-__device__ __forceinline__ int request_tokens(const PagedParams &p, int r) {
-  if (p.query_starts == nullptr) return r < p.T ? 1 : 0;
-  const int n = request_start(p, r + 1) - request_start(p, r);
-  return n > 0 ? n : 0;
-}
-__device__ __forceinline__ int request_kv(const PagedParams &p, int r) {
-  const int kv = p.kv_lens[r];
-  const int64_t cap = (int64_t)p.W * p.block;
-  return kv < 0 ? 0 : (kv < cap ? kv : (int)cap);
-}
-// keys that token t of n new ones sees
-__device__ __forceinline__ int token_keys(int kv, int n, int t) { return max(kv - n + t + 1, 0); }
 // blocks of a unit (at least one: a unit without keys still writes its rows)
 __device__ __forceinline__ int unit_blocks(const PagedParams &p, int kv, int n, int first, int rows, int unit_rows) {
   const int last = min(first + unit_rows, rows) - 1;
@@ -53,21 +29,17 @@ __device__ __forceinline__ int unit_blocks(const PagedParams &p, int kv, int n, 
 
 // Exclusive prefix over the workgroup of one value per thread; total in every thread.
 template <int NTHR>
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t *tmp, int64_t &total) {
+__device__ __forceinline__ int block_scan(int x, int *tmp, int &total) {
   const int lane = lane_id(), w = (int)(threadIdx.x >> 6);
-  int64_t v = x;
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(v, off, 64);
-    if (lane >= off) v += y;
-  }
+  const int v = (int)wv::wave_incl_scan((uint32_t)x);
   __syncthreads();
   if (lane == 63) tmp[w] = v;
   __syncthreads();
-  int64_t before = 0;
+  int before = 0;
   total = 0;
 #pragma unroll
   for (int i = 0; i < NTHR / 64; ++i) {
-    const int64_t t = tmp[i];
+    const int t = tmp[i];
     if (i < w) before += t;
     total += t;
   }
@@ -77,22 +49,23 @@ __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t *tmp, int64_t &
 // The plan, one workgroup: unit_req[u], unit_first[u] (first row), unit_at[u] (first block,
 // unit_at[units] = all), unit0[r] (first unit of request r; unit0[R] = all).
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
-  __shared__ int64_t tmp[16];
-  int64_t total, at = 0;
+  __shared__ int tmp[16];
+  int total, at = 0;
   for (int r0 = 0; r0 < p.R; r0 += 1024) {
     const int r = r0 + (int)threadIdx.x;
-    const int64_t n = r < p.R ? ((int64_t)request_tokens(p, r) * p.H + p.unit_rows - 1) / p.unit_rows : 0;
-    const int64_t x = at + block_scan<1024>(n, tmp, total);
-    if (r < p.R) p.unit0[r] = (int)(x < p.max_units ? x : p.max_units);  // (starts that do not ascend may ask for more)
-    at += total;
+    // (starts that do not ascend may ask for more units than there are: cut)
+    const int n = r < p.R ? min((request_tokens(p, r) * p.H + p.unit_rows - 1) / p.unit_rows, p.max_units) : 0;
+    const int x = at + block_scan<1024>(n, tmp, total);
+    if (r < p.R) p.unit0[r] = min(x, p.max_units);
+    at = min(at + total, p.max_units);
   }
-  const int units = at < p.max_units ? (int)at : p.max_units;
+  const int units = at;
   if (threadIdx.x == 0) p.unit0[p.R] = units;
   __syncthreads();
   at = 0;
   for (int u0 = 0; u0 < units; u0 += 1024) {
     const int u = u0 + (int)threadIdx.x;
-    int64_t nb = 0;
+    int nb = 0;
     if (u < units) {
       int lo = 0, hi = p.R - 1;  // the last request whose first unit is at or before u
       while (lo < hi) {
@@ -104,22 +77,11 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
       p.unit_req[u] = lo;
       p.unit_first[u] = first;
     }
-    const int64_t x = at + block_scan<1024>(nb, tmp, total);
+    const int x = at + block_scan<1024>(nb, tmp, total);
     if (u < units) p.unit_at[u] = x;
     at += total;
   }
   if (threadIdx.x == 0) p.unit_at[units] = at;
-}
-
-// Blocks of a workgroup's range: at least kMinBlocks, so that a piece is worth its prologue.
-constexpr int kMinBlocks = 4;
-__device__ __forceinline__ int64_t range_blocks(const PagedParams &p, int64_t total) {
-  const int64_t per = (total + p.nwg - 1) / p.nwg;
-  return per > kMinBlocks ? per : kMinBlocks;
-}
-
-__device__ __forceinline__ void dma_16_at(uint32_t lds, const unsigned char *src) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
 }
 
 template <int D_QK, int D_V, int NT, int NW_, bool FP4>
@@ -152,8 +114,9 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
   using T = typename C::T;
   using Row = typename C::Row;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int lane = lane_id(), w = wave_id();
-  const int g32 = lane >> 5, l32 = lane & 31, g16 = lane >> 4, l16 = lane & 15;
+  // Lane-dependent values are formed from lane_here() where they are used: kept across a unit's blocks they would
+  // take the registers of O and Q.
+  const int w = wave_id();
   unsigned char *K = smem + C::OFF_K;
   float *Sp = reinterpret_cast<float *>(smem + C::OFF_SP);
   unsigned char *P = smem + C::OFF_P;
@@ -161,52 +124,36 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
   int *FL = reinterpret_cast<int *>(smem + C::OFF_FL);
   const uint32_t k_lds = lds_address(K);
   const unsigned char *zero = reinterpret_cast<const unsigned char *>(kZeroRow);
-
+  // MXFP4: chunks are also permuted by their panel, as neighbouring lanes write one row's blocks, a panel to two of them
+  auto panel_swz = [](int panel) { return FP4 ? (panel & 7) << 4 : 0; };
   const int ht = w / C::KP, kq = w % C::KP;
   constexpr int kPh = 4 / C::KP;
-  int ka[kPh];
-#pragma unroll
-  for (int u = 0; u < kPh; ++u) ka[u] = tile_byte(l32, 2 * (C::KP * u + kq) + g32);
   const int et = w * C::HW / 32;  // row tile of this wave's softmax rows
-  const int eh = (w * C::HW) % 32 + (lane & (C::HW - 1)), eq = lane / C::HW, eg = eq & 1, ei = (eq >> 1) * C::SPL4;
-  const int sr = et * 32 + eh;    // this lane's softmax row of the unit
 
-  const int units = p.unit0[p.R];
-  const int64_t total = p.unit_at[units], per = range_blocks(p, total);
-  int64_t at = (int64_t)blockIdx.x * per;
-  const int64_t end = at + per < total ? at + per : total;
-  if (at >= end) return;
-  int u = 0;
-  {
-    int hi = units - 1;  // the last unit that begins at or before `at`
-    while (u < hi) {
-      const int mid = (u + hi + 1) >> 1;
-      if (p.unit_at[mid] <= at) u = mid; else hi = mid - 1;
-    }
-  }
-  for (; at < end; ++u) {
-    const int64_t ub = p.unit_at[u], ue = p.unit_at[u + 1];
-    const int b0 = (int)(at - ub), b1 = (int)((ue < end ? ue : end) - ub);
-    const bool whole_unit = b0 == 0 && ub + b1 == ue;
-    const int64_t piece = (int64_t)blockIdx.x * 2 + (b0 == 0 ? 1 : 0);
-    at = ub + b1;
-    const int req = p.unit_req[u], first = p.unit_first[u];
-    const int n = request_tokens(p, req), kv = request_kv(p, req);
-    const int nrows = min(n * p.H - first, C::ROWS);
-    const int64_t row0 = (int64_t)request_start(p, req) * p.H + first;  // of q, out, lse
+  const int units = uni(p.unit0[p.R]), total = uni(p.unit_at[units]), per = uni(range_blocks(p, total));
+  if ((int64_t)blockIdx.x * per >= total) return;
+  int at = (int)blockIdx.x * per;
+  const int end = per < total - at ? at + per : total;
+  for (int u = uni(unit_of(p, units, at)); at < end; ++u) {
+    const PagedPiece x = next_piece(p, u, at, end);
+    const int b0 = x.b0, b1 = x.b1, first = x.first, n = x.n, kv = x.kv, nrows = x.nrows;
+    const bool whole_unit = x.whole;
+    const int64_t piece = x.slot, row0 = x.row0;
     const int tok0 = first / p.H, tok1 = (first + nrows - 1) / p.H;
-    const int my_tok = (first + sr) / p.H;
-    const int32_t *table = p.table + (int64_t)req * p.W;
+    const int32_t *table = x.table;
 
-    // this wave's part of Q: row l32 of tile ht, k-steps KP i + kq
+    // this wave's part of Q: row lane % 32 of tile ht, k-steps KP i + kq; and where its operands of K are
     i32x4 q[C::KS];
+    int ka[kPh];
     {
-      const int r = 32 * ht + l32;
+      const int ln = lane_here(), r = 32 * ht + (ln & 31), g32 = ln >> 5;
 #pragma unroll
       for (int i = 0; i < C::KS; ++i) {
         q[i] = i32x4{0, 0, 0, 0};
         if (r < nrows) q[i] = ld_global_16(p.q + ((row0 + r) * D_QK + 16 * (C::KP * i + kq) + 8 * g32) * 2);
       }
+#pragma unroll
+      for (int v = 0; v < kPh; ++v) ka[v] = tile_byte(ln & 31, 2 * (C::KP * v + kq) + g32);
     }
 
     // Runs the piece with the tokens' keys cut at those of token tlim and writes the rows of tokens
@@ -215,25 +162,14 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
     auto run = [&](int tok, int tlim, bool probe) -> bool {
       const int lim = token_keys(kv, n, tlim);           // keys that are read
       const int lim_min = token_keys(kv, n, tok);        // keys that every row sees
-      const int my_lim = token_keys(kv, n, my_tok < tlim ? my_tok : tlim);
+      auto row_keys = [&](int r) {                       // of row r
+        const int t = (first + r) / p.H;
+        return token_keys(kv, n, t < tlim ? t : tlim);
+      };
       const int j1 = min(b1, (lim + 31) / 32);           // blocks past it hold no key
-      auto entry = [&](int j) {                          // table entry of key 32 j + l32, -1: none
-        const int key = 32 * j + l32;
-        int e = -1;
-        if (key < lim) e = table[(uint32_t)key / (uint32_t)p.block];
-        return e;
-      };
-      auto row_at = [&](int j, int e) -> const unsigned char * {
-        const uint32_t key = 32u * (uint32_t)j + (uint32_t)l32;
-        const bool ok = e >= 0 && e < p.num_blocks;
-        const int64_t slot = (int64_t)e * p.block + (key - key / (uint32_t)p.block * (uint32_t)p.block);
-        return ok ? p.cache + slot * Row::BYTES : zero;
-      };
-      auto shfl_ptr = [&](const unsigned char *x, int src) {
-        const uint64_t v = reinterpret_cast<uint64_t>(x);
-        const uint32_t a = (uint32_t)__shfl((int)(uint32_t)v, src, 64), b = (uint32_t)__shfl((int)(uint32_t)(v >> 32), src, 64);
-        return reinterpret_cast<const unsigned char *>(((uint64_t)b << 32) | a);
-      };
+      auto entry = [&](int j) { return key_entry(p, table, j, lim); };
+      auto row_at = [&](int j, int e) { return key_row(p, j, e, Row::BYTES); };
+      auto there = [&](int e) { return (uint32_t)wv::ballot(e >= 0 && e < p.num_blocks); };
       // bf16: the rows; MXFP4: their rope part, into its panels
       auto fetch = [&](int tile, const unsigned char *mine) {
         const int ln = lane_here();
@@ -241,20 +177,21 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
         for (int i = 0; i < T::RG; ++i) {
           const int rg = w + T::NW * i, row = 8 * rg + (ln >> 3);
-          const unsigned char *src = shfl_ptr(mine, row) + SRC + ((ln & 7) ^ row_swz(row)) * 16;
+          const unsigned char *src = shfl_ptr(mine, row) + SRC + ((((ln & 7) ^ row_swz(row)) * 16) ^ panel_swz(P0));
 #pragma unroll
-          for (int pn = P0; pn < T::PANELS; ++pn)
+          for (int pn = P0; pn < T::PANELS; ++pn) {
+            __builtin_amdgcn_sched_barrier(0);  // an address at a time
             dma_16_at(k_lds + (uint32_t)(tile * T::BYTES + pn * T::PANEL + rg * 1024), src + (pn - P0) * 128);
+          }
         }
       };
       // MXFP4 latent: 16 bytes of codes (one 32-channel block of a row) and its exponent per piece
       i32x4 codes[FP4 ? C::CPT : 1];
       uint32_t expo[FP4 ? C::CPT : 1];
-      auto piece_of = [&](int i, int &row, int &blk) {  // lanes: 16 rows, 4 blocks of each
-        const int x = w + NW * i;                         // 64-lane group: blocks 4 (x % (nb / 4)) .., rows 16 (x / (nb / 4)) ..
-        constexpr int NB4 = D_V / 32 >= 4 ? D_V / 128 : 1, BL = D_V / 32 >= 4 ? 4 : D_V / 32;
-        row = 16 * (x / NB4) + (lane & 15) + (BL == 4 ? 0 : 16 * ((lane >> 4) / BL));
-        blk = 4 * (x % NB4) + (lane >> 4) % BL;
+      auto piece_of = [&](int i, int &row, int &blk) {  // a row's codes from neighbouring lanes
+        const int y = (w + NW * i) * 64 + lane_here();
+        row = y / (D_V / 32);
+        blk = y % (D_V / 32);
       };
       auto load_codes = [&](const unsigned char *mine) {
         if constexpr (FP4) {
@@ -286,7 +223,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
             for (int c = 0; c < 4; ++c) {
               i32x4 v = e2m1x8_to_bf16((uint32_t)codes[i][c], s);
               if (expo[i] == 255u) v = i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
-              *reinterpret_cast<i32x4 *>(dst + tile_byte(row, 4 * (blk & 1) + c)) = v;
+              *reinterpret_cast<i32x4 *>(dst + (tile_byte(row, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v;
             }
           }
         }
@@ -315,15 +252,16 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
           const int c = c16 & 3;
-          vt[v] = tile_byte(8 * cg + 4 * v + (c16 >> 2), 2 * (w & 3) + (c >> 1)) + (c & 1) * 8 + (w >> 2) * T::PANEL;
+          vt[v] = tile_byte(8 * cg + 4 * v + (c16 >> 2), 2 * (w & 3) + (c >> 1)) + (c & 1) * 8;
         }
         // P[row][key]: 64-byte rows, 16-byte chunk c of row r at c ^ ((r >> 2) & 3)
         const int p_rd = buf * NT * C::PT_BYTES + c16 * 64 + ((cg ^ ((c16 >> 2) & 3)) * 16);
         i32x4 av[C::DTW];
 #pragma unroll
         for (int i = 0; i < C::DTW; ++i) {
-          const i32x2 r0 = ds_read_tr16(Kb + vt[0] + i * (NW / 4) * T::PANEL);
-          const i32x2 r1 = ds_read_tr16(Kb + vt[1] + i * (NW / 4) * T::PANEL);
+          const int pn = (w >> 2) + i * (NW / 4);
+          const i32x2 r0 = ds_read_tr16(Kb + (vt[0] ^ panel_swz(pn)) + pn * T::PANEL);
+          const i32x2 r1 = ds_read_tr16(Kb + (vt[1] ^ panel_swz(pn)) + pn * T::PANEL);
           av[i] = i32x4{r0[0], r0[1], r1[0], r1[1]};
         }
 #pragma unroll
@@ -335,16 +273,15 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
         }
       };
 
-      int e_nxt = entry(b0);
-      const unsigned char *mine = row_at(b0, e_nxt);
-      uint32_t vm = (uint32_t)wv::ballot(mine != zero);
+      int e_nxt = entry(b0);  // table entry of the block that is fetched next
+      uint32_t vm = there(e_nxt);
       if (b0 < j1) {
+        const unsigned char *mine = row_at(b0, e_nxt);
         if (w < C::FW) fetch(0, mine);
         load_codes(mine);
         store_codes(0);
         e_nxt = entry(b0 + 1);
-        mine = row_at(b0 + 1, e_nxt);
-        load_codes(mine);
+        if constexpr (FP4) load_codes(row_at(b0 + 1, e_nxt));
       }
       int kb = 0, kp = 0;
       for (int j = b0; j < j1; ++j) {
@@ -352,8 +289,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
         const unsigned char *Kj = K + kb * T::BYTES;
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): block j's rows, issued a block ago
         __syncthreads();                     // block j's rows and block j - 1's P are whole; block j - 2's rows are consumed
-        const uint32_t vm_nxt = (uint32_t)wv::ballot(mine != zero);
-        if (w < C::FW) fetch(kn, mine);      // block j + 1 (past the last: zeros)
+        const uint32_t vm_nxt = there(e_nxt);
+        if (w < C::FW) fetch(kn, row_at(j + 1, e_nxt));  // block j + 1 (past the last: zeros)
         store_codes(kn);
         e_nxt = entry(j + 2);
         f32x16 acc;
@@ -361,13 +298,12 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
         for (int a = 0; a < 16; ++a) acc[a] = 0.0f;
 #pragma unroll
         for (int i = 0; i < C::KS; ++i) {
-          const i32x4 a = *reinterpret_cast<const i32x4 *>(Kj + ka[i % kPh] + (i / kPh) * T::PANEL);
+          const i32x4 a = *reinterpret_cast<const i32x4 *>(Kj + (ka[i % kPh] ^ panel_swz(i / kPh)) + (i / kPh) * T::PANEL);
           acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(q[i]), acc, 0, 0, 0);
         }
         put_partial(Sp + w * C::SP_W, acc);
         __syncthreads();  // partial tiles whole
-        mine = row_at(j + 2, e_nxt);
-        load_codes(mine);
+        if constexpr (FP4) load_codes(row_at(j + 2, e_nxt));
         // softmax: row eh of tile et, 4-key groups (i, eg) with i = ei .. ei + SPL4 - 1: keys 8 i + 4 eg ..
         const int ln = lane_here(), eh = (w * C::HW) % 32 + (ln & (C::HW - 1)), sr = et * 32 + eh;
         const int eq = ln / C::HW, eg = eq & 1, ei = (eq >> 1) * C::SPL4;
@@ -385,6 +321,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 
         // online softmax (log2 domain, lazy rescale); key 32 j + 8 (ei + x) + 4 eg + e
         if (vm != 0xffffffffu || 32 * j + 32 > lim_min) {
+          const int my_lim = row_keys(sr);
 #pragma unroll
           for (int x = 0; x < C::SPL4; ++x)
 #pragma unroll
@@ -410,7 +347,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
           m_run = m_new;
         }
         if (eq == 0) AL[cur * C::ROWS + sr] = alpha;
-        if (lane == 0) FL[cur * NW + w] = moved ? 1 : 0;
+        if (ln == 0) FL[cur * NW + w] = moved ? 1 : 0;
 #pragma unroll
         for (int x = 0; x < C::SPL4; ++x) {
           float t[4];
@@ -430,7 +367,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
       for (int off = C::HW; off < 32; off <<= 1) l_run += __shfl_xor(l_run, off, 64);
       l_run = sum_halves(l_run);
-      const bool none = my_lim <= 32 * b0 || l_run == 0.0f;  // no key of this piece
+      const int ln = lane_here(), sr = w * C::HW + (ln & (C::HW - 1)), eq = ln / C::HW;  // this lane's softmax row
+      const bool none = row_keys(sr) <= 32 * b0 || l_run == 0.0f;  // no key of this piece
       if (eq == 0) AL[2 * C::ROWS + sr] = none ? 0.0f : 1.0f / l_run;
       __syncthreads();
       if (b0 < j1) pv_step(K + kp * T::BYTES, (j1 - b0 - 1) & 1);
@@ -456,13 +394,13 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
       }
 #pragma unroll
       for (int h = 0; h < 2 * NT; ++h) {
-        const int r = 16 * h + l16;
+        const int r = 16 * h + (ln & 15);
         const float inv = AL[2 * C::ROWS + r];
         if (r >= rlo && r < rhi) {
 #pragma unroll
           for (int i = 0; i < C::DTW; ++i)
             if (C::NDT % NW == 0 || w + NW * i < C::NDT) {
-              const int d = (w + NW * i) * 16 + 4 * g16;
+              const int d = (w + NW * i) * 16 + 4 * (ln >> 4);
               if (whole_unit) {
                 // an empty row's O is zeros (or what a neighbour's key left): 0
                 const f32x4 x = inv == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o[i][h] * inv;
@@ -517,7 +455,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
   const int u = p.unit0[r] + in_req / p.unit_rows, ur = in_req % p.unit_rows;
   const int units = p.unit0[p.R];
   if (u >= units) return;
-  const int64_t per = range_blocks(p, p.unit_at[units]);
+  const int per = range_blocks(p, p.unit_at[units]);
   const int64_t w0 = p.unit_at[u] / per, w1 = (p.unit_at[u + 1] - 1) / per;
   if (w0 == w1) return;  // one piece: its workgroup wrote the row
   auto at = [&](int64_t w) { return (w * 2 + (w == w0 ? 1 : 0)) * p.unit_rows + ur; };
@@ -546,18 +484,28 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
   if (lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
 }
 
-// 32-row tiles of a unit: as many as the rows that share a key (the heads of a token, and
-// of the other tokens of a prefill chunk) can fill, up to four (the registers of O).
-static int unit_tiles(int64_t T, int64_t R, int64_t H, int64_t d_qk) {
-  const int64_t rows = (T + R - 1) / (R > 0 ? R : 1) * H;  // of a request, on average
-  const int most = d_qk == 576 ? 4 : 2;
-  return rows > 64 && most >= 4 ? 4 : (rows > 32 ? 2 : 1);
-}
-static int64_t max_units(int64_t T, int64_t R, int64_t H, int nt) { return T * H / (32 * nt) + R; }
-static int paged_workgroups(int64_t units, int64_t W, int64_t block) {
-  const int64_t blocks = units * ((W * block + 31) / 32);
-  const int64_t n = (blocks + kMinBlocks - 1) / kMinBlocks;
-  return (int)(n < 1 ? 1 : (n < 256 ? n : 256));
+// How a call is run, from its sizes alone.  Rows that share keys: a request's (token, head) pairs, on average.
+struct PagedPlan {
+  int few;        // 16-row tiles of a unit whose waves split the keys, or 0
+  int nt;         // else 32-row tiles of a unit whose waves share them
+  int unit_rows, max_units, nwg, min_blocks;
+};
+static PagedPlan paged_plan(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk) {
+  PagedPlan r{};
+  const int64_t rows = (T + R - 1) / R * H;
+  if (rows <= (d_qk == 576 ? 16 : 32)) {
+    r.few = rows <= 16 ? 1 : 2;
+    r.unit_rows = 16 * r.few;
+  } else {
+    r.nt = rows > 64 && d_qk == 576 ? 4 : (rows > 32 ? 2 : 1);
+    r.unit_rows = 32 * r.nt;
+  }
+  r.min_blocks = r.few ? 8 : 4;
+  r.max_units = (int)(T * H / r.unit_rows + R);
+  const int64_t blocks = (int64_t)r.max_units * ((W * block + 31) / 32), n = (blocks + r.min_blocks - 1) / r.min_blocks;
+  const int64_t most = r.few && d_qk == 128 ? 768 : 256;  // resident workgroups
+  r.nwg = (int)(n < 1 ? 1 : (n < most ? n : most));
+  return r;
 }
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -565,16 +513,16 @@ struct PagedSections {
   size_t unit0, unit_req, unit_first, unit_at, part_ml, part_o, total;
 };
 static PagedSections paged_sections(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v) {
-  const int nt = unit_tiles(T, R, H, d_qk);
-  const size_t units = (size_t)max_units(T, R, H, nt), wgs = (size_t)paged_workgroups((int64_t)units, W, block);
+  const PagedPlan k = paged_plan(T, R, W, block, H, d_qk);
+  const size_t units = (size_t)k.max_units, pieces = (size_t)k.nwg * 2 * (size_t)k.unit_rows;
   PagedSections s;
   s.unit0 = 0;
   s.unit_req = s.unit0 + up256(((size_t)R + 1) * 4);
   s.unit_first = s.unit_req + up256(units * 4);
   s.unit_at = s.unit_first + up256(units * 4);
-  s.part_ml = s.unit_at + up256((units + 1) * 8);
-  s.part_o = s.part_ml + wgs * 2 * 32 * (size_t)nt * 8;
-  s.total = s.part_o + wgs * 2 * 32 * (size_t)nt * (size_t)d_v * 4;
+  s.part_ml = s.unit_at + up256((units + 1) * 4);
+  s.part_o = s.part_ml + pieces * 8;
+  s.total = s.part_o + pieces * (size_t)d_v * 4;
   return s;
 }
 size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v) {
@@ -587,39 +535,39 @@ static int launch(const PagedParams &p, hipStream_t st) {
   const auto kernel = paged_fwd_kernel<D_QK, D_V, NT, NW, FP4>;
   const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
   if (e != hipSuccess) return set_error(DSA_ERR_HIP, "dsa_paged_latent_mla_fwd: LDS attribute: %s", hipGetErrorString(e));
-  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, st, p);
-  int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
-  if (rc) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)p.nwg), dim3(C::NTHR), C::BYTES, st, p);
-  rc = check_launch("dsa_paged_latent_mla_fwd");
-  if (rc) return rc;
-  hipLaunchKernelGGL(paged_combine_kernel<D_V>, dim3((unsigned)((p.T * p.H + 3) / 4)), dim3(256), 0, st, p);
-  return check_launch("dsa_paged_latent_mla_fwd (combine)");
+  return check_launch("dsa_paged_latent_mla_fwd");
 }
 
 template <bool FP4>
 static int launch_nt(const PagedParams &p, int64_t d_qk, int nt, hipStream_t st) {
-  if (d_qk == 576) {
-    if (nt == 4) return launch<576, 512, 4, 8, FP4>(p, st);
-    if (nt == 2) return launch<576, 512, 2, 8, FP4>(p, st);
-    return launch<576, 512, 1, 4, FP4>(p, st);
-  }
-  return nt == 2 ? launch<128, 64, 2, 4, FP4>(p, st) : launch<128, 64, 1, 4, FP4>(p, st);
+  if (d_qk == 128) return launch<128, 64, 2, 4, FP4>(p, st);
+  if (nt == 1) return launch<576, 512, 1, 4, FP4>(p, st);
+  return nt == 4 ? launch<576, 512, 4, 8, FP4>(p, st) : launch<576, 512, 2, 8, FP4>(p, st);
 }
 
 int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st) {
   const PagedSections s = paged_sections(p.T, p.R, p.W, p.block, p.H, d_qk, d_v);
-  const int nt = unit_tiles(p.T, p.R, p.H, d_qk);
-  p.unit_rows = 32 * nt;
-  p.max_units = (int)max_units(p.T, p.R, p.H, nt);
-  p.nwg = paged_workgroups(p.max_units, p.W, p.block);
+  const PagedPlan k = paged_plan(p.T, p.R, p.W, p.block, p.H, d_qk);
+  p.unit_rows = k.unit_rows;
+  p.max_units = k.max_units;
+  p.nwg = k.nwg;
+  p.min_blocks = k.min_blocks;
   p.unit0 = (int32_t *)(ws + s.unit0);
   p.unit_req = (int32_t *)(ws + s.unit_req);
   p.unit_first = (int32_t *)(ws + s.unit_first);
-  p.unit_at = (int64_t *)(ws + s.unit_at);
+  p.unit_at = (int32_t *)(ws + s.unit_at);
   p.part_ml = (float *)(ws + s.part_ml);
   p.part_o = (float *)(ws + s.part_o);
-  return fp4 ? launch_nt<true>(p, d_qk, nt, st) : launch_nt<false>(p, d_qk, nt, st);
+  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, st, p);
+  int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
+  if (rc) return rc;
+  rc = k.few ? launch_paged_few(p, d_qk, k.few, fp4, st) : (fp4 ? launch_nt<true>(p, d_qk, k.nt, st) : launch_nt<false>(p, d_qk, k.nt, st));
+  if (rc || p.nwg == 1) return rc;  // one workgroup: no unit has several pieces
+  const dim3 grid((unsigned)((p.T * p.H + 3) / 4));
+  if (d_v == 512) hipLaunchKernelGGL(paged_combine_kernel<512>, grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(paged_combine_kernel<64>, grid, dim3(256), 0, st, p);
+  return check_launch("dsa_paged_latent_mla_fwd (combine)");
 }
 
 }  // namespace dsa
