@@ -53,6 +53,7 @@ FILE_FLAGS = {
     "latent_mla_bwd.hip": _MFMA_VGPR,
     "latent_paged.hip": _MFMA_VGPR,
     "latent_paged_few.hip": _MFMA_VGPR,
+    "latent_paged_wide.hip": _MFMA_VGPR,
 }
 
 

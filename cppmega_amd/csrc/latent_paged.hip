@@ -15,16 +15,15 @@
 // 64-bit addresses that the block table gives (MXFP4: as codes in registers, written to
 // the tile as exact bf16 values).  Keys past a request's last, and keys whose table entry
 // is no page, read as zeros and have no weight.
+#include "latent_mla.hpp"
 #include "latent_paged.hpp"
-#include "sparse_mla_wide_tile.hpp"
-#include "wave_ops.hpp"
 
 namespace dsa {
 
 // blocks of a unit (at least one: a unit without keys still writes its rows)
 __device__ __forceinline__ int unit_blocks(const PagedParams &p, int kv, int n, int first, int rows, int unit_rows) {
   const int last = min(first + unit_rows, rows) - 1;
-  return max((token_keys(kv, n, last / p.H) + 31) / 32, 1);
+  return max((token_keys(kv, n, last / p.H) + p.step_keys - 1) / p.step_keys, 1);
 }
 
 // Exclusive prefix over the workgroup of one value per thread; total in every thread.
@@ -84,51 +83,52 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   if (threadIdx.x == 0) p.unit_at[units] = at;
 }
 
-template <int D_QK, int D_V, int NT, int NW_, bool FP4>
+template <int D_QK, int D_V, int NT, int SUB, int NBUF_, bool FP4>
 struct Paged {
-  static constexpr int NW = NW_, NTHR = 64 * NW, KP = NW / NT;
-  static constexpr int FW = NW / 2;                          // waves that fetch by DMA
-  using T = DmaTile<D_QK, FW>;
   using Row = CacheRow<D_QK, D_V, FP4>;
-  static constexpr int KS = D_QK / 16 / KP;
-  static constexpr int NDT = D_V / 16, DTW = (NDT + NW - 1) / NW;
-  static constexpr int ROWS = 32 * NT, HW = ROWS / NW;       // rows per wave in the softmax
-  static constexpr int LPH = 64 / HW, SPL4 = 8 / LPH;
-  static constexpr int SP_W = 32 * 32;
-  static constexpr int PT_BYTES = 32 * 32 * 2;
-  static constexpr int CODES = 32 * (D_V / 32);              // 16-byte pieces of codes in a block
-  static constexpr int CPT = (CODES + NTHR - 1) / NTHR;      // per thread
-  static constexpr int OFF_K = 0;
-  static constexpr int OFF_SP = OFF_K + 3 * T::BYTES;
-  static constexpr int OFF_P = OFF_SP + NW * SP_W * 4;
-  static constexpr int OFF_AL = OFF_P + 2 * NT * PT_BYTES;
-  static constexpr int OFF_FL = OFF_AL + 3 * ROWS * 4;
-  static constexpr int BYTES = OFF_FL + 2 * NW * 4;
-  static_assert(D_QK / 16 % KP == 0 && (KP == 2 || KP == 4) && (HW == 8 || HW == 16), "wave split");
-  static_assert(BYTES <= 159 * 1024, "LDS");
+  static constexpr int NW = 4, KG = NW / NT, ROWS = 32 * NT;  // waves: NT row tiles x KG key groups
+  static constexpr int TILES = KG * SUB, KEYS = 32 * TILES;   // 32-key tiles and keys of a step
+  static constexpr int NBUF = NT == 1 ? 1 : NBUF_;            // steps in LDS; one row tile: a wave's tile is its own
+  static constexpr int AHEAD = NBUF - 1;                      // steps that are fetched ahead
+  static constexpr int KS = D_QK / 16, NDT = D_V / 32;
+  static constexpr int PANELS = D_QK / 64, TILE = PANELS * 4096, STEP = TILES * TILE;
+  static constexpr int DMA = TILES * (FP4 ? PANELS - D_V / 64 : PANELS);  // loads of a wave per step (an 8-row group a tile)
+  static constexpr int NB = D_V / 32, CODES = TILES * 32 * NB;            // code pieces of a row, of a step
+  static constexpr int CPT = (CODES + 255) / 256;                         // per thread and step
+  static constexpr int OFF_T = NBUF * STEP;
+  static constexpr int OFF_ML = OFF_T + kWindow * 4;          // [NW][32][2]
+  static constexpr int BYTES = OFF_ML + NW * 32 * 8;
+  static constexpr int O_BYTES = D_V * 32 * 4;                // a wave's O
+  static_assert(BYTES <= 159 * 1024 && (KG == 1 || (NW / 2) * O_BYTES <= OFF_T), "LDS");
+  static_assert(!FP4 || CODES % 256 == 0 || (CPT == 1 && CODES % 64 == 0 && NT > 1), "code pieces by whole waves");
 };
 
-template <int D_QK, int D_V, int NT, int NW, bool FP4>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4))) paged_fwd_kernel(const PagedParams p) {
-  using C = Paged<D_QK, D_V, NT, NW, FP4>;
-  using T = typename C::T;
+template <int D_QK, int D_V, int NT, int SUB, int NBUF, bool FP4, int OCC>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) paged_rows_kernel(const PagedParams p) {
+  using C = Paged<D_QK, D_V, NT, SUB, NBUF, FP4>;
   using Row = typename C::Row;
+  constexpr int KS = C::KS, NDT = C::NDT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  // Lane-dependent values are formed from lane_here() where they are used: kept across a unit's blocks they would
-  // take the registers of O and Q.
-  const int w = wave_id();
-  unsigned char *K = smem + C::OFF_K;
-  float *Sp = reinterpret_cast<float *>(smem + C::OFF_SP);
-  unsigned char *P = smem + C::OFF_P;
-  float *AL = reinterpret_cast<float *>(smem + C::OFF_AL);
-  int *FL = reinterpret_cast<int *>(smem + C::OFF_FL);
-  const uint32_t k_lds = lds_address(K);
+  const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
+  const int rt = w % NT, kg = w / NT;
+  int *window = reinterpret_cast<int *>(smem + C::OFF_T);
+  float *ML = reinterpret_cast<float *>(smem + C::OFF_ML);
+  const uint32_t lds0 = lds_address(smem);
   const unsigned char *zero = reinterpret_cast<const unsigned char *>(kZeroRow);
   // MXFP4: chunks are also permuted by their panel, as neighbouring lanes write one row's blocks, a panel to two of them
   auto panel_swz = [](int panel) { return FP4 ? (panel & 7) << 4 : 0; };
-  const int ht = w / C::KP, kq = w % C::KP;
-  constexpr int kPh = 4 / C::KP;
-  const int et = w * C::HW / 32;  // row tile of this wave's softmax rows
+  const RowRead row_at;
+  const ColRead col_at;
+  auto row_read = [&](const unsigned char *tile, int ks) {
+    return *reinterpret_cast<const i32x4 *>(tile + (row_at.a[ks & 3] ^ panel_swz(ks >> 2)) + (ks >> 2) * 4096);
+  };
+  auto col_read = [&](const unsigned char *tile, int dt, int u) {
+    const unsigned char *base = tile + (dt >> 1) * 4096 + u * 2048;
+    const i32x2 r0 = ds_read_tr16(base + (col_at.a[0][dt & 1] ^ panel_swz(dt >> 1)));
+    const i32x2 r1 = ds_read_tr16(base + (col_at.a[1][dt & 1] ^ panel_swz(dt >> 1)));
+    return i32x4{r0[0], r0[1], r1[0], r1[1]};
+  };
+  auto page_of = [&](int key) { return p.block_shift >= 0 ? key >> p.block_shift : (int)((uint32_t)key / (uint32_t)p.block); };
 
   const int units = uni(p.unit0[p.R]), total = uni(p.unit_at[units]), per = uni(range_blocks(p, total));
   if ((int64_t)blockIdx.x * per >= total) return;
@@ -136,374 +136,365 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
   const int end = per < total - at ? at + per : total;
   for (int u = uni(unit_of(p, units, at)); at < end; ++u) {
     const PagedPiece x = next_piece(p, u, at, end);
-    const int b0 = x.b0, b1 = x.b1, first = x.first, n = x.n, kv = x.kv, nrows = x.nrows;
-    const bool whole_unit = x.whole;
-    const int64_t piece = x.slot, row0 = x.row0;
-    const int tok0 = first / p.H, tok1 = (first + nrows - 1) / p.H;
-    const int32_t *table = x.table;
-
-    // this wave's part of Q: row lane % 32 of tile ht, k-steps KP i + kq; and where its operands of K are
-    i32x4 q[C::KS];
-    int ka[kPh];
-    {
-      const int ln = lane_here(), r = 32 * ht + (ln & 31), g32 = ln >> 5;
+    const int tok0 = x.first / p.H, tok1 = (x.first + x.nrows - 1) / p.H;
+    const int row = 32 * rt + l32;  // of the unit
+    i32x4 q[KS];
 #pragma unroll
-      for (int i = 0; i < C::KS; ++i) {
-        q[i] = i32x4{0, 0, 0, 0};
-        if (r < nrows) q[i] = ld_global_16(p.q + ((row0 + r) * D_QK + 16 * (C::KP * i + kq) + 8 * g32) * 2);
-      }
-#pragma unroll
-      for (int v = 0; v < kPh; ++v) ka[v] = tile_byte(ln & 31, 2 * (C::KP * v + kq) + g32);
+    for (int ks = 0; ks < KS; ++ks) {
+      q[ks] = i32x4{0, 0, 0, 0};
+      if (row < x.nrows) q[ks] = ld_global_16(p.q + ((x.row0 + row) * D_QK + 16 * ks + 8 * g32) * 2);
     }
-
-    // Runs the piece with the tokens' keys cut at those of token tlim and writes the rows of tokens
-    // [tok, tlim].  All tokens at once; where that leaves something that is not finite, token by
-    // token, since a row's weight of zero does not remove the Inf or NaN of a later token's key.
-    auto run = [&](int tok, int tlim, bool probe) -> bool {
-      const int lim = token_keys(kv, n, tlim);           // keys that are read
-      const int lim_min = token_keys(kv, n, tok);        // keys that every row sees
-      auto row_keys = [&](int r) {                       // of row r
-        const int t = (first + r) / p.H;
-        return token_keys(kv, n, t < tlim ? t : tlim);
-      };
-      const int j1 = min(b1, (lim + 31) / 32);           // blocks past it hold no key
-      auto entry = [&](int j) { return key_entry(p, table, j, lim); };
-      auto row_at = [&](int j, int e) { return key_row(p, j, e, Row::BYTES); };
-      auto there = [&](int e) { return (uint32_t)wv::ballot(e >= 0 && e < p.num_blocks); };
-      // bf16: the rows; MXFP4: their rope part, into its panels
-      auto fetch = [&](int tile, const unsigned char *mine) {
-        const int ln = lane_here();
-        constexpr int P0 = FP4 ? D_V / 64 : 0, SRC = FP4 ? Row::OFF_ROPE : 0;
-#pragma unroll
-        for (int i = 0; i < T::RG; ++i) {
-          const int rg = w + T::NW * i, row = 8 * rg + (ln >> 3);
-          const unsigned char *src = shfl_ptr(mine, row) + SRC + ((((ln & 7) ^ row_swz(row)) * 16) ^ panel_swz(P0));
-#pragma unroll
-          for (int pn = P0; pn < T::PANELS; ++pn) {
-            __builtin_amdgcn_sched_barrier(0);  // an address at a time
-            dma_16_at(k_lds + (uint32_t)(tile * T::BYTES + pn * T::PANEL + rg * 1024), src + (pn - P0) * 128);
-          }
-        }
-      };
-      // MXFP4 latent: 16 bytes of codes (one 32-channel block of a row) and its exponent per piece
-      i32x4 codes[FP4 ? C::CPT : 1];
-      uint32_t expo[FP4 ? C::CPT : 1];
-      auto piece_of = [&](int i, int &row, int &blk) {  // a row's codes from neighbouring lanes
-        const int y = (w + NW * i) * 64 + lane_here();
-        row = y / (D_V / 32);
-        blk = y % (D_V / 32);
-      };
-      auto load_codes = [&](const unsigned char *mine) {
-        if constexpr (FP4) {
-#pragma unroll
-          for (int i = 0; i < C::CPT; ++i) {
-            int row, blk;
-            piece_of(i, row, blk);
-            const bool in = C::CODES % C::NTHR == 0 || (w + NW * i) * 64 < C::CODES;
-            const unsigned char *src = shfl_ptr(mine, row & 31);
-            codes[i] = i32x4{0, 0, 0, 0};
-            expo[i] = 127;
-            if (in && src != zero) {
-              codes[i] = ld_global_16(src + blk * 16);
-              expo[i] = src[Row::OFF_EXP + blk];
+    // Tokens [ta, tb] with the keys cut at tb's: all at once, or, where that left something that is not finite, one by
+    // one, since a weight of zero does not remove the Inf or NaN of a later token's key.
+    int ta = tok0, tb = tok1;
+    bool probe = tok0 != tok1;
+    while (true) {
+      const int lim = token_keys(x.kv, x.n, tb), lim_min = token_keys(x.kv, x.n, ta);
+      const int j1 = min(x.b1, (lim + C::KEYS - 1) / C::KEYS);  // steps past it hold no key
+      const int t = (x.first + row) / p.H, my_lim = token_keys(x.kv, x.n, t < tb ? t : tb);
+      int base = 0;          // first page in the window
+      bool all_there = true;
+      auto refill = [&](int first_page) {
+        base = first_page;
+        const int pages = lim > 0 ? page_of(lim - 1) + 1 : 0;
+        bool ok = true;
+        __syncthreads();  // the window's readers are done
+        for (int i = (int)threadIdx.x; i < kWindow; i += 256) {
+          const int pg = base + i;
+          int e = -1;
+          if (pg < pages) {
+            e = x.table[pg];
+            if (e < 0 || e >= p.num_blocks) {
+              e = -1;
+              ok = false;
             }
           }
+          window[i] = e;
+        }
+        all_there = __syncthreads_and(ok) != 0;
+      };
+      // row of a key, by the window
+      auto key_at = [&](int key) -> const unsigned char * {
+        const int pg = page_of(key), e = key < lim ? window[pg - base] : -1;
+        const int64_t slot = (int64_t)e * p.block + (key - pg * p.block);
+        return e >= 0 ? p.cache + slot * Row::BYTES : zero;
+      };
+      // the wave's 8-row groups of a step's tiles (bf16: their rows; MXFP4: their rope part)
+      auto fetch = [&](int j, int buf) {
+        constexpr int P0 = FP4 ? D_V / 64 : 0;
+#pragma unroll
+        for (int i = 0; i < C::TILES; ++i) {
+          const int grp = NT == 1 ? 4 * w + i : w + 4 * i, r = 8 * (grp & 3) + (lane >> 3);
+          const unsigned char *src = key_at(j * C::KEYS + 8 * grp + (lane >> 3)) + (FP4 ? Row::OFF_ROPE : 0) +
+                                     ((((lane & 7) ^ row_swz(r)) * 16) ^ panel_swz(P0));
+#pragma unroll
+          for (int pn = P0; pn < C::PANELS; ++pn)
+            dma_16_at(lds0 + (uint32_t)(buf * C::STEP + (grp >> 2) * C::TILE + pn * 4096 + (grp & 3) * 1024), src + (pn - P0) * 128);
         }
       };
-      auto store_codes = [&](int tile) {
+      // MXFP4: code pieces of a step, a row's from neighbouring threads (one row tile: of the wave's own tile)
+      i32x4 codes[FP4 ? C::CPT : 1];
+      uint32_t expo[FP4 ? C::CPT : 1];
+      auto piece_at = [&](int i, int &key, int &blk) {
+        const int y = NT == 1 ? w * 64 * C::CPT + i * 64 + lane : i * 256 + w * 64 + lane;
+        key = y / C::NB;
+        blk = y % C::NB;
+      };
+      auto load_codes = [&](int j) {
         if constexpr (FP4) {
 #pragma unroll
           for (int i = 0; i < C::CPT; ++i) {
-            if (!(C::CODES % C::NTHR == 0 || (w + NW * i) * 64 < C::CODES)) continue;
-            int row, blk;
-            piece_of(i, row, blk);
-            const float s = e8m0_scale(expo[i]);
-            unsigned char *dst = K + tile * T::BYTES + (blk >> 1) * T::PANEL;
+            if (C::CODES % 256 != 0 && w * 64 >= C::CODES) continue;  // wave-uniform
+            int key, blk;
+            piece_at(i, key, blk);
+            const unsigned char *src = key_at(j * C::KEYS + key);
+            codes[i] = ld_global_16(src + blk * 16);
+            expo[i] = src[Row::OFF_EXP + blk];
+          }
+        }
+      };
+      auto store_codes = [&](int buf) {
+        if constexpr (FP4) {
+#pragma unroll
+          for (int i = 0; i < C::CPT; ++i) {
+            if (C::CODES % 256 != 0 && w * 64 >= C::CODES) continue;
+            int key, blk;
+            piece_at(i, key, blk);
+            const float sc = e8m0_scale(expo[i]);
+            unsigned char *dst = smem + buf * C::STEP + (key >> 5) * C::TILE + (blk >> 1) * 4096;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              i32x4 v = e2m1x8_to_bf16((uint32_t)codes[i][c], s);
+              i32x4 v = e2m1x8_to_bf16((uint32_t)codes[i][c], sc);
               if (expo[i] == 255u) v = i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
-              *reinterpret_cast<i32x4 *>(dst + (tile_byte(row, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v;
+              *reinterpret_cast<i32x4 *>(dst + (tile_byte(key & 31, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v;
             }
           }
         }
       };
 
       float m_run = kNegBig, l_run = 0.0f;
-      f32x4 o[C::DTW][2 * NT];
+      f32x16 o[NDT];
 #pragma unroll
-      for (int i = 0; i < C::DTW; ++i)
-#pragma unroll
-        for (int h = 0; h < 2 * NT; ++h) o[i][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int dt = 0; dt < NDT; ++dt) o[dt] = zero16();
 
-      auto pv_step = [&](const unsigned char *Kb, int buf) {
-        const int ln = lane_here(), c16 = ln & 15, cg = ln >> 4;
-        if (wv::ballot(FL[buf * NW + (ln & (NW - 1))] != 0) != 0ull) {
+      // one 32-key tile from key0 at LDS tile K
+      auto tile_step = [&](const unsigned char *K, int key0) {
+        auto rows = [&](int ks) { return row_read(K, ks); };
+        auto cols = [&](int i) { return col_read(K, i >> 1, i & 1); };
+        f32x16 acc = zero16();
+        Operands ka;
+        load_group<KS>(ka, 0, rows);
+        stream_operands<KS>(ka, rows, [&](int ks, i32x4 a) {
+          acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(q[ks]), acc, 0, 0, 0);
+        });
+        Operands va;
+        load_group<2 * NDT>(va, 0, cols);
+        __builtin_amdgcn_sched_barrier(0);
+        if (!all_there || key0 + 32 > lim_min) {
+          keep_branch();
+          const uint32_t there = (uint32_t)wv::ballot(key0 + l32 < lim && window[page_of(key0 + l32) - base] >= 0);
 #pragma unroll
-          for (int h = 0; h < 2 * NT; ++h) {
-            const float a = AL[buf * C::ROWS + 16 * h + c16];
-#pragma unroll
-            for (int i = 0; i < C::DTW; ++i) o[i][h] *= a;
+          for (int i = 0; i < 16; ++i) {
+            const int k = acc_row(i, g32);
+            if (!((there >> k) & 1u) || key0 + k >= my_lim) acc[i] = -INFINITY;
           }
         }
-        if (C::NDT < NW && w >= C::NDT) return;
-        // V^T of d tile w + NW i: rows 8 cg + (lane % 16) / 4 (+ 4), columns 4 (lane % 4) .. of the tile
-        int vt[2];
+        float mx = acc[0];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const int c = c16 & 3;
-          vt[v] = tile_byte(8 * cg + 4 * v + (c16 >> 2), 2 * (w & 3) + (c >> 1)) + (c & 1) * 8;
-        }
-        // P[row][key]: 64-byte rows, 16-byte chunk c of row r at c ^ ((r >> 2) & 3)
-        const int p_rd = buf * NT * C::PT_BYTES + c16 * 64 + ((cg ^ ((c16 >> 2) & 3)) * 16);
-        i32x4 av[C::DTW];
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, acc[i]);
+        mx = max_halves(mx) * p.sl2;
+        if (wv::ballot(mx > m_run + 8.0f) != 0ull) {
+          const float m_new = fmaxf(m_run, mx), alpha = exp2_fast(m_run - m_new);
+          m_run = m_new;
+          l_run *= alpha;
 #pragma unroll
-        for (int i = 0; i < C::DTW; ++i) {
-          const int pn = (w >> 2) + i * (NW / 4);
-          const i32x2 r0 = ds_read_tr16(Kb + (vt[0] ^ panel_swz(pn)) + pn * T::PANEL);
-          const i32x2 r1 = ds_read_tr16(Kb + (vt[1] ^ panel_swz(pn)) + pn * T::PANEL);
-          av[i] = i32x4{r0[0], r0[1], r1[0], r1[1]};
+          for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
         }
 #pragma unroll
-        for (int h = 0; h < 2 * NT; ++h) {
-          const i32x4 bv = *reinterpret_cast<const i32x4 *>(P + p_rd + (h >> 1) * C::PT_BYTES + (h & 1) * 1024);
-#pragma unroll
-          for (int i = 0; i < C::DTW; ++i)
-            o[i][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(av[i]), as_bf16x8(bv), o[i][h], 0, 0, 0);
+        for (int i = 0; i < 16; ++i) {
+          acc[i] = exp2_fast(fmaf(acc[i], p.sl2, -m_run));
+          l_run += acc[i];
         }
+        i32x4 pb[2];
+        pack_operand(acc, pb);
+        stream_operands<2 * NDT>(va, cols, [&](int i, i32x4 a) {
+          o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(pb[i & 1]), o[i >> 1], 0, 0, 0);
+        });
       };
 
-      int e_nxt = entry(b0);  // table entry of the block that is fetched next
-      uint32_t vm = there(e_nxt);
-      if (b0 < j1) {
-        const unsigned char *mine = row_at(b0, e_nxt);
-        if (w < C::FW) fetch(0, mine);
-        load_codes(mine);
-        store_codes(0);
-        e_nxt = entry(b0 + 1);
-        if constexpr (FP4) load_codes(row_at(b0 + 1, e_nxt));
+      refill(page_of(x.b0 * C::KEYS));
+      if (x.b0 < j1) {
+        if constexpr (FP4) {
+          load_codes(x.b0);
+          fetch(x.b0, 0);
+          store_codes(0);
+          load_codes(x.b0 + 1);
+        } else if constexpr (NT > 1) {
+#pragma unroll
+          for (int i = 0; i < C::AHEAD; ++i) fetch(x.b0 + i, i);
+        }
       }
-      int kb = 0, kp = 0;
-      for (int j = b0; j < j1; ++j) {
-        const int kn = kb == 2 ? 0 : kb + 1, cur = (j - b0) & 1;
-        const unsigned char *Kj = K + kb * T::BYTES;
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): block j's rows, issued a block ago
-        __syncthreads();                     // block j's rows and block j - 1's P are whole; block j - 2's rows are consumed
-        const uint32_t vm_nxt = there(e_nxt);
-        if (w < C::FW) fetch(kn, row_at(j + 1, e_nxt));  // block j + 1 (past the last: zeros)
-        store_codes(kn);
-        e_nxt = entry(j + 2);
-        f32x16 acc;
-#pragma unroll
-        for (int a = 0; a < 16; ++a) acc[a] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < C::KS; ++i) {
-          const i32x4 a = *reinterpret_cast<const i32x4 *>(Kj + (ka[i % kPh] ^ panel_swz(i / kPh)) + (i / kPh) * T::PANEL);
-          acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(q[i]), acc, 0, 0, 0);
-        }
-        put_partial(Sp + w * C::SP_W, acc);
-        __syncthreads();  // partial tiles whole
-        if constexpr (FP4) load_codes(row_at(j + 2, e_nxt));
-        // softmax: row eh of tile et, 4-key groups (i, eg) with i = ei .. ei + SPL4 - 1: keys 8 i + 4 eg ..
-        const int ln = lane_here(), eh = (w * C::HW) % 32 + (ln & (C::HW - 1)), sr = et * 32 + eh;
-        const int eq = ln / C::HW, eg = eq & 1, ei = (eq >> 1) * C::SPL4;
-        f32x4 s[C::SPL4];
-        {
-          const float *sp = Sp + et * C::KP * C::SP_W + ((ei * 2 + eg) * 32 + eh) * 4;
-#pragma unroll
-          for (int x = 0; x < C::SPL4; ++x) {
-            s[x] = *reinterpret_cast<const f32x4 *>(sp + x * 256);
-#pragma unroll
-            for (int k = 1; k < C::KP; ++k) s[x] += *reinterpret_cast<const f32x4 *>(sp + k * C::SP_W + x * 256);
-          }
-        }
-        if (j > b0) pv_step(K + kp * T::BYTES, cur ^ 1);
-
-        // online softmax (log2 domain, lazy rescale); key 32 j + 8 (ei + x) + 4 eg + e
-        if (vm != 0xffffffffu || 32 * j + 32 > lim_min) {
-          const int my_lim = row_keys(sr);
-#pragma unroll
-          for (int x = 0; x < C::SPL4; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int k = 8 * (ei + x) + 4 * eg + e;
-              if (!((vm >> k) & 1u) || 32 * j + k >= my_lim) s[x][e] = -INFINITY;
+      int buf = 0;
+      for (int j = x.b0; j < j1; ++j) {
+        // what is asked for in this step lies in the window, and what is masked in it
+        if (page_of((j + C::AHEAD + 2) * C::KEYS - 1) >= base + kWindow && page_of(lim - 1) >= base + kWindow) refill(page_of(j * C::KEYS));
+        const unsigned char *S = smem + buf * C::STEP;
+        int nxt = buf + 1 == C::NBUF ? 0 : buf + 1;
+        if constexpr (NT == 1) {
+          if constexpr (FP4) {
+            if (j > x.b0) {
+              wave_lds_sync();
+              fetch(j, 0);
+              store_codes(0);
+              load_codes(j + 1);
             }
-        }
-        float mloc = kNegBig;
-#pragma unroll
-        for (int x = 0; x < C::SPL4; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mloc = fmaxf(mloc, s[x][e]);
-#pragma unroll
-        for (int off = C::HW; off < 32; off <<= 1) mloc = fmaxf(mloc, __shfl_xor(mloc, off, 64));
-        mloc = max_halves(mloc) * p.sl2;
-        const bool moved = wv::ballot(mloc > m_run + 8.0f) != 0ull;
-        float alpha = 1.0f;
-        if (moved) {
-          const float m_new = fmaxf(m_run, mloc);
-          alpha = exp2_fast(m_run - m_new);
-          l_run *= alpha;
-          m_run = m_new;
-        }
-        if (eq == 0) AL[cur * C::ROWS + sr] = alpha;
-        if (ln == 0) FL[cur * NW + w] = moved ? 1 : 0;
-#pragma unroll
-        for (int x = 0; x < C::SPL4; ++x) {
-          float t[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            t[e] = exp2_fast(fmaf(s[x][e], p.sl2, -m_run));
-            l_run += t[e];
+            __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+          } else {
+            fetch(j, 0);
+            __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
           }
-          *reinterpret_cast<i32x2 *>(P + (cur * NT + et) * C::PT_BYTES + eh * 64 + (((ei + x) ^ ((eh >> 2) & 3)) * 16) + eg * 8) =
-              i32x2{(int)pack_bf16x2(t[0], t[1]), (int)pack_bf16x2(t[2], t[3])};
+          wave_lds_sync();
+        } else if constexpr (FP4) {
+          __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+          __syncthreads();          // step j is whole; the step before it is consumed
+          store_codes(nxt);         // step j + 1
+          fetch(j + 1, nxt);
+          load_codes(j + 2);
+        } else {
+          __builtin_amdgcn_s_waitcnt(vmcnt_only((C::AHEAD - 1) * C::DMA));  // this wave's share of step j
+          __syncthreads();
+          fetch(j + C::AHEAD, buf == 0 ? C::NBUF - 1 : buf - 1);           // (past the last step: zeros)
         }
-        vm = vm_nxt;
-        kp = kb;
-        kb = kn;
-      }
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // what was fetched past the last block has landed
 #pragma unroll
-      for (int off = C::HW; off < 32; off <<= 1) l_run += __shfl_xor(l_run, off, 64);
-      l_run = sum_halves(l_run);
-      const int ln = lane_here(), sr = w * C::HW + (ln & (C::HW - 1)), eq = ln / C::HW;  // this lane's softmax row
-      const bool none = row_keys(sr) <= 32 * b0 || l_run == 0.0f;  // no key of this piece
-      if (eq == 0) AL[2 * C::ROWS + sr] = none ? 0.0f : 1.0f / l_run;
-      __syncthreads();
-      if (b0 < j1) pv_step(K + kp * T::BYTES, (j1 - b0 - 1) & 1);
-
+        for (int sub = 0; sub < SUB; ++sub) {
+          const int tl = kg * SUB + sub, key0 = j * C::KEYS + tl * 32;
+          if (key0 < lim) tile_step(S + tl * C::TILE, key0);
+        }
+        if constexpr (NT == 1) wave_lds_sync();  // the tile is read: it may be written again
+        buf = nxt;
+      }
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // what was fetched past the last step has landed
       if (probe) {
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < C::DTW; ++i)
+        for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-          for (int h = 0; h < 2 * NT; ++h)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= (__float_as_uint(o[i][h][e]) & 0x7f800000u) == 0x7f800000u;
-        if (__syncthreads_or(bad)) return false;
-      }
-      const int rlo = tok * p.H - first, rhi = min((tlim + 1) * p.H - first, nrows);  // rows of tokens [tok, tlim]
-      if (!whole_unit) {
-        if (eq == 0 && sr >= rlo && sr < rhi) {
-          p.part_ml[(piece * C::ROWS + sr) * 2] = m_run;
-          p.part_ml[(piece * C::ROWS + sr) * 2 + 1] = none ? 0.0f : l_run;
+          for (int i = 0; i < 16; ++i) bad |= not_finite(o[dt][i]);
+        if (__syncthreads_or(bad)) {
+          probe = false;
+          ta = tb = tok0;
+          continue;
         }
-      } else if (eq == 0 && sr >= rlo && sr < rhi) {
-        p.lse[row0 + sr] = none ? -INFINITY : log2f(l_run) + m_run;
       }
+      l_run = sum_halves(l_run);
+      // the key groups' sums, pairwise: waves of the upper half of them leave theirs for the lower half
 #pragma unroll
-      for (int h = 0; h < 2 * NT; ++h) {
-        const int r = 16 * h + (ln & 15);
-        const float inv = AL[2 * C::ROWS + r];
-        if (r >= rlo && r < rhi) {
+      for (int half = C::KG / 2; half >= 1; half /= 2) {
+        __syncthreads();
+        if (kg >= half && kg < 2 * half) {
+          const int slot = (kg - half) * NT + rt;
+          unsigned char *dst = smem + slot * C::O_BYTES;
 #pragma unroll
-          for (int i = 0; i < C::DTW; ++i)
-            if (C::NDT % NW == 0 || w + NW * i < C::NDT) {
-              const int d = (w + NW * i) * 16 + 4 * (ln >> 4);
-              if (whole_unit) {
-                // an empty row's O is zeros (or what a neighbour's key left): 0
-                const f32x4 x = inv == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o[i][h] * inv;
-                *reinterpret_cast<i32x2 *>(p.out + (row0 + r) * D_V + d) =
-                    i32x2{(int)pack_bf16x2(x[0], x[1]), (int)pack_bf16x2(x[2], x[3])};
-              } else if (inv != 0.0f) {
-                *reinterpret_cast<f32x4 *>(p.part_o + (piece * C::ROWS + r) * D_V + d) = o[i][h];
-              }
+          for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+              *reinterpret_cast<f32x4 *>(dst + ((dt * 4 + m) * 64 + lane) * 16) =
+                  f32x4{o[dt][4 * m], o[dt][4 * m + 1], o[dt][4 * m + 2], o[dt][4 * m + 3]};
+          if (g32 == 0) {
+            ML[(slot * 32 + l32) * 2] = m_run;
+            ML[(slot * 32 + l32) * 2 + 1] = l_run;
+          }
+        }
+        __syncthreads();
+        if (kg < half) {
+          const int slot = kg * NT + rt;
+          const unsigned char *src = smem + slot * C::O_BYTES;
+          const float m2 = ML[(slot * 32 + l32) * 2], l2 = ML[(slot * 32 + l32) * 2 + 1];
+          // (a group without a key of the row has l = 0 and O = 0)
+          const float m_new = l2 == 0.0f ? m_run : (l_run == 0.0f ? m2 : fmaxf(m_run, m2));
+          const float a1 = l_run == 0.0f ? 0.0f : exp2_fast(m_run - m_new), a2 = l2 == 0.0f ? 0.0f : exp2_fast(m2 - m_new);
+          m_run = m_new;
+          l_run = l_run * a1 + l2 * a2;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const f32x4 y = *reinterpret_cast<const f32x4 *>(src + ((dt * 4 + m) * 64 + lane) * 16);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[dt][4 * m + e] = o[dt][4 * m + e] * a1 + y[e] * a2;
             }
         }
       }
-      __syncthreads();  // LDS is free for the next piece
-      return true;
-    };
-    int ta = tok0, tb = tok1;
-    bool probe = tok0 != tok1;
-    while (true) {
-      if (!run(ta, tb, probe)) {
-        probe = false;
-        ta = tb = tok0;
-        __syncthreads();
-        continue;
+      const int rlo = ta * p.H - x.first, rhi = min((tb + 1) * p.H - x.first, x.nrows);  // rows of tokens [ta, tb]
+      if (kg == 0 && row >= rlo && row < rhi) {
+        const bool none = my_lim <= x.b0 * C::KEYS || l_run == 0.0f;  // no key of this piece
+        const float inv = none ? 0.0f : 1.0f / l_run;
+        const int64_t part = (int64_t)x.slot * C::ROWS + row;
+        if (g32 == 0) {
+          if (x.whole) {
+            p.lse[x.row0 + row] = none ? -INFINITY : log2f(l_run) + m_run;
+          } else {
+            p.part_ml[part * 2] = m_run;
+            p.part_ml[part * 2 + 1] = none ? 0.0f : l_run;
+          }
+        }
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const f32x4 v{o[dt][4 * m], o[dt][4 * m + 1], o[dt][4 * m + 2], o[dt][4 * m + 3]};
+            const int col = acc_col(dt, 4 * m, g32);
+            if (x.whole) {
+              // a row without keys: 0, whatever its neighbours' keys left
+              *reinterpret_cast<i32x2 *>(p.out + (x.row0 + row) * D_V + col) =
+                  none ? i32x2{0, 0} : i32x2{(int)pack_bf16x2(v[0] * inv, v[1] * inv), (int)pack_bf16x2(v[2] * inv, v[3] * inv)};
+            } else if (!none) {
+              *reinterpret_cast<f32x4 *>(p.part_o + part * D_V + col) = v;
+            }
+          }
       }
+      __syncthreads();  // LDS is free for the next piece
       if (tb == tok1) break;
       ta = ++tb;
     }
   }
 }
 
-// One wave per row of q: the pieces of its unit, where it has several, brought to their
-// largest maximum and added in order.
+// Workgroup (w, y): where the first of a unit's blocks that is not in the piece of the
+// workgroup that began it is in range w, 16 rows of that unit, a wave four: its pieces
+// brought to their largest maximum and added in order.
 template <int D_V>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p) {
   constexpr int NCH = D_V / 4, CPL = (NCH + 63) / 64;
   const int lane = lane_id();
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave_id();
-  if (row >= p.T * p.H) return;
-  const int tok = (int)(row / p.H);
-  int r = tok;
-  if (p.query_starts != nullptr) {
-    int lo = 0, hi = p.R - 1;  // the last request that starts at or before the token
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (request_start(p, mid) <= tok) lo = mid; else hi = mid - 1;
-    }
-    r = lo;
-    if (tok < request_start(p, r) || tok >= request_start(p, r) + request_tokens(p, r)) return;  // behind the last request
-  } else if (r >= p.R) {
-    return;
-  }
-  const int in_req = (int)(row - (int64_t)request_start(p, r) * p.H);
-  const int u = p.unit0[r] + in_req / p.unit_rows, ur = in_req % p.unit_rows;
-  const int units = p.unit0[p.R];
-  if (u >= units) return;
-  const int per = range_blocks(p, p.unit_at[units]);
-  const int64_t w0 = p.unit_at[u] / per, w1 = (p.unit_at[u + 1] - 1) / per;
-  if (w0 == w1) return;  // one piece: its workgroup wrote the row
-  auto at = [&](int64_t w) { return (w * 2 + (w == w0 ? 1 : 0)) * p.unit_rows + ur; };
-  float m = kNegBig;
-  for (int64_t w = w0; w <= w1; ++w)
-    if (p.part_ml[at(w) * 2 + 1] != 0.0f) m = fmaxf(m, p.part_ml[at(w) * 2]);
-  float l = 0.0f;
-  f32x4 o[CPL];
+  const int units = uni(p.unit0[p.R]), total = uni(p.unit_at[units]), per = uni(range_blocks(p, total));
+  const int64_t cut = ((int64_t)blockIdx.x + 1) * per;
+  if (cut >= total) return;
+  const int u = uni(unit_of(p, units, (int)cut)), ub = uni(p.unit_at[u]), ue = uni(p.unit_at[u + 1]);
+  const int w0 = ub / per, w1 = (ue - 1) / per;
+  if (ub == cut || w0 != (int)blockIdx.x) return;  // no unit is cut here, or it was cut before
+  const int req = uni(p.unit_req[u]), first = uni(p.unit_first[u]);
+  const int nrows = min(uni(request_tokens(p, req)) * p.H - first, p.unit_rows);
+  const int64_t row0 = (int64_t)uni(request_start(p, req)) * p.H + first;
+  for (int ur = (int)blockIdx.y * 16 + wave_id(); ur < min((int)blockIdx.y * 16 + 16, nrows); ur += 4) {
+    const int64_t row = row0 + ur;
+    auto at = [&](int w) { return (int64_t)(w * 2 + (w == w0 ? 1 : 0)) * p.unit_rows + ur; };
+    float m = kNegBig;
+    for (int w = w0; w <= w1; ++w)
+      if (p.part_ml[at(w) * 2 + 1] != 0.0f) m = fmaxf(m, p.part_ml[at(w) * 2]);
+    float l = 0.0f;
+    f32x4 o[CPL];
 #pragma unroll
-  for (int c = 0; c < CPL; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t w = w0; w <= w1; ++w) {
-    const float lw = p.part_ml[at(w) * 2 + 1];
-    if (lw == 0.0f) continue;  // no key of the row in the piece, which left no O (a NaN sum joins)
-    const float a = exp2_fast(p.part_ml[at(w) * 2] - m);
-    l += lw * a;
+    for (int c = 0; c < CPL; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w = w0; w <= w1; ++w) {
+      const float lw = p.part_ml[at(w) * 2 + 1];
+      if (lw == 0.0f) continue;  // no key of the row in the piece, which left no O (a NaN sum joins)
+      const float a = exp2_fast(p.part_ml[at(w) * 2] - m);
+      l += lw * a;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c)
+        if (lane + 64 * c < NCH) o[c] += a * *reinterpret_cast<const f32x4 *>(p.part_o + at(w) * D_V + (lane + 64 * c) * 4);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int c = 0; c < CPL; ++c)
-      if (lane + 64 * c < NCH) o[c] += a * *reinterpret_cast<const f32x4 *>(p.part_o + at(w) * D_V + (lane + 64 * c) * 4);
+      if (lane + 64 * c < NCH)
+        *reinterpret_cast<i32x2 *>(p.out + row * D_V + (lane + 64 * c) * 4) =
+            i32x2{(int)pack_bf16x2(o[c][0] * inv, o[c][1] * inv), (int)pack_bf16x2(o[c][2] * inv, o[c][3] * inv)};
+    if (lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int c = 0; c < CPL; ++c)
-    if (lane + 64 * c < NCH)
-      *reinterpret_cast<i32x2 *>(p.out + row * D_V + (lane + 64 * c) * 4) =
-          i32x2{(int)pack_bf16x2(o[c][0] * inv, o[c][1] * inv), (int)pack_bf16x2(o[c][2] * inv, o[c][3] * inv)};
-  if (lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
 }
 
 // How a call is run, from its sizes alone.  Rows that share keys: a request's (token, head) pairs, on average.
 struct PagedPlan {
-  int few;        // 16-row tiles of a unit whose waves split the keys, or 0
-  int nt;         // else 32-row tiles of a unit whose waves share them
-  int unit_rows, max_units, nwg, min_blocks;
+  int wide;       // 576 / 512: 16-row tiles of a unit
+  int few;        // 128 / 64: 16-row tiles of a unit whose waves split the keys
+  int nt;         // 128 / 64: else 32-row tiles of a unit
+  int unit_rows, step_keys, max_units, nwg, min_blocks;
 };
 static PagedPlan paged_plan(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk) {
   PagedPlan r{};
   const int64_t rows = (T + R - 1) / R * H;
-  if (rows <= (d_qk == 576 ? 16 : 32)) {
+  if (d_qk == 576) {
+    r.wide = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 8));
+    r.unit_rows = 16 * r.wide;
+    r.step_keys = paged_wide_keys(r.wide);
+  } else if (rows <= 32) {
     r.few = rows <= 16 ? 1 : 2;
     r.unit_rows = 16 * r.few;
+    r.step_keys = 32;
   } else {
-    r.nt = rows > 64 && d_qk == 576 ? 4 : (rows > 32 ? 2 : 1);
+    r.nt = rows > 64 ? 4 : 2;
     r.unit_rows = 32 * r.nt;
+    r.step_keys = 64;
   }
-  r.min_blocks = r.few ? 8 : 4;
+  r.min_blocks = 256 / r.step_keys;  // keys that are worth a piece's beginning and end
   r.max_units = (int)(T * H / r.unit_rows + R);
-  const int64_t blocks = (int64_t)r.max_units * ((W * block + 31) / 32), n = (blocks + r.min_blocks - 1) / r.min_blocks;
-  const int64_t most = r.few && d_qk == 128 ? 768 : 256;  // resident workgroups
+  const int64_t blocks = (int64_t)r.max_units * ((W * block + r.step_keys - 1) / r.step_keys);
+  const int64_t n = (blocks + r.min_blocks - 1) / r.min_blocks;
+  const int64_t most = d_qk == 128 ? 768 : 256;  // resident workgroups
   r.nwg = (int)(n < 1 ? 1 : (n < most ? n : most));
   return r;
 }
@@ -529,21 +520,14 @@ size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H
   return paged_sections(T, R, W, block, H, d_qk, d_v).total;
 }
 
-template <int D_QK, int D_V, int NT, int NW, bool FP4>
+template <int D_QK, int D_V, int NT, int SUB, int NBUF, bool FP4, int OCC>
 static int launch(const PagedParams &p, hipStream_t st) {
-  using C = Paged<D_QK, D_V, NT, NW, FP4>;
-  const auto kernel = paged_fwd_kernel<D_QK, D_V, NT, NW, FP4>;
+  using C = Paged<D_QK, D_V, NT, SUB, NBUF, FP4>;
+  const auto kernel = paged_rows_kernel<D_QK, D_V, NT, SUB, NBUF, FP4, OCC>;
   const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
   if (e != hipSuccess) return set_error(DSA_ERR_HIP, "dsa_paged_latent_mla_fwd: LDS attribute: %s", hipGetErrorString(e));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)p.nwg), dim3(C::NTHR), C::BYTES, st, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)p.nwg), dim3(256), C::BYTES, st, p);
   return check_launch("dsa_paged_latent_mla_fwd");
-}
-
-template <bool FP4>
-static int launch_nt(const PagedParams &p, int64_t d_qk, int nt, hipStream_t st) {
-  if (d_qk == 128) return launch<128, 64, 2, 4, FP4>(p, st);
-  if (nt == 1) return launch<576, 512, 1, 4, FP4>(p, st);
-  return nt == 4 ? launch<576, 512, 4, 8, FP4>(p, st) : launch<576, 512, 2, 8, FP4>(p, st);
 }
 
 int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st) {
@@ -553,6 +537,7 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
   p.max_units = k.max_units;
   p.nwg = k.nwg;
   p.min_blocks = k.min_blocks;
+  p.step_keys = k.step_keys;
   p.unit0 = (int32_t *)(ws + s.unit0);
   p.unit_req = (int32_t *)(ws + s.unit_req);
   p.unit_first = (int32_t *)(ws + s.unit_first);
@@ -562,9 +547,12 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
   hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, st, p);
   int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
   if (rc) return rc;
-  rc = k.few ? launch_paged_few(p, d_qk, k.few, fp4, st) : (fp4 ? launch_nt<true>(p, d_qk, k.nt, st) : launch_nt<false>(p, d_qk, k.nt, st));
+  if (k.wide) rc = launch_paged_wide(p, k.wide, fp4, st);
+  else if (k.few) rc = launch_paged_few(p, k.few, fp4, st);
+  else if (k.nt == 4) rc = fp4 ? launch<128, 64, 4, 2, 3, true, 3>(p, st) : launch<128, 64, 4, 2, 3, false, 3>(p, st);
+  else rc = fp4 ? launch<128, 64, 2, 1, 3, true, 3>(p, st) : launch<128, 64, 2, 1, 3, false, 3>(p, st);
   if (rc || p.nwg == 1) return rc;  // one workgroup: no unit has several pieces
-  const dim3 grid((unsigned)((p.T * p.H + 3) / 4));
+  const dim3 grid((unsigned)(p.nwg - 1), (unsigned)(p.unit_rows / 16));
   if (d_v == 512) hipLaunchKernelGGL(paged_combine_kernel<512>, grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL(paged_combine_kernel<64>, grid, dim3(256), 0, st, p);
   return check_launch("dsa_paged_latent_mla_fwd (combine)");

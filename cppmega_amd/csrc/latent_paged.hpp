@@ -16,9 +16,10 @@ struct PagedParams {
   float *lse;                    // [T, H]
   int64_t T;
   int R, W, H, block, num_blocks;
+  int block_shift;               // log2 of a page's rows, -1: no power of two
   float sl2;
   // plan and partial results
-  int unit_rows, max_units, nwg, min_blocks;
+  int unit_rows, step_keys, max_units, nwg, min_blocks;  // rows of a unit, keys of a block of it
   int32_t *unit0, *unit_req, *unit_first;
   int32_t *unit_at;
   float *part_ml, *part_o;       // [2 nwg][unit_rows]: (m, l), [d_v]
@@ -105,7 +106,13 @@ __device__ __forceinline__ const unsigned char *key_row(const PagedParams &p, in
   return entry >= 0 && entry < p.num_blocks ? p.cache + slot * row_bytes : reinterpret_cast<const unsigned char *>(kZeroRow);
 }
 
-int launch_paged_few(const PagedParams &p, int64_t d_qk, int tiles16, bool fp4, hipStream_t st);
+constexpr int kWindow = 1024;  // table entries of a request that a workgroup has in LDS
+// vmcnt(n) alone
+constexpr int vmcnt_only(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+
+int paged_wide_keys(int tiles16);  // keys of a step
+int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
+int launch_paged_few(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
 
 size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v);
 int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st);

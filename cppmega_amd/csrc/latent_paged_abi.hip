@@ -117,6 +117,7 @@ extern "C" int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const 
   p.W = (int)W;
   p.H = (int)H;
   p.block = (int)block_size;
+  p.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)block_size) : -1;
   p.num_blocks = (int)num_blocks;
   p.sl2 = sm_scale * kLog2e;
   return launch_paged_fwd(p, D_qk, D_v, dtype == DSA_DTYPE_MXFP4, (unsigned char *)workspace, (hipStream_t)stream);

@@ -293,8 +293,7 @@ static int launch(const PagedParams &p, hipStream_t st) {
   return check_launch("dsa_paged_latent_mla_fwd");
 }
 
-int launch_paged_few(const PagedParams &p, int64_t d_qk, int tiles16, bool fp4, hipStream_t st) {
-  if (d_qk == 576) return fp4 ? launch<576, 512, 1, true, 1>(p, st) : launch<576, 512, 1, false, 1>(p, st);
+int launch_paged_few(const PagedParams &p, int tiles16, bool fp4, hipStream_t st) {
   if (tiles16 == 1) return fp4 ? launch<128, 64, 1, true, 3>(p, st) : launch<128, 64, 1, false, 3>(p, st);
   return fp4 ? launch<128, 64, 2, true, 3>(p, st) : launch<128, 64, 2, false, 3>(p, st);
 }
