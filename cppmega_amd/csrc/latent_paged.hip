@@ -139,10 +139,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
     const int tok0 = x.first / p.H, tok1 = (x.first + x.nrows - 1) / p.H;
     const int row = 32 * rt + l32;  // of the unit
     i32x4 q[KS];
+    {
+      const unsigned char *src = (row < x.nrows ? p.q + (x.row0 + row) * D_QK * 2 : zero) + 16 * g32;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      q[ks] = i32x4{0, 0, 0, 0};
-      if (row < x.nrows) q[ks] = ld_global_16(p.q + ((x.row0 + row) * D_QK + 16 * ks + 8 * g32) * 2);
+      for (int ks = 0; ks < KS; ++ks) q[ks] = ld_global_16(src + 32 * ks);
     }
     // Tokens [ta, tb] with the keys cut at tb's: all at once, or, where that left something that is not finite, one by
     // one, since a weight of zero does not remove the Inf or NaN of a later token's key.
@@ -423,39 +423,55 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
 }
 
 // Workgroup (w, y): where the first of a unit's blocks that is not in the piece of the
-// workgroup that began it is in range w, 16 rows of that unit, a wave four: its pieces
-// brought to their largest maximum and added in order.
+// workgroup that began it is in range w + 1, some rows of that unit, one a wave after the
+// other: its pieces brought to their largest maximum and added in order.
 template <int D_V>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p) {
-  constexpr int NCH = D_V / 4, CPL = (NCH + 63) / 64;
+  constexpr int NCH = D_V / 4, CPL = (NCH + 63) / 64, AHEAD = 4;
   const int lane = lane_id();
   const int units = uni(p.unit0[p.R]), total = uni(p.unit_at[units]), per = uni(range_blocks(p, total));
   const int64_t cut = ((int64_t)blockIdx.x + 1) * per;
   if (cut >= total) return;
   const int u = uni(unit_of(p, units, (int)cut)), ub = uni(p.unit_at[u]), ue = uni(p.unit_at[u + 1]);
-  const int w0 = ub / per, w1 = (ue - 1) / per;
+  const int w0 = ub / per, pieces = (ue - 1) / per - w0 + 1;
   if (ub == cut || w0 != (int)blockIdx.x) return;  // no unit is cut here, or it was cut before
   const int req = uni(p.unit_req[u]), first = uni(p.unit_first[u]);
   const int nrows = min(uni(request_tokens(p, req)) * p.H - first, p.unit_rows);
   const int64_t row0 = (int64_t)uni(request_start(p, req)) * p.H + first;
-  for (int ur = (int)blockIdx.y * 16 + wave_id(); ur < min((int)blockIdx.y * 16 + 16, nrows); ur += 4) {
+  const int rows = p.unit_rows / (int)gridDim.y;
+  for (int ur = (int)blockIdx.y * rows + wave_id(); ur < min(((int)blockIdx.y + 1) * rows, nrows); ur += 4) {
     const int64_t row = row0 + ur;
-    auto at = [&](int w) { return (int64_t)(w * 2 + (w == w0 ? 1 : 0)) * p.unit_rows + ur; };
+    // piece k's row of partial results: in the second place of the workgroup that began the unit, the first of the others
+    auto at = [&](int k) { return (int64_t)((w0 + k) * 2 + (k == 0 ? 1 : 0)) * p.unit_rows + ur; };
     float m = kNegBig;
-    for (int w = w0; w <= w1; ++w)
-      if (p.part_ml[at(w) * 2 + 1] != 0.0f) m = fmaxf(m, p.part_ml[at(w) * 2]);
+    for (int k = lane; k < pieces; k += 64)
+      if (p.part_ml[at(k) * 2 + 1] != 0.0f) m = fmaxf(m, p.part_ml[at(k) * 2]);
+    m = __uint_as_float(wv::wave_reduce(__float_as_uint(m), wv::MaxF()));
     float l = 0.0f;
     f32x4 o[CPL];
 #pragma unroll
     for (int c = 0; c < CPL; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int w = w0; w <= w1; ++w) {
-      const float lw = p.part_ml[at(w) * 2 + 1];
-      if (lw == 0.0f) continue;  // no key of the row in the piece, which left no O (a NaN sum joins)
-      const float a = exp2_fast(p.part_ml[at(w) * 2] - m);
-      l += lw * a;
+    for (int k0 = 0; k0 < pieces; k0 += AHEAD) {
+      f32x4 x[AHEAD][CPL];
+      float lk[AHEAD], mk[AHEAD];
 #pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (lane + 64 * c < NCH) o[c] += a * *reinterpret_cast<const f32x4 *>(p.part_o + at(w) * D_V + (lane + 64 * c) * 4);
+      for (int i = 0; i < AHEAD; ++i) {
+        const int64_t r = at(min(k0 + i, pieces - 1));
+        mk[i] = p.part_ml[r * 2];
+        lk[i] = k0 + i < pieces ? p.part_ml[r * 2 + 1] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c)
+          if (lane + 64 * c < NCH) x[i][c] = *reinterpret_cast<const f32x4 *>(p.part_o + r * D_V + (lane + 64 * c) * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (lk[i] == 0.0f) continue;  // no key of the row in the piece, which left no O (a NaN sum joins)
+        const float a = exp2_fast(mk[i] - m);
+        l += lk[i] * a;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c)
+          if (lane + 64 * c < NCH) o[c] += a * x[i][c];
+      }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -552,7 +568,7 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
   else if (k.nt == 4) rc = fp4 ? launch<128, 64, 4, 2, 3, true, 3>(p, st) : launch<128, 64, 4, 2, 3, false, 3>(p, st);
   else rc = fp4 ? launch<128, 64, 2, 1, 3, true, 3>(p, st) : launch<128, 64, 2, 1, 3, false, 3>(p, st);
   if (rc || p.nwg == 1) return rc;  // one workgroup: no unit has several pieces
-  const dim3 grid((unsigned)(p.nwg - 1), (unsigned)(p.unit_rows / 16));
+  const dim3 grid((unsigned)(p.nwg - 1), (unsigned)(p.unit_rows / (p.unit_rows < 64 ? 4 : 16)));
   if (d_v == 512) hipLaunchKernelGGL(paged_combine_kernel<512>, grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL(paged_combine_kernel<64>, grid, dim3(256), 0, st, p);
   return check_launch("dsa_paged_latent_mla_fwd (combine)");

@@ -77,14 +77,18 @@ __device__ __forceinline__ PagedPiece next_piece(const PagedParams &p, int u, in
   return x;
 }
 
-// The last unit that begins at or before block `at`.
+// The last unit that begins at or before block `at` (the whole wave: 64 units are looked at in a step).
 __device__ __forceinline__ int unit_of(const PagedParams &p, int units, int at) {
-  int u = 0, hi = units - 1;
-  while (u < hi) {
-    const int mid = (u + hi + 1) >> 1;
-    if (p.unit_at[mid] <= at) u = mid; else hi = mid - 1;
+  const int lane = lane_id();
+  int lo = 0, n = units;  // it is one of lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + 63) / 64, at_lane = lo + lane * step;
+    const uint64_t before = __builtin_amdgcn_ballot_w64(lane * step < n && p.unit_at[at_lane < units ? at_lane : 0] <= at);
+    const int k = (int)__builtin_popcountll(before) - 1;
+    n = n - k * step < step ? n - k * step : step;
+    lo += k * step;
   }
-  return u;
+  return lo;
 }
 
 __device__ __forceinline__ void dma_16_at(uint32_t lds, const unsigned char *src) {

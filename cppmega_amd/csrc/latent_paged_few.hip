@@ -67,12 +67,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
 
     i32x4 q[NR][C::KS];
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt)
+    for (int rt = 0; rt < NR; ++rt) {
+      const unsigned char *src = (16 * rt + l16 < nrows ? p.q + (row0 + 16 * rt + l16) * D_QK * 2 : zero) + 16 * g16;
 #pragma unroll
-      for (int ks = 0; ks < C::KS; ++ks) {
-        q[rt][ks] = i32x4{0, 0, 0, 0};
-        if (16 * rt + l16 < nrows) q[rt][ks] = ld_global_16(p.q + ((row0 + 16 * rt + l16) * D_QK + 32 * ks + 8 * g16) * 2);
-      }
+      for (int ks = 0; ks < C::KS; ++ks) q[rt][ks] = ld_global_16(src + 64 * ks);
+    }
 
     // Tokens [ta, tb] with the keys cut at tb's: all at once, or, where that left something that is not finite, one by
     // one, since a weight of zero does not remove the Inf or NaN of a later token's key.

@@ -37,13 +37,13 @@ struct PagedWide {
   static constexpr int NBUF = 4 * 36864 / STEP;
   static constexpr int KS = 18, NDT = 32;
   static constexpr int LT = 64 * LW;                         // loading threads
-  static constexpr int CPT = KEYS * 16 / LT, RPT = (KEYS * 8 + LT - 1) / LT;  // MXFP4: code pieces, rope chunks per thread
+  static constexpr int TPR = LT / KEYS, CPT = 16 / TPR, RPT = (8 + TPR - 1) / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
   static constexpr int RAW = ROLES ? 2 : 1;                  // steps in a loading wave's registers
   static constexpr int OFF_T = NBUF * STEP;
   static constexpr int OFF_ML = OFF_T + kWindow * 4;         // [2][16][2]
   static constexpr int BYTES = OFF_ML + 2 * 16 * 8;
   static constexpr int O_BYTES = 512 * 16 * 4;
-  static_assert(NBUF == (ROLES ? 2 : 4) && OFF_T == 147456 && BYTES <= 159 * 1024, "LDS");
+  static_assert((TPR == 4 || TPR == 16) && NBUF == (ROLES ? 2 : 4) && OFF_T == 147456 && BYTES <= 159 * 1024, "LDS");
 };
 
 // Chunk c (16 bytes, 0..7) of row r of a panel at r * 128 + ((c ^ swizzle) * 16).  32-row tiles: row_swz.  16-row tiles:
@@ -139,48 +139,46 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           if (w < 4) group(j, buf, w, Zero{}, Mid{}); else group(j, buf, w - 4, Mid{}, All{});
         }
       };
-      // MXFP4: a step's code pieces and rope chunks, a row's from neighbouring threads
+      // MXFP4: TPR neighbouring threads have a row: every TPR-th piece of codes (16 bytes, a 32-channel block) and rope
+      // chunk of it, and all its exponents
       struct Raw {
-        i32x4 codes[C::CPT], rope[C::RPT];
-        uint32_t expo[C::CPT];
+        i32x4 codes[C::CPT], rope[C::RPT], expo;
       };
-      constexpr bool kHalfRope = C::KEYS * 8 < C::LT;  // only the first waves have one
+      const int th = lw * 64 + (C::ROLES ? lane_id() : lane_here()), key_of = th / C::TPR, part = th % C::TPR;
       auto load_raw = [&](Raw &raw, int j) {
-        const int ln = lane_here();
+        const unsigned char *src = key_at(j * C::KEYS + key_of);
 #pragma unroll
-        for (int i = 0; i < C::CPT; ++i) {
-          const int y = i * C::LT + lw * 64 + ln;
-          const unsigned char *src = key_at(j * C::KEYS + (y >> 4));
-          raw.codes[i] = ld_global_16(src + (y & 15) * 16);
-          raw.expo[i] = src[Row::OFF_EXP + (y & 15)];
-        }
+        for (int i = 0; i < C::CPT; ++i) raw.codes[i] = ld_global_16(src + (i * C::TPR + part) * 16);
+        raw.expo = ld_global_16(src + Row::OFF_EXP);
 #pragma unroll
-        for (int i = 0; i < C::RPT; ++i) {
-          const int y = i * C::LT + lw * 64 + ln;
-          if (kHalfRope && lw * 64 >= C::KEYS * 8) continue;  // wave-uniform
-          raw.rope[i] = ld_global_16(key_at(j * C::KEYS + (y >> 3)) + Row::OFF_ROPE + (y & 7) * 16);
-        }
+        for (int i = 0; i < C::RPT; ++i) raw.rope[i] = ld_global_16(src + Row::OFF_ROPE + ((i * C::TPR + part) & 7) * 16);
       };
       auto store_raw = [&](const Raw &raw, int buf) {
-        const int ln = lane_here();
+        unsigned char *tile = smem + buf * C::STEP + (key_of / TK) * C::TILE;
 #pragma unroll
         for (int i = 0; i < C::CPT; ++i) {
-          const int y = i * C::LT + lw * 64 + ln, key = y >> 4, blk = y & 15;
-          const float sc = e8m0_scale(raw.expo[i]);
-          unsigned char *dst = smem + buf * C::STEP + (key / TK) * C::TILE + (blk >> 1) * C::PANEL;
+          const int blk = i * C::TPR + part;
+          // byte blk of the exponents: dword i of four threads' rows, else dword part / 4
+          const uint32_t four = (uint32_t)(C::TPR == 4 ? raw.expo[i] : (part < 8 ? (part < 4 ? raw.expo[0] : raw.expo[1]) : (part < 12 ? raw.expo[2] : raw.expo[3])));
+          const uint32_t e = (four >> (8 * (part & 3))) & 255u;
+          const float sc = e8m0_scale(e);
+          i32x4 v[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            i32x4 v = e2m1x8_to_bf16((uint32_t)raw.codes[i][c], sc);
-            if (raw.expo[i] == 255u) v = i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
-            *reinterpret_cast<i32x4 *>(dst + (wide_byte<TK>(key % TK, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v;
+          for (int c = 0; c < 4; ++c) v[c] = e2m1x8_to_bf16((uint32_t)raw.codes[i][c], sc);
+          if (wv::ballot(e == 255u) != 0ull) {
+            keep_branch();
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (e == 255u) v[c] = i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
           }
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<i32x4 *>(tile + (blk >> 1) * C::PANEL + (wide_byte<TK>(key_of % TK, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v[c];
         }
 #pragma unroll
-        for (int i = 0; i < C::RPT; ++i) {
-          const int y = i * C::LT + lw * 64 + ln, key = y >> 3;
-          if (kHalfRope && lw * 64 >= C::KEYS * 8) continue;
-          *reinterpret_cast<i32x4 *>(smem + buf * C::STEP + (key / TK) * C::TILE + 8 * C::PANEL + wide_byte<TK>(key % TK, y & 7)) = raw.rope[i];
-        }
+        for (int i = 0; i < C::RPT; ++i)
+          if (C::TPR == 4 || part < 8)
+            *reinterpret_cast<i32x4 *>(tile + 8 * C::PANEL + wide_byte<TK>(key_of % TK, (i * C::TPR + part) & 7)) = raw.rope[i];
       };
 
       // steps that are asked for before they are worked on, and their pages in the window
@@ -193,11 +191,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
       bool again = false;
       if (computes) {  // (the registers of Q and O are these waves' alone)
         i32x4 q[KS];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+        {
           const int row = my_row(), g16 = lane_here() >> 4;
-          q[ks] = i32x4{0, 0, 0, 0};
-          if (row < x.nrows) q[ks] = ld_global_16(p.q + ((x.row0 + row) * 576 + 32 * ks + 8 * g16) * 2);
+          const unsigned char *src = (row < x.nrows ? p.q + (x.row0 + row) * 1152 : zero) + 16 * g16;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) q[ks] = ld_global_16(src + 64 * ks);
         }
         float m_run = kNegBig, l_run = 0.0f;
         f32x4 o[NDT];
