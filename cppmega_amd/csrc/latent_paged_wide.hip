@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
       struct Raw {
         i32x4 codes[C::CPT], rope[C::RPT], expo;
       };
-      const int th = lw * 64 + (C::ROLES ? lane_id() : lane_here()), key_of = th / C::TPR, part = th % C::TPR;
       auto load_raw = [&](Raw &raw, int j) {
+        const int th = lw * 64 + lane_here(), key_of = th / C::TPR, part = th % C::TPR;
         const unsigned char *src = key_at(j * C::KEYS + key_of);
 #pragma unroll
         for (int i = 0; i < C::CPT; ++i) raw.codes[i] = ld_global_16(src + (i * C::TPR + part) * 16);
@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
         for (int i = 0; i < C::RPT; ++i) raw.rope[i] = ld_global_16(src + Row::OFF_ROPE + ((i * C::TPR + part) & 7) * 16);
       };
       auto store_raw = [&](const Raw &raw, int buf) {
+        const int th = lw * 64 + lane_here(), key_of = th / C::TPR, part = th % C::TPR;
         unsigned char *tile = smem + buf * C::STEP + (key_of / TK) * C::TILE;
 #pragma unroll
         for (int i = 0; i < C::CPT; ++i) {
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           load_group<KS * H>(a0, 0, rows);
           stream_operands<KS * H>(a0, rows, [&](int i, i32x4 a) {
             s[i % H] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(q[i / H]), s[i % H], 0, 0, 0);
+            if (i % kGroup >= kGroup - H) asm volatile("" : "+v"(s[i % H]));  // here, not where the sum is needed
           });
 #pragma unroll
           for (int h = 0; h < H; ++h) {
@@ -302,11 +304,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           }
         } else if constexpr (FP4) {
           Raw raw;
-          if (x.b0 < j1) {
-            load_raw(raw, x.b0);
-            store_raw(raw, 0);
-            load_raw(raw, x.b0 + 1);
-          }
+          load_raw(raw, x.b0);  // (where there is no step: zeros)
+          store_raw(raw, 0);
+          load_raw(raw, x.b0 + 1);
           for (int j = x.b0; j < j1; ++j) {
             window_for(j);
             __syncthreads();          // step j is whole; the buffer after it is consumed
@@ -401,12 +401,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
       } else {
         if constexpr (C::ROLES && FP4) {
           Raw raw0, raw1;  // the steps after the one that is written next, in turn
-          if (x.b0 < j1) {
-            load_raw(raw0, x.b0);
-            load_raw(raw1, x.b0 + 1);
-            store_raw(raw0, 0);
-            load_raw(raw0, x.b0 + 2);
-          }
+          load_raw(raw0, x.b0);  // (where there is no step: zeros)
+          load_raw(raw1, x.b0 + 1);
+          store_raw(raw0, 0);
+          load_raw(raw0, x.b0 + 2);
           for (int j = x.b0; j < j1; j += 2) {
             window_for(j);
             __syncthreads();        // step j is whole, the other buffer consumed
