@@ -273,12 +273,23 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
   constexpr int KS = DK / 16, VS = DV / 16, NDK = DK / 32, NDV = DV / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
-  // item -> (batch and group, row split, key block): the splits from the last (the causal mask's with most key blocks),
-  // each with the key blocks that its rows reach; consecutive items, which share rows, on one XCD
-  const int64_t item = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  const int64_t bg = item / p.items, b = bg / p.G, g = bg - b * p.G;
-  if (bg >= p.B * p.G) return;
-  int kblk = (int)(item - bg * p.items), split = p.nsplit - 1;
+  // Unsplit: by spread_items (windows leave key blocks that follow each other alike in length).  Else item -> (batch and
+  // group, row split, key block): the splits from the last (the causal mask's with most key blocks), each with the key
+  // blocks that its rows reach; consecutive items, which share rows, on one XCD.
+  int64_t bg, index;
+  int split = 0;
+  if (p.nsplit == 1) {
+    if ((int64_t)blockIdx.x >= p.B * p.G * p.items) return;
+    spread_items(blockIdx.x, p.B * p.G, p.items, bg, index);
+  } else {
+    const int64_t item = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    bg = item / p.items;
+    index = item - bg * p.items;
+    if (bg >= p.B * p.G) return;
+    split = p.nsplit - 1;
+  }
+  const int64_t b = bg / p.G, g = bg - b * p.G;
+  int kblk = (int)index;
   for (int n = split_blocks(p, split, C::KEYS); kblk >= n; n = split_blocks(p, split, C::KEYS)) {
     kblk -= n;
     --split;
@@ -580,11 +591,33 @@ __global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentPara
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= n_own + n_pe) return;
   f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-  auto add = [&](int64_t bg, int64_t key, int col) {
+  // groups bg .. bg + n - 1, each with its splits: the flags of four terms are read together, then what they say is there
+  auto add = [&](int64_t bg, int64_t n, int64_t key, int col) {
+    constexpr int kTerms = 4;
     const int kb = (int)((uint32_t)key / (uint32_t)r.keys);
-    for (int s = 0; s < p.nsplit; ++s) {
-      if (p.nsplit > 1 && (kb >= split_blocks(p, s, r.keys) || p.used[(s * bgs + bg) * p.nkb + kb] == 0)) continue;
-      sum += *reinterpret_cast<const f32x4 *>(p.part + ((s * bgs + bg) * p.S_kv + key) * r.width + col);
+    int64_t gr = bg;
+    int s = 0;
+    for (int64_t i0 = 0; i0 < n * p.nsplit; i0 += kTerms) {
+      int64_t at[kTerms];  // row s * bgs + group of the partial sums
+      int there[kTerms];
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) {
+        const bool in = i0 + i < n * p.nsplit;
+        at[i] = in ? s * bgs + gr : bg;
+        there[i] = in && (p.nsplit == 1 || kb < split_blocks(p, s, r.keys)) ? (p.nsplit == 1 ? 1 : p.used[at[i] * p.nkb + kb]) : 0;
+        if (in && ++s == p.nsplit) {
+          s = 0;
+          ++gr;
+        }
+      }
+      f32x4 x[kTerms];
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) {
+        x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (there[i]) x[i] = *reinterpret_cast<const f32x4 *>(p.part + (at[i] * p.S_kv + key) * r.width + col);
+      }
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) sum += x[i];
     }
   };
   uint16_t *dst;
@@ -593,12 +626,12 @@ __global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentPara
     const int c = (int)(id - row * own) * 4;
     const int64_t b = bg / p.G, orow = (b * p.S_kv + key) * p.G + (bg - b * p.G);
     const bool is_k = c < r.dn;
-    add(bg, key, is_k ? c : c + r.dr);
+    add(bg, 1, key, is_k ? c : c + r.dr);
     dst = is_k ? p.dk + orow * r.dn + c : p.dv + orow * r.dvw + (c - r.dn);
   } else {
     const int64_t x = id - n_own, row = x / (r.dr / 4), b = row / p.S_kv, key = row - b * p.S_kv;
     const int c = (int)(x - row * (r.dr / 4)) * 4;
-    for (int64_t g = 0; g < p.G; ++g) add(b * p.G + g, key, (r.width == r.dr ? 0 : r.dn) + c);
+    add(b * p.G, p.G, key, (r.width == r.dr ? 0 : r.dn) + c);
     dst = p.dkpe + (b * p.S_kv + key) * r.dr + c;
   }
   *reinterpret_cast<i32x2 *>(dst) = i32x2{(int)pack_bf16x2(sum[0], sum[1]), (int)pack_bf16x2(sum[2], sum[3])};
