@@ -591,9 +591,9 @@ __global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentPara
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= n_own + n_pe) return;
   f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-  // groups bg .. bg + n - 1, each with its splits: the flags of four terms are read together, then what they say is there
+  // groups bg .. bg + n - 1, each with its splits: the flags of eight terms are read together, then what they say is there
   auto add = [&](int64_t bg, int64_t n, int64_t key, int col) {
-    constexpr int kTerms = 4;
+    constexpr int kTerms = 8;
     const int kb = (int)((uint32_t)key / (uint32_t)r.keys);
     int64_t gr = bg;
     int s = 0;

@@ -423,12 +423,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
 }
 
 // Workgroup (w, y): where the first of a unit's blocks that is not in the piece of the
-// workgroup that began it is in range w + 1, some rows of that unit, one a wave after the
-// other: its pieces brought to their largest maximum and added in order.
+// workgroup that began it is in range w + 1, some rows of that unit, a row to 64 lanes
+// (64 channels: to 16), one after the other: its pieces brought to their largest maximum
+// and added in order, read AHEAD at a time.
 template <int D_V>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p) {
-  constexpr int NCH = D_V / 4, CPL = (NCH + 63) / 64, AHEAD = 4;
-  const int lane = lane_id();
+  constexpr int NCH = D_V / 4, LANES = NCH < 64 ? NCH : 64, CPL = NCH / LANES, AT_ONCE = 256 / LANES, AHEAD = 4;
+  const int ln = lane_id() % LANES;
   const int units = uni(p.unit0[p.R]), total = uni(p.unit_at[units]), per = uni(range_blocks(p, total));
   const int64_t cut = ((int64_t)blockIdx.x + 1) * per;
   if (cut >= total) return;
@@ -439,14 +440,15 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
   const int nrows = min(uni(request_tokens(p, req)) * p.H - first, p.unit_rows);
   const int64_t row0 = (int64_t)uni(request_start(p, req)) * p.H + first;
   const int rows = p.unit_rows / (int)gridDim.y;
-  for (int ur = (int)blockIdx.y * rows + wave_id(); ur < min(((int)blockIdx.y + 1) * rows, nrows); ur += 4) {
+  for (int ur = (int)blockIdx.y * rows + (int)threadIdx.x / LANES; ur < min(((int)blockIdx.y + 1) * rows, nrows); ur += AT_ONCE) {
     const int64_t row = row0 + ur;
     // piece k's row of partial results: in the second place of the workgroup that began the unit, the first of the others
     auto at = [&](int k) { return (int64_t)((w0 + k) * 2 + (k == 0 ? 1 : 0)) * p.unit_rows + ur; };
     float m = kNegBig;
-    for (int k = lane; k < pieces; k += 64)
+    for (int k = ln; k < pieces; k += LANES)
       if (p.part_ml[at(k) * 2 + 1] != 0.0f) m = fmaxf(m, p.part_ml[at(k) * 2]);
-    m = __uint_as_float(wv::wave_reduce(__float_as_uint(m), wv::MaxF()));
+#pragma unroll
+    for (int x = LANES / 2; x >= 1; x /= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
     float l = 0.0f;
     f32x4 o[CPL];
 #pragma unroll
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
         lk[i] = k0 + i < pieces ? p.part_ml[r * 2 + 1] : 0.0f;
 #pragma unroll
         for (int c = 0; c < CPL; ++c)
-          if (lane + 64 * c < NCH) x[i][c] = *reinterpret_cast<const f32x4 *>(p.part_o + r * D_V + (lane + 64 * c) * 4);
+          x[i][c] = *reinterpret_cast<const f32x4 *>(p.part_o + r * D_V + (ln + LANES * c) * 4);
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
@@ -470,16 +472,15 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
         l += lk[i] * a;
 #pragma unroll
         for (int c = 0; c < CPL; ++c)
-          if (lane + 64 * c < NCH) o[c] += a * x[i][c];
+          o[c] += a * x[i][c];
       }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int c = 0; c < CPL; ++c)
-      if (lane + 64 * c < NCH)
-        *reinterpret_cast<i32x2 *>(p.out + row * D_V + (lane + 64 * c) * 4) =
-            i32x2{(int)pack_bf16x2(o[c][0] * inv, o[c][1] * inv), (int)pack_bf16x2(o[c][2] * inv, o[c][3] * inv)};
-    if (lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
+      *reinterpret_cast<i32x2 *>(p.out + row * D_V + (ln + LANES * c) * 4) =
+          i32x2{(int)pack_bf16x2(o[c][0] * inv, o[c][1] * inv), (int)pack_bf16x2(o[c][2] * inv, o[c][3] * inv)};
+    if (ln == 0) p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
   }
 }
 
@@ -531,6 +532,10 @@ static PagedSections paged_sections(int64_t T, int64_t R, int64_t W, int64_t blo
   s.part_o = s.part_ml + pieces * 8;
   s.total = s.part_o + pieces * (size_t)d_v * 4;
   return s;
+}
+bool paged_countable(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk) {
+  const PagedPlan k = paged_plan(T, R, W, block, H, d_qk);
+  return (T * H / k.unit_rows + R) * ((W * block + k.step_keys - 1) / k.step_keys) < (1ll << 31);
 }
 size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v) {
   return paged_sections(T, R, W, block, H, d_qk, d_v).total;

@@ -118,6 +118,8 @@ int paged_wide_keys(int tiles16);  // keys of a step
 int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
 int launch_paged_few(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
 
+// The blocks of all units can be numbered in 32 bits, whatever the lengths.
+bool paged_countable(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk);
 size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v);
 int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st);
 

@@ -65,27 +65,33 @@ extern "C" int dsa_latent_plan_step(const int32_t *context_lens, const int32_t *
                   (T == 0 || (slots && positions)) &&
                   (R == 0 || (context_lens && query_lens && block_table && block_table_out && kv_lens && context_lens_out && granted)),
               "%s: null pointer", who);
-  DSA_REQUIRE(block_table_out != block_table && free_blocks_out != free_blocks && free_count_out != free_count &&
-                  context_lens_out != context_lens,
-              "%s: an output is an input (the workgroups read the inputs while others write)", who);
+  const void *ins[] = {context_lens, query_lens, block_table, free_blocks, free_count};
+  const void *outs[] = {block_table_out, slots, positions, query_starts, kv_lens, context_lens_out, granted, free_blocks_out,
+                        free_count_out};
+  for (const void *in : ins)
+    for (const void *out : outs)
+      DSA_REQUIRE(in == nullptr || in != out, "%s: an output is an input (the workgroups read the inputs while others write)", who);
   PlanParams p{context_lens, query_lens, block_table, free_blocks, free_count, slots, positions, query_starts, kv_lens,
                context_lens_out, granted, block_table_out, free_blocks_out, free_count_out, T, (int)R, (int)W, (int)F,
                (int)block_size, 0};
   return launch_latent_plan(p, (hipStream_t)stream);
 }
 
-static int check_paged(const char *who, int64_t T, int64_t R, int64_t W, int64_t block, int64_t H) {
+static int check_paged(const char *who, int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk) {
   DSA_REQUIRE(T >= 0 && R >= 0 && W > 0 && H > 0, "%s: bad sizes T=%lld R=%lld W=%lld H=%lld", who, (long long)T, (long long)R,
               (long long)W, (long long)H);
-  DSA_REQUIRE(H <= 4096 && R < (1 << 20) && T < (1ll << 30) && T * H < (1ll << 31) - 256 && W * block < (1ll << 31) - 128,
-              "%s: sizes out of range (H <= 4096, R < 2^20, T * H and W * block_size below 2^31)", who);
+  DSA_REQUIRE(H <= 4096 && R < (1 << 20) && T < (1ll << 30) && T * H < (1ll << 31) - 1024 && W < (1ll << 31) &&
+                  W * block < (1ll << 31) - 1024,
+              "%s: sizes out of range (H <= 4096, R < 2^20, T * H and W * block_size below 2^31 - 1024)", who);
+  DSA_REQUIRE(T == 0 || R == 0 || paged_countable(T, R, W, block, H, d_qk),
+              "%s: sizes out of range (row groups times key blocks must stay below 2^31)", who);
   return DSA_OK;
 }
 
 extern "C" size_t dsa_paged_latent_mla_workspace_size(int64_t T, int64_t R, int64_t W, int64_t block_size, int64_t H, int64_t D_qk,
                                                       int64_t D_v) {
   const char *who = "dsa_paged_latent_mla_workspace_size";
-  if (check_cache(who, 1, block_size, D_qk, D_v, DSA_DTYPE_BF16) || check_paged(who, T, R, W, block_size, H)) return 0;
+  if (check_cache(who, 1, block_size, D_qk, D_v, DSA_DTYPE_BF16) || check_paged(who, T, R, W, block_size, H, D_qk)) return 0;
   return T == 0 || R == 0 ? 0 : paged_workspace(T, R, W, block_size, H, D_qk, D_v);
 }
 
@@ -95,7 +101,7 @@ extern "C" int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const 
                                         int64_t block_size, int dtype, float sm_scale, void *stream) {
   const char *who = "dsa_paged_latent_mla_fwd";
   int rc = check_cache(who, num_blocks, block_size, D_qk, D_v, dtype);
-  if (!rc) rc = check_paged(who, T, R, W, block_size, H);
+  if (!rc) rc = check_paged(who, T, R, W, block_size, H, D_qk);
   if (rc) return rc;
   DSA_REQUIRE(isfinite(sm_scale) && sm_scale > 0.0f, "%s: sm_scale must be positive and finite, got %g", who, (double)sm_scale);
   if (T == 0 || R == 0) return DSA_OK;

@@ -150,10 +150,12 @@ def plan_latent_step(context_lens, query_lens, block_table, free_blocks, free_co
     W, dev = block_table.shape[1], context_lens.device
     stream, here = launch_on(context_lens)
     with here:
-        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=dev)  # noqa: E731
-        p = LatentStepPlan(block_table=new(R, W), slots=torch.empty(num_tokens, dtype=torch.int64, device=dev),
-                           positions=new(num_tokens), query_starts=new(R + 1), kv_lens=new(R), context_lens=new(R),
-                           granted=new(R), free_blocks=new(F), free_count=new(1))
+        # one allocation for the int32 results: nine take half of the call's time on the host
+        table, positions, starts, kv_lens, lens, granted, free, count = torch.empty(
+            R * W + num_tokens + 4 * R + F + 2, dtype=torch.int32, device=dev).split((R * W, num_tokens, R + 1, R, R, R, F, 1))
+        p = LatentStepPlan(block_table=table.view(R, W), slots=torch.empty(num_tokens, dtype=torch.int64, device=dev),
+                           positions=positions, query_starts=starts, kv_lens=kv_lens, context_lens=lens, granted=granted,
+                           free_blocks=free, free_count=count)
         rc = _lib.load().dsa_latent_plan_step(*(t.data_ptr() for t in ins.values()), *(t.data_ptr() for t in p), R, W, F,
                                               num_tokens, block_size, stream)
     _lib.check(rc, "dsa_latent_plan_step")
