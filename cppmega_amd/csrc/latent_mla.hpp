@@ -167,27 +167,29 @@ __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 // use(i, operand) for i in order.  The first group was loaded by the caller (while
 // something else ran); the barriers keep the compiler from sinking a load to its use.
 constexpr int kGroup = 4;
-struct Operands {
-  i32x4 x[kGroup];
+template <int G>
+struct OperandsOf {
+  i32x4 x[G];
 };
-template <int N, class Load>
-__device__ __forceinline__ void load_group(Operands &o, int g, Load load) {
+using Operands = OperandsOf<kGroup>;
+template <int N, int G, class Load>
+__device__ __forceinline__ void load_group(OperandsOf<G> &o, int g, Load load) {
 #pragma unroll
-  for (int i = 0; i < kGroup; ++i)
-    if (g * kGroup + i < N) o.x[i] = load(g * kGroup + i);
+  for (int i = 0; i < G; ++i)
+    if (g * G + i < N) o.x[i] = load(g * G + i);
 }
-template <int N, class Load, class Use>
-__device__ __forceinline__ void stream_operands(const Operands &first, Load load, Use use) {
-  constexpr int NG = (N + kGroup - 1) / kGroup;
-  Operands cur = first;
+template <int N, int G, class Load, class Use>
+__device__ __forceinline__ void stream_operands(const OperandsOf<G> &first, Load load, Use use) {
+  constexpr int NG = (N + G - 1) / G;
+  OperandsOf<G> cur = first;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    Operands nxt;
+    OperandsOf<G> nxt;
     if (g + 1 < NG) load_group<N>(nxt, g + 1, load);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i)
-      if (g * kGroup + i < N) use(g * kGroup + i, cur.x[i]);
+    for (int i = 0; i < G; ++i)
+      if (g * G + i < N) use(g * G + i, cur.x[i]);
     __builtin_amdgcn_sched_barrier(0);
     if (g + 1 < NG) cur = nxt;
   }

@@ -497,7 +497,7 @@ static PagedPlan paged_plan(int64_t T, int64_t R, int64_t W, int64_t block, int6
   if (d_qk == 576) {
     r.wide = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 8));
     r.unit_rows = 16 * r.wide;
-    r.step_keys = paged_wide_keys(r.wide);
+    r.step_keys = paged_wide_keys();
   } else if (rows <= 32) {
     r.few = rows <= 16 ? 1 : 2;
     r.unit_rows = 16 * r.few;

@@ -114,7 +114,7 @@ constexpr int kWindow = 1024;  // table entries of a request that a workgroup ha
 // vmcnt(n) alone
 constexpr int vmcnt_only(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
 
-int paged_wide_keys(int tiles16);  // keys of a step
+int paged_wide_keys();  // keys of a step
 int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
 int launch_paged_few(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
 

@@ -31,19 +31,19 @@ struct PagedWide {
   static constexpr bool ROLES = RG < 8;                      // waves 4..7 bring the rows
   static constexpr int CW = ROLES ? 4 : 8, LW = ROLES ? 4 : 8, KG = CW / RG;  // computing, loading waves
   static constexpr int TK = RG == 1 ? 16 : 32;               // keys of a tile
-  static constexpr int SUB = RG == 4 ? 2 : 1;                // tiles of a computing wave
+  static constexpr int SUB = RG >= 4 ? 2 : 1;                // tiles of a computing wave
   static constexpr int KEYS = KG * SUB * TK;                 // of a step
   static constexpr int PANELS = 9, PANEL = TK * 128, TILE = PANELS * PANEL, STEP = KG * SUB * TILE;
-  static constexpr int NBUF = 4 * 36864 / STEP;
+  static constexpr int GROUP = 3;                            // operands read at once (4: registers spill)
   static constexpr int KS = 18, NDT = 32;
   static constexpr int LT = 64 * LW;                         // loading threads
   static constexpr int TPR = LT / KEYS, CPT = 16 / TPR, RPT = (8 + TPR - 1) / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
   static constexpr int RAW = ROLES ? 2 : 1;                  // steps in a loading wave's registers
-  static constexpr int OFF_T = NBUF * STEP;
+  static constexpr int OFF_T = 2 * STEP;
   static constexpr int OFF_ML = OFF_T + kWindow * 4;         // [2][16][2]
   static constexpr int BYTES = OFF_ML + 2 * 16 * 8;
   static constexpr int O_BYTES = 512 * 16 * 4;
-  static_assert((TPR == 4 || TPR == 16) && NBUF == (ROLES ? 2 : 4) && OFF_T == 147456 && BYTES <= 159 * 1024, "LDS");
+  static_assert((TPR == 4 || TPR == 8) && KEYS == 64 && OFF_T == 147456 && BYTES <= 159 * 1024, "LDS");
 };
 
 // Chunk c (16 bytes, 0..7) of row r of a panel at r * 128 + ((c ^ swizzle) * 16).  32-row tiles: row_swz.  16-row tiles:
@@ -62,7 +62,6 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
   using C = PagedWide<RG, FP4>;
   using Row = typename C::Row;
   constexpr int TK = C::TK, H = TK / 16, KS = C::KS, NDT = C::NDT;
-  static_assert(C::KEYS == (RG == 8 ? 32 : 64), "keys of a step");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int w = wave_id();
   const int rg = w % RG, kg = C::ROLES ? (w & 3) / RG : 0;
@@ -120,23 +119,16 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
         const int64_t slot = (int64_t)e * p.block + (key - pg * p.block);
         return e >= 0 ? p.cache + slot * Row::BYTES : zero;
       };
-      // bf16: a step's 8-row groups: whole groups, or, where there are more waves than groups, parts of their panels
-      auto group = [&](int j, int buf, int grp, auto p0, auto p1) {
-        const int ln = lane_here(), r = 8 * grp + (ln >> 3);
-        const unsigned char *src = key_at(j * C::KEYS + r) + ((ln & 7) ^ wide_swz<TK>(r % TK)) * 16;
-#pragma unroll
-        for (int pn = decltype(p0)::value; pn < decltype(p1)::value; ++pn)
-          dma_16_at(lds0 + (uint32_t)(buf * C::STEP + (8 * grp / TK) * C::TILE + pn * C::PANEL + (8 * grp % TK) * 128), src + pn * 128);
-      };
+      // bf16: a step's eight 8-row groups
       auto fetch = [&](int j, int buf) {
-        using Zero = std::integral_constant<int, 0>;
-        using Mid = std::integral_constant<int, 5>;
-        using All = std::integral_constant<int, 9>;
-        if constexpr (C::ROLES) {
+        const int ln = lane_here();
 #pragma unroll
-          for (int i = 0; i < 2; ++i) group(j, buf, lw + 4 * i, Zero{}, All{});
-        } else {
-          if (w < 4) group(j, buf, w, Zero{}, Mid{}); else group(j, buf, w - 4, Mid{}, All{});
+        for (int grp = lw; grp < 8; grp += C::LW) {
+          const int r = 8 * grp + (ln >> 3);
+          const unsigned char *src = key_at(j * C::KEYS + r) + ((ln & 7) ^ wide_swz<TK>(r % TK)) * 16;
+#pragma unroll
+          for (int pn = 0; pn < C::PANELS; ++pn)
+            dma_16_at(lds0 + (uint32_t)(buf * C::STEP + (8 * grp / TK) * C::TILE + pn * C::PANEL + (8 * grp % TK) * 128), src + pn * 128);
         }
       };
       // MXFP4: TPR neighbouring threads have a row: every TPR-th piece of codes (16 bytes, a 32-channel block) and rope
@@ -159,8 +151,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
         for (int i = 0; i < C::CPT; ++i) {
           const int blk = i * C::TPR + part;
-          // byte blk of the exponents: dword i of four threads' rows, else dword part / 4
-          const uint32_t four = (uint32_t)(C::TPR == 4 ? raw.expo[i] : (part < 8 ? (part < 4 ? raw.expo[0] : raw.expo[1]) : (part < 12 ? raw.expo[2] : raw.expo[3])));
+          const uint32_t four = (uint32_t)(C::TPR == 4 || part < 4 ? raw.expo[C::TPR * i / 4] : raw.expo[C::TPR * i / 4 + C::TPR / 8]);
           const uint32_t e = (four >> (8 * (part & 3))) & 255u;
           const float sc = e8m0_scale(e);
           i32x4 v[4];
@@ -178,12 +169,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
         }
 #pragma unroll
         for (int i = 0; i < C::RPT; ++i)
-          if (C::TPR == 4 || part < 8)
-            *reinterpret_cast<i32x4 *>(tile + 8 * C::PANEL + wide_byte<TK>(key_of % TK, (i * C::TPR + part) & 7)) = raw.rope[i];
+          *reinterpret_cast<i32x4 *>(tile + 8 * C::PANEL + wide_byte<TK>(key_of % TK, (i * C::TPR + part) & 7)) = raw.rope[i];
       };
 
       // steps that are asked for before they are worked on, and their pages in the window
-      constexpr int kAsked = FP4 ? 1 + C::RAW : C::NBUF - 1;
+      constexpr int kAsked = FP4 ? 1 + C::RAW : 1;
       auto window_for = [&](int j) {
         if (page_of((j + kAsked + 1) * C::KEYS - 1) >= base + kWindow && page_of(lim - 1) >= base + kWindow) refill(page_of(j * C::KEYS));
       };
@@ -230,11 +220,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           f32x4 s[H];
 #pragma unroll
           for (int h = 0; h < H; ++h) s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          Operands a0;
+          OperandsOf<C::GROUP> a0;
           load_group<KS * H>(a0, 0, rows);
           stream_operands<KS * H>(a0, rows, [&](int i, i32x4 a) {
             s[i % H] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(q[i / H]), s[i % H], 0, 0, 0);
-            if (i % kGroup >= kGroup - H) asm volatile("" : "+v"(s[i % H]));  // here, not where the sum is needed
+            if (i % C::GROUP >= C::GROUP - H || i >= (KS - 1) * H) asm volatile("" : "+v"(s[i % H]));  // here, not where the sum is needed
           });
 #pragma unroll
           for (int h = 0; h < H; ++h) {
@@ -310,24 +300,20 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           for (int j = x.b0; j < j1; ++j) {
             window_for(j);
             __syncthreads();          // step j is whole; the buffer after it is consumed
-            const int nxt = buf + 1 == C::NBUF ? 0 : buf + 1;
-            store_raw(raw, nxt);      // step j + 1
+            store_raw(raw, buf ^ 1);  // step j + 1
             load_raw(raw, j + 2);
             compute(j, buf);
-            buf = nxt;
+            buf ^= 1;
           }
         } else {
-#pragma unroll
-          for (int i = 0; i < C::NBUF - 1; ++i)
-            if (x.b0 < j1) fetch(x.b0 + i, i);
+          if (x.b0 < j1) fetch(x.b0, 0);
           for (int j = x.b0; j < j1; ++j) {
             window_for(j);
-            // this wave's share of step j has landed: NBUF - 2 later steps' may be on their way
-            if (w < 4) __builtin_amdgcn_s_waitcnt(vmcnt_only((C::NBUF - 2) * 5)); else __builtin_amdgcn_s_waitcnt(vmcnt_only((C::NBUF - 2) * 4));
-            __syncthreads();
-            fetch(j + C::NBUF - 1, buf == 0 ? C::NBUF - 1 : buf - 1);  // (past the last step: zeros)
+            __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+            __syncthreads();      // step j is whole, the other buffer consumed
+            fetch(j + 1, buf ^ 1);  // (past the last step: zeros)
             compute(j, buf);
-            buf = buf + 1 == C::NBUF ? 0 : buf + 1;
+            buf ^= 1;
           }
           __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // what was fetched past the last step has landed
         }
@@ -457,7 +443,7 @@ static int launch(const PagedParams &p, hipStream_t st) {
   return check_launch("dsa_paged_latent_mla_fwd");
 }
 
-int paged_wide_keys(int tiles16) { return tiles16 == 8 ? PagedWide<8, false>::KEYS : PagedWide<4, false>::KEYS; }
+int paged_wide_keys() { return PagedWide<8, false>::KEYS; }
 int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st) {
   if (tiles16 == 8) return fp4 ? launch<8, true>(p, st) : launch<8, false>(p, st);
   if (tiles16 == 4) return fp4 ? launch<4, true>(p, st) : launch<4, false>(p, st);
