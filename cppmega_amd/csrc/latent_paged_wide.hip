@@ -34,7 +34,7 @@ struct PagedWide {
   static constexpr int SUB = RG >= 4 ? 2 : 1;                // tiles of a computing wave
   static constexpr int KEYS = KG * SUB * TK;                 // of a step
   static constexpr int PANELS = 9, PANEL = TK * 128, TILE = PANELS * PANEL, STEP = KG * SUB * TILE;
-  static constexpr int GROUP = 3;                            // operands read at once (4: registers spill)
+  static constexpr int GROUP = 2;                            // operands read at once (3, 4: registers spill)
   static constexpr int KS = 18, NDT = 32;
   static constexpr int LT = 64 * LW;                         // loading threads
   static constexpr int TPR = LT / KEYS, CPT = 16 / TPR, RPT = (8 + TPR - 1) / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
