@@ -1,20 +1,17 @@
 // Latent attention over a paged cache on gfx950 (absorbed form, bf16 or MXFP4 rows):
 // decoding, speculative tokens and prefill chunks of ragged requests.
 //
-// A request's rows are its (new token, head) pairs in that order; a unit is NT * 32 of
-// them with the keys 0 .. of its last token.  The units' 32-key blocks, one after the
+// A request's rows are its (new token, head) pairs in that order; a unit is up to 128 of
+// them with the keys 0 .. of its last token.  The units' blocks of keys, one after the
 // other, are split evenly over the grid's workgroups (stream-wise, so a long request is
 // shared and short ones are packed), whose ends may fall inside a unit: such a piece
 // leaves its unnormalised fp32 O, maximum and sum, and paged_combine_kernel adds a unit's
 // pieces in order.  The plan (units and their first blocks) is made on the device from
 // the lengths: the host knows neither.
 //
-// A block's products follow the wide SparseMLA forward: S^T partial sums over parts of
-// the channels meet through LDS, the softmax of block j runs beside the PV products of
-// block j - 1 (two barriers a block), and block j + 1's rows arrive by LDS-DMA loads from
-// 64-bit addresses that the block table gives (MXFP4: as codes in registers, written to
-// the tile as exact bf16 values).  Keys past a request's last, and keys whose table entry
-// is no page, read as zeros and have no weight.
+// Three kernels take the units: latent_paged_wide.hip rows of 576 channels,
+// latent_paged_few.hip few rows of 128, paged_rows_kernel below many.  Keys past a
+// request's last, and keys whose table entry is no page, read as zeros and have no weight.
 #include "latent_mla.hpp"
 #include "latent_paged.hpp"
 
@@ -83,31 +80,35 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   if (threadIdx.x == 0) p.unit_at[units] = at;
 }
 
-template <int D_QK, int D_V, int NT, int SUB, int NBUF_, bool FP4>
+// Many rows of 128 channels: four waves, NT of them 32 rows each, by 4 / NT key groups; steps of 64 keys, two ahead of
+// the one that is worked on, shared by the waves in three LDS buffers, one barrier a step; three workgroups a CU.
+//   S^T = K Q^T, O^T += V^T P^T on 32x32x16 MFMAs, lane = row.
+// Bound by the MFMAs and the softmax beside them (prefill of 6 requests, 240 tokens each on 1024 .. 4096 keys, 32 heads,
+// MXFP4: 115 us, 310 TFLOP/s; the conversion of the codes, once a unit of 128 rows, is a quarter of it).
+template <int NT, bool FP4>
 struct Paged {
+  static constexpr int D_QK = 128, D_V = 64;
   using Row = CacheRow<D_QK, D_V, FP4>;
   static constexpr int NW = 4, KG = NW / NT, ROWS = 32 * NT;  // waves: NT row tiles x KG key groups
-  static constexpr int TILES = KG * SUB, KEYS = 32 * TILES;   // 32-key tiles and keys of a step
-  static constexpr int NBUF = NT == 1 ? 1 : NBUF_;            // steps in LDS; one row tile: a wave's tile is its own
-  static constexpr int AHEAD = NBUF - 1;                      // steps that are fetched ahead
+  static constexpr int TILES = 2, SUB = TILES / KG, KEYS = 32 * TILES;  // 32-key tiles of a step, of a wave; keys of a step
+  static constexpr int NBUF = 3, AHEAD = NBUF - 1;            // steps in LDS, fetched ahead
   static constexpr int KS = D_QK / 16, NDT = D_V / 32;
   static constexpr int PANELS = D_QK / 64, TILE = PANELS * 4096, STEP = TILES * TILE;
-  static constexpr int DMA = TILES * (FP4 ? PANELS - D_V / 64 : PANELS);  // loads of a wave per step (an 8-row group a tile)
-  static constexpr int NB = D_V / 32, CODES = TILES * 32 * NB;            // code pieces of a row, of a step
-  static constexpr int CPT = (CODES + 255) / 256;                         // per thread and step
+  static constexpr int DMA = TILES * PANELS;                  // bf16: loads of a wave per step (an 8-row group a tile)
+  static constexpr int NB = D_V / 32, CODES = KEYS * NB;      // MXFP4: code pieces of a row, of a step (one to a thread)
   static constexpr int OFF_T = NBUF * STEP;
   static constexpr int OFF_ML = OFF_T + kWindow * 4;          // [NW][32][2]
   static constexpr int BYTES = OFF_ML + NW * 32 * 8;
   static constexpr int O_BYTES = D_V * 32 * 4;                // a wave's O
-  static_assert(BYTES <= 159 * 1024 && (KG == 1 || (NW / 2) * O_BYTES <= OFF_T), "LDS");
-  static_assert(!FP4 || CODES % 256 == 0 || (CPT == 1 && CODES % 64 == 0 && NT > 1), "code pieces by whole waves");
+  static_assert(BYTES <= 64 * 1024 && (KG == 1 || (NW / 2) * O_BYTES <= OFF_T), "LDS");
+  static_assert(CODES % 64 == 0 && CODES <= 256, "code pieces by whole waves");
 };
 
-template <int D_QK, int D_V, int NT, int SUB, int NBUF, bool FP4, int OCC>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC))) paged_rows_kernel(const PagedParams p) {
-  using C = Paged<D_QK, D_V, NT, SUB, NBUF, FP4>;
+template <int NT, bool FP4>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) paged_rows_kernel(const PagedParams p) {
+  using C = Paged<NT, FP4>;
   using Row = typename C::Row;
-  constexpr int KS = C::KS, NDT = C::NDT;
+  constexpr int D_QK = C::D_QK, D_V = C::D_V, KS = C::KS, NDT = C::NDT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const int rt = w % NT, kg = w / NT;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
         constexpr int P0 = FP4 ? D_V / 64 : 0;
 #pragma unroll
         for (int i = 0; i < C::TILES; ++i) {
-          const int grp = NT == 1 ? 4 * w + i : w + 4 * i, r = 8 * (grp & 3) + (lane >> 3);
+          const int grp = w + 4 * i, r = 8 * (grp & 3) + (lane >> 3);
           const unsigned char *src = key_at(j * C::KEYS + 8 * grp + (lane >> 3)) + (FP4 ? Row::OFF_ROPE : 0) +
                                      ((((lane & 7) ^ row_swz(r)) * 16) ^ panel_swz(P0));
 #pragma unroll
@@ -192,43 +193,25 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
             dma_16_at(lds0 + (uint32_t)(buf * C::STEP + (grp >> 2) * C::TILE + pn * 4096 + (grp & 3) * 1024), src + (pn - P0) * 128);
         }
       };
-      // MXFP4: code pieces of a step, a row's from neighbouring threads (one row tile: of the wave's own tile)
-      i32x4 codes[FP4 ? C::CPT : 1];
-      uint32_t expo[FP4 ? C::CPT : 1];
-      auto piece_at = [&](int i, int &key, int &blk) {
-        const int y = NT == 1 ? w * 64 * C::CPT + i * 64 + lane : i * 256 + w * 64 + lane;
-        key = y / C::NB;
-        blk = y % C::NB;
-      };
+      // MXFP4: code pieces of a step, a row's from neighbouring threads
+      i32x4 codes{0, 0, 0, 0};
+      uint32_t expo = 0;
+      const int my_key = (int)threadIdx.x / C::NB, my_blk = (int)threadIdx.x % C::NB;
       auto load_codes = [&](int j) {
-        if constexpr (FP4) {
-#pragma unroll
-          for (int i = 0; i < C::CPT; ++i) {
-            if (C::CODES % 256 != 0 && w * 64 >= C::CODES) continue;  // wave-uniform
-            int key, blk;
-            piece_at(i, key, blk);
-            const unsigned char *src = key_at(j * C::KEYS + key);
-            codes[i] = ld_global_16(src + blk * 16);
-            expo[i] = src[Row::OFF_EXP + blk];
-          }
-        }
+        if (w * 64 >= C::CODES) return;  // wave-uniform
+        const unsigned char *src = key_at(j * C::KEYS + my_key);
+        codes = ld_global_16(src + my_blk * 16);
+        expo = src[Row::OFF_EXP + my_blk];
       };
       auto store_codes = [&](int buf) {
-        if constexpr (FP4) {
+        if (w * 64 >= C::CODES) return;
+        const float sc = e8m0_scale(expo);
+        unsigned char *dst = smem + buf * C::STEP + (my_key >> 5) * C::TILE + (my_blk >> 1) * 4096;
 #pragma unroll
-          for (int i = 0; i < C::CPT; ++i) {
-            if (C::CODES % 256 != 0 && w * 64 >= C::CODES) continue;
-            int key, blk;
-            piece_at(i, key, blk);
-            const float sc = e8m0_scale(expo[i]);
-            unsigned char *dst = smem + buf * C::STEP + (key >> 5) * C::TILE + (blk >> 1) * 4096;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              i32x4 v = e2m1x8_to_bf16((uint32_t)codes[i][c], sc);
-              if (expo[i] == 255u) v = i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
-              *reinterpret_cast<i32x4 *>(dst + (tile_byte(key & 31, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v;
-            }
-          }
+        for (int c = 0; c < 4; ++c) {
+          i32x4 v = e2m1x8_to_bf16((uint32_t)codes[c], sc);
+          if (expo == 255u) v = i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
+          *reinterpret_cast<i32x4 *>(dst + (tile_byte(my_key & 31, 4 * (my_blk & 1) + c) ^ panel_swz(my_blk >> 1))) = v;
         }
       };
 
@@ -291,7 +274,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
           fetch(x.b0, 0);
           store_codes(0);
           load_codes(x.b0 + 1);
-        } else if constexpr (NT > 1) {
+        } else {
 #pragma unroll
           for (int i = 0; i < C::AHEAD; ++i) fetch(x.b0 + i, i);
         }
@@ -301,22 +284,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
         // what is asked for in this step lies in the window, and what is masked in it
         if (page_of((j + C::AHEAD + 2) * C::KEYS - 1) >= base + kWindow && page_of(lim - 1) >= base + kWindow) refill(page_of(j * C::KEYS));
         const unsigned char *S = smem + buf * C::STEP;
-        int nxt = buf + 1 == C::NBUF ? 0 : buf + 1;
-        if constexpr (NT == 1) {
-          if constexpr (FP4) {
-            if (j > x.b0) {
-              wave_lds_sync();
-              fetch(j, 0);
-              store_codes(0);
-              load_codes(j + 1);
-            }
-            __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-          } else {
-            fetch(j, 0);
-            __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-          }
-          wave_lds_sync();
-        } else if constexpr (FP4) {
+        const int nxt = buf + 1 == C::NBUF ? 0 : buf + 1;
+        if constexpr (FP4) {
           __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
           __syncthreads();          // step j is whole; the step before it is consumed
           store_codes(nxt);         // step j + 1
@@ -328,11 +297,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC)))
           fetch(j + C::AHEAD, buf == 0 ? C::NBUF - 1 : buf - 1);           // (past the last step: zeros)
         }
 #pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) {
-          const int tl = kg * SUB + sub, key0 = j * C::KEYS + tl * 32;
+        for (int sub = 0; sub < C::SUB; ++sub) {
+          const int tl = kg * C::SUB + sub, key0 = j * C::KEYS + tl * 32;
           if (key0 < lim) tile_step(S + tl * C::TILE, key0);
         }
-        if constexpr (NT == 1) wave_lds_sync();  // the tile is read: it may be written again
         buf = nxt;
       }
       __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // what was fetched past the last step has landed
@@ -484,26 +452,37 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
   }
 }
 
-// How a call is run, from its sizes alone.  Rows that share keys: a request's (token, head) pairs, on average.
+// How a call is run, from its sizes alone: by the rows that share keys, a request's (token, head) pairs on average.
+// Times of a step of 64 requests, 301 .. 16384 keys, us, the chosen one's first:
+//   576, bf16   up to 64 rows    units of 64: 16 heads 144, 64 heads 160; of 128: 193, 197
+//               more             units of 128: 128 heads 223; of 64: 265
+//   576, MXFP4  up to 32 rows    units of 32: 16 heads 107, 32 heads 110; of 64: 148, 153; of 16: 104, 165
+//               more             units of 64: 64 heads 165, 128 heads 282; of 128 (all waves fetch and compute): 280, 316
+//   128, bf16   up to 16 rows    waves that split the keys, 16 rows: 16 heads 41; 32: 51; units of 64: 58
+//               up to 32         32 rows: 32 heads 56; 16: 59; units of 64: 60
+//               up to 64         units of 64: 64 heads 63; of 128: 71; 16 rows: 97
+//               more             units of 128: 128 heads 78; of 64: 87
+//   128, MXFP4  up to 64 rows    16 rows: 16 heads 38, 64 heads 79; units of 64: 77, 84; of 128: 84, 91
+//               more             units of 128: 128 heads 96; of 64: 120; 16 rows: 133
 struct PagedPlan {
   int wide;       // 576 / 512: 16-row tiles of a unit
   int few;        // 128 / 64: 16-row tiles of a unit whose waves split the keys
   int nt;         // 128 / 64: else 32-row tiles of a unit
   int unit_rows, step_keys, max_units, nwg, min_blocks;
 };
-static PagedPlan paged_plan(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk) {
+static PagedPlan paged_plan(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, bool fp4) {
   PagedPlan r{};
   const int64_t rows = (T + R - 1) / R * H;
   if (d_qk == 576) {
-    r.wide = rows <= 16 ? 1 : (rows <= 32 ? 2 : (rows <= 64 ? 4 : 8));
+    r.wide = fp4 ? (rows <= 32 ? 2 : 4) : (rows <= 64 ? 4 : 8);
     r.unit_rows = 16 * r.wide;
     r.step_keys = paged_wide_keys();
-  } else if (rows <= 32) {
-    r.few = rows <= 16 ? 1 : 2;
+  } else if (rows <= (fp4 ? 64 : 32)) {
+    r.few = fp4 || rows <= 16 ? 1 : 2;
     r.unit_rows = 16 * r.few;
     r.step_keys = 32;
   } else {
-    r.nt = rows > 64 ? 4 : 2;
+    r.nt = fp4 || rows > 64 ? 4 : 2;
     r.unit_rows = 32 * r.nt;
     r.step_keys = 64;
   }
@@ -520,8 +499,8 @@ static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 struct PagedSections {
   size_t unit0, unit_req, unit_first, unit_at, part_ml, part_o, total;
 };
-static PagedSections paged_sections(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v) {
-  const PagedPlan k = paged_plan(T, R, W, block, H, d_qk);
+static PagedSections paged_sections(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v, bool fp4) {
+  const PagedPlan k = paged_plan(T, R, W, block, H, d_qk, fp4);
   const size_t units = (size_t)k.max_units, pieces = (size_t)k.nwg * 2 * (size_t)k.unit_rows;
   PagedSections s;
   s.unit0 = 0;
@@ -534,26 +513,29 @@ static PagedSections paged_sections(int64_t T, int64_t R, int64_t W, int64_t blo
   return s;
 }
 bool paged_countable(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk) {
-  const PagedPlan k = paged_plan(T, R, W, block, H, d_qk);
-  return (T * H / k.unit_rows + R) * ((W * block + k.step_keys - 1) / k.step_keys) < (1ll << 31);
+  bool ok = true;
+  for (int fp4 = 0; fp4 < 2; ++fp4) {
+    const PagedPlan k = paged_plan(T, R, W, block, H, d_qk, fp4 != 0);
+    ok = ok && (T * H / k.unit_rows + R) * ((W * block + k.step_keys - 1) / k.step_keys) < (1ll << 31);
+  }
+  return ok;
 }
 size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v) {
-  return paged_sections(T, R, W, block, H, d_qk, d_v).total;
+  // the larger of the two formats': the query does not know it
+  const size_t a = paged_sections(T, R, W, block, H, d_qk, d_v, false).total, b = paged_sections(T, R, W, block, H, d_qk, d_v, true).total;
+  return a > b ? a : b;
 }
 
-template <int D_QK, int D_V, int NT, int SUB, int NBUF, bool FP4, int OCC>
+template <int NT, bool FP4>
 static int launch(const PagedParams &p, hipStream_t st) {
-  using C = Paged<D_QK, D_V, NT, SUB, NBUF, FP4>;
-  const auto kernel = paged_rows_kernel<D_QK, D_V, NT, SUB, NBUF, FP4, OCC>;
-  const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
-  if (e != hipSuccess) return set_error(DSA_ERR_HIP, "dsa_paged_latent_mla_fwd: LDS attribute: %s", hipGetErrorString(e));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)p.nwg), dim3(256), C::BYTES, st, p);
+  using C = Paged<NT, FP4>;
+  hipLaunchKernelGGL((paged_rows_kernel<NT, FP4>), dim3((unsigned)p.nwg), dim3(256), C::BYTES, st, p);
   return check_launch("dsa_paged_latent_mla_fwd");
 }
 
 int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st) {
-  const PagedSections s = paged_sections(p.T, p.R, p.W, p.block, p.H, d_qk, d_v);
-  const PagedPlan k = paged_plan(p.T, p.R, p.W, p.block, p.H, d_qk);
+  const PagedSections s = paged_sections(p.T, p.R, p.W, p.block, p.H, d_qk, d_v, fp4);
+  const PagedPlan k = paged_plan(p.T, p.R, p.W, p.block, p.H, d_qk, fp4);
   p.unit_rows = k.unit_rows;
   p.max_units = k.max_units;
   p.nwg = k.nwg;
@@ -570,8 +552,8 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
   if (rc) return rc;
   if (k.wide) rc = launch_paged_wide(p, k.wide, fp4, st);
   else if (k.few) rc = launch_paged_few(p, k.few, fp4, st);
-  else if (k.nt == 4) rc = fp4 ? launch<128, 64, 4, 2, 3, true, 3>(p, st) : launch<128, 64, 4, 2, 3, false, 3>(p, st);
-  else rc = fp4 ? launch<128, 64, 2, 1, 3, true, 3>(p, st) : launch<128, 64, 2, 1, 3, false, 3>(p, st);
+  else if (k.nt == 4) rc = fp4 ? launch<4, true>(p, st) : launch<4, false>(p, st);
+  else rc = launch<2, false>(p, st);
   if (rc || p.nwg == 1) return rc;  // one workgroup: no unit has several pieces
   const dim3 grid((unsigned)(p.nwg - 1), (unsigned)(p.unit_rows / (p.unit_rows < 64 ? 4 : 16)));
   if (d_v == 512) hipLaunchKernelGGL(paged_combine_kernel<512>, grid, dim3(256), 0, st, p);

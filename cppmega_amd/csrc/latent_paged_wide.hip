@@ -4,25 +4,26 @@
 //   S^T[key][row] = K Q^T    on 16x16x32 MFMAs (lane = row, its keys in the registers)
 //   running maximum and sum per lane (two exchanges a tile), P^T the operand as it stands
 //   O^T[d][row] += V^T P^T   (V^T by transposed LDS reads)
-// A wave reads a tile's K and V whole (70 KiB a 32-key tile): at 128 rows LDS reads and
-// MFMAs take the same 2176 cycles a tile; with fewer rows a step has KG tiles, a tile for
-// each group, and reading the cache is what bounds it.
-//   RG 8 (128 rows): all eight waves compute and fetch; steps of 32 keys, three ahead of
-//     the one that is worked on (bf16), one barrier a step;
-//   RG 4, 2, 1: four waves compute (RG row groups x KG = 4 / RG key groups; two 32-key
-//     tiles each, one, or one of 16 keys), the other four bring the rows: steps of 64
-//     keys, one ahead in LDS, one barrier a step.
-// bf16 rows come by LDS-DMA loads; MXFP4 rows (a third of the bytes) by registers, up to
-// two steps ahead, converted to exact bf16 values as they are written to LDS.  At a
+// Steps of 64 keys (two 32-key tiles), one ahead in LDS, one barrier a step:
+//   RG 8 (128 rows, bf16): all eight waves fetch and compute;
+//   RG 4, 2: four waves compute (RG row groups x KG = 4 / RG key groups), the other four
+//     bring the rows.
+// bf16 rows come by LDS-DMA loads; MXFP4 rows (a third of the bytes) by registers, two
+// more steps ahead, converted to exact bf16 values as they are written to LDS.  At a
 // piece's end the key groups' O are brought to one maximum and added pairwise through LDS.
-#include <type_traits>
-
+//
+// What bounds it: with up to 64 rows (MXFP4: 32) the reading of the cache, at 144 us for
+// 64 requests of 301 .. 16384 keys, 630 MB (4.4 TB/s; MXFP4: 107 us for 219 MB, where the
+// conversion and its LDS writes come to it).  At 128 rows a wave reads every tile's K and
+// V whole (70 KiB), which is 2176 cycles of LDS reads and as many of MFMAs a tile, against
+// 135 us for the loads alone: 203 us.  Two steps ahead in flight made that 248 us, the
+// loads after the products 228.
 #include "latent_mla.hpp"
 #include "latent_paged.hpp"
 
 namespace dsa {
 
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
+constexpr int kWideKeys = 64;  // keys of a step
 
 template <int RG_, bool FP4>
 struct PagedWide {
@@ -30,38 +31,24 @@ struct PagedWide {
   static constexpr int RG = RG_, ROWS = 16 * RG;
   static constexpr bool ROLES = RG < 8;                      // waves 4..7 bring the rows
   static constexpr int CW = ROLES ? 4 : 8, LW = ROLES ? 4 : 8, KG = CW / RG;  // computing, loading waves
-  static constexpr int TK = RG == 1 ? 16 : 32;               // keys of a tile
-  static constexpr int SUB = RG >= 4 ? 2 : 1;                // tiles of a computing wave
-  static constexpr int KEYS = KG * SUB * TK;                 // of a step
-  static constexpr int PANELS = 9, PANEL = TK * 128, TILE = PANELS * PANEL, STEP = KG * SUB * TILE;
+  static constexpr int SUB = 2 / KG;                         // tiles of a computing wave
+  static constexpr int PANELS = 9, TILE = PANELS * 4096, STEP = 2 * TILE;
   static constexpr int GROUP = 2;                            // operands read at once (3, 4: registers spill)
   static constexpr int KS = 18, NDT = 32;
-  static constexpr int LT = 64 * LW;                         // loading threads
-  static constexpr int TPR = LT / KEYS, CPT = 16 / TPR, RPT = (8 + TPR - 1) / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
-  static constexpr int RAW = ROLES ? 2 : 1;                  // steps in a loading wave's registers
+  static constexpr int TPR = 4, CPT = 16 / TPR, RPT = 8 / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
   static constexpr int OFF_T = 2 * STEP;
   static constexpr int OFF_ML = OFF_T + kWindow * 4;         // [2][16][2]
   static constexpr int BYTES = OFF_ML + 2 * 16 * 8;
   static constexpr int O_BYTES = 512 * 16 * 4;
-  static_assert((TPR == 4 || TPR == 8) && KEYS == 64 && OFF_T == 147456 && BYTES <= 159 * 1024, "LDS");
+  static_assert(BYTES <= 159 * 1024 && (KG == 1 || RG * O_BYTES <= OFF_T), "LDS");
+  static_assert(!FP4 || (ROLES && 64 * LW == kWideKeys * TPR), "MXFP4 rows: by the loading waves");
 };
-
-// Chunk c (16 bytes, 0..7) of row r of a panel at r * 128 + ((c ^ swizzle) * 16).  32-row tiles: row_swz.  16-row tiles:
-// reads take rows 0..15 at one chunk, or rows 0..7 / 8..15 at one chunk pair; both fall on distinct banks so.
-template <int TK>
-__device__ __forceinline__ int wide_swz(int r) {
-  return TK == 32 ? row_swz(r) : ((r >> 1) & 3) * 2 | ((r >> 3) & 1);
-}
-template <int TK>
-__device__ __forceinline__ int wide_byte(int r, int c) {
-  return r * 128 + ((c ^ wide_swz<TK>(r)) * 16);
-}
 
 template <int RG, bool FP4>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) paged_wide_kernel(const PagedParams p) {
   using C = PagedWide<RG, FP4>;
   using Row = typename C::Row;
-  constexpr int TK = C::TK, H = TK / 16, KS = C::KS, NDT = C::NDT;
+  constexpr int KEYS = kWideKeys, KS = C::KS, NDT = C::NDT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int w = wave_id();
   const int rg = w % RG, kg = C::ROLES ? (w & 3) / RG : 0;
@@ -89,7 +76,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
     bool probe = tok0 != tok1;
     while (true) {
       const int lim = token_keys(x.kv, x.n, tb), lim_min = token_keys(x.kv, x.n, ta);
-      const int j1 = min(x.b1, (lim + C::KEYS - 1) / C::KEYS);  // steps past it hold no key
+      const int j1 = min(x.b1, (lim + KEYS - 1) / KEYS);  // steps past it hold no key
       auto row_keys = [&](int row) {
         const int t = (x.first + row) / p.H;
         return token_keys(x.kv, x.n, t < tb ? t : tb);
@@ -125,10 +112,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
         for (int grp = lw; grp < 8; grp += C::LW) {
           const int r = 8 * grp + (ln >> 3);
-          const unsigned char *src = key_at(j * C::KEYS + r) + ((ln & 7) ^ wide_swz<TK>(r % TK)) * 16;
+          const unsigned char *src = key_at(j * KEYS + r) + ((ln & 7) ^ row_swz(r & 31)) * 16;
 #pragma unroll
           for (int pn = 0; pn < C::PANELS; ++pn)
-            dma_16_at(lds0 + (uint32_t)(buf * C::STEP + (8 * grp / TK) * C::TILE + pn * C::PANEL + (8 * grp % TK) * 128), src + pn * 128);
+            dma_16_at(lds0 + (uint32_t)(buf * C::STEP + (grp >> 2) * C::TILE + pn * 4096 + (grp & 3) * 1024), src + pn * 128);
         }
       };
       // MXFP4: TPR neighbouring threads have a row: every TPR-th piece of codes (16 bytes, a 32-channel block) and rope
@@ -138,7 +125,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
       };
       auto load_raw = [&](Raw &raw, int j) {
         const int th = lw * 64 + lane_here(), key_of = th / C::TPR, part = th % C::TPR;
-        const unsigned char *src = key_at(j * C::KEYS + key_of);
+        const unsigned char *src = key_at(j * KEYS + key_of);
 #pragma unroll
         for (int i = 0; i < C::CPT; ++i) raw.codes[i] = ld_global_16(src + (i * C::TPR + part) * 16);
         raw.expo = ld_global_16(src + Row::OFF_EXP);
@@ -147,12 +134,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
       };
       auto store_raw = [&](const Raw &raw, int buf) {
         const int th = lw * 64 + lane_here(), key_of = th / C::TPR, part = th % C::TPR;
-        unsigned char *tile = smem + buf * C::STEP + (key_of / TK) * C::TILE;
+        unsigned char *tile = smem + buf * C::STEP + (key_of >> 5) * C::TILE;
 #pragma unroll
         for (int i = 0; i < C::CPT; ++i) {
           const int blk = i * C::TPR + part;
-          const uint32_t four = (uint32_t)(C::TPR == 4 || part < 4 ? raw.expo[C::TPR * i / 4] : raw.expo[C::TPR * i / 4 + C::TPR / 8]);
-          const uint32_t e = (four >> (8 * (part & 3))) & 255u;
+          const uint32_t e = ((uint32_t)raw.expo[i] >> (8 * part)) & 255u;  // byte blk of the exponents
           const float sc = e8m0_scale(e);
           i32x4 v[4];
 #pragma unroll
@@ -165,19 +151,19 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<i32x4 *>(tile + (blk >> 1) * C::PANEL + (wide_byte<TK>(key_of % TK, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v[c];
+            *reinterpret_cast<i32x4 *>(tile + (blk >> 1) * 4096 + (tile_byte(key_of & 31, 4 * (blk & 1) + c) ^ panel_swz(blk >> 1))) = v[c];
         }
 #pragma unroll
         for (int i = 0; i < C::RPT; ++i)
-          *reinterpret_cast<i32x4 *>(tile + 8 * C::PANEL + wide_byte<TK>(key_of % TK, (i * C::TPR + part) & 7)) = raw.rope[i];
+          *reinterpret_cast<i32x4 *>(tile + 8 * 4096 + tile_byte(key_of & 31, (i * C::TPR + part) & 7)) = raw.rope[i];
       };
 
       // steps that are asked for before they are worked on, and their pages in the window
-      constexpr int kAsked = FP4 ? 1 + C::RAW : 1;
+      constexpr int kAsked = FP4 ? 3 : 1;
       auto window_for = [&](int j) {
-        if (page_of((j + kAsked + 1) * C::KEYS - 1) >= base + kWindow && page_of(lim - 1) >= base + kWindow) refill(page_of(j * C::KEYS));
+        if (page_of((j + kAsked + 1) * KEYS - 1) >= base + kWindow && page_of(lim - 1) >= base + kWindow) refill(page_of(j * KEYS));
       };
-      refill(page_of(x.b0 * C::KEYS));
+      refill(page_of(x.b0 * KEYS));
       int buf = 0;
       bool again = false;
       if (computes) {  // (the registers of Q and O are these waves' alone)
@@ -195,59 +181,51 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
 
         // this wave's tile K of a step, from key0
         auto tile_step = [&](const unsigned char *K, int key0) {
-          // Row m of S^T's 16-key tile h is key 8 (m >> 2) + 4 h + (m & 3) (16-key tiles: key m), so that lane group g16
-          // holds keys 8 g16 + 4 h + i (4 g16 + i): what the second product's operand wants of it.
+          // Row m of S^T's 16-key tile h is key 8 (m >> 2) + 4 h + (m & 3), so that lane group g16 holds keys
+          // 8 g16 + 4 h + i: what the second product's operand wants of it.
           const int ln = lane_here(), g16 = ln >> 4, l16 = ln & 15;
-          int ka[H][2], va[H][4];
+          int ka[2][2], va[2][4];
 #pragma unroll
-          for (int h = 0; h < H; ++h) {
-            const int m = TK == 32 ? 8 * (l16 >> 2) + 4 * h + (l16 & 3) : l16;
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) ka[h][u] = wide_byte<TK>(m, 4 * u + g16);
-          }
+            for (int u = 0; u < 2; ++u) ka[h][u] = tile_byte(8 * (l16 >> 2) + 4 * h + (l16 & 3), 4 * u + g16);
           // operands in the order (k-step, h) of the first product, then of V^T's 16-channel tiles
           auto rows = [&](int i) {
-            const int ks = i / H, h = i % H;
-            return *reinterpret_cast<const i32x4 *>(K + (ka[h][ks & 1] ^ panel_swz(ks >> 1)) + (ks >> 1) * C::PANEL);
+            const int ks = i >> 1, h = i & 1;
+            return *reinterpret_cast<const i32x4 *>(K + (ka[h][ks & 1] ^ panel_swz(ks >> 1)) + (ks >> 1) * 4096);
           };
           auto cols = [&](int dt) {
-            const unsigned char *b = K + (dt >> 2) * C::PANEL;
+            const unsigned char *b = K + (dt >> 2) * 4096;
             const i32x2 r0 = ds_read_tr16(b + (va[0][dt & 3] ^ panel_swz(dt >> 2)));
-            i32x2 r1{0, 0};
-            if constexpr (TK == 32) r1 = ds_read_tr16(b + (va[H - 1][dt & 3] ^ panel_swz(dt >> 2)));
+            const i32x2 r1 = ds_read_tr16(b + (va[1][dt & 3] ^ panel_swz(dt >> 2)));
             return i32x4{r0[0], r0[1], r1[0], r1[1]};
           };
-          f32x4 s[H];
-#pragma unroll
-          for (int h = 0; h < H; ++h) s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          f32x4 s[2]{{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
           OperandsOf<C::GROUP> a0;
-          load_group<KS * H>(a0, 0, rows);
-          stream_operands<KS * H>(a0, rows, [&](int i, i32x4 a) {
-            s[i % H] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(q[i / H]), s[i % H], 0, 0, 0);
-            if (i % C::GROUP >= C::GROUP - H || i >= (KS - 1) * H) asm volatile("" : "+v"(s[i % H]));  // here, not where the sum is needed
+          load_group<KS * 2>(a0, 0, rows);
+          stream_operands<KS * 2>(a0, rows, [&](int i, i32x4 a) {
+            s[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(q[i >> 1]), s[i & 1], 0, 0, 0);
+            asm volatile("" : "+v"(s[i & 1]));  // here, not sunk to where the sum is needed
           });
 #pragma unroll
-          for (int h = 0; h < H; ++h) {
-            const int v = (TK == 32 ? 8 * g16 + 4 * h : 4 * g16) + (l16 >> 2);
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) va[h][u] = wide_byte<TK>(v, 2 * u + ((l16 & 3) >> 1)) + (l16 & 1) * 8;
-          }
+            for (int u = 0; u < 4; ++u) va[h][u] = tile_byte(8 * g16 + 4 * h + (l16 >> 2), 2 * u + ((l16 & 3) >> 1)) + (l16 & 1) * 8;
           load_group<NDT>(a0, 0, cols);
           __builtin_amdgcn_sched_barrier(0);
-          constexpr int KL = TK / 4;  // keys of a lane: KL g16 + e
-          if (!all_there || key0 + TK > lim_min) {
+          if (!all_there || key0 + 32 > lim_min) {
             keep_branch();
-            const int kl = key0 + (ln & (TK - 1)), my_lim = row_keys(16 * rg + l16);
+            const int kl = key0 + (ln & 31), my_lim = row_keys(16 * rg + l16);
             const uint32_t there = (uint32_t)wv::ballot(kl < lim && window[page_of(kl) - base] >= 0);
 #pragma unroll
-            for (int e = 0; e < KL; ++e) {
-              const int k = KL * g16 + e;
+            for (int e = 0; e < 8; ++e) {
+              const int k = 8 * g16 + e;
               if (!((there >> k) & 1u) || key0 + k >= my_lim) s[e >> 2][e & 3] = -INFINITY;
             }
           }
           float mx = s[0][0];
 #pragma unroll
-          for (int e = 1; e < KL; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+          for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
           mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
           mx = max_halves(mx) * p.sl2;
           if (wv::ballot(mx > m_run + 8.0f) != 0ull) {
@@ -257,31 +235,23 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
           }
-          float e2[KL];
+          float e2[8];
 #pragma unroll
-          for (int e = 0; e < KL; ++e) {
+          for (int e = 0; e < 8; ++e) {
             e2[e] = exp2_fast(fmaf(s[e >> 2][e & 3], p.sl2, -m_run));
             l_run += e2[e];
           }
-          i32x4 pb{(int)pack_bf16x2(e2[0], e2[1]), (int)pack_bf16x2(e2[2], e2[3]), 0, 0};
-          if constexpr (TK == 32) {
-            pb[2] = (int)pack_bf16x2(e2[KL - 4], e2[KL - 3]);
-            pb[3] = (int)pack_bf16x2(e2[KL - 2], e2[KL - 1]);
-          }
+          const i32x4 pb{(int)pack_bf16x2(e2[0], e2[1]), (int)pack_bf16x2(e2[2], e2[3]), (int)pack_bf16x2(e2[4], e2[5]),
+                         (int)pack_bf16x2(e2[6], e2[7])};
           stream_operands<NDT>(a0, cols, [&](int dt, i32x4 a) {
-            if constexpr (TK == 32) {
-              o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(pb), o[dt], 0, 0, 0);
-            } else {
-              const i32x2 al{a[0], a[1]}, pl{pb[0], pb[1]};
-              o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, al), __builtin_bit_cast(s16x4_t, pl), o[dt], 0, 0, 0);
-            }
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(pb), o[dt], 0, 0, 0);
           });
         };
 
         auto compute = [&](int j, int buf) {
 #pragma unroll
           for (int sub = 0; sub < C::SUB; ++sub) {
-            const int tl = kg * C::SUB + sub, key0 = j * C::KEYS + tl * TK;
+            const int tl = kg * C::SUB + sub, key0 = j * KEYS + tl * 32;
             if (key0 < lim) tile_step(smem + buf * C::STEP + tl * C::TILE, key0);
           }
         };
@@ -289,19 +259,6 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           for (int j = x.b0; j < j1; ++j) {
             window_for(j);
             __syncthreads();  // step j is whole
-            compute(j, buf);
-            buf ^= 1;
-          }
-        } else if constexpr (FP4) {
-          Raw raw;
-          load_raw(raw, x.b0);  // (where there is no step: zeros)
-          store_raw(raw, 0);
-          load_raw(raw, x.b0 + 1);
-          for (int j = x.b0; j < j1; ++j) {
-            window_for(j);
-            __syncthreads();          // step j is whole; the buffer after it is consumed
-            store_raw(raw, buf ^ 1);  // step j + 1
-            load_raw(raw, j + 2);
             compute(j, buf);
             buf ^= 1;
           }
@@ -360,7 +317,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           const int rlo = ta * p.H - x.first, rhi = min((tb + 1) * p.H - x.first, x.nrows);  // rows of tokens [ta, tb]
           const int row = my_row(), g16 = lane_here() >> 4;
           if (kg == 0 && row >= rlo && row < rhi) {
-            const bool none = row_keys(row) <= x.b0 * C::KEYS || l_run == 0.0f;  // no key of this piece
+            const bool none = row_keys(row) <= x.b0 * KEYS || l_run == 0.0f;  // no key of this piece
             const float inv = none ? 0.0f : 1.0f / l_run;
             const int64_t part = (int64_t)x.slot * C::ROWS + row;
             if (g16 == 0) {
@@ -443,12 +400,10 @@ static int launch(const PagedParams &p, hipStream_t st) {
   return check_launch("dsa_paged_latent_mla_fwd");
 }
 
-int paged_wide_keys() { return PagedWide<8, false>::KEYS; }
+int paged_wide_keys() { return kWideKeys; }
 int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st) {
-  if (tiles16 == 8) return fp4 ? launch<8, true>(p, st) : launch<8, false>(p, st);
-  if (tiles16 == 4) return fp4 ? launch<4, true>(p, st) : launch<4, false>(p, st);
-  if (tiles16 == 2) return fp4 ? launch<2, true>(p, st) : launch<2, false>(p, st);
-  return fp4 ? launch<1, true>(p, st) : launch<1, false>(p, st);
+  if (fp4) return tiles16 == 2 ? launch<2, true>(p, st) : launch<4, true>(p, st);
+  return tiles16 == 4 ? launch<4, false>(p, st) : launch<8, false>(p, st);
 }
 
 }  // namespace dsa
