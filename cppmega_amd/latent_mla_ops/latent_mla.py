@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..sparse_mla_ops._common import check_same_device, normalize_sm_scale, unwrap_quantized
@@ -210,6 +211,7 @@ class LatentMLA(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output, grad_lse):
         if grad_output is None:
             return (None,) * 7
@@ -233,6 +235,7 @@ class LatentMLAExpanded(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output, grad_lse):
         if grad_output is None:
             return (None,) * 8
