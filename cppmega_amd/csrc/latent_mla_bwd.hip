@@ -67,6 +67,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
       latent_window(p, b, t, lo[rt], hi[rt]);
       span_add(mine, lo[rt], hi[rt]);
       span_add(span, lo[rt], hi[rt]);
+    } else {
+      span_add(mine, 0, 0);  // no row admits nothing: its weight 0 must not meet a key that is not finite
     }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {

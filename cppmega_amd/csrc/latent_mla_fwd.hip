@@ -198,7 +198,13 @@ if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) bad |= not_finite(o[rt][dt][i]);
+      for (int i = 0; i < 16; ++i) {
+        // the bits by way of a register that the compiler does not see through: this file is compiled as if there were no
+        // NaNs (the maxima above need no canonical operands so), which would make this a test for Inf alone
+        uint32_t bits = __float_as_uint(o[rt][dt][i]);
+        asm("" : "+v"(bits));
+        bad |= (bits & 0x7f800000u) == 0x7f800000u;
+      }
   if (__syncthreads_or(bad)) pass(std::true_type{});  // a masked Inf or NaN may have reached a row: once more, without it
 
 #pragma unroll
