@@ -168,11 +168,11 @@ _SIGNATURES = {
                                        + [_f32, _i32, _c_void_p]),
     "dsa_topk_index_mask": (_i32, [_c_void_p, _i32, _i64, _c_void_p, _i64, _i64, _i64, _i64, _i64,
                                    _f32, _f32, _i32, _c_void_p]),
-    "dsa_latent_mla_fwd": (_i32, [_c_void_p] * 6 + [_i64] * 7 + [_f32, _i32, _c_void_p]),
-    "dsa_latent_mla_expanded_fwd": (_i32, [_c_void_p] * 8 + [_i64] * 7 + [ctypes.POINTER(_i64), _f32, _i32, _c_void_p]),
+    "dsa_latent_mla_fwd": (_i32, [_c_void_p] * 7 + [_i64] * 7 + [_f32, _i32, _c_void_p]),
+    "dsa_latent_mla_expanded_fwd": (_i32, [_c_void_p] * 9 + [_i64] * 7 + [ctypes.POINTER(_i64), _f32, _i32, _c_void_p]),
     "dsa_latent_mla_bwd_workspace_size": (_size_t, [_i64] * 7 + [_i32]),
-    "dsa_latent_mla_bwd": (_i32, [_c_void_p] * 10 + [_size_t] + [_i64] * 7 + [_f32, _i32, _c_void_p]),
-    "dsa_latent_mla_expanded_bwd": (_i32, [_c_void_p] * 14 + [_size_t] + [_i64] * 7
+    "dsa_latent_mla_bwd": (_i32, [_c_void_p] * 11 + [_size_t] + [_i64] * 7 + [_f32, _i32, _c_void_p]),
+    "dsa_latent_mla_expanded_bwd": (_i32, [_c_void_p] * 15 + [_size_t] + [_i64] * 7
                                     + [ctypes.POINTER(_i64), _f32, _i32, _c_void_p]),
     "dsa_latent_cache_row_bytes": (_i64, [_i64, _i64, _i32]),
     "dsa_latent_cache_append": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p] + [_i64] * 5

@@ -16,14 +16,14 @@ struct LatentParams {
   const unsigned char *q;              // [B, S, H, DK] bf16
   const unsigned char *k, *kpe, *v;    // bf16; kpe, v: expanded only
   int64_t k_b, k_t, k_g, pe_b, pe_t, v_b, v_t, v_g;  // strides in bytes: batch, token, group
-  uint16_t *out;                       // [B, S, H, DV]
+  uint16_t *out, *out_lo;              // [B, S, H, DV]; what rounding took from out, or null
   float *lse;                          // [B, S, H]
   const int32_t *starts, *ends;        // [B, S] key windows, or null
   int64_t B, S, S_kv, H, G, rows;      // rows = S * hpg
   int hpg, causal;
   float sl2, scale;                    // sm_scale * log2(e), sm_scale
   // backward
-  const unsigned char *o, *dO;
+  const unsigned char *o, *o_lo, *dO;  // (o_lo may be null)
   const float *lse_in;
   uint16_t *dq, *dk, *dkpe, *dv;       // absorbed: dk = dkv [B, S_kv, G, DK]
   float *stat;                         // [B * G][nt64][4][64]: -lse2 / sl2, -delta, lo, hi (int bits) of a row

@@ -1,7 +1,6 @@
 // C entry points of dense latent attention: argument checks and parameter blocks.
 #include <math.h>
 
-
 #include "latent_mla.hpp"
 
 namespace dsa {
@@ -87,35 +86,39 @@ static int check_shape(const char *who, int64_t d_qk, int64_t d_v, bool expanded
 
 using namespace dsa;
 
-extern "C" int dsa_latent_mla_fwd(const void *q, const void *kv, const int32_t *starts, const int32_t *ends, void *out, float *lse2,
-                                  int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t D_qk, int64_t D_v,
+extern "C" int dsa_latent_mla_fwd(const void *q, const void *kv, const int32_t *starts, const int32_t *ends, void *out,
+                                  void *out_lo, float *lse2, int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t D_qk, int64_t D_v,
                                   float sm_scale, int causal, void *stream) {
   int rc = check_common("dsa_latent_mla_fwd", B, S, S_kv, H, G, sm_scale, causal, starts, ends);
   if (!rc) rc = check_shape("dsa_latent_mla_fwd", D_qk, D_v, false);
   if (rc) return rc;
   DSA_REQUIRE(G * D_qk < (1ll << 23), "dsa_latent_mla_fwd: G * D_qk must be below 2^23");
   if (B * S == 0) return DSA_OK;
-  DSA_REQUIRE(given(q, 1) && given(kv, S_kv) && given(out, 1) && lse2 != nullptr, "dsa_latent_mla_fwd: null or misaligned pointer");
+  DSA_REQUIRE(given(q, 1) && given(kv, S_kv) && given(out, 1) && aligned16(out_lo) && lse2 != nullptr,
+              "dsa_latent_mla_fwd: null or misaligned pointer");
   LatentParams p = common_params(q, starts, ends, B, S, S_kv, H, G, sm_scale, causal);
   absorbed_kv(p, kv, D_qk);
   p.out = (uint16_t *)out;
+  p.out_lo = (uint16_t *)out_lo;
   p.lse = lse2;
   return launch_latent_fwd(p, D_qk, D_v, false, (hipStream_t)stream);
 }
 
 extern "C" int dsa_latent_mla_expanded_fwd(const void *q, const void *k_nope, const void *k_pe, const void *v, const int32_t *starts,
-                                           const int32_t *ends, void *out, float *lse2, int64_t B, int64_t S, int64_t S_kv,
-                                           int64_t H, int64_t D_nope, int64_t D_pe, int64_t D_v, const int64_t *strides,
+                                           const int32_t *ends, void *out, void *out_lo, float *lse2, int64_t B, int64_t S,
+                                           int64_t S_kv, int64_t H, int64_t D_nope, int64_t D_pe, int64_t D_v, const int64_t *strides,
                                            float sm_scale, int causal, void *stream) {
   int rc = check_common("dsa_latent_mla_expanded_fwd", B, S, S_kv, H, H, sm_scale, causal, starts, ends);
   if (!rc) rc = check_shape("dsa_latent_mla_expanded_fwd", D_pe == 64 ? D_nope + D_pe : -1, D_v, true);
   if (rc) return rc;
   if (B * S == 0) return DSA_OK;
-  DSA_REQUIRE(given(q, 1) && given(out, 1) && lse2 != nullptr, "dsa_latent_mla_expanded_fwd: null or misaligned pointer");
+  DSA_REQUIRE(given(q, 1) && given(out, 1) && aligned16(out_lo) && lse2 != nullptr,
+              "dsa_latent_mla_expanded_fwd: null or misaligned pointer");
   LatentParams p = common_params(q, starts, ends, B, S, S_kv, H, H, sm_scale, causal);
   rc = expanded_kv("dsa_latent_mla_expanded_fwd", p, k_nope, k_pe, v, strides, D_nope, D_pe, D_v);
   if (rc) return rc;
   p.out = (uint16_t *)out;
+  p.out_lo = (uint16_t *)out_lo;
   p.lse = lse2;
   return launch_latent_fwd(p, D_nope + D_pe, D_v, true, (hipStream_t)stream);
 }
@@ -127,22 +130,23 @@ extern "C" size_t dsa_latent_mla_bwd_workspace_size(int64_t B, int64_t S, int64_
   return latent_bwd_workspace(common_params(nullptr, nullptr, nullptr, B, S, S_kv, H, G, 1.0f, 0), D_qk, D_v, expanded != 0);
 }
 
-static int backward(const char *who, LatentParams &p, const void *o, const void *dO, const float *lse2, void *dq, int64_t d_qk,
+static int backward(const char *who, LatentParams &p, const void *o, const void *o_lo, const void *dO, const float *lse2, void *dq, int64_t d_qk,
                     int64_t d_v, bool expanded, void *ws, size_t ws_bytes, void *stream) {
   const int64_t n = p.B * p.S;
-  DSA_REQUIRE(given(p.q, n) && given(o, n) && given(dO, n) && given(dq, n) && (n == 0 || lse2 != nullptr),
+  DSA_REQUIRE(given(p.q, n) && given(o, n) && aligned16(o_lo) && given(dO, n) && given(dq, n) && (n == 0 || lse2 != nullptr),
               "%s: null or misaligned pointer", who);
   const size_t need = latent_bwd_workspace(p, d_qk, d_v, expanded);
   if (need > 0 && (ws == nullptr || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u)))
     return set_error(DSA_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", who, need, ws_bytes);
   p.o = (const unsigned char *)o;
+  p.o_lo = (const unsigned char *)o_lo;
   p.dO = (const unsigned char *)dO;
   p.lse_in = lse2;
   p.dq = (uint16_t *)dq;
   return launch_latent_bwd(p, d_qk, d_v, expanded, (unsigned char *)ws, (hipStream_t)stream);
 }
 
-extern "C" int dsa_latent_mla_bwd(const void *q, const void *kv, const void *o, const void *dO, const float *lse2,
+extern "C" int dsa_latent_mla_bwd(const void *q, const void *kv, const void *o, const void *o_lo, const void *dO, const float *lse2,
                                   const int32_t *starts, const int32_t *ends, void *dq, void *dkv, void *workspace,
                                   size_t workspace_bytes, int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G, int64_t D_qk,
                                   int64_t D_v, float sm_scale, int causal, void *stream) {
@@ -155,11 +159,11 @@ extern "C" int dsa_latent_mla_bwd(const void *q, const void *kv, const void *o, 
   LatentParams p = common_params(q, starts, ends, B, S, S_kv, H, G, sm_scale, causal);
   absorbed_kv(p, kv, D_qk);
   p.dk = (uint16_t *)dkv;
-  return backward("dsa_latent_mla_bwd", p, o, dO, lse2, dq, D_qk, D_v, false, workspace, workspace_bytes, stream);
+  return backward("dsa_latent_mla_bwd", p, o, o_lo, dO, lse2, dq, D_qk, D_v, false, workspace, workspace_bytes, stream);
 }
 
 extern "C" int dsa_latent_mla_expanded_bwd(const void *q, const void *k_nope, const void *k_pe, const void *v, const void *o,
-                                           const void *dO, const float *lse2, const int32_t *starts, const int32_t *ends, void *dq,
+                                           const void *o_lo, const void *dO, const float *lse2, const int32_t *starts, const int32_t *ends, void *dq,
                                            void *dk_nope, void *dk_pe, void *dv, void *workspace, size_t workspace_bytes,
                                            int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t D_nope, int64_t D_pe,
                                            int64_t D_v, const int64_t *strides, float sm_scale, int causal, void *stream) {
@@ -175,5 +179,5 @@ extern "C" int dsa_latent_mla_expanded_bwd(const void *q, const void *k_nope, co
   p.dk = (uint16_t *)dk_nope;
   p.dkpe = (uint16_t *)dk_pe;
   p.dv = (uint16_t *)dv;
-  return backward(who, p, o, dO, lse2, dq, D_nope + D_pe, D_v, true, workspace, workspace_bytes, stream);
+  return backward(who, p, o, o_lo, dO, lse2, dq, D_nope + D_pe, D_v, true, workspace, workspace_bytes, stream);
 }

@@ -81,13 +81,17 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
       dO[rt][vs] = i32x4{0, 0, 0, 0};
       if (orow[rt] >= 0) {
         dO[rt][vs] = ld_global_16(p.dO + (orow[rt] * DV + 16 * vs + 8 * g32) * 2);
-        const i32x4 ov = ld_global_16(p.o + (orow[rt] * DV + 16 * vs + 8 * g32) * 2);
+        auto dot = [&](const unsigned char *o) {
+          const i32x4 ov = ld_global_16(o + (orow[rt] * DV + 16 * vs + 8 * g32) * 2);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t a = (uint32_t)ov[e], c = (uint32_t)dO[rt][vs][e];
-          dl = fmaf(__uint_as_float(a << 16), __uint_as_float(c << 16), dl);
-          dl = fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(c & 0xffff0000u), dl);
-        }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t a = (uint32_t)ov[e], c = (uint32_t)dO[rt][vs][e];
+            dl = fmaf(__uint_as_float(a << 16), __uint_as_float(c << 16), dl);
+            dl = fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(c & 0xffff0000u), dl);
+          }
+        };
+        dot(p.o);
+        if (p.o_lo != nullptr) dot(p.o_lo);
       }
     }
     const bool any = hi[rt] > lo[rt];

@@ -221,8 +221,15 @@ if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
           // an empty row's O is 0 (or what a neighbour's NaN left): 0
           const float a0 = empty ? 0.0f : x[4 * m] * inv, a1 = empty ? 0.0f : x[4 * m + 1] * inv;
           const float a2 = empty ? 0.0f : x[4 * m + 2] * inv, a3 = empty ? 0.0f : x[4 * m + 3] * inv;
-          *reinterpret_cast<i32x2 *>(p.out + orow[rt] * DV + acc_col(dt, 4 * m, g32)) =
-              i32x2{(int)pack_bf16x2(a0, a1), (int)pack_bf16x2(a2, a3)};
+          const i32x2 hi2{(int)pack_bf16x2(a0, a1), (int)pack_bf16x2(a2, a3)};
+          const int64_t at = orow[rt] * DV + acc_col(dt, 4 * m, g32);
+          *reinterpret_cast<i32x2 *>(p.out + at) = hi2;
+          if (p.out_lo != nullptr) {
+            auto low = [](int two, float x, float y) {
+              return (int)pack_bf16x2(x - __uint_as_float((uint32_t)two << 16), y - __uint_as_float((uint32_t)two & 0xffff0000u));
+            };
+            *reinterpret_cast<i32x2 *>(p.out_lo + at) = i32x2{low(hi2[0], a0, a1), low(hi2[1], a2, a3)};
+          }
         }
       if (g32 == 0) p.lse[orow[rt]] = empty ? -INFINITY : log2f(l) + m_run[rt];
     }

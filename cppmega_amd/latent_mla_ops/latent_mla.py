@@ -62,6 +62,13 @@ def _check_dense(**ts):
         assert t.data_ptr() % 16 == 0, f"{name} must be 16-byte aligned"
 
 
+def _check_residual(residual, o):
+    if residual is not None:
+        assert residual.shape == o.shape, f"residual must be of out's shape {tuple(o.shape)}, got {tuple(residual.shape)}"
+        _check_bf16(residual=residual)
+        _check_dense(residual=residual)
+
+
 def _batched(*ts):
     """3-D tensors as a batch of one."""
     return tuple(t.unsqueeze(0) for t in ts)
@@ -78,8 +85,9 @@ def _absorbed_dims(q, kv, d_v):
     return B, S, S_kv, H, G, D
 
 
-def latent_mla_fwd_interface(q, kv, sm_scale=None, d_v=512, causal=None, starts=None, ends=None):
-    """Absorbed forward: (out, lse).  Arguments as in the module's description."""
+def latent_mla_fwd_interface(q, kv, sm_scale=None, d_v=512, causal=None, starts=None, ends=None, residual=False):
+    """Absorbed forward: (out, lse), with ``residual`` (out, lse, what rounding took from out, for the backward).
+    Arguments as in the module's description."""
     q, kv = unwrap_quantized(q), unwrap_quantized(kv)
     squeeze = q.ndim == 3
     if squeeze:
@@ -95,19 +103,22 @@ def latent_mla_fwd_interface(q, kv, sm_scale=None, d_v=512, causal=None, starts=
     with here:
         out = torch.empty((B, S, H, d_v), dtype=torch.bfloat16, device=q.device)
         lse = torch.empty((B, S, H), dtype=torch.float32, device=q.device)
+        low = torch.empty_like(out) if residual else None
         rc = _lib.load().dsa_latent_mla_fwd(q.data_ptr(), kv.data_ptr(), _lib.ptr(starts), _lib.ptr(ends), out.data_ptr(),
-                                            lse.data_ptr(), B, S, S_kv, H, G, D, d_v, scale, flag, stream)
+                                            _lib.ptr(low), lse.data_ptr(), B, S, S_kv, H, G, D, d_v, scale, flag, stream)
     _lib.check(rc, "dsa_latent_mla_fwd")
-    return (out[0], lse[0]) if squeeze else (out, lse)
+    got = (out, lse, low) if residual else (out, lse)
+    return tuple(t[0] for t in got) if squeeze else got
 
 
-def latent_mla_bwd(q, kv, o, do, lse, sm_scale=None, causal=None, starts=None, ends=None):
-    """Absorbed backward: (dq, dkv) bf16, from the forward's out and lse.  Deterministic: repeated
-    calls give the same bits."""
+def latent_mla_bwd(q, kv, o, do, lse, sm_scale=None, causal=None, starts=None, ends=None, residual=None):
+    """Absorbed backward: (dq, dkv) bf16, from the forward's out, lse and (for rows of few keys more exactly)
+    residual.  Deterministic: repeated calls give the same bits."""
     q, kv, o, do = unwrap_quantized(q), unwrap_quantized(kv), unwrap_quantized(o), unwrap_quantized(do)
     squeeze = q.ndim == 3
     if squeeze:
         q, kv, o, do, lse = _batched(q, kv, o, do, lse)
+        residual = None if residual is None else residual.unsqueeze(0)
         starts, ends = (x if x is None or x.ndim == 2 else x.unsqueeze(0) for x in (starts, ends))
     d_v = o.shape[-1]
     B, S, S_kv, H, G, D = _absorbed_dims(q, kv, d_v)
@@ -115,7 +126,8 @@ def latent_mla_bwd(q, kv, o, do, lse, sm_scale=None, causal=None, starts=None, e
     _check_bf16(q=q, kv=kv, o=o, do=do)
     assert lse.dtype == torch.float32
     _check_dense(q=q, kv=kv, o=o, do=do, lse=lse)
-    check_same_device(q, kv, o, do, lse, starts, ends)
+    _check_residual(residual, o)
+    check_same_device(q, kv, o, do, lse, starts, ends, residual)
     flag = _mask(causal, starts, ends, B, S)
     scale = _scale(sm_scale, D)
     stream, here = launch_on(q)
@@ -124,8 +136,8 @@ def latent_mla_bwd(q, kv, o, do, lse, sm_scale=None, causal=None, starts=None, e
         dq, dkv = torch.empty_like(q), torch.empty_like(kv)
         n = int(L.dsa_latent_mla_bwd_workspace_size(B, S, S_kv, H, G, D, d_v, 0))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        rc = L.dsa_latent_mla_bwd(q.data_ptr(), kv.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), _lib.ptr(starts),
-                                  _lib.ptr(ends), dq.data_ptr(), dkv.data_ptr(), ws.data_ptr(), n, B, S, S_kv, H, G, D, d_v,
+        rc = L.dsa_latent_mla_bwd(q.data_ptr(), kv.data_ptr(), o.data_ptr(), _lib.ptr(residual), do.data_ptr(), lse.data_ptr(),
+                                  _lib.ptr(starts), _lib.ptr(ends), dq.data_ptr(), dkv.data_ptr(), ws.data_ptr(), n, B, S, S_kv, H, G, D, d_v,
                                   scale, flag, stream)
     _lib.check(rc, "dsa_latent_mla_bwd")
     return (dq[0], dkv[0]) if squeeze else (dq, dkv)
@@ -153,8 +165,8 @@ def _expanded_args(q, k_nope, k_pe, v):
     return B, S, S_kv, H, dn, dr, dv, strides
 
 
-def latent_mla_expanded_fwd(q, k_nope, k_pe, v, sm_scale=None, causal=None, starts=None, ends=None):
-    """Expanded forward: (out, lse).  k_nope, k_pe and v may be strided views (last axis dense)."""
+def latent_mla_expanded_fwd(q, k_nope, k_pe, v, sm_scale=None, causal=None, starts=None, ends=None, residual=False):
+    """Expanded forward: (out, lse), with ``residual`` a third as the absorbed form.  k_nope, k_pe and v may be strided views (last axis dense)."""
     k_nope, k_pe, v = _rows(k_nope), _rows(k_pe), _rows(v)
     B, S, S_kv, H, dn, dr, dv, strides = _expanded_args(q, k_nope, k_pe, v)
     check_same_device(q, k_nope, k_pe, v, starts, ends)
@@ -164,14 +176,15 @@ def latent_mla_expanded_fwd(q, k_nope, k_pe, v, sm_scale=None, causal=None, star
     with here:
         out = torch.empty((B, S, H, dv), dtype=torch.bfloat16, device=q.device)
         lse = torch.empty((B, S, H), dtype=torch.float32, device=q.device)
+        low = torch.empty_like(out) if residual else None
         rc = _lib.load().dsa_latent_mla_expanded_fwd(
             q.data_ptr(), k_nope.data_ptr(), k_pe.data_ptr(), v.data_ptr(), _lib.ptr(starts), _lib.ptr(ends), out.data_ptr(),
-            lse.data_ptr(), B, S, S_kv, H, dn, dr, dv, strides, scale, flag, stream)
+            _lib.ptr(low), lse.data_ptr(), B, S, S_kv, H, dn, dr, dv, strides, scale, flag, stream)
     _lib.check(rc, "dsa_latent_mla_expanded_fwd")
-    return out, lse
+    return (out, lse, low) if residual else (out, lse)
 
 
-def latent_mla_expanded_bwd(q, k_nope, k_pe, v, o, do, lse, sm_scale=None, causal=None, starts=None, ends=None):
+def latent_mla_expanded_bwd(q, k_nope, k_pe, v, o, do, lse, sm_scale=None, causal=None, starts=None, ends=None, residual=None):
     """Expanded backward: (dq, dk_nope, dk_pe, dv) bf16, dk_pe summed over the heads.  Deterministic."""
     k_nope, k_pe, v = _rows(k_nope), _rows(k_pe), _rows(v)
     B, S, S_kv, H, dn, dr, dv, strides = _expanded_args(q, k_nope, k_pe, v)
@@ -179,7 +192,8 @@ def latent_mla_expanded_bwd(q, k_nope, k_pe, v, o, do, lse, sm_scale=None, causa
     _check_bf16(o=o, do=do)
     assert lse.dtype == torch.float32
     _check_dense(o=o, do=do, lse=lse)
-    check_same_device(q, k_nope, k_pe, v, o, do, lse, starts, ends)
+    _check_residual(residual, o)
+    check_same_device(q, k_nope, k_pe, v, o, do, lse, starts, ends, residual)
     flag = _mask(causal, starts, ends, B, S)
     scale = _scale(sm_scale, dn + dr)
     stream, here = launch_on(q)
@@ -190,8 +204,8 @@ def latent_mla_expanded_bwd(q, k_nope, k_pe, v, o, do, lse, sm_scale=None, causa
         n = int(L.dsa_latent_mla_bwd_workspace_size(B, S, S_kv, H, H, dn + dr, dv, 1))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         rc = L.dsa_latent_mla_expanded_bwd(
-            q.data_ptr(), k_nope.data_ptr(), k_pe.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-            _lib.ptr(starts), _lib.ptr(ends), dq.data_ptr(), dk_nope.data_ptr(), dk_pe.data_ptr(), dvv.data_ptr(),
+            q.data_ptr(), k_nope.data_ptr(), k_pe.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(residual), do.data_ptr(),
+            lse.data_ptr(), _lib.ptr(starts), _lib.ptr(ends), dq.data_ptr(), dk_nope.data_ptr(), dk_pe.data_ptr(), dvv.data_ptr(),
             ws.data_ptr(), n, B, S, S_kv, H, dn, dr, dv, strides, scale, flag, stream)
     _lib.check(rc, "dsa_latent_mla_expanded_bwd")
     return dq, dk_nope, dk_pe, dvv
@@ -204,8 +218,9 @@ class LatentMLA(torch.autograd.Function):
     def forward(ctx, q, kv, scaling=None, d_v=None, causal=None, starts=None, ends=None):
         q, kv = unwrap_quantized(q).contiguous(), unwrap_quantized(kv).contiguous()
         ctx.args = dict(sm_scale=scaling, causal=causal)
-        out, lse = latent_mla_fwd_interface(q, kv, d_v=q.shape[-1] if d_v is None else d_v, starts=starts, ends=ends, **ctx.args)
-        ctx.save_for_backward(q, kv, out, lse, starts, ends)
+        out, lse, *low = latent_mla_fwd_interface(q, kv, d_v=q.shape[-1] if d_v is None else d_v, starts=starts, ends=ends,
+                                                  residual=any(ctx.needs_input_grad), **ctx.args)
+        ctx.save_for_backward(q, kv, out, lse, starts, ends, *low)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -215,8 +230,8 @@ class LatentMLA(torch.autograd.Function):
     def backward(ctx, grad_output, grad_lse):
         if grad_output is None:
             return (None,) * 7
-        q, kv, out, lse, starts, ends = ctx.saved_tensors
-        dq, dkv = latent_mla_bwd(q, kv, out, grad_output.contiguous(), lse, starts=starts, ends=ends, **ctx.args)
+        q, kv, out, lse, starts, ends, low = ctx.saved_tensors
+        dq, dkv = latent_mla_bwd(q, kv, out, grad_output.contiguous(), lse, starts=starts, ends=ends, residual=low, **ctx.args)
         return dq, dkv, None, None, None, None, None
 
 
@@ -228,8 +243,9 @@ class LatentMLAExpanded(torch.autograd.Function):
     def forward(ctx, q, k_nope, k_pe, v, scaling=None, causal=None, starts=None, ends=None):
         q = q.contiguous()
         ctx.args = dict(sm_scale=scaling, causal=causal)
-        out, lse = latent_mla_expanded_fwd(q, k_nope, k_pe, v, starts=starts, ends=ends, **ctx.args)
-        ctx.save_for_backward(q, k_nope, k_pe, v, out, lse, starts, ends)
+        out, lse, *low = latent_mla_expanded_fwd(q, k_nope, k_pe, v, starts=starts, ends=ends, residual=any(ctx.needs_input_grad),
+                                                 **ctx.args)
+        ctx.save_for_backward(q, k_nope, k_pe, v, out, lse, starts, ends, *low)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -239,6 +255,7 @@ class LatentMLAExpanded(torch.autograd.Function):
     def backward(ctx, grad_output, grad_lse):
         if grad_output is None:
             return (None,) * 8
-        q, k_nope, k_pe, v, out, lse, starts, ends = ctx.saved_tensors
-        grads = latent_mla_expanded_bwd(q, k_nope, k_pe, v, out, grad_output.contiguous(), lse, starts=starts, ends=ends, **ctx.args)
+        q, k_nope, k_pe, v, out, lse, starts, ends, low = ctx.saved_tensors
+        grads = latent_mla_expanded_bwd(q, k_nope, k_pe, v, out, grad_output.contiguous(), lse, starts=starts, ends=ends, residual=low,
+                                        **ctx.args)
         return (*grads, None, None, None, None)

@@ -617,8 +617,11 @@ int dsa_topk_index_mask(const void *topk_indices, int topk_dtype, int64_t topk,
  *   Keys outside a row's window reach neither its results nor its gradients, whatever
  *   they hold.
  *   out [B, S, H, D_v] bf16, lse2 [B, S, H] f32 (log2 units); sm_scale > 0.
+ *   out_lo (may be NULL) [B, S, H, D_v] bf16: what rounding took from out.
  *
- * Backward, from the forward's out (o) and lse2 and the upstream gradient dO:
+ * Backward, from the forward's out (o), out_lo (o_lo, may be NULL: the rows' o . dO is then
+ * that of the rounded out, which costs up to a half more error in dq and dk where rows
+ * have few keys), lse2 and the upstream gradient dO:
  *   dq, and dkv (absorbed) or dk_nope, dk_pe (summed over the heads), dv (expanded),
  *   all dense bf16.  No float atomics: repeated calls give the same bits.  workspace:
  *   dsa_latent_mla_bwd_workspace_size() bytes, 256-byte aligned (expanded: G = H,
@@ -626,22 +629,23 @@ int dsa_topk_index_mask(const void *topk_indices, int topk_dtype, int64_t topk,
  * Device pointers are 16-byte aligned.  Outputs and workspace overlap no input.
  */
 int dsa_latent_mla_fwd(const void *q, const void *kv, const int32_t *starts, const int32_t *ends,
-                       void *out, float *lse2, int64_t B, int64_t S, int64_t S_kv, int64_t H,
-                       int64_t G, int64_t D_qk, int64_t D_v, float sm_scale, int causal, void *stream);
+                       void *out, void *out_lo, float *lse2, int64_t B, int64_t S, int64_t S_kv,
+                       int64_t H, int64_t G, int64_t D_qk, int64_t D_v, float sm_scale, int causal,
+                       void *stream);
 int dsa_latent_mla_expanded_fwd(const void *q, const void *k_nope, const void *k_pe, const void *v,
-                                const int32_t *starts, const int32_t *ends, void *out, float *lse2,
-                                int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t D_nope,
+                                const int32_t *starts, const int32_t *ends, void *out, void *out_lo,
+                                float *lse2, int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t D_nope,
                                 int64_t D_pe, int64_t D_v, const int64_t *strides, float sm_scale,
                                 int causal, void *stream);
 size_t dsa_latent_mla_bwd_workspace_size(int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G,
                                          int64_t D_qk, int64_t D_v, int expanded);
-int dsa_latent_mla_bwd(const void *q, const void *kv, const void *o, const void *dO, const float *lse2,
-                       const int32_t *starts, const int32_t *ends, void *dq, void *dkv, void *workspace,
+int dsa_latent_mla_bwd(const void *q, const void *kv, const void *o, const void *o_lo,
+                       const void *dO, const float *lse2, const int32_t *starts, const int32_t *ends, void *dq, void *dkv, void *workspace,
                        size_t workspace_bytes, int64_t B, int64_t S, int64_t S_kv, int64_t H, int64_t G,
                        int64_t D_qk, int64_t D_v, float sm_scale, int causal, void *stream);
 int dsa_latent_mla_expanded_bwd(const void *q, const void *k_nope, const void *k_pe, const void *v,
-                                const void *o, const void *dO, const float *lse2, const int32_t *starts,
-                                const int32_t *ends, void *dq, void *dk_nope, void *dk_pe, void *dv,
+                                const void *o, const void *o_lo, const void *dO, const float *lse2,
+                                const int32_t *starts, const int32_t *ends, void *dq, void *dk_nope, void *dk_pe, void *dv,
                                 void *workspace, size_t workspace_bytes, int64_t B, int64_t S,
                                 int64_t S_kv, int64_t H, int64_t D_nope, int64_t D_pe, int64_t D_v,
                                 const int64_t *strides, float sm_scale, int causal, void *stream);

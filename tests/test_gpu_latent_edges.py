@@ -454,3 +454,23 @@ def test_both_forms_are_one_attention(dev):
     assert ((a.double().cpu() - b[..., :64].double().cpu()).abs() <= move + 2 * ref["e_out"] + 2.0 ** -8 * big).all()
     assert ((lse_a.double().cpu() - lse_b.double().cpu()).abs() <= eps / 0.6931 + 2 * ref["e_lse"] + 1e-5).all()
     assert (b[..., 64:] == 0).all()
+
+
+def test_residual_is_what_rounding_took(dev):
+    """out + residual is the output to 2^-17 beyond the products' own error, and with it the gradients' error falls to that
+    of the weights' and the results' rounding (two of them, each at most half a step)."""
+    gen = torch.Generator().manual_seed(23)
+    S, H = 400, 4
+    q, kv, do = _normal(gen, 1, S, H, 128), _normal(gen, 1, S, 1, 128), _normal(gen, 1, S, H, 64)
+    m = dict(zip(("starts", "ends"), _docs(gen, 1, S)))
+    ref = om.absorbed(q, kv, 64, 0.1, *om.windows(1, S, S, **m), do)
+    w = {k: v.to(dev) for k, v in m.items()}
+    plain = ops.latent_mla_fwd_interface(q.to(dev), kv.to(dev), 0.1, 64, **w)
+    out, lse, low = ops.latent_mla_fwd_interface(q.to(dev), kv.to(dev), 0.1, 64, **w, residual=True)
+    assert torch.equal(out, plain[0]) and torch.equal(lse, plain[1])
+    assert (low.float().abs() <= 2.0 ** -8 * out.float().abs() + 1e-30).all()
+    both = [ops.latent_mla_bwd(q.to(dev), kv.to(dev), out, do.to(dev), lse, 0.1, **w, residual=r) for r in (low, None)]
+    off = [[float((g.double().cpu() - ref[n]).norm() / ref[n].norm()) for n, g in zip(("dq", "dkv"), x)] for x in both]
+    assert all(a <= b for a, b in zip(*off)), off
+    got = run_absorbed(dev, q, kv, 64, do, 0.1, m)
+    assert torch.equal(got["dq"], both[0][0]) and torch.equal(got["dkv"], both[0][1])

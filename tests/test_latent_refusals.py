@@ -48,6 +48,8 @@ def test_dense_arguments():
         _refused(ValueError, fwd, q, kv, scale, 64)
     _refused(RuntimeError, fwd, q, kv, None, 64)                       # no GPU tensor
     out, lse = _t(1, 4, 2, 64), _t(1, 4, 2, dtype=torch.float32)
+    _refused(AssertionError, ops.latent_mla_bwd, q, kv, out, out, lse, residual=out[:, :2])
+    _refused(AssertionError, ops.latent_mla_bwd, q, kv, out, out, lse, residual=out.float())
     for a in ((q, kv, _t(1, 4, 2, 128)[..., :64], out, lse), (q, kv, out, _t(1, 3, 2, 64), lse), (q, kv, out, out, lse.double()),
               (q, kv, out, out.float(), lse), (q, kv, out, out, lse[:, :3])):
         _refused(AssertionError, ops.latent_mla_bwd, *a)
@@ -118,17 +120,17 @@ P = 1 << 20  # a pointer that is aligned and never read: each call ends at its c
 
 def test_c_dense():
     L = _lib.load()
-    fwd = lambda **k: L.dsa_latent_mla_fwd(*({**dict(q=P, kv=P, s=None, e=None, o=P, l=P, B=1, S=4, Sk=4, H=2, G=1, D=128, V=64, scale=0.1,  # noqa: E731
+    fwd = lambda **k: L.dsa_latent_mla_fwd(*({**dict(q=P, kv=P, s=None, e=None, o=P, lo=None, l=P, B=1, S=4, Sk=4, H=2, G=1, D=128, V=64, scale=0.1,  # noqa: E731
                                                      causal=1, st=None), **k}).values())
     for k in (dict(B=-1), dict(S=-1), dict(H=0), dict(G=3), dict(H=8192), dict(S=1 << 30), dict(Sk=1 << 30), dict(scale=0.0),
               dict(scale=float("nan")), dict(causal=2), dict(s=P), dict(s=P, e=P), dict(q=None), dict(kv=P + 2), dict(o=P + 8),
-              dict(l=None), dict(S=1 << 29, H=4096)):
+              dict(l=None), dict(lo=P + 2), dict(S=1 << 29, H=4096)):
         assert fwd(**k) == INVALID, k
     for k in (dict(D=576, V=512), dict(D=192, V=64), dict(V=32)):
         assert fwd(**k) == UNSUPPORTED, k
     assert fwd(B=0, q=None) == OK and fwd(S=0, q=None, o=None, l=None) == OK
     st = (ctypes.c_int64 * 8)(1024, 256, 128, 256, 64, 1024, 256, 128)
-    ex = lambda **k: L.dsa_latent_mla_expanded_fwd(*({**dict(q=P, kn=P, pe=P, v=P, s=None, e=None, o=P, l=P, B=1, S=4, Sk=4, H=2, dn=128,  # noqa: E731
+    ex = lambda **k: L.dsa_latent_mla_expanded_fwd(*({**dict(q=P, kn=P, pe=P, v=P, s=None, e=None, o=P, lo=None, l=P, B=1, S=4, Sk=4, H=2, dn=128,  # noqa: E731
                                                              dr=64, V=128, strides=st, scale=0.1, causal=1, stream=None), **k}).values())
     for k in (dict(strides=None), dict(strides=(ctypes.c_int64 * 8)(4, *st[1:])), dict(strides=(ctypes.c_int64 * 8)(*st[:4], -8, *st[5:])),
               dict(strides=(ctypes.c_int64 * 8)(st[0], 1 << 23, *st[2:])), dict(pe=P + 8), dict(v=None), dict(q=None)):
@@ -137,10 +139,10 @@ def test_c_dense():
     size = L.dsa_latent_mla_bwd_workspace_size
     assert size(1, 4, 4, 2, 1, 128, 64, 0) > 0 and size(1, 4, 4, 2, 1, 576, 512, 0) == 0 and size(1, 4, 4, 2, 3, 128, 64, 0) == 0
     n = size(1, 4, 4, 2, 1, 128, 64, 0)
-    bwd = lambda **k: L.dsa_latent_mla_bwd(*({**dict(q=P, kv=P, o=P, do=P, l=P, s=None, e=None, dq=P, dkv=P, ws=P, n=n, B=1, S=4, Sk=4, H=2,  # noqa: E731
+    bwd = lambda **k: L.dsa_latent_mla_bwd(*({**dict(q=P, kv=P, o=P, lo=None, do=P, l=P, s=None, e=None, dq=P, dkv=P, ws=P, n=n, B=1, S=4, Sk=4, H=2,  # noqa: E731
                                                      G=1, D=128, V=64, scale=0.1, causal=1, st=None), **k}).values())
     assert bwd(ws=None) == WORKSPACE and bwd(n=n - 1) == WORKSPACE and bwd(ws=P + 16) == WORKSPACE
-    for k in (dict(dq=None), dict(dkv=None), dict(do=P + 2), dict(l=None), dict(scale=-1.0)):
+    for k in (dict(dq=None), dict(dkv=None), dict(do=P + 2), dict(lo=P + 8), dict(l=None), dict(scale=-1.0)):
         assert bwd(**k) == INVALID, k
 
 
