@@ -4,7 +4,8 @@ Host code mirrors cppmega's Python surface (``sparse_mla_ops``,
 ``dsa_indexer_fused_patch``, top-k, ``index_cache_patch``,
 ``dsa_splitk_indexer_loss``, ``dsa_index_mask``) and calls the
 hand-written HIP kernels of ``_lib/libdsa_hip.so`` through the C-ABI declared
-in ``include/dsa_hip.h``.
+in ``include/dsa_hip.h``.  ``latent_mla_ops`` is the dense attention of the same
+layers, in training and from a paged cache.
 """
 from . import _lib
 from .dsa_fused_indexer_loss import FusedDSAIndexerLoss, apply_fused_indexer_loss_patch, fused_dsa_indexer_loss

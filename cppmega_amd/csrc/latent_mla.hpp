@@ -196,6 +196,16 @@ __device__ __forceinline__ void stream_operands(const OperandsOf<G> &first, Load
 }
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+// Tile dt of a row per lane pair (l, l + 32) as bf16, v[m] its columns acc_col(dt, 4 m, l / 32) .. + 3 (m and m + 1: 16 that lie together):
+// halves exchanged, so that a lane stores 16 bytes (8 at a time, the forward's results took a tenth of its time).
+__device__ __forceinline__ void store_tile(uint16_t *row, int dt, const i32x2 (&v)[4], int g32) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)v[2 * u][0], (uint32_t)v[2 * u + 1][0], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v[2 * u][1], (uint32_t)v[2 * u + 1][1], false, false);
+    *reinterpret_cast<i32x4 *>(row + acc_col(dt, 8 * u, 0) + 8 * g32) = i32x4{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
+  }
+}
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
 #pragma unroll
