@@ -22,7 +22,7 @@
 // Bound by the MFMAs, with the exponentials and the packing of P and dS beside them.
 // Causal, 4096 tokens: 128 / 64 absorbed, batch 2, 32 heads: rows 340 us (1010 TFLOP/s of
 // its three products), keys 525 (785 of its four), reduction 17; 192 / 128 expanded, 128
-// heads: 1325 (830), 1990 (690), 34.  The wider form has registers for one wave a SIMD, so
+// heads: 1325 (830), 1990 (690), 28.  The wider form has registers for one wave a SIMD, so
 // that nothing runs beside its softmax.  delta is a sum over out: where out_lo is given,
 // over out + out_lo, since the rounding of out alone shows in dq and dk of rows with few
 // keys (packed documents: relative error 0.0026 against 0.0024).
@@ -596,31 +596,33 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
   }
 }
 
-// One thread per 4 columns: partial rows added in split order (k_pe: group by group,
-// each group's splits in order) and rounded once.
+// 2^lg threads per 4 columns, each a run of the terms: partial rows in split order (k_pe: group by group, each group's
+// splits in order), then the threads' sums in order, rounded once.
 struct LatentReduce {
-  int keys, width, dn, dr, dvw;  // keys of a block; width of a partial row: dn + dr + dvw, or dr
+  int keys, width, dn, dr, dvw, lg;  // keys of a block; width of a partial row: dn + dr + dvw, or dr
 };
 __global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentParams p, const LatentReduce r) {
+  __shared__ f32x4 sums[256];
   const int64_t bgs = p.B * p.G;
   const int own = (r.width - r.dr) / 4;  // columns of the group's own rows
   const int64_t n_own = bgs * p.S_kv * own, n_pe = p.B * p.S_kv * (r.dr / 4);
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= n_own + n_pe) return;
+  const int items = 256 >> r.lg, part = (int)threadIdx.x >> (8 - r.lg);
+  const int64_t id = (int64_t)blockIdx.x * items + ((int)threadIdx.x & (items - 1));
   f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
   // groups bg .. bg + n - 1, each with its splits: the flags of eight terms are read together, then what they say is there
   auto add = [&](int64_t bg, int64_t n, int64_t key, int col) {
     constexpr int kTerms = 8;
     const int kb = (int)((uint32_t)key / (uint32_t)r.keys);
-    int64_t gr = bg;
-    int s = 0;
-    for (int64_t i0 = 0; i0 < n * p.nsplit; i0 += kTerms) {
+    const int terms = (int)n * p.nsplit, per = (terms + (1 << r.lg) - 1) >> r.lg;
+    const int end = min(terms, (part + 1) * per);
+    int gr = part * per / p.nsplit, s = part * per - gr * p.nsplit;
+    for (int i0 = part * per; i0 < end; i0 += kTerms) {
       int64_t at[kTerms];  // row s * bgs + group of the partial sums
       int there[kTerms];
 #pragma unroll
       for (int i = 0; i < kTerms; ++i) {
-        const bool in = i0 + i < n * p.nsplit;
-        at[i] = in ? s * bgs + gr : bg;
+        const bool in = i0 + i < end;
+        at[i] = in ? s * bgs + bg + gr : bg;
         there[i] = in && (p.nsplit == 1 || kb < split_blocks(p, s, r.keys)) ? (p.nsplit == 1 ? 1 : p.used[at[i] * p.nkb + kb]) : 0;
         if (in && ++s == p.nsplit) {
           s = 0;
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentPara
       for (int i = 0; i < kTerms; ++i) sum += x[i];
     }
   };
-  uint16_t *dst;
+  uint16_t *dst = nullptr;
   if (id < n_own) {
     const int64_t row = id / own, bg = row / p.S_kv, key = row - bg * p.S_kv;
     const int c = (int)(id - row * own) * 4;
@@ -645,13 +647,19 @@ __global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentPara
     const bool is_k = c < r.dn;
     add(bg, 1, key, is_k ? c : c + r.dr);
     dst = is_k ? p.dk + orow * r.dn + c : p.dv + orow * r.dvw + (c - r.dn);
-  } else {
+  } else if (id < n_own + n_pe) {
     const int64_t x = id - n_own, row = x / (r.dr / 4), b = row / p.S_kv, key = row - b * p.S_kv;
     const int c = (int)(x - row * (r.dr / 4)) * 4;
     add(b * p.G, p.G, key, (r.width == r.dr ? 0 : r.dn) + c);
     dst = p.dkpe + (b * p.S_kv + key) * r.dr + c;
   }
-  *reinterpret_cast<i32x2 *>(dst) = i32x2{(int)pack_bf16x2(sum[0], sum[1]), (int)pack_bf16x2(sum[2], sum[3])};
+  if (r.lg > 0) {
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (part > 0) return;
+    for (int i = 1; i < 1 << r.lg; ++i) sum += sums[threadIdx.x + i * items];
+  }
+  if (dst != nullptr) *reinterpret_cast<i32x2 *>(dst) = i32x2{(int)pack_bf16x2(sum[0], sum[1]), (int)pack_bf16x2(sum[2], sum[3])};
 }
 
 // Waves per SIMD of the key-major kernel: two where its 32 keys a wave and their gradients leave the registers for it.
@@ -746,8 +754,12 @@ static int launch(LatentParams p, unsigned char *ws, hipStream_t st) {
   hipLaunchKernelGGL(kk, dim3((unsigned)nk), dim3(64 * NW), K::BYTES, st, p);
   rc = check_launch("dsa_latent_mla_bwd (keys)");
   if (rc || (!expanded && k.nsplit == 1)) return rc;
-  const LatentReduce r{k.keys, k.width, DN, DK - DN, expanded ? DV : 0};
-  const int64_t n = bgs * p.S_kv * ((r.width - r.dr) / 4) + p.B * p.S_kv * (r.dr / 4), wgs = (n + 255) / 256;
+  // threads of an output: one for every eight terms, up to eight (32 splits of 512 rows: 18 us with one, 6.6 with four; where
+  // rows are many, one and two are alike)
+  LatentReduce r{k.keys, k.width, DN, DK - DN, expanded ? DV : 0, 0};
+  const int64_t terms = k.nsplit > 1 ? k.nsplit : p.G;
+  while (r.lg < 3 && (8 << r.lg) < terms) ++r.lg;
+  const int64_t n = bgs * p.S_kv * ((r.width - r.dr) / 4) + p.B * p.S_kv * (r.dr / 4), wgs = (n + (256 >> r.lg) - 1) / (256 >> r.lg);
   DSA_REQUIRE(wgs < (1ll << 31), "dsa_latent_mla_bwd: grid too large");
   hipLaunchKernelGGL(latent_bwd_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, p, r);
   return check_launch("dsa_latent_mla_bwd (reduction)");
