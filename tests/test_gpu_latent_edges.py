@@ -474,3 +474,60 @@ def test_residual_is_what_rounding_took(dev):
     assert all(a <= b for a, b in zip(*off)), off
     got = run_absorbed(dev, q, kv, 64, do, 0.1, m)
     assert torch.equal(got["dq"], both[0][0]) and torch.equal(got["dkv"], both[0][1])
+
+
+@pytest.mark.parametrize("d_qk,d_v", DIMS)
+@pytest.mark.parametrize("fmt,H", [("bf16", 16), ("bf16", 100), ("mxfp4", 16), ("mxfp4", 100)])
+def test_graph_of_paged_attention(dev, d_qk, d_v, fmt, H):
+    """Captured on a side stream and replayed with other queries, lengths and tables, eager work between."""
+    gen = torch.Generator().manual_seed(H)
+    cache, table, kv, _, q = _paged_case(dev, gen, fmt, d_qk, d_v, H, [700, 64, 1], [1, 1, 1], 16)
+    q, table, kv = q.to(dev), table.to(dev), kv.to(dev)
+    s = torch.cuda.Stream(dev)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        ops.paged_latent_mla_fwd(q, cache, table, kv, sm_scale=0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        held = ops.paged_latent_mla_fwd(q, cache, table, kv, sm_scale=0.1)
+    for i, lens in enumerate(([700, 64, 1], [13, 700, 0], [1, 33, 650], [300, 300, 300])):
+        q.copy_(_normal(gen, *q.shape))
+        kv.copy_(torch.tensor(lens))
+        table.copy_(table.roll(1, 0))
+        want = ops.paged_latent_mla_fwd(q, cache, table, kv, sm_scale=0.1)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1]), i
+
+
+def test_plan_keeps_its_inputs_and_results_apart(dev):
+    """The inputs are not written, results of two calls share nothing, and a step repeated from the same state is the same."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    a = [i32([5, 0, 30]), i32([1, 20, -1]), i32([[3, -1, -1], [-1, -1, -1], [0, 1, -1]]), i32([2, 4, 5, 6, 7, 8]), i32([5])]
+    before = [t.clone() for t in a]
+    one = ops.plan_latent_step(*a, 24, 16)
+    kept = [t.clone() for t in one]
+    two = ops.plan_latent_step(*a, 24, 16)
+    assert all(torch.equal(x, y) for x, y in zip(a, before))
+    for t in two:
+        t.fill_(-9)
+    assert all(torch.equal(x, y) for x, y in zip(one, kept))
+    for i, t in enumerate(one):      # nor do a call's own results overlap
+        t.fill_(100 + i)
+    assert all((t == 100 + i).all() for i, t in enumerate(one))
+
+
+def test_gradient_of_a_sum(dev):
+    """An upstream gradient that is a broadcast scalar, into leaves of which one takes none."""
+    gen = torch.Generator().manual_seed(41)
+    q, kv = _normal(gen, 1, 65, 4, 128), _normal(gen, 1, 65, 1, 128)
+    ref = om.absorbed(q, kv, 64, 0.1, *om.windows(1, 65, 65), torch.ones(1, 65, 4, 64))
+    a, b = q.to(dev), kv.to(dev).requires_grad_()
+    out, lse = ops.LatentMLA.apply(a, b, 0.1, 64, None, None, None)
+    out.sum().backward()
+    check(dict(dkv=b.grad), ref, ("dkv",))
+    assert not lse.requires_grad
+    with torch.no_grad():
+        assert torch.equal(ops.LatentMLA.apply(a, b, 0.1, 64, None, None, None)[0], out)
