@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
     {
       const unsigned char *src = (row < x.nrows ? p.q + (x.row0 + row) * D_QK * 2 : zero) + 16 * g32;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) q[ks] = ld_global_16(src + 32 * ks);
+      for (int ks = 0; ks < KS; ++ks) q[ks] = ld_row_16(src + 32 * ks);
     }
     // Tokens [ta, tb] with the keys cut at tb's: all at once, or, where that left something that is not finite, one by
     // one, since a weight of zero does not remove the Inf or NaN of a later token's key.
@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
       auto load_codes = [&](int j) {
         if (w * 64 >= C::CODES) return;  // wave-uniform
         const unsigned char *src = key_at(j * C::KEYS + my_key);
-        codes = ld_global_16(src + my_blk * 16);
-        expo = src[Row::OFF_EXP + my_blk];
+        codes = ld_row_16(src + my_blk * 16);
+        expo = ld_row_1(src + Row::OFF_EXP + my_blk);
       };
       auto store_codes = [&](int buf) {
         if (w * 64 >= C::CODES) return;

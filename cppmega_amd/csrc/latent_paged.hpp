@@ -26,6 +26,14 @@ struct PagedParams {
 };
 
 static __device__ const i32x4 kZeroRow[80] = {};  // a masked key's row
+// A load from p.cache, p.q or kZeroRow, chosen by a select: said to be global, since the compiler takes the choice for a flat
+// address, whose loads are also counted as LDS operations, so that the next barrier waits for them.
+__device__ __forceinline__ i32x4 ld_row_16(const unsigned char *x) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) i32x4 *>(reinterpret_cast<uint64_t>(x));
+}
+__device__ __forceinline__ uint32_t ld_row_1(const unsigned char *x) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) unsigned char *>(reinterpret_cast<uint64_t>(x));
+}
 
 __device__ __forceinline__ int request_start(const PagedParams &p, int r) {
   return p.query_starts == nullptr ? r : min(max(p.query_starts[r], 0), (int)p.T);

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
     for (int rt = 0; rt < NR; ++rt) {
       const unsigned char *src = (16 * rt + l16 < nrows ? p.q + (row0 + 16 * rt + l16) * D_QK * 2 : zero) + 16 * g16;
 #pragma unroll
-      for (int ks = 0; ks < C::KS; ++ks) q[rt][ks] = ld_global_16(src + 64 * ks);
+      for (int ks = 0; ks < C::KS; ++ks) q[rt][ks] = ld_row_16(src + 64 * ks);
     }
 
     // Tokens [ta, tb] with the keys cut at tb's: all at once, or, where that left something that is not finite, one by
@@ -105,11 +105,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
 #pragma unroll
           for (int x = 0; x < C::CPL; ++x) {
             const unsigned char *src = shfl_ptr(mine, x * (64 / C::NB) + lane / C::NB);
-            codes[x] = ld_global_16(src + (lane % C::NB) * 16);
-            expo[x] = src[Row::OFF_EXP + lane % C::NB];
+            codes[x] = ld_row_16(src + (lane % C::NB) * 16);
+            expo[x] = ld_row_1(src + Row::OFF_EXP + lane % C::NB);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) rope[i] = ld_global_16(shfl_ptr(mine, 8 * i + (lane >> 3)) + Row::OFF_ROPE + (lane & 7) * 16);
+          for (int i = 0; i < 4; ++i) rope[i] = ld_row_16(shfl_ptr(mine, 8 * i + (lane >> 3)) + Row::OFF_ROPE + (lane & 7) * 16);
         }
       };
       auto put_block = [&](int row, int blk, i32x4 c, uint32_t e) {  // 32 channels of a row

@@ -127,10 +127,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
         const int th = lw * 64 + lane_here(), key_of = th / C::TPR, part = th % C::TPR;
         const unsigned char *src = key_at(j * KEYS + key_of);
 #pragma unroll
-        for (int i = 0; i < C::CPT; ++i) raw.codes[i] = ld_global_16(src + (i * C::TPR + part) * 16);
-        raw.expo = ld_global_16(src + Row::OFF_EXP);
+        for (int i = 0; i < C::CPT; ++i) raw.codes[i] = ld_row_16(src + (i * C::TPR + part) * 16);
+        raw.expo = ld_row_16(src + Row::OFF_EXP);
 #pragma unroll
-        for (int i = 0; i < C::RPT; ++i) raw.rope[i] = ld_global_16(src + Row::OFF_ROPE + ((i * C::TPR + part) & 7) * 16);
+        for (int i = 0; i < C::RPT; ++i) raw.rope[i] = ld_row_16(src + Row::OFF_ROPE + ((i * C::TPR + part) & 7) * 16);
       };
       auto store_raw = [&](const Raw &raw, int buf) {
         const int th = lw * 64 + lane_here(), key_of = th / C::TPR, part = th % C::TPR;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
           const int row = my_row(), g16 = lane_here() >> 4;
           const unsigned char *src = (row < x.nrows ? p.q + (x.row0 + row) * 1152 : zero) + 16 * g16;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) q[ks] = ld_global_16(src + 64 * ks);
+          for (int ks = 0; ks < KS; ++ks) q[ks] = ld_row_16(src + 64 * ks);
         }
         float m_run = kNegBig, l_run = 0.0f;
         f32x4 o[NDT];
