@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
 // the one that is worked on, shared by the waves in three LDS buffers, one barrier a step; three workgroups a CU.
 //   S^T = K Q^T, O^T += V^T P^T on 32x32x16 MFMAs, lane = row.
 // Bound by the MFMAs and the softmax beside them (prefill of 6 requests, 240 tokens each on 1024 .. 4096 keys, 32 heads,
-// MXFP4: 115 us, 310 TFLOP/s; the conversion of the codes, once a unit of 128 rows, is a quarter of it).
+// MXFP4: 111 us, 325 TFLOP/s; the conversion of the codes, once a unit of 128 rows, is a quarter of it).
 template <int NT, bool FP4>
 struct Paged {
   static constexpr int D_QK = 128, D_V = 64;
@@ -454,16 +454,16 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
 
 // How a call is run, from its sizes alone: by the rows that share keys, a request's (token, head) pairs on average.
 // Times of a step of 64 requests, 301 .. 16384 keys, us, the chosen one's first:
-//   576, bf16   up to 64 rows    units of 64: 16 heads 144, 64 heads 160; of 128: 193, 197
-//               more             units of 128: 128 heads 223; of 64: 265
-//   576, MXFP4  up to 32 rows    units of 32: 16 heads 107, 32 heads 110; of 64: 148, 153; of 16: 104, 165
-//               more             units of 64: 64 heads 165, 128 heads 282; of 128 (all waves fetch and compute): 280, 316
-//   128, bf16   up to 16 rows    waves that split the keys, 16 rows: 16 heads 41; 32: 51; units of 64: 58
+//   576, bf16   up to 64 rows    units of 64: 16 heads 143, 64 heads 159; of 128: 189, 204
+//               more             units of 128: 128 heads 229; of 64: 260
+//   576, MXFP4  up to 32 rows    units of 32: 16 heads 103, 32 heads 107; of 64: 144, 146
+//               more             units of 64: 64 heads 158, 128 heads 274; of 32: 177, 309
+//   128, bf16   up to 16 rows    waves that split the keys, 16 rows: 16 heads 41; 32: 50; units of 64: 58
 //               up to 32         32 rows: 32 heads 56; 16: 59; units of 64: 60
-//               up to 64         units of 64: 64 heads 63; of 128: 71; 16 rows: 97
-//               more             units of 128: 128 heads 78; of 64: 87
-//   128, MXFP4  up to 64 rows    16 rows: 16 heads 38, 64 heads 79; units of 64: 77, 84; of 128: 84, 91
-//               more             units of 128: 128 heads 96; of 64: 120; 16 rows: 133
+//               up to 64         units of 64: 64 heads 63; of 128: 70; 32 rows: 78
+//               more             units of 128: 128 heads 79; of 64: 86
+//   128, MXFP4  up to 64 rows    16 rows: 16 heads 37, 64 heads 78; units of 128: 83, 88
+//               more             units of 128: 128 heads 94; 16 rows: 128
 struct PagedPlan {
   int wide;       // 576 / 512: 16-row tiles of a unit
   int few;        // 128 / 64: 16-row tiles of a unit whose waves split the keys

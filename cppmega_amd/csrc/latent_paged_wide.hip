@@ -12,12 +12,13 @@
 // more steps ahead, converted to exact bf16 values as they are written to LDS.  At a
 // piece's end the key groups' O are brought to one maximum and added pairwise through LDS.
 //
-// What bounds it: with up to 64 rows (MXFP4: 32) the reading of the cache, at 144 us for
-// 64 requests of 301 .. 16384 keys, 630 MB (4.4 TB/s; MXFP4: 107 us for 219 MB, where the
-// conversion and its LDS writes come to it).  At 128 rows a wave reads every tile's K and
-// V whole (70 KiB), which is 2176 cycles of LDS reads and as many of MFMAs a tile, against
-// 135 us for the loads alone: 203 us.  Two steps ahead in flight made that 248 us, the
-// loads after the products 228.
+// What bounds it: bf16 with up to 64 rows the reading of the cache, 143 us with plan and
+// joining for 64 requests of 301 .. 16384 keys, 630 MB (4.8 TB/s in this kernel).  MXFP4
+// with up to 32 rows the computing waves, one a SIMD: for 96 requests, 338 MB, the kernel
+// takes 124 us, its loads alone 65, these with the conversion 84, the products alone 108.
+// At 128 rows a wave reads every tile's K and V whole (70 KiB), which is 2176 cycles of LDS
+// reads and as many of MFMAs a tile, against 135 us for the loads alone: 203 to 214 us.
+// Two steps ahead in flight made that 248 us, the loads after the products 228.
 #include "latent_mla.hpp"
 #include "latent_paged.hpp"
 
