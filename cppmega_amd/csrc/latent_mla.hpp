@@ -38,6 +38,7 @@ struct LatentParams {
 constexpr int kKeyTile = 64;           // keys (or, in the key-major kernel, rows) of an LDS tile
 constexpr uint32_t kTileRecords = 0x80000000u;  // a tile's resource: kMaskedOff lies past it, its rows below it
 constexpr int kNoLo = 0x7fffffff;
+constexpr float kLeastScale = 0x1p-100f;  // of sm_scale: the backward's lse2 / (sm_scale log2 e) stays finite
 
 // Keys [lo, hi) of token t of batch b, within [0, S_kv); an empty row has lo = hi = 0.
 __device__ __forceinline__ void latent_window(const LatentParams &p, int64_t b, int64_t t, int &lo, int &hi) {

@@ -17,7 +17,8 @@ static int check_common(const char *who, int64_t B, int64_t S, int64_t S_kv, int
               (long long)H, (long long)G);
   DSA_REQUIRE(H <= 4096 && S < (1ll << 30) && S_kv < (1ll << 30) && S * (H / G) < (1ll << 31) - 256 && B * G < (1ll << 24),
               "%s: sizes out of range (H <= 4096, S * H / G < 2^31 - 256, S_kv < 2^30, B * G < 2^24)", who);
-  DSA_REQUIRE(isfinite(sm_scale) && sm_scale > 0.0f, "%s: sm_scale must be positive and finite, got %g", who, (double)sm_scale);
+  DSA_REQUIRE(isfinite(sm_scale) && sm_scale >= kLeastScale, "%s: sm_scale must be finite and at least 2^-100, got %g", who,
+              (double)sm_scale);
   DSA_REQUIRE(causal == 0 || causal == 1, "%s: causal must be 0 or 1", who);
   DSA_REQUIRE((starts == nullptr) == (ends == nullptr), "%s: starts and ends come together", who);
   DSA_REQUIRE(starts == nullptr || !causal, "%s: row windows carry the mask: pass causal = 0 with them", who);
@@ -50,8 +51,8 @@ static void absorbed_kv(LatentParams &p, const void *kv, int64_t D) {
   p.k_b = p.S_kv * p.k_t;
 }
 
-static int expanded_kv(const char *who, LatentParams &p, const void *k_nope, const void *k_pe, const void *v, const int64_t *st,
-                       int64_t d_nope, int64_t d_pe, int64_t d_v) {
+static int expanded_kv(const char *who, LatentParams &p, const void *k_nope, const void *k_pe, const void *v,
+                       const int64_t *st) {
   DSA_REQUIRE(st != nullptr, "%s: null strides", who);
   const int64_t n = p.B * p.S_kv;
   DSA_REQUIRE(given(k_nope, n) && given(k_pe, n) && given(v, n), "%s: k_nope, k_pe and v must be 16-byte aligned device pointers", who);
@@ -115,7 +116,7 @@ extern "C" int dsa_latent_mla_expanded_fwd(const void *q, const void *k_nope, co
   DSA_REQUIRE(given(q, 1) && given(out, 1) && aligned16(out_lo) && lse2 != nullptr,
               "dsa_latent_mla_expanded_fwd: null or misaligned pointer");
   LatentParams p = common_params(q, starts, ends, B, S, S_kv, H, H, sm_scale, causal);
-  rc = expanded_kv("dsa_latent_mla_expanded_fwd", p, k_nope, k_pe, v, strides, D_nope, D_pe, D_v);
+  rc = expanded_kv("dsa_latent_mla_expanded_fwd", p, k_nope, k_pe, v, strides);
   if (rc) return rc;
   p.out = (uint16_t *)out;
   p.out_lo = (uint16_t *)out_lo;
@@ -174,7 +175,7 @@ extern "C" int dsa_latent_mla_expanded_bwd(const void *q, const void *k_nope, co
   if (B == 0) return DSA_OK;
   DSA_REQUIRE(given(dk_nope, S_kv) && given(dk_pe, S_kv) && given(dv, S_kv), "%s: null or misaligned gradient", who);
   LatentParams p = common_params(q, starts, ends, B, S, S_kv, H, H, sm_scale, causal);
-  rc = expanded_kv(who, p, k_nope, k_pe, v, strides, D_nope, D_pe, D_v);
+  rc = expanded_kv(who, p, k_nope, k_pe, v, strides);
   if (rc) return rc;
   p.dk = (uint16_t *)dk_nope;
   p.dkpe = (uint16_t *)dk_pe;

@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(256) latent_bwd_reduce_kernel(const LatentPara
 }
 
 // Waves per SIMD of the key-major kernel: two where its 32 keys a wave and their gradients leave the registers for it.
-constexpr int kv_waves(int64_t d_qk, int64_t d_v, bool expanded) { return !expanded && d_qk == 128 ? 2 : 1; }
+constexpr int kv_waves(int64_t d_qk, bool expanded) { return !expanded && d_qk == 128 ? 2 : 1; }
 
 // Row splits of the key-major kernel: what takes least of the rounds of its workgroups on the card (1.3 us a row tile,
 // 8 tiles' time for a workgroup's beginning and end) and of the partial sums' way to memory and back.
@@ -675,7 +675,7 @@ static BwdKvPlan kv_plan(LatentParams p, int64_t d_qk, int64_t d_v, bool expande
   BwdKvPlan r{};
   r.keys = 4 * 32;
   p.nkb = r.nkb = (int)((p.S_kv + r.keys - 1) / r.keys);
-  const int64_t tiles = (p.rows + 63) / 64, bgs = p.B * p.G, slots = kv_waves(d_qk, d_v, expanded) * 256;
+  const int64_t tiles = (p.rows + 63) / 64, bgs = p.B * p.G, slots = kv_waves(d_qk, expanded) * 256;
   const double row_us = (double)(bgs * p.S_kv * (expanded ? d_qk + d_v : d_qk)) * 8 / 4.9e6 * (p.causal ? 0.5 : 1.0);
   double least = 0;
   for (int64_t n = 1; n <= 64 && (n == 1 || n * 4 <= tiles); ++n) {
@@ -722,7 +722,7 @@ size_t latent_bwd_workspace(LatentParams p, int64_t d_qk, int64_t d_v, bool expa
 
 template <int DK, int DN, int DV, int RT, int OQ>
 static int launch(LatentParams p, unsigned char *ws, hipStream_t st) {
-  constexpr int NW = 4, CT = 1, OK = kv_waves(DK, DV, DN != DK);
+  constexpr int NW = 4, CT = 1, OK = kv_waves(DK, DN != DK);
   using Q = LatentBwdQ<DK, DN, DV, RT, NW>;
   using K = LatentBwdKv<DK, DN, DV, CT, NW>;
   constexpr bool expanded = DN != DK;

@@ -103,7 +103,7 @@ extern "C" int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const 
   int rc = check_cache(who, num_blocks, block_size, D_qk, D_v, dtype);
   if (!rc) rc = check_paged(who, T, R, W, block_size, H, D_qk);
   if (rc) return rc;
-  DSA_REQUIRE(isfinite(sm_scale) && sm_scale > 0.0f, "%s: sm_scale must be positive and finite, got %g", who, (double)sm_scale);
+  DSA_REQUIRE(isfinite(sm_scale) && sm_scale >= 0x1p-100f, "%s: sm_scale must be finite and at least 2^-100, got %g", who, (double)sm_scale);
   if (T == 0 || R == 0) return DSA_OK;
   DSA_REQUIRE(q && cache && block_table && kv_lens && out && lse2 && aligned16(q) && aligned16(cache) && aligned16(out),
               "%s: null or misaligned pointer", who);

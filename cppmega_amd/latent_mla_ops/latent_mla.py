@@ -34,8 +34,8 @@ _STRIDES = ctypes.c_int64 * 8
 
 def _scale(sm_scale, d_qk):
     scale = normalize_sm_scale(sm_scale, d_qk)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"sm_scale must be positive and finite, got {scale}")
+    if not 2.0 ** -100 <= scale < float("inf"):
+        raise ValueError(f"sm_scale must be finite and at least 2^-100, got {scale}")
     return scale
 
 

@@ -616,7 +616,7 @@ int dsa_topk_index_mask(const void *topk_indices, int topk_dtype, int64_t topk,
  *   to position t + S_kv - S; else all.  A row without keys: out 0, lse2 -inf, no gradient.
  *   Keys outside a row's window reach neither its results nor its gradients, whatever
  *   they hold.
- *   out [B, S, H, D_v] bf16, lse2 [B, S, H] f32 (log2 units); sm_scale > 0.
+ *   out [B, S, H, D_v] bf16, lse2 [B, S, H] f32 (log2 units); sm_scale >= 2^-100.
  *   out_lo (may be NULL) [B, S, H, D_v] bf16: what rounding took from out.
  *
  * Backward, from the forward's out (o), out_lo (o_lo, may be NULL: the rows' o . dO is then

@@ -531,3 +531,17 @@ def test_gradient_of_a_sum(dev):
     assert not lse.requires_grad
     with torch.no_grad():
         assert torch.equal(ops.LatentMLA.apply(a, b, 0.1, 64, None, None, None)[0], out)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -40, 4.0])
+def test_scales(dev, scale):
+    """From the least that is served (every weight 1 / n) to one where a row sees one key."""
+    gen = torch.Generator().manual_seed(50)
+    q, kv, do = _normal(gen, 1, 100, 4, 128), _normal(gen, 1, 100, 1, 128), _normal(gen, 1, 100, 4, 64)
+    ref = om.absorbed(q, kv, 64, scale, *om.windows(1, 100, 100), do)
+    if scale < 1:
+        check(run_absorbed(dev, q, kv, 64, do, scale, dict(causal=True)), ref, ("out", "lse", "dkv"))
+    else:
+        got = run_absorbed(dev, q, kv, 64, do, scale, dict(causal=True))
+        check(got, ref, ("lse",))
+        assert all(torch.isfinite(t.float()).all() for t in got.values())

@@ -44,7 +44,7 @@ def test_dense_arguments():
         ((q, kv), dict(starts=_i32(1, 4), ends=_i32(1, 4), causal=True)),
     ):
         _refused(AssertionError, fwd, *a, **({"d_v": 64} | k))
-    for scale in (0.0, -1.0, float("inf"), float("nan")):
+    for scale in (0.0, -1.0, 1e-38, float("inf"), float("nan")):
         _refused(ValueError, fwd, q, kv, scale, 64)
     _refused(RuntimeError, fwd, q, kv, None, 64)                       # no GPU tensor
     out, lse = _t(1, 4, 2, 64), _t(1, 4, 2, dtype=torch.float32)
@@ -123,7 +123,7 @@ def test_c_dense():
     fwd = lambda **k: L.dsa_latent_mla_fwd(*({**dict(q=P, kv=P, s=None, e=None, o=P, lo=None, l=P, B=1, S=4, Sk=4, H=2, G=1, D=128, V=64, scale=0.1,  # noqa: E731
                                                      causal=1, st=None), **k}).values())
     for k in (dict(B=-1), dict(S=-1), dict(H=0), dict(G=3), dict(H=8192), dict(S=1 << 30), dict(Sk=1 << 30), dict(scale=0.0),
-              dict(scale=float("nan")), dict(causal=2), dict(s=P), dict(s=P, e=P), dict(q=None), dict(kv=P + 2), dict(o=P + 8),
+              dict(scale=1e-38), dict(scale=float("nan")), dict(causal=2), dict(s=P), dict(s=P, e=P), dict(q=None), dict(kv=P + 2), dict(o=P + 8),
               dict(l=None), dict(lo=P + 2), dict(S=1 << 29, H=4096)):
         assert fwd(**k) == INVALID, k
     for k in (dict(D=576, V=512), dict(D=192, V=64), dict(V=32)):
