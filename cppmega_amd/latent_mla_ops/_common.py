@@ -6,8 +6,17 @@ import contextlib
 import torch
 
 from .. import _lib
+from ..sparse_mla_ops._common import check_same_device
 
 _HERE = contextlib.nullcontext()
+
+
+def same_device(first, *rest):
+    """``check_same_device`` at less time on the host where they are on one."""
+    dev = first.device
+    for t in rest:
+        if t is not None and t.device != dev:
+            check_same_device(first, *rest)
 
 
 def launch_on(t: torch.Tensor):

@@ -18,8 +18,8 @@ from typing import NamedTuple
 import torch
 
 from .. import _lib
-from ..sparse_mla_ops._common import check_same_device, unwrap_quantized
-from ._common import launch_on
+from ..sparse_mla_ops._common import unwrap_quantized
+from ._common import launch_on, same_device
 from .latent_mla import _check_bf16, _check_dense, _scale
 
 _DIMS = ((576, 512), (128, 64))
@@ -63,14 +63,15 @@ class LatentCache:
 
 
 def _check_slots(slots, T):
-    assert slots.dtype == torch.int64 and tuple(slots.shape) == (T,) and slots.is_contiguous(), \
+    assert slots.dtype == torch.int64 and slots.shape == (T,) and slots.is_contiguous(), \
         f"slots must be contiguous int64 [{T}], got {slots.dtype} {tuple(slots.shape)}"
 
 
 def _strided(t, width, name):
-    assert t.ndim == 2 and t.shape[1] == width, f"{name} must be [tokens, {width}], got {tuple(t.shape)}"
-    ok = t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+    shape = t.shape
+    assert len(shape) == 2 and shape[1] == width, f"{name} must be [tokens, {width}], got {tuple(shape)}"
+    row, col = t.stride()
+    return t if col == 1 and row % 8 == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
 
 
 def latent_cache_append(cache, latent, rope, slots):
@@ -84,7 +85,7 @@ def latent_cache_append(cache, latent, rope, slots):
     assert rope.shape[0] == T, f"latent has {T} tokens, rope {rope.shape[0]}"
     _check_bf16(latent=latent, rope=rope)
     _check_slots(slots, T)
-    check_same_device(cache.data, latent, rope, slots)
+    same_device(cache.data, latent, rope, slots)
     stream, here = launch_on(cache.data)
     with here:
         rc = _lib.load().dsa_latent_cache_append(cache.data.data_ptr(), latent.data_ptr(), latent.stride(0), rope.data_ptr(),
@@ -98,7 +99,7 @@ def latent_cache_gather(cache, slots):
     for a slot outside the cache: cached prefixes for the expanded form's up-projections."""
     T = slots.shape[0]
     _check_slots(slots, T)
-    check_same_device(cache.data, slots)
+    same_device(cache.data, slots)
     stream, here = launch_on(cache.data)
     with here:
         out = torch.empty((T, cache.d_qk), dtype=torch.bfloat16, device=slots.device)
@@ -146,7 +147,7 @@ def plan_latent_step(context_lens, query_lens, block_table, free_blocks, free_co
         f"block_table must be [{R}, pages], got {tuple(block_table.shape)}"
     assert free_count.numel() == 1 and F > 0, "free_blocks must hold a page at least, free_count one number"
     assert num_tokens >= 0 and block_size > 0, f"bad num_tokens={num_tokens} or block_size={block_size}"
-    check_same_device(*ins.values())
+    same_device(*ins.values())
     W, dev = block_table.shape[1], context_lens.device
     stream, here = launch_on(context_lens)
     with here:
@@ -186,7 +187,7 @@ def paged_latent_mla_fwd(q, cache, block_table, kv_lens, query_starts=None, sm_s
         assert T == R, f"without query_starts every request has one token: {T} tokens, {R} requests"
     else:
         assert tuple(query_starts.shape) == (R + 1,), f"query_starts must be [{R + 1}], got {tuple(query_starts.shape)}"
-    check_same_device(q, cache.data, block_table, kv_lens, query_starts, out, lse)
+    same_device(q, cache.data, block_table, kv_lens, query_starts, out, lse)
     scale = _scale(sm_scale, D)
     stream, here = launch_on(q)
     L = _lib.load()

@@ -26,8 +26,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ..sparse_mla_ops._common import check_same_device, normalize_sm_scale, unwrap_quantized
-from ._common import launch_on
+from ..sparse_mla_ops._common import normalize_sm_scale, unwrap_quantized
+from ._common import launch_on, same_device
 
 _STRIDES = ctypes.c_int64 * 8
 
@@ -96,7 +96,7 @@ def latent_mla_fwd_interface(q, kv, sm_scale=None, d_v=512, causal=None, starts=
     B, S, S_kv, H, G, D = _absorbed_dims(q, kv, d_v)
     _check_bf16(q=q, kv=kv)
     _check_dense(q=q, kv=kv)
-    check_same_device(q, kv, starts, ends)
+    same_device(q, kv, starts, ends)
     flag = _mask(causal, starts, ends, B, S)
     scale = _scale(sm_scale, D)
     stream, here = launch_on(q)
@@ -127,7 +127,7 @@ def latent_mla_bwd(q, kv, o, do, lse, sm_scale=None, causal=None, starts=None, e
     assert lse.dtype == torch.float32
     _check_dense(q=q, kv=kv, o=o, do=do, lse=lse)
     _check_residual(residual, o)
-    check_same_device(q, kv, o, do, lse, starts, ends, residual)
+    same_device(q, kv, o, do, lse, starts, ends, residual)
     flag = _mask(causal, starts, ends, B, S)
     scale = _scale(sm_scale, D)
     stream, here = launch_on(q)
@@ -169,7 +169,7 @@ def latent_mla_expanded_fwd(q, k_nope, k_pe, v, sm_scale=None, causal=None, star
     """Expanded forward: (out, lse), with ``residual`` a third as the absorbed form.  k_nope, k_pe and v may be strided views (last axis dense)."""
     k_nope, k_pe, v = _rows(k_nope), _rows(k_pe), _rows(v)
     B, S, S_kv, H, dn, dr, dv, strides = _expanded_args(q, k_nope, k_pe, v)
-    check_same_device(q, k_nope, k_pe, v, starts, ends)
+    same_device(q, k_nope, k_pe, v, starts, ends)
     flag = _mask(causal, starts, ends, B, S)
     scale = _scale(sm_scale, dn + dr)
     stream, here = launch_on(q)
@@ -193,7 +193,7 @@ def latent_mla_expanded_bwd(q, k_nope, k_pe, v, o, do, lse, sm_scale=None, causa
     assert lse.dtype == torch.float32
     _check_dense(o=o, do=do, lse=lse)
     _check_residual(residual, o)
-    check_same_device(q, k_nope, k_pe, v, o, do, lse, starts, ends, residual)
+    same_device(q, k_nope, k_pe, v, o, do, lse, starts, ends, residual)
     flag = _mask(causal, starts, ends, B, S)
     scale = _scale(sm_scale, dn + dr)
     stream, here = launch_on(q)
