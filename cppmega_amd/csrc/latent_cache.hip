@@ -11,7 +11,7 @@
 // hundred integers) and writes what belongs to its own ones, so the plan is one launch.
 //
 // 16384 rows of 576 channels into MXFP4 pages 11 us, back 7.6 (26 MB each: 2.3, 3.4 TB/s,
-// the launch among it); the plan of 16 requests 6.5 us, of 768 with 16384 tokens 17:
+// the launch among it); the plan of 16 requests 6.5 us, of 768 with 16384 tokens 14:
 // latencies of the prefix sums, one after the other.
 #include "latent_cache.hpp"
 

@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
 // Many rows of 128 channels: four waves, NT of them 32 rows each, by 4 / NT key groups; steps of 64 keys, two ahead of
 // the one that is worked on, shared by the waves in three LDS buffers, one barrier a step; three workgroups a CU.
 //   S^T = K Q^T, O^T += V^T P^T on 32x32x16 MFMAs, lane = row.
-// Bound by the MFMAs and the softmax beside them (prefill of 6 requests, 240 tokens each on 1024 .. 4096 keys, 32 heads,
-// MXFP4: 111 us, 325 TFLOP/s; the conversion of the codes, once a unit of 128 rows, is a quarter of it).
+// Bound by the MFMAs and the softmax beside them: prefill of 6 requests, 40 .. 512 tokens each on 1024 .. 4096 keys, 32
+// heads, MXFP4: 111 us, 325 TFLOP/s.  Widening the codes costs a sixth (decode of 128 heads: 94 us against 79 in bf16).
 template <int NT, bool FP4>
 struct Paged {
   static constexpr int D_QK = 128, D_V = 64;
