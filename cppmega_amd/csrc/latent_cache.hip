@@ -11,7 +11,7 @@
 // hundred integers) and writes what belongs to its own ones, so the plan is one launch.
 //
 // 16384 rows of 576 channels into MXFP4 pages 11 us, back 7.6 (26 MB each: 2.3, 3.4 TB/s,
-// the launch among it); the plan of 16 requests 6.5 us, of 768 with 16384 tokens 14:
+// the launch among it); the plan of 16 requests 6.7 us, of 768 with 16384 tokens 15:
 // latencies of the prefix sums, one after the other.
 #include "latent_cache.hpp"
 
@@ -133,6 +133,25 @@ struct PlanOwn {
   int ctx, n, held, got, before, back, granted, done;  // before: new blocks of earlier requests; back: blocks given back by them
 };
 
+// Blocks that a request holds: its context's, and those behind them up to the first negative entry of its table (tokens of
+// an earlier step that were not kept).  The search doubles its stride, then halves it: one load where nothing is behind.
+__device__ __forceinline__ int blocks_held(const int32_t *row, int of_context, int W) {
+  int lo = of_context, hi = W;  // entries before lo are blocks; entry hi, if there is one, is none
+  for (int step = 1; lo < hi; step *= 2) {
+    const int at = step <= hi - lo ? lo + step - 1 : hi - 1;
+    if (row[at] < 0) {
+      hi = at;
+      break;
+    }
+    lo = at + 1;
+  }
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (row[mid] < 0) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
 // Inclusive prefix over the workgroup of two values per thread, and their totals.
 __device__ __forceinline__ void scan2(int64_t &a, int64_t &b, int64_t (*tmp)[2], int64_t &ta, int64_t &tb) {
   const int lane = lane_id(), w = (int)(threadIdx.x >> 6);
@@ -182,7 +201,7 @@ __global__ void __launch_bounds__(kPlanThreads) latent_plan_kernel(const PlanPar
       const int asked = p.query_lens[r];
       x.done = asked < 0;
       x.n = asked > 0 ? asked : 0;
-      x.held = (int)(((int64_t)x.ctx + p.block - 1) / p.block);
+      x.held = blocks_held(p.table + (int64_t)r * p.W, (int)(((int64_t)x.ctx + p.block - 1) / p.block), p.W);
       a = x.n;
     }
     // tokens first: whether a request's fit decides what it needs
@@ -191,7 +210,7 @@ __global__ void __launch_bounds__(kPlanThreads) latent_plan_kernel(const PlanPar
     scan2(a, b, tmp, ta, tb);
     const int64_t tok_end = tokens + a, back_end = back + b;
     const bool fits = r < p.R && !x.done && tok_end <= p.T && (int64_t)x.ctx + x.n <= cap;
-    if (fits) need = (int)(((int64_t)x.ctx + x.n + p.block - 1) / p.block) - x.held;
+    if (fits) need = max((int)(((int64_t)x.ctx + x.n + p.block - 1) / p.block) - x.held, 0);
     int64_t d = need, z = 0, td, tz;
     scan2(d, z, tmp, td, tz);
     const int64_t upto = needed + d;

@@ -128,9 +128,12 @@ def plan_latent_step(context_lens, query_lens, block_table, free_blocks, free_co
 
     context_lens [R] int32: cached tokens of every request; query_lens [R] int32: its new tokens, in the order in
     which they lie in the step's token batch (0: none, -1: the request is done and gives its pages back);
-    block_table [R, W] int32: its pages; free_blocks [F] int32, of which the first free_count [1] int32 are free
+    block_table [R, W] int32: its pages, without gaps from the front, -1 behind them (a new request: -1 alone);
+    free_blocks [F] int32, of which the first free_count [1] int32 are free
     (F at least the cache's pages, so that every page can come back); num_tokens: length of the token batch.
 
+    A context may be shorter than the step before left it (speculative tokens that were not kept): the request keeps the
+    pages behind it for its next tokens, and gives all back when it is done.
     New pages come from the end of the free list, request by request.  A request is granted its tokens where they
     lie within the batch and within W pages and the pages that it and the requests before it need are there (one
     that needs no page is granted all the same); otherwise its tokens get no slot, its kv length is 0 and its

@@ -681,10 +681,13 @@ int dsa_latent_cache_gather(const void *cache, const int64_t *slots, void *out, 
  *   block_table_out [R, W]; slots int64 [T], positions [T] of the token batch (-1: none);
  *   query_starts [R + 1]; kv_lens [R] (context + new tokens, 0 where not granted);
  *   context_lens_out [R]; granted [R]; free_blocks_out [F], free_count_out [1].
+ * A request's pages lie at the front of its row of block_table without gaps, a negative
+ * entry ends them: its context's, and those of earlier tokens that were not kept (its
+ * context may have shrunk since), which its next tokens take first.
  * New pages are taken from the end of the free list in request order; a request is
  * granted its tokens where they lie within T and W pages and the pages needed up to and
- * with it are free (or it needs none).  Pages of done requests are appended to what is
- * left.  Lengths and counts are clipped to their ranges.  No output may be an input.
+ * with it are free (or it needs none).  All pages of done requests are appended to what
+ * is left.  Lengths and counts are clipped to their ranges.  No output may be an input.
  */
 int dsa_latent_plan_step(const int32_t *context_lens, const int32_t *query_lens, const int32_t *block_table,
                          const int32_t *free_blocks, const int32_t *free_count, int32_t *block_table_out,

@@ -63,14 +63,16 @@ def plan(ctx, new, table, free, count, T, bs):
     at = upto = used = 0
     for r in range(R):
         c, n = max(0, min(ctx[r], W * bs)), max(new[r], 0)
-        held = -(-c // bs)
+        held = -(-c // bs)                       # its context's pages, and what lies behind them up to the first -1
+        while held < W and table[r][held] >= 0:
+            held += 1
         starts.append(min(at, T))
         if new[r] < 0:
             back += table[r][:held]
             kv.append(0), nxt.append(0), granted.append(0)
             continue
         ok = at + n <= T and c + n <= W * bs
-        need = -(-(c + n) // bs) - held if ok else 0
+        need = max(-(-(c + n) // bs) - held, 0) if ok else 0
         ok = ok and (need == 0 or upto + need <= have)
         out[r][:held] = table[r][:held]
         if ok:

@@ -123,6 +123,60 @@ def test_plan(dev, ctx, new, W, F, count, T, bs):
         assert getattr(got, name).cpu().tolist() == ref[name], name
 
 
+HELD = [
+    # context, pages in the table, new, W, free pages, count, T, block
+    ([16], [2], [1], 4, 8, 8, 1, 16),                                       # a page that a draft took: not taken anew
+    ([16, 1, 0, 33], [3, 1, 2, 3], [17, 40, 0, -1], 6, 20, 12, 60, 16),     # partly enough; unused; done with one behind
+    ([5] * 300, [1 + i % 5 for i in range(300)], [i % 61 - 1 for i in range(300)], 70, 900, 700, 9001, 16),
+    ([10, 3], [64, 0], [600, 900], 64, 90, 3, 1500, 16),                    # a table reserved whole; the pool runs out
+    ([0, 20, 7], [5, 9, 8], [-1, -1, -1], 9, 30, 8, 4, 8),
+]
+
+
+@pytest.mark.parametrize("ctx,held,new,W,F,count,T,bs", HELD)
+def test_plan_keeps_pages_behind_a_context(dev, ctx, held, new, W, F, count, T, bs):
+    """Pages of tokens that were not kept: used before new ones, given back at the end."""
+    gen = torch.Generator().manual_seed(W)
+    held = [max(h, -(-c // bs)) for c, h in zip(ctx, held)]
+    order = torch.randperm(F + sum(held), generator=gen).tolist()
+    free, at, table = order[:F], F, []
+    for n in held:
+        table.append(order[at:at + n] + [-1] * (W - n))
+        at += n
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    got = ops.plan_latent_step(i32(ctx), i32(new), i32(table), i32(free), i32([count]), T, bs)
+    ref = orc.plan(ctx, new, table, free, count, T, bs)
+    for name in got._fields:
+        assert getattr(got, name).cpu().tolist() == ref[name], name
+
+
+def test_rejected_drafts_lose_no_page(dev):
+    """Many steps of draft tokens of which few are kept, across page borders, with requests that end and begin: every page
+    is in exactly one table row or on the free list, and a kept token's page stays its own."""
+    gen = torch.Generator().manual_seed(13)
+    R, W, bs, F = 5, 6, 4, 26
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    table, free, count = i32([[-1] * W] * R), i32(list(range(F))), i32([F])
+    ctx = [0] * R
+    for step in range(80):
+        draft = torch.randint(0, 7, (R,), generator=gen).tolist()
+        new = [-1 if c + d > W * bs - 6 else d for c, d in zip(ctx, draft)]
+        before = table.cpu().tolist()
+        p = ops.plan_latent_step(i32(ctx), i32(new), table, free, count, 40, bs)
+        table, free, count = p.block_table, p.free_blocks, p.free_count
+        rows, n, ok = table.cpu().tolist(), int(count), p.granted.cpu().tolist()
+        pages = [e for r in rows for e in r if e >= 0] + free.cpu().tolist()[:n]
+        assert sorted(pages) == list(range(F)), step
+        for r in range(R):
+            if new[r] < 0:
+                ctx[r] = 0
+                continue
+            kept = -(-ctx[r] // bs)
+            assert rows[r][:kept] == before[r][:kept]
+            if ok[r]:
+                ctx[r] += int(torch.randint(0, new[r] + 1, (1,), generator=gen))
+
+
 # ---------------------------------------------------------------- attention
 
 

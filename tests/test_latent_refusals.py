@@ -186,6 +186,17 @@ def test_c_plan():
 # ---------------------------------------------------------------- the oracle itself
 
 
+def test_oracle_plan_keeps_pages_behind_a_context():
+    """Context 15, four drafts, one kept: the page that the drafts took serves position 16, and a finished request gives it back."""
+    one = oc.plan([15], [4], [[3, -1, -1]], [5, 6, 7, -1], 3, 4, 16)
+    assert one["block_table"] == [[3, 7, -1]] and one["free_count"] == [2]
+    two = oc.plan([16], [1], one["block_table"], one["free_blocks"], 2, 1, 16)
+    assert two["block_table"] == [[3, 7, -1]] and two["slots"] == [7 * 16] and two["free_blocks"] == [5, 6, -1, -1]
+    end = oc.plan([15], [-1], two["block_table"], two["free_blocks"], 2, 0, 16)
+    assert end["free_blocks"] == [5, 6, 3, 7] and end["free_count"] == [4]
+
+
+
 def test_oracle_gradients_are_differences():
     """The formulas of the oracle's gradients against central differences of its forward, in 64 bits."""
     gen = torch.Generator().manual_seed(1)
