@@ -23,39 +23,52 @@ __device__ __forceinline__ int unit_blocks(const PagedParams &p, int kv, int n, 
   return max((token_keys(kv, n, last / p.H) + p.step_keys - 1) / p.step_keys, 1);
 }
 
-// Exclusive prefix over the workgroup of one value per thread; total in every thread.
+// Sums that stop at 2^32 - 1: starts that do not ascend may count a token many times over.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ uint32_t wave_scan_sat(uint32_t x) {  // wv::wave_incl_scan's steps
+  x = add_sat(x, wv::dpp<0x111, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x112, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x114, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x118, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x142, 0xa>(x));
+  x = add_sat(x, wv::dpp<0x143, 0xc>(x));
+  return x;
+}
+// Exclusive prefix over the workgroup of one value below 2^31 per thread; total in every thread.  Exact below 2^32 - 1,
+// at least 2^31 (the stop, less the thread's value) past it.
 template <int NTHR>
-__device__ __forceinline__ int block_scan(int x, int *tmp, int &total) {
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *tmp, uint32_t &total) {
   const int lane = lane_id(), w = (int)(threadIdx.x >> 6);
-  const int v = (int)wv::wave_incl_scan((uint32_t)x);
+  const uint32_t v = wave_scan_sat(x);
   __syncthreads();
   if (lane == 63) tmp[w] = v;
   __syncthreads();
-  int before = 0;
+  uint32_t before = 0;
   total = 0;
 #pragma unroll
   for (int i = 0; i < NTHR / 64; ++i) {
-    const int t = tmp[i];
-    if (i < w) before += t;
-    total += t;
+    const uint32_t t = tmp[i];
+    if (i < w) before = add_sat(before, t);
+    total = add_sat(total, t);
   }
-  return before + v - x;
+  return add_sat(before, v) - x;
 }
 
 // The plan, one workgroup: unit_req[u], unit_first[u] (first row), unit_at[u] (first block,
 // unit_at[units] = all), unit0[r] (first unit of request r; unit0[R] = all).
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
-  __shared__ int tmp[16];
-  int total, at = 0;
+  __shared__ uint32_t tmp[16];
+  const uint32_t most = (uint32_t)p.max_units;
+  uint32_t total, at = 0;
   for (int r0 = 0; r0 < p.R; r0 += 1024) {
     const int r = r0 + (int)threadIdx.x;
     // (starts that do not ascend may ask for more units than there are: cut)
     const int n = r < p.R ? min((request_tokens(p, r) * p.H + p.unit_rows - 1) / p.unit_rows, p.max_units) : 0;
-    const int x = at + block_scan<1024>(n, tmp, total);
-    if (r < p.R) p.unit0[r] = min(x, p.max_units);
-    at = min(at + total, p.max_units);
+    const uint32_t x = add_sat(at, block_scan<1024>((uint32_t)n, tmp, total));
+    if (r < p.R) p.unit0[r] = (int)min(x, most);
+    at = min(add_sat(at, total), most);
   }
-  const int units = at;
+  const int units = (int)at;
   if (threadIdx.x == 0) p.unit0[p.R] = units;
   __syncthreads();
   at = 0;
@@ -73,11 +86,11 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
       p.unit_req[u] = lo;
       p.unit_first[u] = first;
     }
-    const int x = at + block_scan<1024>(nb, tmp, total);
-    if (u < units) p.unit_at[u] = x;
+    const uint32_t x = at + block_scan<1024>((uint32_t)nb, tmp, total);  // (all of them below 2^31: paged_countable)
+    if (u < units) p.unit_at[u] = (int)x;
     at += total;
   }
-  if (threadIdx.x == 0) p.unit_at[units] = at;
+  if (threadIdx.x == 0) p.unit_at[units] = (int)at;
 }
 
 // Many rows of 128 channels: four waves, NT of them 32 rows each, by 4 / NT key groups; steps of 64 keys, two ahead of

@@ -326,6 +326,37 @@ def test_starts_out_of_order_stay_in_bounds(dev):
     assert out.shape == (6, 4, 64)
 
 
+def test_many_starts_out_of_order(dev):
+    """Row groups asked for pass 31 bits (512 requests that each claim nearly the whole batch of 2^29 rows: 512 * (2^22 + 11)
+    groups of 128): the plan stays within its buffers, and the one sound request has its results."""
+    T, H, R, bs = (1 << 22) + 16, 128, 1030, 16
+    if torch.cuda.get_device_properties(dev).total_memory < 260 << 30:
+        pytest.skip("208 GB of queries and results")
+    gen = torch.Generator().manual_seed(77)
+    cache = ops.LatentCache.empty(4, bs, 128, 64, "bf16", dev)
+    rows = _normal(gen, 64, 128).to(dev)
+    ops.latent_cache_append(cache, rows[:, :64], rows[:, 64:], torch.arange(64, device=dev))
+    starts = torch.full((R + 1,), T, dtype=torch.int32)
+    starts[0], starts[1:1026:2] = 0, 5              # request 0: five tokens; then every other one from token 5 to the end
+    kv = torch.zeros(R, dtype=torch.int32)
+    kv[0] = 60
+    table = torch.arange(4, dtype=torch.int32)[None].expand(R, 4).contiguous()
+    torch.cuda.empty_cache()
+    try:
+        q = torch.empty(T, H, 128, dtype=torch.bfloat16, device=dev)
+        out, lse = torch.empty(T, H, 64, dtype=torch.bfloat16, device=dev), torch.empty(T, H, device=dev)
+    except torch.OutOfMemoryError:
+        pytest.skip("208 GB of queries and results")
+    q[:5] = _normal(gen, 5, H, 128).to(dev)
+    ops.paged_latent_mla_fwd(q, cache, table.to(dev), kv.to(dev), starts.to(dev), 0.1, out, lse)
+    got, few = (out[:5].clone(), lse[:5].clone()), q[:5].cpu()
+    torch.cuda.synchronize()
+    del q, out, lse
+    torch.cuda.empty_cache()
+    ref = oc.paged(few, _cache_rows(cache), table[:1], starts[:2], kv[:1], bs, 64, 0.1)
+    _check(got, ref)
+
+
 @pytest.mark.parametrize("fmt,blocks", [("bf16", 60000), ("mxfp4", 176000)])
 def test_offsets_past_32_bits(dev, fmt, blocks):
     """Rows behind 4 GiB of cache: append, gather and attention."""
