@@ -32,7 +32,7 @@
 
 namespace dsa {
 
-constexpr float kNoRow = 1.0e30f;  // lse2 of a row without keys: 2^(x - it) = 0
+constexpr float kNoRow = 1.0e30f;  // in place of the lse2 of a row without weights: 2^(x - it) = 0
 
 template <int DK, int DN, int DV, int RT, int NW>
 struct LatentBwdQ {
@@ -102,10 +102,12 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
         if (p.o_lo != nullptr) dot(p.o_lo);
       }
     }
-    const bool any = hi[rt] > lo[rt];
+    // a row with weights: one without keys, or with scores of -Inf alone (lse2 -Inf), has no gradient
+    const float lse_row = hi[rt] > lo[rt] ? p.lse_in[orow[rt]] : -INFINITY;
+    const bool any = lse_row != -INFINITY;
     dl = sum_halves(dl);
     delta[rt] = any ? dl * p.scale : 0.0f;
-    lse[rt] = any ? p.lse_in[orow[rt]] : kNoRow;
+    lse[rt] = any ? lse_row : kNoRow;
     // what the key-major kernel needs of these rows
     const int64_t r32 = (int64_t)blk * (C::ROWS / 32) + w * RT + rt, t64 = r32 >> 1;
     if (t64 < p.nt64) {
@@ -247,7 +249,7 @@ if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
     if (orow[rt] >= 0) {
-      const bool empty = hi[rt] <= lo[rt];
+      const bool empty = lse[rt] == kNoRow;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
         const f32x16 &x = acc[rt][dt];

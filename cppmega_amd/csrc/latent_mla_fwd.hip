@@ -216,7 +216,7 @@ if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float l = sum_halves(l_run[rt]);
-    const bool empty = hi[rt] <= lo[rt];
+    const bool empty = hi[rt] <= lo[rt] || l == 0.0f;  // no key, or a score of -Inf with each: no weight
     const float inv = empty ? 0.0f : 1.0f / l;
     if (orow[rt] >= 0) {
 #pragma unroll

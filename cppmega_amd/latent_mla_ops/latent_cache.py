@@ -172,8 +172,8 @@ def paged_latent_mla_fwd(q, cache, block_table, kv_lens, query_starts=None, sm_s
     q [T, H, d_qk] bf16; block_table [R, W] int32; kv_lens [R] int32: keys of every request, those of its new tokens
     among them; query_starts [R + 1] int32, ascending: request r has the tokens query_starts[r] .. query_starts[r + 1],
     the last of its kv_lens[r] positions, and each sees the positions up to its own; without query_starts token r is
-    request r's one new token (decoding; T = R).  A page outside the cache hides its keys, and a token without keys has
-    out 0 and lse -inf.  Rows of tokens that belong to no request are not written: pass ``out`` and ``lse`` to keep
+    request r's one new token (decoding; T = R).  A page outside the cache hides its keys, and a token without keys
+    (or with scores of -Inf alone) has out 0 and lse -inf.  Rows of tokens that belong to no request are not written: pass ``out`` and ``lse`` to keep
     what they hold.  Keys that a token does not see may hold anything, Inf and NaN too.
     """
     q = unwrap_quantized(q)

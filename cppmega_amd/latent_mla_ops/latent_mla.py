@@ -14,7 +14,8 @@ attention) and layers without an indexer need it.
 (query token t sees the keys up to position t + S_kv - S: the last S of S_kv tokens),
 every key (``causal=False``), or per-row key windows ``starts`` / ``ends`` [B, S] int32
 (keys [start, end), clipped to [0, S_kv): packed documents, padding, sliding windows),
-which take causal's place.  A row without keys has out 0, lse -inf and zero gradients.
+which take causal's place.  A row without keys, or whose every score is -Inf, has out 0,
+lse -inf and zero gradients.
 Keys that a row does not see may hold anything, Inf and NaN too.  The gradient of lse is
 not taken, as SparseMLA does not take it.
 """

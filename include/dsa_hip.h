@@ -613,7 +613,8 @@ int dsa_topk_index_mask(const void *topk_indices, int topk_dtype, int64_t topk,
  *   of 8 (0 broadcasts), token strides below 2^23; the last axes are dense.
  * Row t sees the keys [starts[b, t], ends[b, t]) clipped to [0, S_kv) where the int32
  *   [B, S] windows are given (both or neither, causal 0); else, with causal, the keys up
- *   to position t + S_kv - S; else all.  A row without keys: out 0, lse2 -inf, no gradient.
+ *   to position t + S_kv - S; else all.  A row without keys, or with scores of -Inf alone:
+ *   out 0, lse2 -inf, no gradient.
  *   Keys outside a row's window reach neither its results nor its gradients, whatever
  *   they hold.
  *   out [B, S, H, D_v] bf16, lse2 [B, S, H] f32 (log2 units); sm_scale >= 2^-100.
@@ -702,7 +703,7 @@ int dsa_latent_plan_step(const int32_t *context_lens, const int32_t *query_lens,
  * the last of its kv_lens[r] positions; a token sees the positions up to its own.
  * block_table [R, W] int32: an entry outside [0, num_blocks) hides its keys; lengths
  * past W * block_size are cut.  out [T, H, D_v] bf16, lse2 [T, H] f32; a token without
- * keys: 0 and -inf; tokens of no request are not written.  Keys that a token does not
+ * keys, or with scores of -Inf alone: 0 and -inf; tokens of no request are not written.  Keys that a token does not
  * see do not reach it, whatever they hold.  workspace:
  * dsa_paged_latent_mla_workspace_size() bytes, 256-byte aligned.
  */

@@ -78,6 +78,39 @@ def test_a_document_is_not_reached_by_another(dev, what, expanded):
     assert not torch.isfinite(got["out"][:, 90:120].float()).all()
 
 
+@pytest.mark.parametrize("q_at,k_at", [(1.0, -INF), (3.0e38, -3.0e38)])
+@pytest.mark.parametrize("form", ["absorbed", "expanded", "paged"])
+def test_scores_of_minus_infinity(dev, q_at, k_at, form):
+    """A document whose every score is -Inf (an Inf in its keys' rope part, or a product past fp32's range) has no weights:
+    out 0, lse -Inf and no gradient, in every form; its neighbours are as without it."""
+    gen = torch.Generator().manual_seed(19)
+    S, H, D, V = 150, 4, 128, 64
+    starts = torch.tensor([[0] * 60 + [60] * 50 + [110] * 40], dtype=torch.int32)
+    m = dict(starts=starts, ends=torch.arange(1, S + 1, dtype=torch.int32)[None].contiguous())
+    lo, hi = om.windows(1, S, S, **m)
+    hi_ref = torch.where(starts == 60, lo, hi)      # the reference: that document sees no key
+    q, do = _normal(gen, 1, S, H, D), _normal(gen, 1, S, H, V)
+    q[:, 60:110, :, D - 1] = q_at
+    if form == "expanded":
+        x = [_normal(gen, 1, S, H, 64), _normal(gen, 1, S, 64), _normal(gen, 1, S, H, V)]
+        ref, names = om.expanded(q, *x, 0.1, lo, hi_ref, do), ("out", "lse", "dq", "dk_nope", "dk_pe", "dv")
+        x[1][:, 60:110, 63] = k_at
+        got = run_expanded(dev, q, *x, do, 0.1, m)
+    else:
+        kv = _normal(gen, 1, S, 1, D)
+        ref, names = om.absorbed(q, kv, V, 0.1, lo, hi_ref, do), ("out", "lse", "dq", "dkv")
+        kv[:, 60:110, :, D - 1] = k_at
+        if form == "absorbed":
+            got = run_absorbed(dev, q, kv, V, do, 0.1, m)
+        else:                                       # a document is a request, its tokens new
+            cache = ops.LatentCache(kv.to(dev).view(15, 10, D), D, V)
+            table = torch.tensor([[0, 1, 2, 3, 4, 5], [6, 7, 8, 9, 10, -1], [11, 12, 13, 14, -1, -1]], dtype=torch.int32)
+            lens, at = torch.tensor([60, 50, 40], dtype=torch.int32), torch.tensor([0, 60, 110, 150], dtype=torch.int32)
+            out, lse = ops.paged_latent_mla_fwd(q[0].to(dev), cache, table.to(dev), lens.to(dev), at.to(dev), 0.1)
+            got, names = dict(out=out[None], lse=lse[None]), ("out", "lse")
+    check({n: got[n] for n in names}, ref, names)
+
+
 @pytest.mark.parametrize("S,S_kv", [(0, 5), (5, 0), (0, 0), (3, 1)])
 @pytest.mark.parametrize("expanded", [False, True])
 def test_empty_and_single(dev, S, S_kv, expanded):
