@@ -49,7 +49,7 @@ FILE_FLAGS = {
     "sparse_mla_wide_bwd.hip": _MFMA_VGPR,
     "indexer_kl_loss.hip": _MFMA_VGPR,
     "indexer_bwd.hip": _MFMA_VGPR,
-    "latent_mla_fwd.hip": _MFMA_VGPR + ["-fno-honor-nans", "-mno-amdgpu-ieee"],
+    "latent_mla_fwd.hip": _MFMA_VGPR,
     "latent_mla_bwd.hip": _MFMA_VGPR,
     "latent_paged.hip": _MFMA_VGPR,
     "latent_paged_few.hip": _MFMA_VGPR,

@@ -14,8 +14,8 @@
 // product; l sums the weights before that rounding.
 //
 // Bound by the MFMAs and the softmax beside them, which overlap across the two or three
-// waves of a SIMD only.  Causal, 4096 tokens: 128 / 64 absorbed, batch 2, 32 heads, 230 us
-// (900 TFLOP/s of the admitted pairs); 192 / 128 expanded, 128 heads, 975 us (705); a large
+// waves of a SIMD only.  Causal, 4096 tokens: 128 / 64 absorbed, batch 2, 32 heads, 224 us
+// (920 TFLOP/s of the admitted pairs); 192 / 128 expanded, 128 heads, 975 us (705); a large
 // product runs at 1173.  Of these 5 and 20 us go to out_lo, what rounding took from out.
 // 32 rows a wave (RT 1): with 64 the operands do not fit beside O.
 #include <type_traits>
@@ -163,7 +163,7 @@ if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
         for (int rt = 0; rt < RT; ++rt) {
           float mx = acc[rt][0];
 #pragma unroll
-          for (int i = 1; i < 16; ++i) mx = fmaxf(mx, acc[rt][i]);
+          for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, acc[rt][i]);  // (fmaxf quiets operands first)
           mx = max_halves(mx) * p.sl2;
           if (wv::ballot(mx > m_run[rt] + 8.0f) != 0ull) {
             const float m_new = fmaxf(m_run[rt], mx), alpha = exp2_fast(m_run[rt] - m_new);
@@ -204,13 +204,7 @@ if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        // the bits by way of a register that the compiler does not see through: this file is compiled as if there were no
-        // NaNs (the maxima above need no canonical operands so), which would make this a test for Inf alone
-        uint32_t bits = __float_as_uint(o[rt][dt][i]);
-        asm("" : "+v"(bits));
-        bad |= (bits & 0x7f800000u) == 0x7f800000u;
-      }
+      for (int i = 0; i < 16; ++i) bad |= not_finite(o[rt][dt][i]);
   if (__syncthreads_or(bad)) pass(std::true_type{});  // a masked Inf or NaN may have reached a row: once more, without it
 
 #pragma unroll

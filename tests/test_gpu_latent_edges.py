@@ -111,6 +111,27 @@ def test_scores_of_minus_infinity(dev, q_at, k_at, form):
     check({n: got[n] for n in names}, ref, names)
 
 
+@pytest.mark.parametrize("expanded", [False, True])
+def test_a_row_of_nan_has_nan_results(dev, expanded):
+    """A query row, or one key that rows admit, with NaN: out and lse of the rows that it reaches are NaN, of the others as
+    without it."""
+    gen = torch.Generator().manual_seed(27)
+    S, H = 130, 2
+    x = [_normal(gen, 1, S, H, 128), *((_normal(gen, 1, S, H, 64), _normal(gen, 1, S, 64), _normal(gen, 1, S, H, 64)) if expanded
+                                       else (_normal(gen, 1, S, 1, 128),))]
+    w = om.windows(1, S, S)
+    ref = om.expanded(*x, 0.1, *w) if expanded else om.absorbed(*x, 64, 0.1, *w)
+    x[0][:, 7, 1] = NAN
+    x[1][:, 100:101, 0, 0] = NAN                    # expanded: of head 0 alone
+    on = [t.to(dev) for t in x]
+    out, lse = ops.latent_mla_expanded_fwd(*on, 0.1) if expanded else ops.latent_mla_fwd_interface(*on, 0.1, 64)
+    hit = torch.zeros(1, S, H, dtype=torch.bool)
+    hit[:, 7, 1] = True
+    hit[:, 100:, :1 if expanded else H] = True
+    assert out[hit.to(dev)].isnan().all() and lse[hit.to(dev)].isnan().all()
+    check(dict(out=out[~hit.to(dev)], lse=lse[~hit.to(dev)]), {k: v[~hit] for k, v in ref.items()}, ("out", "lse"))
+
+
 @pytest.mark.parametrize("S,S_kv", [(0, 5), (5, 0), (0, 0), (3, 1)])
 @pytest.mark.parametrize("expanded", [False, True])
 def test_empty_and_single(dev, S, S_kv, expanded):
