@@ -19,6 +19,12 @@ def same_device(first, *rest):
             check_same_device(first, *rest)
 
 
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """``t`` if it is contiguous and 16-byte aligned, else a copy that is (``contiguous()`` leaves a misaligned tensor, and
+    any strides of axes of one, as they are)."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def launch_on(t: torch.Tensor):
     """(stream pointer, context) for a launch on ``t``'s device: the context makes that device current
     where another one is, as a launch on a stream of its own needs."""

@@ -71,7 +71,7 @@ def _strided(t, width, name):
     shape = t.shape
     assert len(shape) == 2 and shape[1] == width, f"{name} must be [tokens, {width}], got {tuple(shape)}"
     row, col = t.stride()
-    return t if col == 1 and row % 8 == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
+    return t if col == 1 and row % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def latent_cache_append(cache, latent, rope, slots):

@@ -28,7 +28,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..sparse_mla_ops._common import normalize_sm_scale, unwrap_quantized
-from ._common import launch_on, same_device
+from ._common import dense, launch_on, same_device
 
 _STRIDES = ctypes.c_int64 * 8
 
@@ -149,7 +149,7 @@ def _rows(t):
     up-projection are taken as they are), else a contiguous copy."""
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(0 <= s < 1 << 23 and s % 8 == 0 for s in t.stride()[1:-1]) \
         and t.stride(0) % 8 == 0
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _expanded_args(q, k_nope, k_pe, v):
@@ -217,7 +217,7 @@ class LatentMLA(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, kv, scaling=None, d_v=None, causal=None, starts=None, ends=None):
-        q, kv = unwrap_quantized(q).contiguous(), unwrap_quantized(kv).contiguous()
+        q, kv = dense(unwrap_quantized(q)), dense(unwrap_quantized(kv))
         ctx.args = dict(sm_scale=scaling, causal=causal)
         out, lse, *low = latent_mla_fwd_interface(q, kv, d_v=q.shape[-1] if d_v is None else d_v, starts=starts, ends=ends,
                                                   residual=any(ctx.needs_input_grad), **ctx.args)
@@ -232,7 +232,7 @@ class LatentMLA(torch.autograd.Function):
         if grad_output is None:
             return (None,) * 7
         q, kv, out, lse, starts, ends, low = ctx.saved_tensors
-        dq, dkv = latent_mla_bwd(q, kv, out, grad_output.contiguous(), lse, starts=starts, ends=ends, residual=low, **ctx.args)
+        dq, dkv = latent_mla_bwd(q, kv, out, dense(grad_output), lse, starts=starts, ends=ends, residual=low, **ctx.args)
         return dq, dkv, None, None, None, None, None
 
 
@@ -242,7 +242,7 @@ class LatentMLAExpanded(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k_nope, k_pe, v, scaling=None, causal=None, starts=None, ends=None):
-        q = q.contiguous()
+        q = dense(q)
         ctx.args = dict(sm_scale=scaling, causal=causal)
         out, lse, *low = latent_mla_expanded_fwd(q, k_nope, k_pe, v, starts=starts, ends=ends, residual=any(ctx.needs_input_grad),
                                                  **ctx.args)
@@ -257,6 +257,6 @@ class LatentMLAExpanded(torch.autograd.Function):
         if grad_output is None:
             return (None,) * 8
         q, k_nope, k_pe, v, out, lse, starts, ends, low = ctx.saved_tensors
-        grads = latent_mla_expanded_bwd(q, k_nope, k_pe, v, out, grad_output.contiguous(), lse, starts=starts, ends=ends, residual=low,
+        grads = latent_mla_expanded_bwd(q, k_nope, k_pe, v, out, dense(grad_output), lse, starts=starts, ends=ends, residual=low,
                                         **ctx.args)
         return (*grads, None, None, None, None)

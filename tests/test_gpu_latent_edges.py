@@ -186,6 +186,54 @@ def test_broadcast_and_misaligned_views(dev):
     assert ((g.double().cpu() - want).abs() <= tol + 2.0 ** -8 * ref["dk_nope"].abs().sum(2, keepdim=True)).all()
 
 
+def _off(t, dev):
+    """``t`` on the device, contiguous, 2 bytes past an aligned address."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=dev)[1:]
+    got = flat.view(t.shape).copy_(t)
+    assert got.is_contiguous() and got.data_ptr() % 16 == 2
+    return got
+
+
+@pytest.mark.parametrize("expanded", [False, True])
+def test_contiguous_but_misaligned(dev, expanded):
+    """Leaves, and an upstream gradient (that of a concatenation behind an odd number of values), 2 bytes off."""
+    gen = torch.Generator().manual_seed(61)
+    S, H = 66, 2
+    q, do = _normal(gen, 1, S, H, 128), _normal(gen, 1, S, H, 64)
+    x = [_normal(gen, 1, S, H, 64), _normal(gen, 1, S, 64), _normal(gen, 1, S, H, 64)] if expanded else [_normal(gen, 1, S, 1, 128)]
+    w = om.windows(1, S, S)
+    ref = om.expanded(q, *x, 0.1, *w, do) if expanded else om.absorbed(q, *x, 64, 0.1, *w, do)
+    leaves = [_off(t, dev).requires_grad_() for t in (q, *x)]
+    out, lse = ops.LatentMLAExpanded.apply(*leaves, 0.1) if expanded else ops.LatentMLA.apply(*leaves, 0.1, 64)
+    odd = torch.zeros(3, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    both = torch.cat([odd, out.flatten()])
+    grads = torch.autograd.grad(both, leaves, torch.cat([torch.zeros(3, dtype=torch.bfloat16), do.flatten()]).to(dev))
+    names = ("dq", "dk_nope", "dk_pe", "dv") if expanded else ("dq", "dkv")
+    check(dict(zip(names, grads)) | dict(out=out, lse=lse), ref, ("out", "lse", *names))
+
+
+def test_strides_of_axes_of_one(dev):
+    """One key, one token: the stride of an axis of one says nothing, whatever it is."""
+    gen = torch.Generator().manual_seed(62)
+    q, do = _normal(gen, 1, 1, 2, 128), _normal(gen, 1, 1, 2, 64)
+    x = [_normal(gen, 1, 1, 2, 64), _normal(gen, 1, 1, 64), _normal(gen, 1, 1, 2, 64)]
+    odd = [t.to(dev).as_strided(t.shape, (5, 1 << 24, *t.stride()[2:])) for t in x]
+    ref = om.expanded(q, *x, 0.1, *om.windows(1, 1, 1), do)
+    out, lse = ops.latent_mla_expanded_fwd(q.to(dev), *odd, 0.1)
+    got = ops.latent_mla_expanded_bwd(q.to(dev), *odd, out, do.to(dev), lse, 0.1)
+    names = ("out", "lse", "dq", "dk_nope", "dk_pe", "dv")
+    check(dict(zip(names, (out, lse, *got))), ref, names)
+    for d_qk, d_v in DIMS:       # one token's row of a wider projection, at an odd place; then several, packed but off
+        cache = ops.LatentCache.empty(1, 16, d_qk, d_v, "bf16", dev)
+        row = _normal(gen, 1, d_qk + 3)
+        on = row.to(dev)
+        ops.latent_cache_append(cache, on[:, 3:3 + d_v], on[:, 3 + d_v:], torch.tensor([4], device=dev))
+        assert torch.equal(cache.data[0, 4].cpu(), row[0, 3:])
+        rows = _normal(gen, 5, d_qk)
+        ops.latent_cache_append(cache, _off(rows[:, :d_v], dev), _off(rows[:, d_v:], dev), torch.arange(5, 10, device=dev))
+        assert torch.equal(cache.data[0, 5:10].cpu(), rows)
+
+
 def test_three_axes_are_a_batch_of_one(dev):
     gen = torch.Generator().manual_seed(3)
     q, kv, do = (_normal(gen, 60, 4, 128).to(dev), _normal(gen, 60, 1, 128).to(dev), _normal(gen, 60, 4, 64).to(dev))
