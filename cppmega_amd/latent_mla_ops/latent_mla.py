@@ -86,10 +86,11 @@ def _absorbed_dims(q, kv, d_v):
     return B, S, S_kv, H, G, D
 
 
-def latent_mla_fwd_interface(q, kv, sm_scale=None, d_v=512, causal=None, starts=None, ends=None, residual=False):
+def latent_mla_fwd_interface(q, kv, sm_scale=None, d_v=None, causal=None, starts=None, ends=None, residual=False):
     """Absorbed forward: (out, lse), with ``residual`` (out, lse, what rounding took from out, for the backward).
-    Arguments as in the module's description."""
+    Arguments as in the module's description; d_v: all channels where it is not given."""
     q, kv = unwrap_quantized(q), unwrap_quantized(kv)
+    d_v = q.shape[-1] if d_v is None else d_v
     squeeze = q.ndim == 3
     if squeeze:
         q, kv = _batched(q, kv)
@@ -219,8 +220,8 @@ class LatentMLA(torch.autograd.Function):
     def forward(ctx, q, kv, scaling=None, d_v=None, causal=None, starts=None, ends=None):
         q, kv = dense(unwrap_quantized(q)), dense(unwrap_quantized(kv))
         ctx.args = dict(sm_scale=scaling, causal=causal)
-        out, lse, *low = latent_mla_fwd_interface(q, kv, d_v=q.shape[-1] if d_v is None else d_v, starts=starts, ends=ends,
-                                                  residual=any(ctx.needs_input_grad), **ctx.args)
+        out, lse, *low = latent_mla_fwd_interface(q, kv, d_v=d_v, starts=starts, ends=ends, residual=any(ctx.needs_input_grad),
+                                                  **ctx.args)
         ctx.save_for_backward(q, kv, out, lse, starts, ends, *low)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)

@@ -234,6 +234,14 @@ def test_strides_of_axes_of_one(dev):
         assert torch.equal(cache.data[0, 5:10].cpu(), rows)
 
 
+def test_default_value_channels(dev):
+    gen = torch.Generator().manual_seed(63)
+    q, kv = _normal(gen, 1, 40, 2, 128).to(dev), _normal(gen, 1, 40, 1, 128).to(dev)
+    want = ops.latent_mla_fwd_interface(q, kv, d_v=128)
+    for got in (ops.latent_mla_fwd_interface(q, kv), ops.LatentMLA.apply(q, kv)):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_three_axes_are_a_batch_of_one(dev):
     gen = torch.Generator().manual_seed(3)
     q, kv, do = (_normal(gen, 60, 4, 128).to(dev), _normal(gen, 60, 1, 128).to(dev), _normal(gen, 60, 4, 64).to(dev))

@@ -55,6 +55,14 @@ def test_dense_arguments():
         _refused(AssertionError, ops.latent_mla_bwd, *a)
 
 
+def test_default_value_channels():
+    """Without d_v a row is its own value, in the functional form as in LatentMLA: no check before the device's refuses it."""
+    q, kv = _t(1, 4, 2, 128), _t(1, 4, 1, 128)
+    _refused(RuntimeError, ops.latent_mla_fwd_interface, q, kv)
+    _refused(RuntimeError, ops.latent_mla_fwd_interface, q[0], kv[0])
+    _refused(RuntimeError, ops.LatentMLA.apply, q, kv)
+
+
 def test_expanded_arguments():
     q, kn, pe, v = _t(1, 4, 2, 192), _t(1, 4, 2, 128), _t(1, 4, 64), _t(1, 4, 2, 128)
     f = ops.latent_mla_expanded_fwd
