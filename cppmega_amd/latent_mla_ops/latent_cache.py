@@ -5,11 +5,13 @@ A serving step of a latent-attention layer:
 
     plan = plan_latent_step(context_lens, query_lens, block_table, free_blocks, free_count, num_tokens, cache.block_size)
     latent_cache_append(cache, c_kv, k_pe, plan.slots)                     # every layer: the new tokens' rows
-    out, lse = paged_latent_mla_fwd(q, cache, plan.block_table, plan.kv_lens, plan.query_starts)
+    out, lse = paged_latent_mla_fwd(q, cache, plan.block_table, plan.kv_lens, plan.query_starts, sm_scale=scale)
     # next step: plan.context_lens, plan.block_table, plan.free_blocks, plan.free_count
 
 Nothing synchronises with the host, so a step of fixed sizes can be captured in a HIP
 graph.  (d_qk, d_v) in {(576, 512), (128, 64)}: the latent's d_v channels, then the rope part.
+``scale`` is the layer's: of the un-absorbed head, (d_nope + d_rope)^-0.5 (192^-0.5 where
+LatentMLAExpanded trained it with its default), not of the cached row.
 """
 from __future__ import annotations
 
@@ -174,7 +176,8 @@ def paged_latent_mla_fwd(q, cache, block_table, kv_lens, query_starts=None, sm_s
     the last of its kv_lens[r] positions, and each sees the positions up to its own; without query_starts token r is
     request r's one new token (decoding; T = R).  A page outside the cache hides its keys, and a token without keys
     (or with scores of -Inf alone) has out 0 and lse -inf.  Rows of tokens that belong to no request are not written: pass ``out`` and ``lse`` to keep
-    what they hold.  Keys that a token does not see may hold anything, Inf and NaN too.
+    what they hold.  Keys that a token does not see may hold anything, Inf and NaN too.  sm_scale None is d_qk^-0.5, of
+    the cached row's width: a layer whose scale is that of its un-absorbed heads (LatentMLAExpanded's default) passes its own.
     """
     q = unwrap_quantized(q)
     assert q.ndim == 3 and q.shape[2] == cache.d_qk, f"q must be [tokens, heads, {cache.d_qk}], got {tuple(q.shape)}"

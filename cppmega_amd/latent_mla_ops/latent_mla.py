@@ -10,6 +10,9 @@ attention) and layers without an indexer need it.
              head, v [B, S_kv, H, d_v]; (d_nope, d_v) in {(128, 128), (64, 64)}
   returns    (out [B, S, H, d_v] bf16, lse [B, S, H] f32, log2 units)
 
+The default scale is (width of q)^-0.5: the two forms of one layer have different widths,
+so the absorbed form of a layer trained expanded takes the expanded form's scale.
+
 3-D q / kv without the batch are accepted as SparseMLA accepts them.  Masks: ``causal``
 (query token t sees the keys up to position t + S_kv - S: the last S of S_kv tokens),
 every key (``causal=False``), or per-row key windows ``starts`` / ``ends`` [B, S] int32

@@ -597,6 +597,36 @@ def test_both_forms_are_one_attention(dev):
     assert (b[..., 64:] == 0).all()
 
 
+def test_trained_expanded_served_absorbed(dev):
+    """A layer in its expanded form at the default scale, and served from the cache at that scale: one attention.  (The cached
+    row's own width would give another scale.)"""
+    gen = torch.Generator().manual_seed(18)
+    S, H, r, dn, dr = 50, 3, 64, 128, 64
+    lat, pe, q = _normal(gen, S, r), _normal(gen, S, dr), _normal(gen, S, H, dn + dr)
+    wk = (torch.randn(H, dn, r, generator=gen) / 16).to(torch.bfloat16)
+    kn = torch.einsum("sr,hdr->shd", lat.double(), wk.double()).to(torch.bfloat16)
+    qa = torch.einsum("shd,hdr->shr", q[..., :dn].double(), wk.double()).to(torch.bfloat16)
+    v = torch.cat([lat[:, None].expand(S, H, r), torch.zeros(S, H, 128 - r, dtype=torch.bfloat16)], -1)
+    b, lse_b = (t[0] for t in ops.LatentMLAExpanded.apply(q[None].to(dev), kn[None].to(dev), pe[None].to(dev), v[None].to(dev)))
+    cache = ops.LatentCache.empty(4, 16, 128, 64, "bf16", dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    plan = ops.plan_latent_step(i32([0]), i32([S]), i32([[-1] * 4]), i32([2, 0, 3, 1]), i32([4]), S, 16)
+    ops.latent_cache_append(cache, lat.to(dev), pe.to(dev), plan.slots)
+    scale = (dn + dr) ** -0.5
+    a, lse_a = ops.paged_latent_mla_fwd(torch.cat([qa, q[..., dn:]], -1).to(dev), cache, plan.block_table, plan.kv_lens,
+                                        plan.query_starts, sm_scale=scale)
+    # qa and kn are each rounded once: a score moves by at most 2^-8 of sum |q| |k| on either side
+    seen = torch.ones(S, S).tril().bool()
+    move = (torch.einsum("shd,thd->hst", q[..., :dn].double().abs(), kn.double().abs())
+            + torch.einsum("shr,tr->hst", qa.double().abs(), lat.double().abs())) * 2.0 ** -8 * scale
+    eps = move.masked_fill(~seen, 0).amax(-1).T * 1.01
+    ref = om.absorbed(torch.cat([qa, q[..., dn:]], -1)[None], torch.cat([lat, pe], -1)[None, :, None], 64, scale, *om.windows(1, S, S))
+    big = lat.double().abs().amax()
+    assert ((lse_a.double().cpu() - lse_b.double().cpu()).abs() <= eps / 0.6931 + 2 * ref["e_lse"][0] + 1e-5).all()
+    assert ((a.double().cpu() - b[..., :64].double().cpu()).abs()
+            <= torch.expm1(2 * eps)[..., None] * big + 2 * ref["e_out"][0] + 2.0 ** -8 * big).all()
+
+
 def test_residual_is_what_rounding_took(dev):
     """out + residual is the output to 2^-17 beyond the products' own error, and with it the gradients' error falls to that
     of the weights' and the results' rounding (two of them, each at most half a step)."""
