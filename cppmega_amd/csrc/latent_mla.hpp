@@ -196,6 +196,22 @@ __device__ __forceinline__ void stream_operands(const OperandsOf<G> &first, Load
   }
 }
 
+// Whether a lane of the workgroup's NW waves has x: by the first NW words of LDS at `words`, free before and after
+// (__syncthreads_or takes 256 bytes of its own beside what a kernel asks for).
+template <int NW>
+__device__ __forceinline__ bool any_wave(bool x, unsigned char *words) {
+  int *at = reinterpret_cast<int *>(words);
+  const int mine = wv::ballot(x) != 0ull;
+  if (lane_id() == 0) at[wave_id()] = mine;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) any |= at[i];
+  __syncthreads();  // read: they may be written again
+  return __builtin_amdgcn_readfirstlane(any) != 0;
+}
+constexpr int kLdsOfCu = 160 * 1024;
+
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 // Tile dt of a row per lane pair (l, l + 32) as bf16, v[m] its columns acc_col(dt, 4 m, l / 32) .. + 3 (m and m + 1: 16 that lie together):
 // halves exchanged, so that a lane stores 16 bytes (8 at a time, the forward's results took a tenth of its time).

@@ -14,10 +14,12 @@
 // product; l sums the weights before that rounding.
 //
 // Bound by the MFMAs and the softmax beside them, which overlap across the two or three
-// waves of a SIMD only.  Causal, 4096 tokens: 128 / 64 absorbed, batch 2, 32 heads, 224 us
-// (920 TFLOP/s of the admitted pairs); 192 / 128 expanded, 128 heads, 975 us (705); a large
-// product runs at 1173.  Of these 5 and 20 us go to out_lo, what rounding took from out.
-// 32 rows a wave (RT 1): with 64 the operands do not fit beside O.
+// waves of a SIMD only.  Causal, 4096 tokens: 128 / 64 absorbed, batch 2, 32 heads, 222 us
+// (930 TFLOP/s of the admitted pairs); 192 / 128 expanded, 128 heads, 707 us (970; 946 us when
+// 336 bytes more of LDS left room for one workgroup a CU); a large product runs at 1173.
+// Of these 5 and 20 us go to out_lo, what rounding took from out.
+// 32 rows a wave (RT 1): with 64, Q, O, the scores and an operand group take 190 (128 / 64)
+// to 290 registers (192 / 128), which leaves a SIMD two waves or one.
 #include <type_traits>
 
 #include "latent_mla.hpp"
@@ -31,14 +33,15 @@ struct LatentFwd {
   static constexpr int K_BYTES = 2 * KP * 4096, V_BYTES = SHARED ? 0 : 2 * VP * 4096;
   static constexpr int BUF = K_BYTES + V_BYTES;
   static constexpr int ROWS = NW * RT * 32;
-  static constexpr int OFF_SPAN = 2 * BUF;             // [NW][4] the waves' spans, then one flag
-  static constexpr int BYTES = OFF_SPAN + NW * 16 + 16;
+  static constexpr int BYTES = 2 * BUF;                // (the waves' spans lie in the first buffer before a tile does)
 };
 
+// OCC workgroups a CU.
 template <int DK, int DN, int DV, int RT, int NW, int OCC>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) latent_fwd_kernel(const LatentParams p) {
   using C = LatentFwd<DK, DN, DV, RT, NW>;
   constexpr int KS = DK / 16, NDT = DV / 32;
+  static_assert(NW == 4 && OCC * C::BYTES <= kLdsOfCu, "a wave a SIMD and workgroup; LDS of all of them (no static LDS beside it)");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const int nblk = (int)((p.rows + C::ROWS - 1) / C::ROWS);
@@ -46,7 +49,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
   spread_items(blockIdx.x, p.B * p.G, nblk, bg, index);
   const int64_t b = bg / p.G, g = bg - b * p.G;
   const int blk = nblk - 1 - (int)index;  // the causal mask's longest first
-  int *span_lds = reinterpret_cast<int *>(smem + C::OFF_SPAN);
+  int *span_lds = reinterpret_cast<int *>(smem);
 
   // this lane's rows
   int lo[RT], hi[RT];
@@ -82,6 +85,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
     klo = min(klo, span_lds[2 * i]);
     khi = max(khi, span_lds[2 * i + 1]);
   }
+  __syncthreads();  // read: a tile may lie there
   klo = __builtin_amdgcn_readfirstlane(klo);
   khi = __builtin_amdgcn_readfirstlane(khi);
   const int t0 = khi > klo ? klo / kKeyTile : 0, t1 = khi > klo ? (khi + kKeyTile - 1) / kKeyTile : 0;
@@ -205,7 +209,7 @@ if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) bad |= not_finite(o[rt][dt][i]);
-  if (__syncthreads_or(bad)) pass(std::true_type{});  // a masked Inf or NaN may have reached a row: once more, without it
+  if (any_wave<NW>(bad, smem)) pass(std::true_type{});  // a masked Inf or NaN may have reached a row: once more, without it
 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
