@@ -97,7 +97,8 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
 // the one that is worked on, shared by the waves in three LDS buffers, one barrier a step; three workgroups a CU.
 //   S^T = K Q^T, O^T += V^T P^T on 32x32x16 MFMAs, lane = row.
 // Bound by the MFMAs and the softmax beside them: prefill of 6 requests, 40 .. 512 tokens each on 1024 .. 4096 keys, 32
-// heads, MXFP4: 111 us, 325 TFLOP/s.  Widening the codes costs a sixth (decode of 128 heads: 94 us against 79 in bf16).
+// heads, MXFP4: 83 us, 430 TFLOP/s (two workgroups a CU: 112).  Widening the codes costs a sixth (decode of 128 heads: 76 us
+// against 64 in bf16).
 template <int NT, bool FP4>
 struct Paged {
   static constexpr int D_QK = 128, D_V = 64;
@@ -109,16 +110,19 @@ struct Paged {
   static constexpr int PANELS = D_QK / 64, TILE = PANELS * 4096, STEP = TILES * TILE;
   static constexpr int DMA = TILES * PANELS;                  // bf16: loads of a wave per step (an 8-row group a tile)
   static constexpr int NB = D_V / 32, CODES = KEYS * NB;      // MXFP4: code pieces of a row, of a step (one to a thread)
-  static constexpr int OFF_T = NBUF * STEP;
-  static constexpr int OFF_ML = OFF_T + kWindow * 4;          // [NW][32][2]
-  static constexpr int BYTES = OFF_ML + NW * 32 * 8;
+  static constexpr int OFF_T = NBUF * STEP;                   // table entries, then words of any_wave
+  static constexpr int WINDOW = 1024 - 16, OFF_ANY = OFF_T + WINDOW * 4;
+  static constexpr int BYTES = OFF_ANY + 16 * 4;
   static constexpr int O_BYTES = D_V * 32 * 4;                // a wave's O
-  static_assert(BYTES <= 64 * 1024 && (KG == 1 || (NW / 2) * O_BYTES <= OFF_T), "LDS");
+  static constexpr int OFF_ML = (NW / 2) * O_BYTES;           // [NW / 2][32][2], behind the O that lie over the tiles
+  static constexpr int WGS = 3;                               // workgroups a CU (LDS by blocks of at most 2 KiB)
+  static_assert(WGS * ((BYTES + 2047) / 2048 * 2048) <= kLdsOfCu && OFF_ML + (NW / 2) * 32 * 8 <= OFF_T, "LDS");
+  static_assert(KEYS * (AHEAD + 2) < WINDOW, "the steps that are asked for lie in the window, also where pages have one row");
   static_assert(CODES % 64 == 0 && CODES <= 256, "code pieces by whole waves");
 };
 
 template <int NT, bool FP4>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) paged_rows_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Paged<NT, FP4>::WGS))) paged_rows_kernel(const PagedParams p) {
   using C = Paged<NT, FP4>;
   using Row = typename C::Row;
   constexpr int D_QK = C::D_QK, D_V = C::D_V, KS = C::KS, NDT = C::NDT;
@@ -173,7 +177,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
         const int pages = lim > 0 ? page_of(lim - 1) + 1 : 0;
         bool ok = true;
         __syncthreads();  // the window's readers are done
-        for (int i = (int)threadIdx.x; i < kWindow; i += 256) {
+        for (int i = (int)threadIdx.x; i < C::WINDOW; i += 256) {
           const int pg = base + i;
           int e = -1;
           if (pg < pages) {
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
           }
           window[i] = e;
         }
-        all_there = __syncthreads_and(ok) != 0;
+        all_there = !any_wave<C::NW>(!ok, smem + C::OFF_ANY);  // (its barriers stand behind the entries too)
       };
       // row of a key, by the window
       auto key_at = [&](int key) -> const unsigned char * {
@@ -295,7 +299,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
       int buf = 0;
       for (int j = x.b0; j < j1; ++j) {
         // what is asked for in this step lies in the window, and what is masked in it
-        if (page_of((j + C::AHEAD + 2) * C::KEYS - 1) >= base + kWindow && page_of(lim - 1) >= base + kWindow) refill(page_of(j * C::KEYS));
+        if (page_of((j + C::AHEAD + 2) * C::KEYS - 1) >= base + C::WINDOW && page_of(lim - 1) >= base + C::WINDOW) refill(page_of(j * C::KEYS));
         const unsigned char *S = smem + buf * C::STEP;
         const int nxt = buf + 1 == C::NBUF ? 0 : buf + 1;
         if constexpr (FP4) {
@@ -323,7 +327,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) bad |= not_finite(o[dt][i]);
-        if (__syncthreads_or(bad)) {
+        if (any_wave<C::NW>(bad, smem + C::OFF_ANY)) {
           probe = false;
           ta = tb = tok0;
           continue;
@@ -503,7 +507,7 @@ static PagedPlan paged_plan(int64_t T, int64_t R, int64_t W, int64_t block, int6
   r.max_units = (int)(T * H / r.unit_rows + R);
   const int64_t blocks = (int64_t)r.max_units * ((W * block + r.step_keys - 1) / r.step_keys);
   const int64_t n = (blocks + r.min_blocks - 1) / r.min_blocks;
-  const int64_t most = d_qk == 128 ? 768 : 256;  // resident workgroups
+  const int64_t most = 256 * (d_qk == 128 ? Paged<4, true>::WGS : 1);  // resident workgroups (few rows: as many fit)
   r.nwg = (int)(n < 1 ? 1 : (n < most ? n : most));
   return r;
 }
