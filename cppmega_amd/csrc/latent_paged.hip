@@ -475,15 +475,14 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
 //               more             units of 128: 128 heads 229; of 64: 260
 //   576, MXFP4  up to 32 rows    units of 32: 16 heads 103, 32 heads 107; of 64: 144, 146
 //               more             units of 64: 64 heads 158, 128 heads 274; of 32: 177, 309
-//   128, bf16   up to 16 rows    waves that split the keys, 16 rows: 16 heads 41; 32: 50; units of 64: 58
-//               up to 32         32 rows: 32 heads 56; 16: 59; units of 64: 60
-//               up to 64         units of 64: 64 heads 63; of 128: 70; 32 rows: 78
-//               more             units of 128: 128 heads 79; of 64: 86
-//   128, MXFP4  up to 64 rows    16 rows: 16 heads 37, 64 heads 78; units of 128: 83, 88
-//               more             units of 128: 128 heads 94; 16 rows: 128
+//   128, bf16   up to 16 rows    waves that split the keys, 16 rows: 16 heads 40; units of 64: 49
+//               up to 64         units of 64: 32 heads 50, 64 heads 53; of 128: 54, 56; 16 rows: 59, 97
+//               more             units of 128: 128 heads 64; of 64: 73
+//   128, MXFP4  up to 32 rows    16 rows: 16 heads 37, 32 heads 49; units of 128: 63, 65
+//               more             units of 128: 64 heads 69, 128 heads 76; 16 rows: 78, 129
 struct PagedPlan {
   int wide;       // 576 / 512: 16-row tiles of a unit
-  int few;        // 128 / 64: 16-row tiles of a unit whose waves split the keys
+  bool few;       // 128 / 64: 16 rows a unit, whose waves split the keys
   int nt;         // 128 / 64: else 32-row tiles of a unit
   int unit_rows, step_keys, max_units, nwg, min_blocks;
 };
@@ -494,9 +493,9 @@ static PagedPlan paged_plan(int64_t T, int64_t R, int64_t W, int64_t block, int6
     r.wide = fp4 ? (rows <= 32 ? 2 : 4) : (rows <= 64 ? 4 : 8);
     r.unit_rows = 16 * r.wide;
     r.step_keys = paged_wide_keys();
-  } else if (rows <= (fp4 ? 64 : 32)) {
-    r.few = fp4 || rows <= 16 ? 1 : 2;
-    r.unit_rows = 16 * r.few;
+  } else if (rows <= (fp4 ? 32 : 16)) {
+    r.few = true;
+    r.unit_rows = 16;
     r.step_keys = 32;
   } else {
     r.nt = fp4 || rows > 64 ? 4 : 2;
@@ -568,7 +567,7 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
   int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
   if (rc) return rc;
   if (k.wide) rc = launch_paged_wide(p, k.wide, fp4, st);
-  else if (k.few) rc = launch_paged_few(p, k.few, fp4, st);
+  else if (k.few) rc = launch_paged_few(p, fp4, st);
   else if (k.nt == 4) rc = fp4 ? launch<4, true>(p, st) : launch<4, false>(p, st);
   else rc = launch<2, false>(p, st);
   if (rc || p.nwg == 1) return rc;  // one workgroup: no unit has several pieces

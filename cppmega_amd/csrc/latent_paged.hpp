@@ -124,7 +124,7 @@ constexpr int vmcnt_only(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
 
 int paged_wide_keys();  // keys of a step
 int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
-int launch_paged_few(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
+int launch_paged_few(const PagedParams &p, bool fp4, hipStream_t st);
 
 // The blocks of all units can be numbered in 32 bits, whatever the lengths.
 bool paged_countable(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk);

@@ -1,10 +1,10 @@
-// Latent attention over a paged cache, rows of 128 channels (64 latent), for units of at
-// most 32 rows (MXFP4: 16 rows, used for up to 64): bound by reading the cache, so nothing
-// is shared that would make a wave wait for another.
+// Latent attention over a paged cache, rows of 128 channels (64 latent), for units of 16
+// rows: bound by reading the cache, so nothing is shared that would make a wave wait for
+// another.
 //
 // The four waves of a workgroup take the unit's 32-key blocks in turn, each in its own
-// LDS tile, with all rows' Q and O in its registers:
-//   S^T[key][row] = K Q^T    on 16x16x32 MFMAs (16 rows a tile; lane = row, 8 of the keys)
+// LDS tile, with the rows' Q and O in its registers:
+//   S^T[key][row] = K Q^T    on 16x16x32 MFMAs (lane = row, 8 of the keys)
 //   running maximum and sum per lane (two exchanges a block), P^T the operand as it stands
 //   O^T[d][row] += V^T P^T   (V^T by transposed reads of the tile)
 // No barrier until a piece's end, where the waves' O are brought to one maximum and added
@@ -19,11 +19,11 @@
 
 namespace dsa {
 
-template <int NR, bool FP4>
+template <bool FP4>
 struct PagedFew {
   static constexpr int D_QK = 128, D_V = 64;
   using Row = CacheRow<D_QK, D_V, FP4>;
-  static constexpr int NW = 4, ROWS = 16 * NR;
+  static constexpr int NW = 4, ROWS = 16;
   static constexpr int KS = D_QK / 32, NDT = D_V / 16;    // k-steps, 16-channel tiles of O
   static constexpr int PANELS = D_QK / 64, TILE = PANELS * 4096;
   static constexpr int O_ROW = D_V + 4;                   // floats of an O row in LDS
@@ -31,12 +31,12 @@ struct PagedFew {
   static constexpr int CPL = NB / 2;                      // 16-byte pieces of codes per lane
   static constexpr int OFF_ML = NW * TILE;                // [NW][ROWS][2]
   static constexpr int BYTES = OFF_ML + NW * ROWS * 8;
-  static_assert(16 * O_ROW * 4 <= TILE && BYTES <= 159 * 1024, "LDS");
+  static_assert(ROWS * O_ROW * 4 <= TILE, "a wave's O over its tile");
 };
 
-template <int NR, bool FP4>
+template <bool FP4>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) paged_few_kernel(const PagedParams p) {
-  using C = PagedFew<NR, FP4>;
+  using C = PagedFew<FP4>;
   using Row = typename C::Row;
   constexpr int D_QK = C::D_QK, D_V = C::D_V;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -69,13 +69,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
     const int tok0 = first / p.H, tok1 = (first + nrows - 1) / p.H;
     const int32_t *table = x.table;
 
-    i32x4 q[NR][C::KS];
+    i32x4 q[C::KS];
+    const unsigned char *src = (l16 < nrows ? p.q + (row0 + l16) * D_QK * 2 : zero) + 16 * g16;
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) {
-      const unsigned char *src = (16 * rt + l16 < nrows ? p.q + (row0 + 16 * rt + l16) * D_QK * 2 : zero) + 16 * g16;
-#pragma unroll
-      for (int ks = 0; ks < C::KS; ++ks) q[rt][ks] = ld_row_16(src + 64 * ks);
-    }
+    for (int ks = 0; ks < C::KS; ++ks) q[ks] = ld_row_16(src + 64 * ks);
 
     // Tokens [ta, tb] with the keys cut at tb's: all at once, or, where that left something that is not finite, one by
     // one, since a weight of zero does not remove the Inf or NaN of a later token's key.
@@ -84,18 +81,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
     while (true) {
       const int lim = token_keys(kv, n, tb), lim_min = token_keys(kv, n, ta);
       const int j1 = min(b1, (lim + 31) / 32);
-      int my_lim[NR];
-      float m_run[NR], l_run[NR];
-      f32x4 o[NR][C::NDT];
+      const int my_lim = token_keys(kv, n, min((first + l16) / p.H, tb));
+      float m_run = kNegBig, l_run = 0.0f;
+      f32x4 o[C::NDT];
 #pragma unroll
-      for (int rt = 0; rt < NR; ++rt) {
-        const int t = (first + 16 * rt + l16) / p.H;
-        my_lim[rt] = token_keys(kv, n, t < tb ? t : tb);
-        m_run[rt] = kNegBig;
-        l_run[rt] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < C::NDT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
+      for (int dt = 0; dt < C::NDT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       // MXFP4, a block ahead in registers: code pieces (row, blk), their rows' exponent bytes, the rope part
       i32x4 codes[FP4 ? C::CPL : 1], rope[FP4 ? 4 : 1];
       uint32_t expo[FP4 ? C::CPL : 1];
@@ -157,61 +147,49 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
           __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the tile
           wave_lds_sync();
         }
-        f32x4 s[2][NR];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int rt = 0; rt < NR; ++rt) s[h][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 s[2]{{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int ks = 0; ks < C::KS; ++ks)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const i32x4 a = *reinterpret_cast<const i32x4 *>(K + (ka[h][ks & 1] ^ panel_swz(ks >> 1)) + (ks >> 1) * 4096);
-#pragma unroll
-            for (int rt = 0; rt < NR; ++rt)
-              s[h][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(q[rt][ks]), s[h][rt], 0, 0, 0);
+            s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(q[ks]), s[h], 0, 0, 0);
           }
-        i32x4 pb[NR];
+        if (vm != 0xffffffffu || 32 * j + 32 > lim_min) {
 #pragma unroll
-        for (int rt = 0; rt < NR; ++rt) {
-          if (vm != 0xffffffffu || 32 * j + 32 > lim_min) {
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int k = 8 * g16 + 4 * h + i;
-                if (!((vm >> k) & 1u) || 32 * j + k >= my_lim[rt]) s[h][rt][i] = -INFINITY;
-              }
-          }
-          float mx = s[0][rt][0];
-#pragma unroll
-          for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][rt][i & 3]);
-          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-          mx = max_halves(mx) * p.sl2;
-          if (wv::ballot(mx > m_run[rt] + 8.0f) != 0ull) {
-            const float m_new = fmaxf(m_run[rt], mx), alpha = exp2_fast(m_run[rt] - m_new);
-            m_run[rt] = m_new;
-            l_run[rt] *= alpha;
-#pragma unroll
-            for (int dt = 0; dt < C::NDT; ++dt) o[rt][dt] *= alpha;
-          }
-          float t[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            t[i] = exp2_fast(fmaf(s[i >> 2][rt][i & 3], p.sl2, -m_run[rt]));
-            l_run[rt] += t[i];
-          }
-          pb[rt] = i32x4{(int)pack_bf16x2(t[0], t[1]), (int)pack_bf16x2(t[2], t[3]), (int)pack_bf16x2(t[4], t[5]),
-                         (int)pack_bf16x2(t[6], t[7])};
+            for (int i = 0; i < 4; ++i) {
+              const int k = 8 * g16 + 4 * h + i;
+              if (!((vm >> k) & 1u) || 32 * j + k >= my_lim) s[h][i] = -INFINITY;
+            }
         }
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = max_halves(mx) * p.sl2;
+        if (wv::ballot(mx > m_run + 8.0f) != 0ull) {
+          const float m_new = fmaxf(m_run, mx), alpha = exp2_fast(m_run - m_new);
+          m_run = m_new;
+          l_run *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < C::NDT; ++dt) o[dt] *= alpha;
+        }
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          t[i] = exp2_fast(fmaf(s[i >> 2][i & 3], p.sl2, -m_run));
+          l_run += t[i];
+        }
+        const i32x4 pb{(int)pack_bf16x2(t[0], t[1]), (int)pack_bf16x2(t[2], t[3]), (int)pack_bf16x2(t[4], t[5]),
+                       (int)pack_bf16x2(t[6], t[7])};
 #pragma unroll
         for (int dt = 0; dt < C::NDT; ++dt) {
           const i32x2 r0 = ds_read_tr16(K + (va[0][dt & 3] ^ panel_swz(dt >> 2)) + (dt >> 2) * 4096);
           const i32x2 r1 = ds_read_tr16(K + (va[1][dt & 3] ^ panel_swz(dt >> 2)) + (dt >> 2) * 4096);
           const i32x4 a{r0[0], r0[1], r1[0], r1[1]};
-#pragma unroll
-          for (int rt = 0; rt < NR; ++rt)
-            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(pb[rt]), o[rt][dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(pb), o[dt], 0, 0, 0);
         }
         wave_lds_sync();  // the tile is read: it may be written again
       }
@@ -219,11 +197,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
       if (probe) {
         bool bad = false;
 #pragma unroll
-        for (int rt = 0; rt < NR; ++rt)
+        for (int dt = 0; dt < C::NDT; ++dt)
 #pragma unroll
-          for (int dt = 0; dt < C::NDT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= (__float_as_uint(o[rt][dt][e]) & 0x7f800000u) == 0x7f800000u;
+          for (int e = 0; e < 4; ++e) bad |= (__float_as_uint(o[dt][e]) & 0x7f800000u) == 0x7f800000u;
         if (__syncthreads_or(bad)) {
           probe = false;
           ta = tb = tok0;
@@ -231,72 +207,64 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
         }
       }
       // the waves' sums, by row
-#pragma unroll
-      for (int rt = 0; rt < NR; ++rt) {
-        float l = l_run[rt];
-        l += __shfl_xor(l, 16, 64);
-        l = sum_halves(l);
-        if (g16 == 0) {
-          ML[(w * C::ROWS + 16 * rt + l16) * 2] = m_run[rt];
-          ML[(w * C::ROWS + 16 * rt + l16) * 2 + 1] = l;
-        }
+      l_run += __shfl_xor(l_run, 16, 64);
+      l_run = sum_halves(l_run);
+      if (g16 == 0) {
+        ML[(w * C::ROWS + l16) * 2] = m_run;
+        ML[(w * C::ROWS + l16) * 2 + 1] = l_run;
       }
       const int rlo = ta * p.H - first, rhi = min((tb + 1) * p.H - first, nrows);  // rows of tokens [ta, tb]
+      float *mine_o = reinterpret_cast<float *>(K);
 #pragma unroll
-      for (int rt = 0; rt < NR; ++rt) {
-        float *mine_o = reinterpret_cast<float *>(K);
+      for (int dt = 0; dt < C::NDT; ++dt) *reinterpret_cast<f32x4 *>(mine_o + l16 * C::O_ROW + dt * 16 + 4 * g16) = o[dt];
+      __syncthreads();  // every wave's O tile and sums
+      constexpr int QUADS = C::ROWS * D_V / 4;
+      for (int x = (int)threadIdx.x; x < QUADS; x += 256) {
+        const int ur = x / (D_V / 4), d = (x - ur * (D_V / 4)) * 4;
+        if (ur < rlo || ur >= rhi) continue;
+        float m = kNegBig, l = 0.0f;
 #pragma unroll
-        for (int dt = 0; dt < C::NDT; ++dt) *reinterpret_cast<f32x4 *>(mine_o + l16 * C::O_ROW + dt * 16 + 4 * g16) = o[rt][dt];
-        __syncthreads();  // every wave's O tile and sums
-        constexpr int QUADS = 16 * D_V / 4;
-        for (int x = (int)threadIdx.x; x < QUADS; x += 256) {
-          const int r = x / (D_V / 4), d = (x - r * (D_V / 4)) * 4, ur = 16 * rt + r;
-          if (ur < rlo || ur >= rhi) continue;
-          float m = kNegBig, l = 0.0f;
+        for (int k = 0; k < C::NW; ++k)
+          if (ML[(k * C::ROWS + ur) * 2 + 1] != 0.0f) m = fmaxf(m, ML[(k * C::ROWS + ur) * 2]);
+        f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int k = 0; k < C::NW; ++k)
-            if (ML[(k * C::ROWS + ur) * 2 + 1] != 0.0f) m = fmaxf(m, ML[(k * C::ROWS + ur) * 2]);
-          f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int k = 0; k < C::NW; ++k) {
-            const float lk = ML[(k * C::ROWS + ur) * 2 + 1];
-            if (lk == 0.0f) continue;  // the wave saw no key of the row (a NaN sum joins)
-            const float a = exp2_fast(ML[(k * C::ROWS + ur) * 2] - m);
-            l += lk * a;
-            sum += a * *reinterpret_cast<const f32x4 *>(smem + k * C::TILE + (r * C::O_ROW + d) * 4);
-          }
-          if (whole_unit) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            *reinterpret_cast<i32x2 *>(p.out + (row0 + ur) * D_V + d) =
-                i32x2{(int)pack_bf16x2(sum[0] * inv, sum[1] * inv), (int)pack_bf16x2(sum[2] * inv, sum[3] * inv)};
-            if (d == 0) p.lse[row0 + ur] = l == 0.0f ? -INFINITY : log2f(l) + m;
-          } else {
-            if (l != 0.0f) *reinterpret_cast<f32x4 *>(p.part_o + (piece * C::ROWS + ur) * D_V + d) = sum;
-            if (d == 0) {
-              p.part_ml[(piece * C::ROWS + ur) * 2] = m;
-              p.part_ml[(piece * C::ROWS + ur) * 2 + 1] = l;
-            }
+        for (int k = 0; k < C::NW; ++k) {
+          const float lk = ML[(k * C::ROWS + ur) * 2 + 1];
+          if (lk == 0.0f) continue;  // the wave saw no key of the row (a NaN sum joins)
+          const float a = exp2_fast(ML[(k * C::ROWS + ur) * 2] - m);
+          l += lk * a;
+          sum += a * *reinterpret_cast<const f32x4 *>(smem + k * C::TILE + (ur * C::O_ROW + d) * 4);
+        }
+        if (whole_unit) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          *reinterpret_cast<i32x2 *>(p.out + (row0 + ur) * D_V + d) =
+              i32x2{(int)pack_bf16x2(sum[0] * inv, sum[1] * inv), (int)pack_bf16x2(sum[2] * inv, sum[3] * inv)};
+          if (d == 0) p.lse[row0 + ur] = l == 0.0f ? -INFINITY : log2f(l) + m;
+        } else {
+          if (l != 0.0f) *reinterpret_cast<f32x4 *>(p.part_o + (piece * C::ROWS + ur) * D_V + d) = sum;
+          if (d == 0) {
+            p.part_ml[(piece * C::ROWS + ur) * 2] = m;
+            p.part_ml[(piece * C::ROWS + ur) * 2 + 1] = l;
           }
         }
-        __syncthreads();  // read: the tiles may be written again
       }
+      __syncthreads();  // read: the tiles may be written again
       if (tb == tok1) break;
       ta = ++tb;
     }
   }
 }
 
-template <int NR, bool FP4>
+template <bool FP4>
 static int launch(const PagedParams &p, hipStream_t st) {
-  using C = PagedFew<NR, FP4>;
+  using C = PagedFew<FP4>;
   static_assert(C::BYTES <= 64 * 1024, "LDS of an ordinary launch");
-  hipLaunchKernelGGL((paged_few_kernel<NR, FP4>), dim3((unsigned)p.nwg), dim3(256), C::BYTES, st, p);
+  hipLaunchKernelGGL((paged_few_kernel<FP4>), dim3((unsigned)p.nwg), dim3(256), C::BYTES, st, p);
   return check_launch("dsa_paged_latent_mla_fwd");
 }
 
-int launch_paged_few(const PagedParams &p, int tiles16, bool fp4, hipStream_t st) {
-  if (fp4) return launch<1, true>(p, st);
-  return tiles16 == 1 ? launch<1, false>(p, st) : launch<2, false>(p, st);
+int launch_paged_few(const PagedParams &p, bool fp4, hipStream_t st) {
+  return fp4 ? launch<true>(p, st) : launch<false>(p, st);
 }
 
 }  // namespace dsa
