@@ -34,7 +34,9 @@ struct PagedWide {
   static constexpr int CW = ROLES ? 4 : 8, LW = ROLES ? 4 : 8, KG = CW / RG;  // computing, loading waves
   static constexpr int SUB = 2 / KG;                         // tiles of a computing wave
   static constexpr int PANELS = 9, TILE = PANELS * 4096, STEP = 2 * TILE;
-  static constexpr int GROUP = 2;                            // operands read at once (3, 4: registers spill)
+  // operands read at once (3, 4: registers spill in the step; 2: none does there, MXFP4 with RG 2 spills 21 around a piece's
+  // joining and the window's refill)
+  static constexpr int GROUP = 2;
   static constexpr int KS = 18, NDT = 32;
   static constexpr int TPR = 4, CPT = 16 / TPR, RPT = 8 / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
   static constexpr int OFF_T = 2 * STEP;
