@@ -148,6 +148,29 @@ def test_empty_and_single(dev, S, S_kv, expanded):
               ("out", "lse", "dq", "dkv"))
 
 
+@pytest.mark.parametrize("poison", [False, True])
+def test_more_row_tiles_than_a_search_holds(dev, poison):
+    """Key gradients from 68 row tiles in one workgroup (128 heads: unsplit), few of which admit its keys: the search passes
+    its 64 tiles, and with NaN in rows without keys it begins anew for the careful pass."""
+    gen = torch.Generator().manual_seed(65)
+    S, S_kv, H, heads = 4300, 256, 128, [0, 77, 127]
+    starts, ends = torch.zeros(1, S, dtype=torch.int32), torch.zeros(1, S, dtype=torch.int32)
+    for a, b, lo, hi in ((10, 150, 0, 100), (4170, 4200, 128, 250), (4230, 4290, 30, 120)):
+        starts[:, a:b], ends[:, a:b] = lo, hi
+    m = dict(starts=starts, ends=ends)
+    q, do = _normal(gen, 1, S, H, 128), _normal(gen, 1, S, H, 64)
+    x = [_normal(gen, 1, S_kv, H, 64), _normal(gen, 1, S_kv, 64), _normal(gen, 1, S_kv, H, 64)]
+    some = lambda t: t[:, :, heads] if t.ndim == 4 else t  # noqa: E731
+    ref = om.expanded(some(q), *(some(t) for t in x), 0.1, *om.windows(1, S, S_kv, **m), some(do))
+    if poison:
+        for t in (q, do):
+            t[:, [0, 151, 4169, 4201, 4229, 4299]] = NAN
+    got = run_expanded(dev, q, *x, do, 0.1, m)
+    names = ("dq", "dk_nope", "dv")
+    check({n: got[n][:, :, heads] for n in names}, ref, names)
+    assert torch.isfinite(got["dk_pe"].float()).all()
+
+
 def test_large_scores(dev):
     """Scores of hundreds: the running maximum moves, weights underflow, lse stays exact to its bound."""
     gen = torch.Generator().manual_seed(2)
@@ -434,6 +457,26 @@ def test_starts_out_of_order_stay_in_bounds(dev):
     out, lse = ops.paged_latent_mla_fwd(q.to(dev), cache, table.to(dev), kv.to(dev), starts.to(dev), sm_scale=0.1)
     torch.cuda.synchronize()
     assert out.shape == (6, 4, 64)
+
+
+@pytest.mark.parametrize("d_qk,d_v", DIMS)
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("H", [4, 100])
+def test_sound_requests_beside_bad_starts(dev, d_qk, d_v, fmt, H):
+    """Negative starts, starts past the batch and one that falls claim no token: the two sound requests have their results,
+    and nothing is written around them."""
+    gen = torch.Generator().manual_seed(H)
+    cache, table, kv, _, q = _paged_case(dev, gen, fmt, d_qk, d_v, H, [50, 60, 170, 40, 30], [1, 3, 4, 1, 1], 16)
+    T = 7
+    q = q[:T].contiguous()
+    starts = torch.tensor([-9, 0, 3, T, 900, -3], dtype=torch.int32)
+    ref = oc.paged(q, _cache_rows(cache), table[1:3], torch.tensor([0, 3, T]), kv[1:3], 16, d_v, 0.1)
+    out = torch.full((T + 16, H, d_v), 7.0, dtype=torch.bfloat16, device=dev)
+    lse = torch.full((T + 16, H), -7.0, device=dev)
+    ops.paged_latent_mla_fwd(q.to(dev), cache, table.to(dev), kv.to(dev), starts.to(dev), 0.1, out[8:8 + T], lse[8:8 + T])
+    _check((out[8:8 + T], lse[8:8 + T]), ref)
+    for x, held in ((out, 7.0), (lse, -7.0)):
+        assert (x[:8] == held).all() and (x[8 + T:] == held).all()
 
 
 def test_many_starts_out_of_order(dev):
