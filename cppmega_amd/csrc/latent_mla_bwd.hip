@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
       __syncthreads();
       if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
       const unsigned char *Kt = smem + buf * C::BUF, *Vt = C::SHARED ? Kt : Kt + C::K_BYTES;
-if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
+      if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
       // operands 0 .. KS - 1: K; absorbed: the first VS of them V too; expanded: V after them
       constexpr int NR = C::SHARED ? KS : KS + VS;
       auto rows_of = [&](int sub) {
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
       then = spans(nxt);
       const unsigned char *Qt = smem + buf * C::BUF, *Dt = Qt + C::Q_BYTES;
       const float *st = reinterpret_cast<const float *>(Qt + C::OFF_STAT);
-// operands 0 .. KS - 1: Q, then the VS of dO
+      // operands 0 .. KS - 1: Q, then the VS of dO
       auto rows_of = [&](int sub) {
         return [=](int i) { return i < KS ? row_read(Qt + sub * C::KP * 4096, i) : row_read(Dt + sub * C::VP * 4096, i - KS); };
       };

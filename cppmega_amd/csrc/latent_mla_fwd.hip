@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
       __syncthreads();                     // the tile is whole; the other buffer is consumed
       if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
       const unsigned char *Kt = smem + buf * C::BUF, *Vt = C::SHARED ? Kt : Kt + C::K_BYTES;
-if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
+      if (k0 >= span.hi || k0 + kKeyTile <= span.lo) continue;  // wave-uniform
       auto rows_of = [&](int sub) { return [=](int ks) { return row_read(Kt + sub * C::KP * 4096, ks); }; };
       Operands ka;
       load_group<KS>(ka, 0, rows_of(0));
