@@ -21,6 +21,9 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 constexpr int kWave = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1.0e30f;  // finite "minus infinity" for running maxima
+// Least running maximum of latent attention (log2 units).  A weight is 2^(s c - m) with s c unrounded and m rounded: below
+// -2^31, where half a step of m is 128 and more, that could be Inf for a score that a later key's makes nothing of.
+constexpr float kLeastMax = -0x1p31f;
 
 // ---------------------------------------------------------------------------
 // bf16 <-> f32 (bit exact, round-to-nearest-even; NaN stays NaN)

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OC
     constexpr bool careful = decltype(careful_t)::value;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      m_run[rt] = kNegBig;
+      m_run[rt] = kLeastMax;
       l_run[rt] = 0.0f;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) o[rt][dt] = zero16();

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Paged<
         }
       };
 
-      float m_run = kNegBig, l_run = 0.0f;
+      float m_run = kLeastMax, l_run = 0.0f;
       f32x16 o[NDT];
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) o[dt] = zero16();
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p)
     const int64_t row = row0 + ur;
     // piece k's row of partial results: in the second place of the workgroup that began the unit, the first of the others
     auto at = [&](int k) { return (int64_t)((w0 + k) * 2 + (k == 0 ? 1 : 0)) * p.unit_rows + ur; };
-    float m = kNegBig;
+    float m = kLeastMax;
     for (int k = ln; k < pieces; k += LANES)
       if (p.part_ml[at(k) * 2 + 1] != 0.0f) m = fmaxf(m, p.part_ml[at(k) * 2]);
 #pragma unroll

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
       const int lim = token_keys(kv, n, tb), lim_min = token_keys(kv, n, ta);
       const int j1 = min(b1, (lim + 31) / 32);
       const int my_lim = token_keys(kv, n, min((first + l16) / p.H, tb));
-      float m_run = kNegBig, l_run = 0.0f;
+      float m_run = kLeastMax, l_run = 0.0f;
       f32x4 o[C::NDT];
 #pragma unroll
       for (int dt = 0; dt < C::NDT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) p
       for (int x = (int)threadIdx.x; x < QUADS; x += 256) {
         const int ur = x / (D_V / 4), d = (x - ur * (D_V / 4)) * 4;
         if (ur < rlo || ur >= rhi) continue;
-        float m = kNegBig, l = 0.0f;
+        float m = kLeastMax, l = 0.0f;
 #pragma unroll
         for (int k = 0; k < C::NW; ++k)
           if (ML[(k * C::ROWS + ur) * 2 + 1] != 0.0f) m = fmaxf(m, ML[(k * C::ROWS + ur) * 2]);

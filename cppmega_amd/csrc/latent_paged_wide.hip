@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) q[ks] = ld_row_16(src + 64 * ks);
         }
-        float m_run = kNegBig, l_run = 0.0f;
+        float m_run = kLeastMax, l_run = 0.0f;
         f32x4 o[NDT];
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};

@@ -18,7 +18,7 @@ so the absorbed form of a layer trained expanded takes the expanded form's scale
 every key (``causal=False``), or per-row key windows ``starts`` / ``ends`` [B, S] int32
 (keys [start, end), clipped to [0, S_kv): packed documents, padding, sliding windows),
 which take causal's place.  A row without keys, or whose every score is -Inf, has out 0,
-lse -inf and zero gradients.
+lse -inf and zero gradients; scores below -2^31 (log2 units) count as -Inf.
 Keys that a row does not see may hold anything, Inf and NaN too.  The gradient of lse is
 not taken, as SparseMLA does not take it.
 """

@@ -617,6 +617,8 @@ int dsa_topk_index_mask(const void *topk_indices, int topk_dtype, int64_t topk,
  *   out 0, lse2 -inf, no gradient.
  *   Keys outside a row's window reach neither its results nor its gradients, whatever
  *   they hold.
+ *   Scores below -2^31 in log2 units (sm_scale log2(e) q . k) count as -Inf; a row whose
+ *   largest score passes 2^24 in magnitude has an lse2 that does not tell its weights apart.
  *   out [B, S, H, D_v] bf16, lse2 [B, S, H] f32 (log2 units); sm_scale >= 2^-100.
  *   out_lo (may be NULL) [B, S, H, D_v] bf16: what rounding took from out.
  *
@@ -703,7 +705,7 @@ int dsa_latent_plan_step(const int32_t *context_lens, const int32_t *query_lens,
  * the last of its kv_lens[r] positions; a token sees the positions up to its own.
  * block_table [R, W] int32: an entry outside [0, num_blocks) hides its keys; lengths
  * past W * block_size are cut.  out [T, H, D_v] bf16, lse2 [T, H] f32; a token without
- * keys, or with scores of -Inf alone: 0 and -inf; tokens of no request are not written.  Keys that a token does not
+ * keys, keys, or with scores of -Inf alone: 0 and -inf;  Keys that a token does not
  * see do not reach it, whatever they hold.  workspace:
  * dsa_paged_latent_mla_workspace_size() bytes, 256-byte aligned.
  */

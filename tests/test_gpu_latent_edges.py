@@ -111,6 +111,50 @@ def test_scores_of_minus_infinity(dev, q_at, k_at, form):
     check({n: got[n] for n in names}, ref, names)
 
 
+@pytest.mark.parametrize("k_at", [-1.0e11, -1.0e14, -1.0e20, -1.0e29, -3.0e38])
+@pytest.mark.parametrize("form", ["absorbed", "expanded"])
+def test_scores_far_below_the_others(dev, k_at, form):
+    """Finite keys whose scores lie below -2^31 have no weight beside keys that come after them, and none by themselves."""
+    gen = torch.Generator().manual_seed(29)
+    S, H, D, V, n = 150, 4, 128, 64, 40
+    t = torch.arange(1, S + 1)[None]
+    lo, hi = torch.full((1, S), n), torch.where(t > n, t, n)     # the reference: the first n keys are not there
+    lo[:, :n] = hi[:, :n] = 0
+    q, do = _normal(gen, 1, S, H, D), _normal(gen, 1, S, H, V)
+    q[..., D - 1] = 1.0
+    if form == "expanded":
+        x = [_normal(gen, 1, S, H, 64), _normal(gen, 1, S, 64), _normal(gen, 1, S, H, V)]
+        ref, names = om.expanded(q, *x, 0.1, lo, hi, do), ("out", "lse", "dq", "dk_nope", "dk_pe", "dv")
+        x[1][:, :n, 63] = k_at
+        got = run_expanded(dev, q, *x, do, 0.1, dict(causal=True))
+    else:
+        kv = _normal(gen, 1, S, 1, D)
+        ref, names = om.absorbed(q, kv, V, 0.1, lo, hi, do), ("out", "lse", "dq", "dkv")
+        kv[:, :n, :, D - 1] = k_at
+        got = run_absorbed(dev, q, kv, V, do, 0.1, dict(causal=True))
+    check(got, ref, names)
+
+
+@pytest.mark.parametrize("k_at", [-1.0e11, -1.0e20, -3.0e38])
+@pytest.mark.parametrize("d_qk,d_v", DIMS)
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("H", [4, 40, 128])
+def test_paged_scores_far_below_the_others(dev, k_at, d_qk, d_v, fmt, H):
+    """The same over pages, in one piece and in several, for every kernel: the first pages' rows carry such a value in their
+    rope part; the reference sees those pages as none."""
+    gen = torch.Generator().manual_seed(H)
+    cache, table, kv, starts, q = _paged_case(dev, gen, fmt, d_qk, d_v, H, [4100, 90], [1, 2], 16)
+    q[..., d_qk - 1] = 1.0
+    rows = _cache_rows(cache)
+    hidden = table.clone()
+    hidden[0, :130], hidden[1, :2] = -1, -1
+    ref = oc.paged(q, rows, hidden, starts, kv, 16, d_v, 0.1)
+    pages = torch.cat([table[0, :130], table[1, :2]]).long()
+    at = 2 * d_qk - 2 if fmt == "bf16" else d_v // 2 + 2 * (d_qk - d_v) - 2       # the last rope channel's bytes
+    cache.data.view(torch.uint8)[pages.to(dev), :, at:at + 2] = torch.tensor([k_at], dtype=torch.bfloat16).view(torch.uint8).to(dev)
+    _check(ops.paged_latent_mla_fwd(q.to(dev), cache, table.to(dev), kv.to(dev), starts.to(dev), sm_scale=0.1), ref)
+
+
 @pytest.mark.parametrize("expanded", [False, True])
 def test_a_row_of_nan_has_nan_results(dev, expanded):
     """A query row, or one key that rows admit, with NaN: out and lse of the rows that it reaches are NaN, of the others as
