@@ -175,8 +175,8 @@ def paged_latent_mla_fwd(q, cache, block_table, kv_lens, query_starts=None, sm_s
     among them; query_starts [R + 1] int32, ascending: request r has the tokens query_starts[r] .. query_starts[r + 1],
     the last of its kv_lens[r] positions, and each sees the positions up to its own; without query_starts token r is
     request r's one new token (decoding; T = R).  A page outside the cache hides its keys, and a token without keys
-    (or with scores of -Inf alone, or below -2^31 in log2 units) has out 0 and lse -inf.  Rows of tokens that belong to no request are not written: pass ``out`` and ``lse`` to keep
-    what they hold.  Keys that a token does not see may hold anything, Inf and NaN too.  sm_scale None is d_qk^-0.5, of
+    (or with scores of -Inf alone, or below -2^31 in log2 units) has out 0 and lse -inf.  Rows of tokens that belong to no
+    request are not written: pass ``out`` and ``lse`` to keep what they hold.  Keys that a token does not see may hold anything, Inf and NaN too.  sm_scale None is d_qk^-0.5, of
     the cached row's width: a layer whose scale is that of its un-absorbed heads (LatentMLAExpanded's default) passes its own.
     """
     q = unwrap_quantized(q)

@@ -705,8 +705,9 @@ int dsa_latent_plan_step(const int32_t *context_lens, const int32_t *query_lens,
  * the last of its kv_lens[r] positions; a token sees the positions up to its own.
  * block_table [R, W] int32: an entry outside [0, num_blocks) hides its keys; lengths
  * past W * block_size are cut.  out [T, H, D_v] bf16, lse2 [T, H] f32; a token without
- * keys, keys, or with scores of -Inf alone: 0 and -inf;  Keys that a token does not
- * see do not reach it, whatever they hold.  workspace:
+ * keys, or with scores of -Inf (below -2^31) alone: 0 and -inf; tokens of no request are
+ * not written.  Keys that a token does not see do not reach it, whatever they hold.
+ * workspace:
  * dsa_paged_latent_mla_workspace_size() bytes, 256-byte aligned.
  */
 size_t dsa_paged_latent_mla_workspace_size(int64_t T, int64_t R, int64_t W, int64_t block_size, int64_t H,
