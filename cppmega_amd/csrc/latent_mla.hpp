@@ -210,7 +210,7 @@ __device__ __forceinline__ bool any_wave(bool x, unsigned char *words) {
   __syncthreads();  // read: they may be written again
   return __builtin_amdgcn_readfirstlane(any) != 0;
 }
-constexpr int kLdsOfCu = 160 * 1024;
+constexpr int kLdsOfCu = 160 * 1024, kAnyBytes = 256;  // LDS of a CU; what __syncthreads_or takes of it
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 // Tile dt of a row per lane pair (l, l + 32) as bf16, v[m] its columns acc_col(dt, 4 m, l / 32) .. + 3 (m and m + 1: 16 that lie together):

@@ -49,6 +49,7 @@ template <int DK, int DN, int DV, int RT, int NW, int OCC>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) latent_bwd_q_kernel(const LatentParams p) {
   using C = LatentBwdQ<DK, DN, DV, RT, NW>;
   constexpr int KS = DK / 16, VS = DV / 16, NDT = DK / 32;
+  static_assert(NW == 4 && OCC * (C::BYTES + kAnyBytes) <= kLdsOfCu, "a wave a SIMD and workgroup; LDS of all of them");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const int nblk = (int)((p.rows + C::ROWS - 1) / C::ROWS);
@@ -290,6 +291,7 @@ template <int DK, int DN, int DV, int CT, int NW, int OCC>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) latent_bwd_kv_kernel(const LatentParams p) {
   using C = LatentBwdKv<DK, DN, DV, CT, NW>;
   constexpr int KS = DK / 16, VS = DV / 16, NDK = DK / 32, NDV = DV / 32;
+  static_assert(NW == 4 && OCC * (C::BYTES + kAnyBytes) <= kLdsOfCu, "a wave a SIMD and workgroup; LDS of all of them");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   // Unsplit: by spread_items (windows leave key blocks that follow each other alike in length).  Else item -> (batch and

@@ -131,8 +131,8 @@ def plan_latent_step(context_lens, query_lens, block_table, free_blocks, free_co
     context_lens [R] int32: cached tokens of every request; query_lens [R] int32: its new tokens, in the order in
     which they lie in the step's token batch (0: none, -1: the request is done and gives its pages back);
     block_table [R, W] int32: its pages, without gaps from the front, -1 behind them (a new request: -1 alone);
-    free_blocks [F] int32, of which the first free_count [1] int32 are free
-    (F at least the cache's pages, so that every page can come back); num_tokens: length of the token batch.
+    free_blocks [F] int32, of which the first free_count [1] int32 are free (F at least the cache's pages, so that every
+    page can come back); num_tokens: length of the token batch.
 
     A context may be shorter than the step before left it (speculative tokens that were not kept): the request keeps the
     pages behind it for its next tokens, and gives all back when it is done.
@@ -176,8 +176,9 @@ def paged_latent_mla_fwd(q, cache, block_table, kv_lens, query_starts=None, sm_s
     the last of its kv_lens[r] positions, and each sees the positions up to its own; without query_starts token r is
     request r's one new token (decoding; T = R).  A page outside the cache hides its keys, and a token without keys
     (or with scores of -Inf alone, or below -2^31 in log2 units) has out 0 and lse -inf.  Rows of tokens that belong to no
-    request are not written: pass ``out`` and ``lse`` to keep what they hold.  Keys that a token does not see may hold anything, Inf and NaN too.  sm_scale None is d_qk^-0.5, of
-    the cached row's width: a layer whose scale is that of its un-absorbed heads (LatentMLAExpanded's default) passes its own.
+    request are not written: pass ``out`` and ``lse`` to keep what they hold.  Keys that a token does not see may hold
+    anything, Inf and NaN too.  sm_scale None is d_qk^-0.5, of the cached row's width: a layer whose scale is that of its
+    un-absorbed heads (LatentMLAExpanded's default) passes its own.
     """
     q = unwrap_quantized(q)
     assert q.ndim == 3 and q.shape[2] == cache.d_qk, f"q must be [tokens, heads, {cache.d_qk}], got {tuple(q.shape)}"
