@@ -1,0 +1,565 @@
+"""Sparse attention from a paged cache, and the layer norm of the index keys: timed workloads and their plain forms.
+
+Each case is one call, or one training step, through the package's public entry points; ``kind`` names the operator:
+
+  norm    LayerNorm step: y and the gradients of x, weight and bias
+  keys    index_key_append of new tokens' index keys, then index_key_gather of the same slots
+  scores  paged_index_scores: the indexer's scores of new tokens over the paged index keys (bf16, MXFP8 or MXFP4)
+  sparse  paged_sparse_mla_fwd: attention of new tokens over the cached latent rows that a top-k names (bf16 or MXFP4)
+
+``run`` computes them with elementary torch operations in 32 bits, or, where ``own`` is true, by the package's calls.
+"""
+from __future__ import annotations
+
+import math
+import random
+
+import torch
+
+own = False
+
+LOG2E = 1.4426950408889634
+# (d_qk, d_v): 64 latent + 64 rope (NAM56R) and 512 latent + 64 rope (DeepSeek-V3.2)
+_LATENT = ((128, 64), (576, 512))
+# (heads, channels) of the indexer: cfg3's and cfg5's, and those between
+_INDEXER = ((16, 64), (32, 128), (64, 128))
+_TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def _norm(name, rows, n, dtype, wdtype):
+    return dict(name=name, kind="norm", rows=rows, n=n, dtype=dtype, wdtype=wdtype)
+
+
+def _keys(name, fmt, T, d, block, blocks):
+    return dict(name=name, kind="keys", fmt=fmt, T=T, d=d, block=block, blocks=blocks)
+
+
+def _scores(name, fmt, R, n_lo, n_hi, kv_lo, kv_hi, H, d, block):
+    return dict(name=name, kind="scores", fmt=fmt, R=R, n_lo=n_lo, n_hi=n_hi, kv_lo=kv_lo, kv_hi=kv_hi, H=H, d=d, block=block)
+
+
+def _sparse(name, fmt, R, n_lo, n_hi, kv_lo, kv_hi, topk, H, d_qk, d_v, block):
+    return dict(name=name, kind="sparse", fmt=fmt, R=R, n_lo=n_lo, n_hi=n_hi, kv_lo=kv_lo, kv_hi=kv_hi, topk=topk, H=H,
+                d_qk=d_qk, d_v=d_v, block=block)
+
+
+def listed():
+    return [
+        # the index keys of a training step (cfg3: 2 x 4096 tokens)
+        _norm("norm_index_keys", 8192, 64, "bf16", "bf16"),
+        # a layer's hidden state over a long sequence, weights kept in 32 bits
+        _norm("norm_hidden", 16384, 4096, "bf16", "f32"),
+        # a width that no vector of elements divides, in 32 bits
+        _norm("norm_odd", 2051, 1001, "f32", "f32"),
+        # a decode step's new index keys
+        _keys("keys_step", "mxfp8", 64, 128, 64, 512),
+        # a prefill batch's index keys, in 4 bits
+        _keys("keys_prefill", "mxfp4", 65536, 128, 64, 1280),
+        # one new token of one short conversation on a small model: latency
+        _scores("scores_one", "bf16", 1, 1, 1, 1025, 1025, 16, 64, 64),
+        # generation: 64 conversations of mixed length, up to long ones
+        _scores("scores_decode", "mxfp8", 64, 1, 1, 301, 65536, 64, 128, 64),
+        # chunked prefill on cached prompts, keys in 4 bits
+        _scores("scores_prefill", "mxfp4", 5, 33, 512, 1024, 16384, 32, 128, 64),
+        # one new token of one short conversation on a small model: latency
+        _sparse("sparse_one", "bf16", 1, 1, 1, 777, 777, 256, 16, 128, 64, 64),
+        # generation, every head on one card; the shortest conversations have fewer keys than the top-k
+        _sparse("sparse_decode", "bf16", 64, 1, 1, 1023, 32768, 2048, 128, 576, 512, 64),
+        # generation with the heads split over eight cards, cache in 4 bits
+        _sparse("sparse_decode_mxfp4", "mxfp4", 96, 1, 1, 1023, 16384, 2048, 16, 576, 512, 64),
+        # chunked prefill (NAM56R's heads and top-k) on cached prompts, cache in 4 bits
+        _sparse("sparse_prefill", "mxfp4", 6, 40, 512, 513, 4096, 256, 32, 128, 64, 16),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _draw_once(rng):
+    kind = rng.choice(("norm", "norm", "norm", "keys", "scores", "scores", "scores", "sparse", "sparse", "sparse"))
+    if kind == "norm":
+        n = rng.choice((64, 128, 576)) if rng.random() < 0.4 else _log(rng, 8, 8192)
+        dtype = rng.choice(("bf16", "bf16", "f32"))
+        c = _norm("", _log(rng, 1, 32768), n, dtype, "f32" if dtype == "f32" else rng.choice(("bf16", "f32")))
+    elif kind == "keys":
+        T, block = _log(rng, 1, 65536), rng.choice((16, 64, 128))
+        c = _keys("", rng.choice(("bf16", "mxfp8", "mxfp4")), T, rng.choice((64, 128)), block, T // block + rng.randint(2, 256))
+    else:
+        one = rng.random() < 0.6
+        R = _log(rng, 1, 96 if one else 12)
+        n_hi = 1 if one else _log(rng, 2, 512)
+        kv_hi = _log(rng, 600, 65536 if one and kind == "scores" else 32768 if one else 8192)
+        kv_lo = max(n_hi, _log(rng, 300, kv_hi))
+        shape = (R, 1 if one else rng.randint(1, n_hi), n_hi, kv_lo, max(kv_lo, kv_hi))
+        if kind == "scores":
+            c = _scores("", rng.choice(("bf16", "mxfp8", "mxfp4")), *shape, *rng.choice(_INDEXER), rng.choice((16, 64, 64, 128)))
+        else:
+            c = _sparse("", rng.choice(("bf16", "mxfp4")), *shape, rng.choice((64, 256, 512, 1000, 2048)),
+                        rng.choice((8, 16, 32, 64, 128)), *rng.choice(_LATENT), rng.choice((16, 64, 64, 128)))
+    del c["name"]
+    return c
+
+
+def draw(rng):
+    most = [work(c) for c in listed()]
+    flops, size = max(w["flops"] for w in most), max(w["bytes"] for w in most)
+    while True:
+        c = _draw_once(rng)
+        w = work(c)
+        if w["flops"] <= flops and w["bytes"] <= size and _plain_bytes(c) <= 30e9:
+            return c
+
+
+def _plain_bytes(c):
+    """What the plain form holds, at most."""
+    if c["kind"] == "scores":
+        return 4 * c["n_hi"] * c["kv_hi"] * c["H"] + 4 * sum(kv for kv, _ in _requests(c)) * c["d"]
+    if c["kind"] == "sparse":
+        return 4 * sum(n for _, n in _requests(c)) * c["topk"] * (c["d_qk"] + 2 * c["H"])
+    return 0
+
+
+# ---------------------------------------------------------------- inputs
+
+
+def _spread(lo, hi, n):
+    """n whole numbers from lo to hi, evenly spread (one of them: hi)."""
+    return [hi] if n == 1 else [lo + (hi - lo) * i // (n - 1) for i in range(n)]
+
+
+def _requests(c):
+    """(kv length, new tokens) of a case's requests: the same numbers for every seed."""
+    return list(zip(_spread(c["kv_lo"], c["kv_hi"], c["R"]), reversed(_spread(c["n_lo"], c["n_hi"], c["R"]))))
+
+
+def _randn(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+def _normal(g, *shape):
+    return _randn(g, *shape).to(torch.bfloat16)
+
+
+def _int32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _latent_bytes(d_qk, d_v):
+    """An MXFP4 latent row: d_v / 2 bytes of codes (element 2 i in the low half of byte i), the rope part in bf16, one
+    exponent byte per 32 latent channels, padded to 16 bytes."""
+    return (d_v // 2 + 2 * (d_qk - d_v) + d_v // 32 + 15) // 16 * 16
+
+
+def _code_bytes(fmt, d):
+    return d if fmt == "mxfp8" else d // 2
+
+
+def _key_pages(fmt, blocks, block, d):
+    """Empty pages of index keys: bf16 [blocks, block, d], or uint8 [blocks, block, code bytes + 4], a page of which holds
+    the codes of its keys and then four exponent bytes a key."""
+    if fmt == "bf16":
+        return torch.zeros(blocks, block, d, dtype=torch.bfloat16, device="cuda")
+    return torch.zeros(blocks, block, _code_bytes(fmt, d) + 4, dtype=torch.uint8, device="cuda")
+
+
+def _page_parts(pages, fmt, d):
+    """Views of MX pages: codes [blocks, block, code bytes], exponents [blocks, block, 4]."""
+    blocks, block, _ = pages.shape
+    flat, n = pages.view(blocks, -1), block * _code_bytes(fmt, d)
+    return flat[:, :n].unflatten(1, (block, -1)), flat[:, n:].unflatten(1, (block, 4))
+
+
+def _tables(c, g, reqs):
+    """Pages of the requests, scattered over the pool: block table, number of pages."""
+    need = [-(-kv // c["block"]) for kv, _ in reqs]
+    W, blocks = max(need) + 1, sum(need) + 3
+    order, at, table = torch.randperm(blocks, generator=g, device="cuda").tolist(), 0, []
+    for n in need:
+        table.append(order[at:at + n] + [-1] * (W - n))
+        at += n
+    return _int32(table), blocks
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rng = random.Random(seed)
+    c, kind = case, case["kind"]
+    s = dict(case=c)
+    if kind == "norm":
+        t, wt = _TYPES[c["dtype"]], _TYPES[c["wdtype"]]
+        # rows of different size and mean, as a projection gives them
+        x = _randn(g, c["rows"], c["n"]) * torch.exp(0.5 * _randn(g, c["rows"], 1)) + 0.5 * _randn(g, c["rows"], 1)
+        s["x"], s["dy"] = x.to(t).requires_grad_(), _randn(g, c["rows"], c["n"]).to(t)
+        s["weight"] = (1 + 0.1 * _randn(g, c["n"])).to(wt).requires_grad_()
+        s["bias"] = (0.1 * _randn(g, c["n"])).to(wt).requires_grad_()
+        s["eps"] = 1e-6
+    elif kind == "keys":
+        # magnitudes differ from channel to channel
+        s["k"] = _normal(g, c["T"], c["d"]) * torch.exp(_randn(g, c["d"])).to(torch.bfloat16)
+        s["slots"] = torch.randperm(c["block"] * c["blocks"], generator=g, device="cuda")[: c["T"]]
+        s["cache"] = _key_pages(c["fmt"], c["blocks"], c["block"], c["d"])
+    else:
+        reqs = _requests(c)
+        rng.shuffle(reqs)
+        s["table"], blocks = _tables(c, g, reqs)
+        starts = [0]
+        for _, n in reqs:
+            starts.append(starts[-1] + n)
+        T = starts[-1]
+        s["lens"], s["first"] = [kv for kv, _ in reqs], starts       # (a scheduler knows them on the host as well)
+        s["kv_lens"], s["query_starts"] = _int32(s["lens"]), _int32(starts)
+        s["one"] = c["n_hi"] == 1
+        # visible keys of every token
+        s["lims"] = [kv - n + i + 1 for kv, n in reqs for i in range(n)]
+        if kind == "scores":
+            s["q"], s["num_keys"] = _normal(g, T, c["H"], c["d"]), c["kv_hi"]
+            s["w"] = _randn(g, T, c["H"]) * (c["H"] * c["d"]) ** -0.5
+            s["cache"] = _key_pages(c["fmt"], blocks, c["block"], c["d"])
+            for i in range(0, blocks, 4096):
+                part = s["cache"][i:i + 4096]
+                _put_keys(part, c["fmt"], slice(None), _normal(g, part.shape[0] * c["block"], c["d"]))
+        else:
+            s["q"] = _normal(g, T, c["H"], c["d_qk"])
+            rows = _normal(g, blocks * c["block"], c["d_qk"])
+            if c["fmt"] == "mxfp4":
+                rows = _pack_latent(rows[:, : c["d_v"]], rows[:, c["d_v"]:])
+            s["cache"] = rows.view(blocks, c["block"], -1)
+            s["scale"] = c["d_qk"] ** -0.5
+            # a top-k of random scores: distinct visible positions, ascending, -1 behind them
+            k, lim, picks = c["topk"], _int32(s["lims"])[:, None], []
+            pos = torch.arange(max(c["kv_hi"], k), device="cuda")
+            for at in range(0, T, 256):
+                score = torch.rand(min(256, T - at), pos.shape[0], generator=g, device="cuda")
+                score = score.masked_fill_(pos >= lim[at:at + 256], -1.0)
+                val, idx = score.topk(k, dim=1)
+                idx = torch.where(val < 0, torch.full_like(idx, 1 << 30), idx).sort(dim=1).values
+                picks.append(torch.where(idx == 1 << 30, torch.full_like(idx, -1), idx).to(torch.int32))
+            s["indices"] = torch.cat(picks)
+    return s
+
+
+# ---------------------------------------------------------------- MX formats
+
+
+def _blocks_of(x):
+    """x [T, d] in blocks of 32 channels, 32 bits; their largest magnitudes; which hold Inf or NaN."""
+    x = x.float().unflatten(-1, (-1, 32))
+    amax = x.abs().amax(-1)
+    return x, amax, ~torch.isfinite(x).all(-1)
+
+
+def _e4m3_blocks(x):
+    """Codes (float8_e4m3fn) [T, d / 32, 32] and exponents [T, d / 32]: the scale of 32 channels is the least power of two
+    under which their largest magnitude is at most 448, its exponent held to +-125 (all zeros: 2^0)."""
+    x, amax, bad = _blocks_of(x)
+    mant, e = torch.frexp(amax)                                  # amax = mant 2^e, mant in [1/2, 1)
+    e = (e - 9 + (mant > 0.875)).clamp(-125, 125)
+    e = torch.where((amax == 0) | bad, torch.zeros_like(e), e)
+    v = torch.where(bad[..., None], torch.zeros_like(x), torch.ldexp(x, -e[..., None]))
+    return v.to(torch.float8_e4m3fn), e, bad
+
+
+def _e2m1_blocks(x):
+    """Codes 0 .. 15 [T, d / 32, 32] and exponents: scale 2^(floor(log2 amax) - 2), its exponent held to +-125, codes to
+    nearest, ties to even, at most 6."""
+    x, amax, bad = _blocks_of(x)
+    e = (torch.frexp(amax).exponent - 3).clamp(-125, 125)
+    e = torch.where((amax == 0) | bad, torch.zeros_like(e), e)
+    a = torch.where(bad[..., None], torch.zeros_like(x), torch.ldexp(x.abs(), -e[..., None]))
+    # nearest of 0 0.5 1 1.5 2 3 4 6, whose codes are 0..7: a tie goes to the even code
+    code = (a > 0.25).int() + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0)
+    return (code | (torch.signbit(x).int() << 3)).to(torch.uint8), e, bad
+
+
+def _exponent_bytes(e, bad):
+    return torch.where(bad, torch.full_like(e, 255), e + 127).to(torch.uint8)
+
+
+def _scale_of(byte, dtype):
+    scale = torch.ldexp(torch.ones((), dtype=dtype, device=byte.device), byte.int() - 127)
+    return torch.where(byte == 255, torch.full_like(scale, math.nan), scale)
+
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _e2m1_values(codes, dtype):
+    value = torch.tensor(_E2M1, dtype=dtype, device=codes.device)[(codes & 7).long()]
+    return torch.where(codes > 7, -value, value)
+
+
+def _put_keys(pages, fmt, slots, k):
+    """Index keys k [T, d] into the pages' slots (each once)."""
+    d = k.shape[1]
+    if fmt == "bf16":
+        pages.flatten(0, 1)[slots] = k
+        return
+    codes, expo = _page_parts(pages, fmt, d)
+    v, e, bad = _e4m3_blocks(k) if fmt == "mxfp8" else _e2m1_blocks(k)
+    v = v.view(torch.uint8).flatten(1)
+    if fmt == "mxfp4":
+        v = v[:, 0::2] | v[:, 1::2] << 4
+    block = pages.shape[1]
+    at = torch.arange(pages.shape[0] * block, device=k.device)[slots]
+    codes[at // block, at % block] = v
+    byte = torch.zeros(k.shape[0], 4, dtype=torch.uint8, device=k.device)
+    byte[:, : d // 32] = _exponent_bytes(e, bad)
+    expo[at // block, at % block] = byte
+
+
+def _get_keys(pages, fmt, d, slots, dtype):
+    """The values of the index keys in slots: [.., d]."""
+    if fmt == "bf16":
+        return pages.flatten(0, 1)[slots].to(dtype)
+    codes, expo = _page_parts(pages, fmt, d)
+    block = pages.shape[1]
+    c, e = codes[slots // block, slots % block], expo[slots // block, slots % block][..., : d // 32]
+    if fmt == "mxfp8":
+        v = c.contiguous().view(torch.float8_e4m3fn).to(dtype)
+    else:
+        v = _e2m1_values(torch.stack([c & 15, c >> 4], dim=-1).flatten(-2), dtype)
+    return (v.unflatten(-1, (-1, 32)) * _scale_of(e, dtype)[..., None]).flatten(-2)
+
+
+def _pack_latent(latent, rope):
+    """bf16 [T, d_v], [T, d_rope] -> MXFP4 latent rows uint8 [T, row bytes]."""
+    T, V = latent.shape
+    codes, e, bad = _e2m1_blocks(latent)
+    codes = codes.flatten(1)
+    row = torch.zeros(T, _latent_bytes(V + rope.shape[1], V), dtype=torch.uint8, device=latent.device)
+    at = V // 2 + 2 * rope.shape[1]
+    row[:, : V // 2] = codes[:, 0::2] | codes[:, 1::2] << 4
+    row[:, V // 2: at] = rope.contiguous().view(torch.uint8)
+    row[:, at: at + V // 32] = _exponent_bytes(e, bad)
+    return row
+
+
+def _unpack_latent(rows, d_qk, d_v, dtype):
+    """MXFP4 latent rows uint8 [..., row bytes] -> [..., d_qk] values."""
+    at = d_v // 2 + 2 * (d_qk - d_v)
+    codes = torch.stack([rows[..., : d_v // 2] & 15, rows[..., : d_v // 2] >> 4], dim=-1).flatten(-2)
+    latent = (_e2m1_values(codes, dtype).unflatten(-1, (-1, 32)) * _scale_of(rows[..., at: at + d_v // 32], dtype)[..., None]).flatten(-2)
+    return torch.cat([latent, rows[..., d_v // 2: at].contiguous().view(torch.bfloat16).to(dtype)], dim=-1)
+
+
+# ---------------------------------------------------------------- plain forms
+
+
+def _norm_plain(s):
+    x, dy, w, b = (s[n].detach().float() for n in ("x", "dy", "weight", "bias"))
+    mean = x.mean(1, keepdim=True)
+    xc = x - mean
+    rstd = torch.rsqrt((xc * xc).mean(1, keepdim=True) + s["eps"])
+    xhat = xc * rstd
+    g = dy * w
+    dx = (g - g.mean(1, keepdim=True) - xhat * (g * xhat).mean(1, keepdim=True)) * rstd
+    t, wt = s["x"].dtype, s["weight"].dtype
+    return dict(y=(xhat * w + b).to(t), dx=dx.to(t), dweight=(dy * xhat).sum(0).to(wt), dbias=dy.sum(0).to(wt))
+
+
+def _keys_plain(s):
+    c = s["case"]
+    _put_keys(s["cache"], c["fmt"], s["slots"], s["k"])
+    return dict(rows=_get_keys(s["cache"], c["fmt"], c["d"], s["slots"], torch.float32).bfloat16())
+
+
+def _slots_of(s, r, positions):
+    """Cache slots of positions of request r (every position has its page)."""
+    bs = s["case"]["block"]
+    return s["table"][r].long()[positions // bs] * bs + positions % bs
+
+
+def _scores_plain(s):
+    """Request by request; over an MX cache the queries are rounded as MXFP8 keys are."""
+    c = s["case"]
+    q = s["q"]
+    if c["fmt"] != "bf16":
+        v, e, _ = _e4m3_blocks(q.flatten(0, 1))
+        q = torch.ldexp(v.float(), e[..., None]).flatten(1).view(q.shape)
+    out = torch.full((q.shape[0], s["num_keys"]), -math.inf, dtype=torch.float32, device="cuda")
+    for r, kv in enumerate(s["lens"]):
+        a, b = s["first"][r], s["first"][r + 1]
+        pos = torch.arange(kv, device="cuda")
+        k = _get_keys(s["cache"], c["fmt"], c["d"], _slots_of(s, r, pos), torch.float32)
+        x = torch.matmul(q[a:b].float(), k.T).relu_()
+        score = torch.matmul(s["w"][a:b, None], x)[:, 0]
+        seen = pos <= torch.arange(kv - (b - a), kv, device="cuda")[:, None]
+        out[a:b, :kv] = torch.where(seen, score, torch.full_like(score, -math.inf))
+    return dict(scores=out)
+
+
+def _sparse_plain(s):
+    """All tokens at once: their picked rows side by side."""
+    c = s["case"]
+    V, bs, T = c["d_v"], c["block"], s["q"].shape[0]
+    owner = torch.searchsorted(s["query_starts"][1:].long(), torch.arange(T, device="cuda"), right=True)
+    idx = s["indices"].long()
+    off = idx < 0
+    pos = idx.clamp(min=0)
+    slot = s["table"].long()[owner[:, None], pos // bs].clamp(min=0) * bs + pos % bs
+    rows = s["cache"].flatten(0, 1)[slot]
+    k = _unpack_latent(rows, c["d_qk"], V, torch.float32) if c["fmt"] == "mxfp4" else rows.float()
+    z = torch.matmul(s["q"].float(), k.transpose(1, 2)).mul_(s["scale"]).masked_fill_(off[:, None], -math.inf)
+    top = z.amax(-1, keepdim=True)
+    p = z.sub_(top).exp_()
+    total = p.sum(-1, keepdim=True)
+    out = torch.matmul(p, k[..., :V].contiguous()) / total
+    return dict(out=out.bfloat16(), lse=(total.log() + top)[..., 0] * LOG2E)
+
+
+# ---------------------------------------------------------------- one pass
+
+
+def _own(s):
+    c, kind = s["case"], s["case"]["kind"]
+    if kind == "norm":
+        from cppmega_amd import LayerNorm
+
+        y = LayerNorm.apply(s["x"], s["weight"], s["bias"], s["eps"])
+        dx, dw, db = torch.autograd.grad(y, (s["x"], s["weight"], s["bias"]), s["dy"])
+        return dict(y=y.detach(), dx=dx, dweight=dw, dbias=db)
+    from cppmega_amd import paged_sparse_ops as ops
+
+    if kind == "keys":
+        cache = ops.IndexKeyCache(s["cache"], c["d"])
+        ops.index_key_append(cache, s["k"], s["slots"])
+        return dict(rows=ops.index_key_gather(cache, s["slots"]))
+    starts = None if s["one"] else s["query_starts"]
+    if kind == "scores":
+        cache = ops.IndexKeyCache(s["cache"], c["d"])
+        return dict(scores=ops.paged_index_scores(s["q"], s["w"], cache, s["table"], s["kv_lens"], starts, num_keys=s["num_keys"]))
+    from cppmega_amd.latent_mla_ops import LatentCache
+
+    cache = LatentCache(s["cache"], c["d_qk"], c["d_v"])
+    out, lse = ops.paged_sparse_mla_fwd(s["q"], cache, s["indices"], s["table"], s["kv_lens"], starts, sm_scale=s["scale"])
+    return dict(out=out, lse=lse)
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return {"norm": _norm_plain, "keys": _keys_plain, "scores": _scores_plain, "sparse": _sparse_plain}[state["case"]["kind"]](state)
+
+
+# ---------------------------------------------------------------- what a pass cannot do without
+
+
+def work(case):
+    c, kind = case, case["kind"]
+    if kind == "norm":
+        size = 4 if c["dtype"] == "f32" else 2
+        return dict(bytes=4 * c["rows"] * c["n"] * size + 4 * c["n"] * (4 if c["wdtype"] == "f32" else 2),
+                    flops=16 * c["rows"] * c["n"])
+    if kind == "keys":
+        row = 2 * c["d"] if c["fmt"] == "bf16" else _code_bytes(c["fmt"], c["d"]) + c["d"] // 32
+        return dict(bytes=c["T"] * (4 * c["d"] + 2 * row + 16), flops=c["T"] * c["d"])
+    reqs = _requests(c)
+    tokens = sum(n for _, n in reqs)
+    if kind == "scores":
+        row = 2 * c["d"] if c["fmt"] == "bf16" else _code_bytes(c["fmt"], c["d"]) + c["d"] // 32
+        pairs = sum(n * kv - n * (n - 1) // 2 for kv, n in reqs)
+        return dict(bytes=sum(kv for kv, _ in reqs) * row + tokens * (c["H"] * (2 * c["d"] + 4) + 4 * c["kv_hi"]),
+                    flops=2 * c["H"] * (c["d"] + 1) * pairs)
+    D, V, H, k = c["d_qk"], c["d_v"], c["H"], c["topk"]
+    row = 2 * D if c["fmt"] == "bf16" else V // 2 + 2 * (D - V) + V // 32
+    # rows that a token picks; neighbouring tokens of a request may pick the same, of which each is read once
+    picks = sum(min(kv - n + i + 1, k) for kv, n in reqs for i in range(n))
+    rows = sum(min(kv, sum(min(kv - n + i + 1, k) for i in range(n))) for kv, n in reqs)
+    return dict(bytes=rows * row + tokens * (H * (2 * D + 2 * V + 4) + 4 * k), flops=2 * H * (D + V) * picks)
+
+
+# ---------------------------------------------------------------- the same in 64 bits
+
+
+def _mx64(x, largest):
+    """The values that an MX format holds of x [.., d], in 64 bits, by distance from the grid of 32 channels' scale.
+    largest 448: e4m3 under the least power of two that keeps the block within it; 6: e2m1 under 2^(floor(log2 amax) - 2)."""
+    x = x.double().unflatten(-1, (-1, 32))
+    amax = x.abs().amax(-1, keepdim=True).clamp(min=2.0 ** -140)
+    if largest == 448:
+        scale = torch.exp2(torch.ceil(torch.log2(amax / 448)).clamp(-125, 125))
+        scale = torch.where(amax > scale * 448, scale * 2, scale)       # log2 rounds: settle the border by comparison
+        scale = torch.where(amax <= scale * 224, scale / 2, scale).clamp(min=2.0 ** -125)
+        a = x.abs() / scale
+        step = torch.exp2(torch.floor(torch.log2(a.clamp(min=2.0 ** -6))).clamp(-6, 8) - 3)
+        near = (a / step).round() * step                                  # (a power of two's log2 is exact)
+    else:
+        scale = torch.exp2(torch.floor(torch.log2(amax)).clamp(-123, 127) - 2)
+        # even codes first: they take ties
+        grid = torch.tensor([0.0, 1.0, 2.0, 4.0, 0.5, 1.5, 3.0, 6.0], dtype=torch.float64, device=x.device)
+        near = grid[(torch.minimum(x.abs() / scale, grid[-1])[..., None] - grid).abs().argmin(-1)]
+    return (torch.copysign(near, x) * scale).flatten(-2)
+
+
+def _stored64(c, s, slots):
+    """Cached rows of slots in 64 bits, decoded by their bits' meaning."""
+    bs = c["block"]
+    if c["fmt"] == "bf16":
+        return s["cache"][slots // bs, slots % bs].double()
+    page = s["cache"].flatten(1)[slots // bs]
+    if c["kind"] == "sparse":
+        row, n_code, V = s["cache"][slots // bs, slots % bs], c["d_v"] // 2, c["d_v"]
+        raw, expo = row[:, :n_code].int(), row[:, n_code + 2 * (c["d_qk"] - V):][:, : V // 32].double()
+    else:
+        n_code = _code_bytes(c["fmt"], c["d"])
+        at = (slots % bs)[:, None]
+        raw = page.gather(1, at * n_code + torch.arange(n_code, device="cuda")).int()
+        expo = page.gather(1, bs * n_code + 4 * at + torch.arange(c["d"] // 32, device="cuda")).double()
+    if c["fmt"] == "mxfp8":  # e4m3: sign, 4 bits of exponent (bias 7), 3 of mantissa
+        x, m = (raw // 8 % 16).double(), (raw % 8).double()
+        v = torch.where(x == 0, m * 2.0 ** -9, torch.exp2(x - 7) * (1 + m / 8))
+        v = torch.where(raw > 127, -v, v)
+    else:                    # e2m1: code 2 x + m is 2^(x - 1) (1 + m / 2), codes 0 and 1 are 0 and 1/2
+        code = torch.stack([raw % 16, raw // 16], dim=2).flatten(1)
+        mag = (code % 8).double()
+        v = torch.where(mag < 2, mag / 2, torch.exp2(torch.floor(mag / 2) - 1) * (1 + mag % 2 / 2))
+        v = torch.where(code > 7, -v, v)
+    v = (v.unflatten(1, (-1, 32)) * torch.exp2(expo - 127)[..., None]).flatten(1)
+    if c["kind"] == "sparse":
+        rope = row[:, n_code: n_code + 2 * (c["d_qk"] - V)].contiguous().view(torch.bfloat16).double()
+        v = torch.cat([v, rope], dim=1)
+    return v
+
+
+def exact(case, seed):
+    s, c = prepare(case, seed), case
+    kind = c["kind"]
+    if kind == "norm":
+        x, dy, w, b = (s[n].detach().double() for n in ("x", "dy", "weight", "bias"))
+        var, mean = torch.var_mean(x, dim=1, keepdim=True, correction=0)
+        sigma = (var + s["eps"]).sqrt()
+        xhat = (x - mean) / sigma
+        n, g = c["n"], dy * w
+        # the projection of the gradient off the constant vector and off xhat
+        dx = (g * n - g.sum(1, keepdim=True) - xhat * (g * xhat).sum(1, keepdim=True)) / (n * sigma)
+        return dict(y=xhat * w + b, dx=dx, dweight=torch.einsum("ij,ij->j", dy, xhat), dbias=dy.sum(0))
+    if kind == "keys":
+        return dict(rows=s["k"].double() if c["fmt"] == "bf16" else _mx64(s["k"], 448 if c["fmt"] == "mxfp8" else 6))
+    bs, first = c["block"], s["first"]
+    q = s["q"].double()
+    if kind == "scores":
+        if c["fmt"] != "bf16":
+            q = _mx64(s["q"], 448)
+        out = torch.full((q.shape[0], s["num_keys"]), -math.inf, dtype=torch.float64, device="cuda")
+        for r, kv in enumerate(s["lens"]):
+            pages = s["table"][r, : -(-kv // bs)].long()
+            slots = (pages[:, None] * bs + torch.arange(bs, device="cuda")).flatten()[:kv]
+            k = _stored64(c, s, slots)
+            for t in range(first[r], first[r + 1]):
+                n = s["lims"][t]
+                out[t, :n] = s["w"][t].double() @ torch.clamp(q[t] @ k[:n].T, min=0)
+        return dict(scores=out)
+    V = c["d_v"]
+    out = torch.zeros(q.shape[0], c["H"], V, dtype=torch.float64, device="cuda")
+    lse = torch.zeros(q.shape[0], c["H"], dtype=torch.float64, device="cuda")
+    lims = s["lims"]
+    for r in range(c["R"]):
+        pages = s["table"][r].long()
+        for t in range(first[r], first[r + 1]):
+            at = s["indices"][t, : min(c["topk"], lims[t])].long()      # the visible picks come first
+            k = _stored64(c, s, pages[at // bs] * bs + at % bs)
+            z = q[t] @ k.T * s["scale"]
+            total = torch.logsumexp(z, dim=1, keepdim=True)
+            out[t], lse[t] = torch.exp(z - total) @ k[:, :V], total[:, 0] / math.log(2)
+    return dict(out=out, lse=lse)
