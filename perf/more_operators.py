@@ -251,13 +251,14 @@ def _blocks_of(x):
 
 def _e4m3_blocks(x):
     """Codes (float8_e4m3fn) [T, d / 32, 32] and exponents [T, d / 32]: the scale of 32 channels is the least power of two
-    under which their largest magnitude is at most 448, its exponent held to +-125 (all zeros: 2^0)."""
+    under which their largest magnitude is at most 448, its exponent held to -117 .. 119 (all zeros: 2^0), so that every
+    code stands for a bf16 value; codes to nearest, ties to even, at most 448."""
     x, amax, bad = _blocks_of(x)
     mant, e = torch.frexp(amax)                                  # amax = mant 2^e, mant in [1/2, 1)
-    e = (e - 9 + (mant > 0.875)).clamp(-125, 125)
+    e = (e - 9 + (mant > 0.875)).clamp(-117, 119)
     e = torch.where((amax == 0) | bad, torch.zeros_like(e), e)
     v = torch.where(bad[..., None], torch.zeros_like(x), torch.ldexp(x, -e[..., None]))
-    return v.to(torch.float8_e4m3fn), e, bad
+    return v.clamp(-448, 448).to(torch.float8_e4m3fn), e, bad
 
 
 def _e2m1_blocks(x):
@@ -371,12 +372,8 @@ def _slots_of(s, r, positions):
 
 
 def _scores_plain(s):
-    """Request by request; over an MX cache the queries are rounded as MXFP8 keys are."""
-    c = s["case"]
-    q = s["q"]
-    if c["fmt"] != "bf16":
-        v, e, _ = _e4m3_blocks(q.flatten(0, 1))
-        q = torch.ldexp(v.float(), e[..., None]).flatten(1).view(q.shape)
+    """Request by request."""
+    c, q = s["case"], s["q"]
     out = torch.full((q.shape[0], s["num_keys"]), -math.inf, dtype=torch.float32, device="cuda")
     for r, kv in enumerate(s["lens"]):
         a, b = s["first"][r], s["first"][r + 1]
@@ -478,10 +475,10 @@ def _mx64(x, largest):
     x = x.double().unflatten(-1, (-1, 32))
     amax = x.abs().amax(-1, keepdim=True).clamp(min=2.0 ** -140)
     if largest == 448:
-        scale = torch.exp2(torch.ceil(torch.log2(amax / 448)).clamp(-125, 125))
+        scale = torch.exp2(torch.ceil(torch.log2(amax / 448)).clamp(-117, 119))
         scale = torch.where(amax > scale * 448, scale * 2, scale)       # log2 rounds: settle the border by comparison
-        scale = torch.where(amax <= scale * 224, scale / 2, scale).clamp(min=2.0 ** -125)
-        a = x.abs() / scale
+        scale = torch.where(amax <= scale * 224, scale / 2, scale).clamp(2.0 ** -117, 2.0 ** 119)
+        a = torch.clamp(x.abs() / scale, max=448)
         step = torch.exp2(torch.floor(torch.log2(a.clamp(min=2.0 ** -6))).clamp(-6, 8) - 3)
         near = (a / step).round() * step                                  # (a power of two's log2 is exact)
     else:
@@ -539,8 +536,6 @@ def exact(case, seed):
     bs, first = c["block"], s["first"]
     q = s["q"].double()
     if kind == "scores":
-        if c["fmt"] != "bf16":
-            q = _mx64(s["q"], 448)
         out = torch.full((q.shape[0], s["num_keys"]), -math.inf, dtype=torch.float64, device="cuda")
         for r, kv in enumerate(s["lens"]):
             pages = s["table"][r, : -(-kv // bs)].long()
