@@ -84,6 +84,15 @@ EXPORTED_SYMBOLS = (
     "dsa_latent_plan_step",
     "dsa_paged_latent_mla_workspace_size",
     "dsa_paged_latent_mla_fwd",
+    "dsa_index_key_row_bytes",
+    "dsa_index_key_append",
+    "dsa_index_key_gather",
+    "dsa_paged_index_scores",
+    "dsa_paged_sparse_mla_workspace_size",
+    "dsa_paged_sparse_mla_fwd",
+    "dsa_layer_norm_fwd",
+    "dsa_layer_norm_bwd_workspace_size",
+    "dsa_layer_norm_bwd",
     "dsa_stage_timing",
     "dsa_stage_times",
 )
@@ -181,6 +190,15 @@ _SIGNATURES = {
     "dsa_latent_plan_step": (_i32, [_c_void_p] * 14 + [_i64] * 5 + [_c_void_p]),
     "dsa_paged_latent_mla_workspace_size": (_size_t, [_i64] * 7),
     "dsa_paged_latent_mla_fwd": (_i32, [_c_void_p] * 8 + [_size_t] + [_i64] * 8 + [_i32, _f32, _c_void_p]),
+    "dsa_index_key_row_bytes": (_i64, [_i64, _i32]),
+    "dsa_index_key_append": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p] + [_i64] * 4 + [_i32, _c_void_p]),
+    "dsa_index_key_gather": (_i32, [_c_void_p] * 3 + [_i64] * 4 + [_i32, _c_void_p]),
+    "dsa_paged_index_scores": (_i32, [_c_void_p] * 8 + [_i64] * 10 + [_i32] * 3 + [_c_void_p]),
+    "dsa_paged_sparse_mla_workspace_size": (_size_t, [_i64] * 5),
+    "dsa_paged_sparse_mla_fwd": (_i32, [_c_void_p] * 9 + [_size_t] + [_i64] * 9 + [_i32, _f32, _c_void_p]),
+    "dsa_layer_norm_fwd": (_i32, [_c_void_p] * 6 + [_i64] * 3 + [_f32, _i32, _i32, _c_void_p]),
+    "dsa_layer_norm_bwd_workspace_size": (_size_t, [_i64] * 2),
+    "dsa_layer_norm_bwd": (_i32, [_c_void_p] * 9 + [_size_t] + [_i64] * 4 + [_i32, _i32, _c_void_p]),
     "dsa_stage_timing": (_i32, [_i32]),
     "dsa_stage_times": (_i32, [_i32, ctypes.POINTER(ctypes.c_float), _i32]),
 }

@@ -549,7 +549,8 @@ static int launch(const PagedParams &p, hipStream_t st) {
   return check_launch("dsa_paged_latent_mla_fwd");
 }
 
-int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st) {
+// The fields of p that the sizes decide, and its places in the workspace.
+void paged_setup(PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws) {
   const PagedSections s = paged_sections(p.T, p.R, p.W, p.block, p.H, d_qk, d_v, fp4);
   const PagedPlan k = paged_plan(p.T, p.R, p.W, p.block, p.H, d_qk, fp4);
   p.unit_rows = k.unit_rows;
@@ -563,9 +564,11 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
   p.unit_at = (int32_t *)(ws + s.unit_at);
   p.part_ml = (float *)(ws + s.part_ml);
   p.part_o = (float *)(ws + s.part_o);
-  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, st, p);
-  int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
-  if (rc) return rc;
+}
+// Attention over the units that stand in p's arrays.
+int launch_paged_units(const PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, hipStream_t st) {
+  const PagedPlan k = paged_plan(p.T, p.R, p.W, p.block, p.H, d_qk, fp4);
+  int rc;
   if (k.wide) rc = launch_paged_wide(p, k.wide, fp4, st);
   else if (k.few) rc = launch_paged_few(p, fp4, st);
   else if (k.nt == 4) rc = fp4 ? launch<4, true>(p, st) : launch<4, false>(p, st);
@@ -575,6 +578,12 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
   if (d_v == 512) hipLaunchKernelGGL(paged_combine_kernel<512>, grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL(paged_combine_kernel<64>, grid, dim3(256), 0, st, p);
   return check_launch("dsa_paged_latent_mla_fwd (combine)");
+}
+int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st) {
+  paged_setup(p, d_qk, d_v, fp4, ws);
+  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, st, p);
+  const int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
+  return rc ? rc : launch_paged_units(p, d_qk, d_v, fp4, st);
 }
 
 }  // namespace dsa

@@ -129,6 +129,13 @@ int launch_paged_few(const PagedParams &p, bool fp4, hipStream_t st);
 // The blocks of all units can be numbered in 32 bits, whatever the lengths.
 bool paged_countable(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk);
 size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v);
+void paged_setup(PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws);
+int launch_paged_units(const PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, hipStream_t st);
 int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st);
+
+// Attention over the cached rows that indices [T, topk] name by their positions in p.table's requests; p as for launch_paged_fwd.
+size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t d_v);
+int launch_paged_sparse(const PagedParams &p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4,
+                        unsigned char *ws, hipStream_t st);
 
 }  // namespace dsa

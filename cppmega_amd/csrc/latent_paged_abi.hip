@@ -128,3 +128,57 @@ extern "C" int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const 
   p.sl2 = sm_scale * kLog2e;
   return launch_paged_fwd(p, D_qk, D_v, dtype == DSA_DTYPE_MXFP4, (unsigned char *)workspace, (hipStream_t)stream);
 }
+
+static int check_sparse(const char *who, int64_t T, int64_t H, int64_t topk, int64_t d_qk) {
+  DSA_REQUIRE(T >= 0 && H > 0 && topk > 0, "%s: bad sizes T=%lld H=%lld topk=%lld", who, (long long)T, (long long)H, (long long)topk);
+  DSA_REQUIRE(H <= 4096 && T < (1ll << 30) && T * H < (1ll << 31) - 1024 && topk < (1ll << 31) - 1024,
+              "%s: sizes out of range (H <= 4096, T * H and topk below 2^31 - 1024)", who);
+  DSA_REQUIRE(T == 0 || paged_countable(T, T, topk, 1, H, d_qk), "%s: sizes out of range (row groups times blocks of picks must stay below 2^31)",
+              who);
+  return DSA_OK;
+}
+
+extern "C" size_t dsa_paged_sparse_mla_workspace_size(int64_t T, int64_t H, int64_t topk, int64_t D_qk, int64_t D_v) {
+  const char *who = "dsa_paged_sparse_mla_workspace_size";
+  if (check_cache(who, 1, 1, D_qk, D_v, DSA_DTYPE_BF16) || check_sparse(who, T, H, topk, D_qk)) return 0;
+  return T == 0 ? 0 : paged_sparse_workspace(T, topk, H, D_qk, D_v);
+}
+
+extern "C" int dsa_paged_sparse_mla_fwd(const void *q, const void *cache, const int32_t *indices, const int32_t *block_table,
+                                        const int32_t *query_starts, const int32_t *kv_lens, void *out, float *lse2, void *workspace,
+                                        size_t workspace_bytes, int64_t T, int64_t R, int64_t W, int64_t H, int64_t topk, int64_t D_qk,
+                                        int64_t D_v, int64_t num_blocks, int64_t block_size, int dtype, float sm_scale, void *stream) {
+  const char *who = "dsa_paged_sparse_mla_fwd";
+  int rc = check_cache(who, num_blocks, block_size, D_qk, D_v, dtype);
+  if (!rc) rc = check_sparse(who, T, H, topk, D_qk);
+  if (rc) return rc;
+  DSA_REQUIRE(R >= 0 && R < (1 << 20) && W > 0 && W < (1ll << 31) && W * block_size < (1ll << 31) - 1024,
+              "%s: sizes out of range (R < 2^20, W * block_size below 2^31 - 1024)", who);
+  DSA_REQUIRE(num_blocks * block_size < (1ll << 31), "%s: num_blocks * block_size must stay below 2^31", who);
+  DSA_REQUIRE(query_starts != nullptr || T == R, "%s: without query_starts every request has one token: %lld tokens, %lld requests", who,
+              (long long)T, (long long)R);
+  DSA_REQUIRE(isfinite(sm_scale) && sm_scale >= 0x1p-100f, "%s: sm_scale must be finite and at least 2^-100, got %g", who, (double)sm_scale);
+  if (T == 0 || R == 0) return DSA_OK;
+  DSA_REQUIRE(q && cache && indices && block_table && kv_lens && out && lse2 && aligned16(q) && aligned16(cache) && aligned16(out),
+              "%s: null or misaligned pointer", who);
+  const size_t need = paged_sparse_workspace(T, topk, H, D_qk, D_v);
+  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return set_error(DSA_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", who, need, workspace_bytes);
+  PagedParams p{};
+  p.q = (const unsigned char *)q;
+  p.cache = (const unsigned char *)cache;
+  p.table = block_table;
+  p.query_starts = query_starts;
+  p.kv_lens = kv_lens;
+  p.out = (uint16_t *)out;
+  p.lse = lse2;
+  p.T = T;
+  p.R = (int)R;
+  p.W = (int)W;
+  p.H = (int)H;
+  p.block = (int)block_size;
+  p.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)block_size) : -1;
+  p.num_blocks = (int)num_blocks;
+  p.sl2 = sm_scale * kLog2e;
+  return launch_paged_sparse(p, indices, topk, D_qk, D_v, dtype == DSA_DTYPE_MXFP4, (unsigned char *)workspace, (hipStream_t)stream);
+}

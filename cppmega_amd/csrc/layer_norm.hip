@@ -1,0 +1,411 @@
+// Layer norm over the last axis, forward and backward, on gfx950 (bf16 or f32 rows).
+//
+//   y = (x - mean) rstd weight + bias,   rstd = (mean((x - mean)^2) + eps)^-1/2
+//   g = dy weight,  xhat = (x - mean) rstd
+//   dx = rstd (g - mean(g) - xhat mean(g xhat)),  dweight = sum dy xhat,  dbias = sum dy  (over rows)
+//
+// GL lanes have a row, 8 neighbouring elements a lane and chunk (CH chunks), all in registers, so the variance is that of
+// the differences from the mean and the row is read once; the index keys' 64 channels take 8 lanes, a hidden state's 4096
+// a workgroup.  Rows need no alignment beyond their elements': the loads and stores are 16 bytes wide wherever a row begins.
+// The backward adds a lane's columns over the rows that it meets, then its workgroup's lanes in order through LDS, and
+// layer_norm_reduce_kernel the workgroups' sums: no atomics, the order depends on the sizes alone.  All of it is bound by
+// the bytes moved.
+#include <math.h>
+
+#include "dsa_common.hpp"
+#include "wave_ops.hpp"
+
+namespace dsa {
+
+struct NormParams {
+  const unsigned char *x, *dy;
+  const void *weight, *bias;
+  unsigned char *y, *dx;     // dense
+  float *mean, *rstd;        // [rows]
+  float *part;               // [nwg][2][n] sums of dy xhat and dy, or null
+  void *dweight, *dbias;     // nwg == 1: written at once
+  int64_t rows, x_stride, dy_stride;  // strides in elements
+  int n, w_f32, nwg;
+  float eps, inv_n;
+};
+
+// 16 bytes wherever an element may begin
+typedef int u16x16b __attribute__((ext_vector_type(4), aligned(2)));
+typedef int f32x16b __attribute__((ext_vector_type(4), aligned(4)));
+
+template <bool F32>
+__device__ __forceinline__ void load_8(const unsigned char *p, int left, float (&v)[8]) {  // elements past `left` are zeros
+  if (left >= 8) {
+    if constexpr (F32) {
+      const f32x16b a = *reinterpret_cast<const f32x16b *>(p), b = *reinterpret_cast<const f32x16b *>(p + 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = __int_as_float(a[i]);
+        v[4 + i] = __int_as_float(b[i]);
+      }
+    } else {
+      const u16x16b a = *reinterpret_cast<const u16x16b *>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = bf16_bits_to_f32((uint32_t)a[i] & 0xffffu);
+        v[2 * i + 1] = __uint_as_float((uint32_t)a[i] & 0xffff0000u);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = 0.0f;
+    if (i < left) v[i] = F32 ? reinterpret_cast<const float *>(p)[i] : bf16_bits_to_f32(reinterpret_cast<const uint16_t *>(p)[i]);
+  }
+}
+template <bool F32>
+__device__ __forceinline__ void store_8(unsigned char *p, int left, const float (&v)[8]) {
+  if (left >= 8) {
+    if constexpr (F32) {
+      *reinterpret_cast<f32x16b *>(p) = f32x16b{__float_as_int(v[0]), __float_as_int(v[1]), __float_as_int(v[2]), __float_as_int(v[3])};
+      *reinterpret_cast<f32x16b *>(p + 16) = f32x16b{__float_as_int(v[4]), __float_as_int(v[5]), __float_as_int(v[6]), __float_as_int(v[7])};
+    } else {
+      *reinterpret_cast<u16x16b *>(p) = u16x16b{(int)pack_bf16x2(v[0], v[1]), (int)pack_bf16x2(v[2], v[3]),
+                                                (int)pack_bf16x2(v[4], v[5]), (int)pack_bf16x2(v[6], v[7])};
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) {
+      if constexpr (F32) reinterpret_cast<float *>(p)[i] = v[i];
+      else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)pack_bf16x2(v[i], 0.0f);
+    }
+}
+// weight or bias of 8 columns (none: `value`)
+__device__ __forceinline__ void load_param(const void *w, int f32, int col, int left, float value, float (&v)[8]) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = value;
+  } else if (f32) {
+    load_8<true>(static_cast<const unsigned char *>(w) + (int64_t)col * 4, left, v);
+  } else {
+    load_8<false>(static_cast<const unsigned char *>(w) + (int64_t)col * 2, left, v);
+  }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __uint_as_float(wv::dpp<CTRL>(__float_as_uint(v)));
+}
+__device__ __forceinline__ float sum_rows16(float x) {  // x(lane) + x(lane ^ 16)
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Sum over the GL lanes of a row, in each of them.  GL > 64: the whole workgroup, through tmp [2][GL / 64] in turn.
+template <int GL>
+__device__ __forceinline__ float row_sum(float v, float *tmp) {
+  v = add_dpp<0xB1>(v);   // quad_perm [1,0,3,2]
+  v = add_dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+  v = add_dpp<0x141>(v);  // row_half_mirror
+  if constexpr (GL >= 16) v = add_dpp<0x140>(v);  // row_mirror
+  if constexpr (GL >= 32) v = sum_rows16(v);
+  if constexpr (GL >= 64) v = sum_halves(v);
+  if constexpr (GL > 64) {
+    if (lane_id() == 0) tmp[wave_id()] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GL / 64; ++i) v += tmp[i];
+  }
+  return v;
+}
+
+template <int GL>
+struct NormGroup {
+  static constexpr int NTHR = GL > 256 ? GL : 256, RPW = NTHR / GL, NW = GL / 64;  // threads; rows at once; waves of a row
+};
+
+template <int GL, int CH, bool F32>
+__global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(const NormParams p) {
+  using C = NormGroup<GL>;
+  constexpr int ELT = F32 ? 4 : 2;
+  __shared__ float tmp[2][GL > 64 ? C::NW : 1];
+  const int gl = (int)threadIdx.x % GL;
+  const int64_t row = (int64_t)blockIdx.x * C::RPW + (int)threadIdx.x / GL;
+  const bool there = row < p.rows;  // (whole rows of lanes)
+  float v[CH][8], sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = 8 * (gl + GL * c);
+    load_8<F32>(p.x + ((there ? row : 0) * p.x_stride + col) * ELT, p.n - col, v[c]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[c][i];
+  }
+  const float mean = row_sum<GL>(sum, tmp[0]) * p.inv_n;
+  float sq = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[c][i] = 8 * (gl + GL * c) + i < p.n ? v[c][i] - mean : 0.0f;
+      sq = fmaf(v[c][i], v[c][i], sq);
+    }
+  const float rstd = 1.0f / sqrtf(row_sum<GL>(sq, tmp[1]) * p.inv_n + p.eps);
+  if (!there) return;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = 8 * (gl + GL * c), left = p.n - col;
+    if (left <= 0) continue;
+    float w[8], b[8];
+    load_param(p.weight, p.w_f32, col, left, 1.0f, w);
+    load_param(p.bias, p.w_f32, col, left, 0.0f, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[c][i] = fmaf(v[c][i] * rstd, w[i], b[i]);
+    store_8<F32>(p.y + (row * p.n + col) * ELT, left, v[c]);
+  }
+  if (gl == 0 && p.mean != nullptr) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+}
+
+__device__ __forceinline__ void put_sum(void *dst, int f32, int col, float v) {
+  if (f32) static_cast<float *>(dst)[col] = v;
+  else static_cast<uint16_t *>(dst)[col] = (uint16_t)pack_bf16x2(v, 0.0f);
+}
+
+template <int GL, int CH, bool F32>
+__global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_bwd_kernel(const NormParams p) {
+  using C = NormGroup<GL>;
+  constexpr int ELT = F32 ? 4 : 2;
+  __shared__ float tmp[2][GL > 64 ? C::NW : 1];
+  __shared__ float sums[C::RPW > 1 ? C::RPW * GL * CH * 8 : 1];
+  const int gl = (int)threadIdx.x % GL, grp = (int)threadIdx.x / GL;
+  float w[CH][8], dw[CH][8], db[CH][8];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = 8 * (gl + GL * c);
+    load_param(p.weight, p.w_f32, col, p.n - col, 1.0f, w[c]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[c][i] = db[c][i] = 0.0f;
+  }
+  for (int64_t row0 = (int64_t)blockIdx.x * C::RPW; row0 < p.rows; row0 += (int64_t)p.nwg * C::RPW) {
+    const int64_t row = row0 + grp;
+    const bool there = row < p.rows;
+    const int64_t r = there ? row : 0;
+    const float mean = p.mean[r], rstd = p.rstd[r];
+    float x[CH][8], g[CH][8], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = 8 * (gl + GL * c), left = there ? p.n - col : 0;
+      load_8<F32>(p.x + (r * p.x_stride + col) * ELT, left, x[c]);
+      load_8<F32>(p.dy + (r * p.dy_stride + col) * ELT, left, g[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[c][i] = there && 8 * (gl + GL * c) + i < p.n ? (x[c][i] - mean) * rstd : 0.0f;
+        dw[c][i] = fmaf(g[c][i], x[c][i], dw[c][i]);
+        db[c][i] += g[c][i];
+        g[c][i] *= w[c][i];
+        s1 += g[c][i];
+        s2 = fmaf(g[c][i], x[c][i], s2);
+      }
+    if (p.dx == nullptr) continue;  // (uniform)
+    s1 = row_sum<GL>(s1, tmp[0]) * p.inv_n;
+    s2 = row_sum<GL>(s2, tmp[1]) * p.inv_n;
+    if (there) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = 8 * (gl + GL * c), left = p.n - col;
+        if (left <= 0) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[c][i] = rstd * (g[c][i] - s1 - x[c][i] * s2);
+        store_8<F32>(p.dx + (row * p.n + col) * ELT, left, g[c]);
+      }
+    }
+    if constexpr (GL > 64) __syncthreads();  // tmp is read
+  }
+  if (p.part == nullptr && p.dweight == nullptr && p.dbias == nullptr) return;
+  // the workgroup's sums: its row groups in order
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    auto put = [&](int col, float v) {
+      if (p.nwg > 1) p.part[((int64_t)blockIdx.x * 2 + which) * p.n + col] = v;
+      else if (void *dst = which ? p.dbias : p.dweight) put_sum(dst, p.w_f32, col, v);
+    };
+    if constexpr (C::RPW == 1) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int col = 8 * (gl + GL * c) + i;
+          if (col < p.n) put(col, which ? db[c][i] : dw[c][i]);
+        }
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[grp * GL * CH * 8 + 8 * (gl + GL * c) + i] = which ? db[c][i] : dw[c][i];
+      __syncthreads();
+      for (int col = (int)threadIdx.x; col < p.n; col += C::NTHR) {
+        float v = 0.0f;
+        for (int k = 0; k < C::RPW; ++k) v += sums[k * GL * CH * 8 + col];
+        put(col, v);
+      }
+    }
+  }
+}
+
+// dweight (y = 0), dbias (y = 1): the workgroups' sums, 64 columns a workgroup, wave w those of w, w + 16, ..; nwg = 0: zeros.
+__global__ void __launch_bounds__(1024) layer_norm_reduce_kernel(const NormParams p) {
+  __shared__ float sums[16][64];
+  const int lane = lane_id(), w = wave_id(), which = (int)blockIdx.y, col = (int)blockIdx.x * 64 + lane;
+  void *dst = which ? p.dbias : p.dweight;
+  if (dst == nullptr) return;
+  float v = 0.0f;
+  if (col < p.n) {
+#pragma unroll 8
+    for (int k = w; k < p.nwg; k += 16) v += p.part[((int64_t)k * 2 + which) * p.n + col];
+  }
+  sums[w][lane] = v;
+  __syncthreads();
+  if (w != 0 || col >= p.n) return;
+  for (int k = 1; k < 16; ++k) v += sums[k][lane];
+  put_sum(dst, p.w_f32, col, v);
+}
+
+// Lanes of a row and chunks a lane, by the width.
+struct NormShape {
+  int gl, ch;
+};
+static NormShape norm_shape(int64_t n) {
+  if (n <= 512) return {n <= 64 ? 8 : n <= 128 ? 16 : n <= 256 ? 32 : 64, 1};
+  if (n <= 1024) return {64, 2};
+  if (n <= 4096) return {256, n <= 2048 ? 1 : 2};
+  return {1024, n <= 8192 ? 1 : 2};
+}
+constexpr int64_t kNormMost = 16384;
+// Workgroups of the backward: their sums cost 16 bytes a column, a row's step 6 to 12.
+static int64_t norm_bwd_wgs(int64_t rows, int64_t n) {
+  const int gl = norm_shape(n).gl, rpw = gl > 256 ? 1 : 256 / gl;
+  const int64_t steps = (rows + rpw - 1) / rpw, most = gl > 256 ? 256 : 512;
+  return steps < most ? steps : most;
+}
+
+template <int GL, int CH>
+static void launch_norm(bool bwd, bool f32, const NormParams &p, hipStream_t st) {
+  using C = NormGroup<GL>;
+  const dim3 grid((unsigned)(bwd ? p.nwg : (p.rows + C::RPW - 1) / C::RPW)), block(C::NTHR);
+  if (bwd) {
+    if (f32) hipLaunchKernelGGL((layer_norm_bwd_kernel<GL, CH, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((layer_norm_bwd_kernel<GL, CH, false>), grid, block, 0, st, p);
+  } else {
+    if (f32) hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, false>), grid, block, 0, st, p);
+  }
+}
+static void launch_norm(bool bwd, bool f32, const NormParams &p, hipStream_t st) {
+  const NormShape s = norm_shape(p.n);
+  switch (s.gl) {
+    case 8: return launch_norm<8, 1>(bwd, f32, p, st);
+    case 16: return launch_norm<16, 1>(bwd, f32, p, st);
+    case 32: return launch_norm<32, 1>(bwd, f32, p, st);
+    case 64: return s.ch == 1 ? launch_norm<64, 1>(bwd, f32, p, st) : launch_norm<64, 2>(bwd, f32, p, st);
+    case 256: return s.ch == 1 ? launch_norm<256, 1>(bwd, f32, p, st) : launch_norm<256, 2>(bwd, f32, p, st);
+    default: return s.ch == 1 ? launch_norm<1024, 1>(bwd, f32, p, st) : launch_norm<1024, 2>(bwd, f32, p, st);
+  }
+}
+
+static int check_norm(const char *who, int64_t rows, int64_t n, int dtype, int w_dtype) {
+  DSA_REQUIRE(rows >= 0 && rows < (1ll << 31) && n > 0, "%s: bad sizes rows=%lld n=%lld", who, (long long)rows, (long long)n);
+  DSA_REQUIRE((dtype == DSA_DTYPE_BF16 || dtype == DSA_DTYPE_F32) && (w_dtype == DSA_DTYPE_BF16 || w_dtype == DSA_DTYPE_F32),
+              "%s: rows and weights are bf16 or f32, got dtypes %d, %d", who, dtype, w_dtype);
+  if (n > kNormMost)
+    return set_error(DSA_ERR_UNSUPPORTED, "%s: rows of %lld elements (at most %lld)", who, (long long)n, (long long)kNormMost);
+  return DSA_OK;
+}
+static bool aligned_to(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
+}  // namespace dsa
+
+using namespace dsa;
+
+extern "C" int dsa_layer_norm_fwd(const void *x, const void *weight, const void *bias, void *y, float *mean, float *rstd, int64_t rows,
+                                  int64_t n, int64_t x_stride, float eps, int dtype, int w_dtype, void *stream) {
+  const char *who = "dsa_layer_norm_fwd";
+  const int rc = check_norm(who, rows, n, dtype, w_dtype);
+  if (rc) return rc;
+  DSA_REQUIRE(isfinite(eps) && eps >= 0.0f, "%s: eps must be finite and not negative, got %g", who, (double)eps);
+  DSA_REQUIRE(x_stride >= 0, "%s: negative row stride", who);
+  if (rows == 0) return DSA_OK;
+  const int elt = dtype == DSA_DTYPE_F32 ? 4 : 2, welt = w_dtype == DSA_DTYPE_F32 ? 4 : 2;
+  DSA_REQUIRE(x && y && (mean == nullptr) == (rstd == nullptr), "%s: null pointer (mean and rstd come together)", who);
+  DSA_REQUIRE(aligned_to(x, elt) && aligned_to(y, elt) && aligned_to(weight, welt) && aligned_to(bias, welt) && aligned_to(mean, 4) && aligned_to(rstd, 4),
+              "%s: misaligned pointer", who);
+  NormParams p{};
+  p.x = (const unsigned char *)x;
+  p.weight = weight;
+  p.bias = bias;
+  p.y = (unsigned char *)y;
+  p.mean = mean;
+  p.rstd = rstd;
+  p.rows = rows;
+  p.x_stride = x_stride;
+  p.n = (int)n;
+  p.w_f32 = w_dtype == DSA_DTYPE_F32;
+  p.eps = eps;
+  p.inv_n = 1.0f / (float)n;
+  launch_norm(false, dtype == DSA_DTYPE_F32, p, (hipStream_t)stream);
+  return check_launch(who);
+}
+
+extern "C" size_t dsa_layer_norm_bwd_workspace_size(int64_t rows, int64_t n) {
+  if (check_norm("dsa_layer_norm_bwd_workspace_size", rows, n, DSA_DTYPE_F32, DSA_DTYPE_F32)) return 0;
+  const int64_t nwg = norm_bwd_wgs(rows, n);
+  return nwg > 1 ? (size_t)nwg * 2 * (size_t)n * 4 : 0;
+}
+
+extern "C" int dsa_layer_norm_bwd(const void *dy, const void *x, const void *weight, const float *mean, const float *rstd, void *dx,
+                                  void *dweight, void *dbias, void *workspace, size_t workspace_bytes, int64_t rows, int64_t n,
+                                  int64_t dy_stride, int64_t x_stride, int dtype, int w_dtype, void *stream) {
+  const char *who = "dsa_layer_norm_bwd";
+  const int rc = check_norm(who, rows, n, dtype, w_dtype);
+  if (rc) return rc;
+  DSA_REQUIRE(x_stride >= 0 && dy_stride >= 0, "%s: negative row stride", who);
+  const int elt = dtype == DSA_DTYPE_F32 ? 4 : 2, welt = w_dtype == DSA_DTYPE_F32 ? 4 : 2;
+  DSA_REQUIRE(rows == 0 || (dy && x && mean && rstd), "%s: null pointer", who);
+  DSA_REQUIRE(aligned_to(dy, elt) && aligned_to(x, elt) && aligned_to(dx, elt) && aligned_to(weight, welt) && aligned_to(dweight, welt) &&
+                  aligned_to(dbias, welt) && aligned_to(mean, 4) && aligned_to(rstd, 4),
+              "%s: misaligned pointer", who);
+  NormParams p{};
+  p.dy = (const unsigned char *)dy;
+  p.x = (const unsigned char *)x;
+  p.weight = weight;
+  p.mean = const_cast<float *>(mean);
+  p.rstd = const_cast<float *>(rstd);
+  p.dx = (unsigned char *)dx;
+  p.dweight = dweight;
+  p.dbias = dbias;
+  p.rows = rows;
+  p.x_stride = x_stride;
+  p.dy_stride = dy_stride;
+  p.n = (int)n;
+  p.w_f32 = w_dtype == DSA_DTYPE_F32;
+  p.inv_n = 1.0f / (float)n;
+  p.nwg = (int)norm_bwd_wgs(rows, n);
+  const bool sums = dweight != nullptr || dbias != nullptr;
+  if (sums && p.nwg > 1) {
+    const size_t need = (size_t)p.nwg * 2 * (size_t)n * 4;
+    if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 4))
+      return set_error(DSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace_bytes);
+    p.part = (float *)workspace;
+  }
+  if (rows > 0 && (sums || dx != nullptr)) {
+    launch_norm(true, dtype == DSA_DTYPE_F32, p, (hipStream_t)stream);
+    const int rc2 = check_launch(who);
+    if (rc2) return rc2;
+  }
+  if (!sums || p.nwg == 1) return DSA_OK;
+  hipLaunchKernelGGL(layer_norm_reduce_kernel, dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, (hipStream_t)stream, p);
+  return check_launch("dsa_layer_norm_bwd (reduce)");
+}

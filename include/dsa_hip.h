@@ -719,6 +719,83 @@ int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const int32_t *bl
                              int dtype, float sm_scale, void *stream);
 
 /*
+ * Paged cache of index keys (the indexer's k), pages of the same numbers as the latent
+ * cache's: [num_blocks] pages of block_size keys of D channels, D in {64, 128}.
+ *   DSA_DTYPE_BF16   D bf16 a key
+ *   DSA_DTYPE_MXFP8  the page's keys of D e4m3 codes, then four exponent bytes a key: byte b
+ *                    is that of channels 32 b .. 32 b + 31 (scale 2^(e - 127), 255: NaN),
+ *                    bytes past the last channel 0
+ *   DSA_DTYPE_MXFP4  the same with D / 2 bytes of e2m1 codes a key (channel 2 i in the low
+ *                    half of byte i)
+ * block_size is a multiple of 4 for the MX formats.  dsa_index_key_row_bytes: a page's bytes
+ * per key (0 where the sizes are refused).  A slot is page * block_size + offset.
+ * append: k [T, D] bf16 (row stride k_stride elements) to slots[t]; slots outside the cache
+ *   are skipped; a slot may be given once.  MXFP8: the scale of 32 channels is the least power
+ *   of two under which their largest magnitude is at most 448, its exponent held to -117 ..
+ *   119 (all zeros: 2^0); MXFP4: 2^(floor(log2 amax) - 2), held to +-125; codes to nearest
+ *   even, saturating; a block with Inf or NaN gets 255.
+ * gather: out [T, D] bf16 of slots (zeros outside the cache), exact.
+ * Pointers of rows are 16-byte aligned, k_stride a multiple of 8.
+ */
+int64_t dsa_index_key_row_bytes(int64_t D, int dtype);
+int dsa_index_key_append(void *cache, const void *k, int64_t k_stride, const int64_t *slots, int64_t T,
+                         int64_t num_blocks, int64_t block_size, int64_t D, int dtype, void *stream);
+int dsa_index_key_gather(const void *cache, const int64_t *slots, void *out, int64_t T, int64_t num_blocks,
+                         int64_t block_size, int64_t D, int dtype, void *stream);
+
+/*
+ * Indexer scores over the paged index keys: for tokens first .. first + tokens - 1 of a batch
+ * of T,
+ *   scores[t - first, s] = sum_h w[t, h] act(q[t, h] . k[s])   0 <= s < L (L <= W * block_size)
+ * with act = ReLU when use_relu != 0, for the positions s of token t's request up to its own,
+ * -inf for the others and for keys whose page lies outside the cache.  q [T, H, D] bf16, w
+ * [T, H] bf16 or f32 (w_dtype), H in {16, 32, 64}; requests, block_table [R, W], query_starts
+ * and kv_lens as in dsa_paged_latent_mla_fwd.  A NaN or Inf of a key, a query or a weight
+ * reaches the scores of that key, token and no other.  Rows of tokens of no request are not
+ * written.  limits [tokens] int32 (or NULL): the columns that each token sees, 0 for a token
+ * of no request: with 0 as the starts, the windows of a top-k over the scores.
+ */
+int dsa_paged_index_scores(const void *q, const void *w, const void *cache, const int32_t *block_table,
+                           const int32_t *query_starts, const int32_t *kv_lens, float *scores, int32_t *limits,
+                           int64_t T, int64_t R, int64_t W, int64_t first, int64_t tokens, int64_t L, int64_t H,
+                           int64_t D, int64_t num_blocks, int64_t block_size, int dtype, int w_dtype, int use_relu,
+                           void *stream);
+
+/*
+ * SparseMLA over the paged latent cache: token t attends to the cached rows at indices[t]
+ * (int32 [T, topk], positions in its request, any order; a position outside the token's own
+ * ones, in particular -1, is masked; a repeated one counts every time).  Everything else as
+ * in dsa_paged_latent_mla_fwd, whose results for the same rows it gives; num_blocks *
+ * block_size < 2^31.  workspace: dsa_paged_sparse_mla_workspace_size() bytes, 256-byte aligned.
+ */
+size_t dsa_paged_sparse_mla_workspace_size(int64_t T, int64_t H, int64_t topk, int64_t D_qk, int64_t D_v);
+int dsa_paged_sparse_mla_fwd(const void *q, const void *cache, const int32_t *indices, const int32_t *block_table,
+                             const int32_t *query_starts, const int32_t *kv_lens, void *out, float *lse2,
+                             void *workspace, size_t workspace_bytes, int64_t T, int64_t R, int64_t W, int64_t H,
+                             int64_t topk, int64_t D_qk, int64_t D_v, int64_t num_blocks, int64_t block_size,
+                             int dtype, float sm_scale, void *stream);
+
+/*
+ * Layer norm over rows of n <= 16384 elements (the index keys', or any other):
+ *   y = (x - mean) rstd weight + bias,  rstd = (mean((x - mean)^2) + eps)^-1/2
+ * x [rows, n] bf16 or f32 (dtype; row stride x_stride elements, 0 repeats a row), weight and
+ * bias [n] bf16 or f32 (w_dtype; NULL: ones, zeros), y [rows, n] of x's type; mean, rstd
+ * [rows] f32 for the backward (or both NULL).
+ * Backward, from dy [rows, n] of x's type (row stride dy_stride): dx [rows, n], dweight and
+ * dbias [n] of the weights' type; each may be NULL.  No atomics: repeated calls give the same
+ * bits.  workspace: dsa_layer_norm_bwd_workspace_size() bytes, 4-byte aligned (needed for
+ * dweight and dbias).  Pointers are aligned to their elements.  Outputs overlap no input.
+ */
+int dsa_layer_norm_fwd(const void *x, const void *weight, const void *bias, void *y, float *mean, float *rstd,
+                       int64_t rows, int64_t n, int64_t x_stride, float eps, int dtype, int w_dtype,
+                       void *stream);
+size_t dsa_layer_norm_bwd_workspace_size(int64_t rows, int64_t n);
+int dsa_layer_norm_bwd(const void *dy, const void *x, const void *weight, const float *mean, const float *rstd,
+                       void *dx, void *dweight, void *dbias, void *workspace, size_t workspace_bytes,
+                       int64_t rows, int64_t n, int64_t dy_stride, int64_t x_stride, int dtype, int w_dtype,
+                       void *stream);
+
+/*
  * Stage timing (measurement aid; no counterpart in the reference, which
  * times whole calls with CUDA events in its benchmark scripts).  With
  * dsa_stage_timing(1) on a thread, every later dsa_sparse_mla_bwd call on
