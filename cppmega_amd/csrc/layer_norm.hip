@@ -33,31 +33,47 @@ struct NormParams {
 typedef int u16x16b __attribute__((ext_vector_type(4), aligned(2)));
 typedef int f32x16b __attribute__((ext_vector_type(4), aligned(4)));
 
+// 8 neighbouring elements as they lie in memory; those past `left` are zeros.
 template <bool F32>
-__device__ __forceinline__ void load_8(const unsigned char *p, int left, float (&v)[8]) {  // elements past `left` are zeros
+struct Raw8 {
+  i32x4 v[F32 ? 2 : 1];
+};
+template <bool F32>
+__device__ __forceinline__ Raw8<F32> load_raw(const unsigned char *p, int left) {
+  Raw8<F32> r;
   if (left >= 8) {
     if constexpr (F32) {
-      const f32x16b a = *reinterpret_cast<const f32x16b *>(p), b = *reinterpret_cast<const f32x16b *>(p + 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = __int_as_float(a[i]);
-        v[4 + i] = __int_as_float(b[i]);
-      }
+      r.v[0] = *reinterpret_cast<const f32x16b *>(p);
+      r.v[1] = *reinterpret_cast<const f32x16b *>(p + 16);
     } else {
-      const u16x16b a = *reinterpret_cast<const u16x16b *>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = bf16_bits_to_f32((uint32_t)a[i] & 0xffffu);
-        v[2 * i + 1] = __uint_as_float((uint32_t)a[i] & 0xffff0000u);
-      }
+      r.v[0] = *reinterpret_cast<const u16x16b *>(p);
     }
-    return;
+    return r;
   }
+  if constexpr (F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i >> 2][i & 3] = i < left ? reinterpret_cast<const int *>(p)[i] : 0;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = 2 * i < left ? reinterpret_cast<const uint16_t *>(p)[2 * i] : 0u;
+      const uint32_t hi = 2 * i + 1 < left ? reinterpret_cast<const uint16_t *>(p)[2 * i + 1] : 0u;
+      r.v[0][i] = (int)(lo | hi << 16);
+    }
+  }
+  return r;
+}
+template <bool F32>
+__device__ __forceinline__ void widen(const Raw8<F32> &r, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    v[i] = 0.0f;
-    if (i < left) v[i] = F32 ? reinterpret_cast<const float *>(p)[i] : bf16_bits_to_f32(reinterpret_cast<const uint16_t *>(p)[i]);
+    if constexpr (F32) v[i] = __int_as_float(r.v[i >> 2][i & 3]);
+    else v[i] = __uint_as_float((i & 1) ? (uint32_t)r.v[0][i >> 1] & 0xffff0000u : (uint32_t)r.v[0][i >> 1] << 16);
   }
+}
+template <bool F32>
+__device__ __forceinline__ void load_8(const unsigned char *p, int left, float (&v)[8]) {
+  widen<F32>(load_raw<F32>(p, left), v);
 }
 template <bool F32>
 __device__ __forceinline__ void store_8(unsigned char *p, int left, const float (&v)[8]) {
@@ -98,23 +114,31 @@ __device__ __forceinline__ float sum_rows16(float x) {  // x(lane) + x(lane ^ 16
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// Sum over the GL lanes of a row, in each of them.  GL > 64: the whole workgroup, through tmp [2][GL / 64] in turn.
-template <int GL>
-__device__ __forceinline__ float row_sum(float v, float *tmp) {
-  v = add_dpp<0xB1>(v);   // quad_perm [1,0,3,2]
-  v = add_dpp<0x4E>(v);   // quad_perm [2,3,0,1]
-  v = add_dpp<0x141>(v);  // row_half_mirror
-  if constexpr (GL >= 16) v = add_dpp<0x140>(v);  // row_mirror
-  if constexpr (GL >= 32) v = sum_rows16(v);
-  if constexpr (GL >= 64) v = sum_halves(v);
-  if constexpr (GL > 64) {
-    if (lane_id() == 0) tmp[wave_id()] = v;
-    __syncthreads();
-    v = 0.0f;
+// Sums over the GL lanes of a row, in each of them.  GL > 64: the whole workgroup through tmp [N][GL / 64], one barrier.
+template <int GL, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float *tmp) {
 #pragma unroll
-    for (int i = 0; i < GL / 64; ++i) v += tmp[i];
+  for (int i = 0; i < N; ++i) {
+    v[i] = add_dpp<0xB1>(v[i]);   // quad_perm [1,0,3,2]
+    v[i] = add_dpp<0x4E>(v[i]);   // quad_perm [2,3,0,1]
+    v[i] = add_dpp<0x141>(v[i]);  // row_half_mirror
+    if constexpr (GL >= 16) v[i] = add_dpp<0x140>(v[i]);  // row_mirror
+    if constexpr (GL >= 32) v[i] = sum_rows16(v[i]);
+    if constexpr (GL >= 64) v[i] = sum_halves(v[i]);
   }
-  return v;
+  if constexpr (GL > 64) {
+    constexpr int NW = GL / 64;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane_id() == 0) tmp[i * NW + wave_id()] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) v[i] += tmp[i * NW + k];
+    }
+  }
 }
 
 template <int GL>
@@ -138,7 +162,9 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(c
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += v[c][i];
   }
-  const float mean = row_sum<GL>(sum, tmp[0]) * p.inv_n;
+  float total[1] = {sum};
+  row_sums<GL>(total, tmp[0]);
+  const float mean = total[0] * p.inv_n;
   float sq = 0.0f;
 #pragma unroll
   for (int c = 0; c < CH; ++c)
@@ -147,7 +173,9 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(c
       v[c][i] = 8 * (gl + GL * c) + i < p.n ? v[c][i] - mean : 0.0f;
       sq = fmaf(v[c][i], v[c][i], sq);
     }
-  const float rstd = 1.0f / sqrtf(row_sum<GL>(sq, tmp[1]) * p.inv_n + p.eps);
+  total[0] = sq;
+  row_sums<GL>(total, tmp[1]);
+  const float rstd = 1.0f / sqrtf(total[0] * p.inv_n + p.eps);
   if (!there) return;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -175,9 +203,27 @@ template <int GL, int CH, bool F32>
 __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_bwd_kernel(const NormParams p) {
   using C = NormGroup<GL>;
   constexpr int ELT = F32 ? 4 : 2;
-  __shared__ float tmp[2][GL > 64 ? C::NW : 1];
+  __shared__ float tmp[2][GL > 64 ? 2 * C::NW : 1];
   __shared__ float sums[C::RPW > 1 ? C::RPW * GL * CH * 8 : 1];
   const int gl = (int)threadIdx.x % GL, grp = (int)threadIdx.x / GL;
+  const int64_t step = (int64_t)p.nwg * C::RPW;
+  // a row, fetched while the one before it is worked on
+  Raw8<F32> rx[CH], rg[CH];
+  float mean, rstd;
+  auto fetch = [&](int64_t row) {
+    const bool there = row < p.rows;
+    const int64_t r = there ? row : 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = 8 * (gl + GL * c), left = there ? p.n - col : 0;
+      rx[c] = load_raw<F32>(p.x + (r * p.x_stride + col) * ELT, left);
+      rg[c] = load_raw<F32>(p.dy + (r * p.dy_stride + col) * ELT, left);
+    }
+    mean = p.mean[r];
+    rstd = p.rstd[r];
+  };
+  int64_t row = (int64_t)blockIdx.x * C::RPW + grp;
+  fetch(row);
   float w[CH][8], dw[CH][8], db[CH][8];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -186,43 +232,38 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_bwd_kernel(c
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[c][i] = db[c][i] = 0.0f;
   }
-  for (int64_t row0 = (int64_t)blockIdx.x * C::RPW; row0 < p.rows; row0 += (int64_t)p.nwg * C::RPW) {
-    const int64_t row = row0 + grp;
+  for (int turn = 0; row - grp < p.rows; row += step, turn ^= 1) {
     const bool there = row < p.rows;
-    const int64_t r = there ? row : 0;
-    const float mean = p.mean[r], rstd = p.rstd[r];
-    float x[CH][8], g[CH][8], s1 = 0.0f, s2 = 0.0f;
+    const float r = rstd;
+    float x[CH][8], g[CH][8], s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int col = 8 * (gl + GL * c), left = there ? p.n - col : 0;
-      load_8<F32>(p.x + (r * p.x_stride + col) * ELT, left, x[c]);
-      load_8<F32>(p.dy + (r * p.dy_stride + col) * ELT, left, g[c]);
-    }
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
+      widen<F32>(rx[c], x[c]);
+      widen<F32>(rg[c], g[c]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[c][i] = there && 8 * (gl + GL * c) + i < p.n ? (x[c][i] - mean) * rstd : 0.0f;
+        x[c][i] = there && 8 * (gl + GL * c) + i < p.n ? (x[c][i] - mean) * r : 0.0f;
         dw[c][i] = fmaf(g[c][i], x[c][i], dw[c][i]);
         db[c][i] += g[c][i];
         g[c][i] *= w[c][i];
-        s1 += g[c][i];
-        s2 = fmaf(g[c][i], x[c][i], s2);
+        s[0] += g[c][i];
+        s[1] = fmaf(g[c][i], x[c][i], s[1]);
       }
+    }
+    fetch(row + step);
     if (p.dx == nullptr) continue;  // (uniform)
-    s1 = row_sum<GL>(s1, tmp[0]) * p.inv_n;
-    s2 = row_sum<GL>(s2, tmp[1]) * p.inv_n;
+    row_sums<GL>(s, tmp[turn]);     // (two places in turn: no wait for the readers)
+    const float m1 = s[0] * p.inv_n, m2 = s[1] * p.inv_n;
     if (there) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int col = 8 * (gl + GL * c), left = p.n - col;
         if (left <= 0) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] = rstd * (g[c][i] - s1 - x[c][i] * s2);
+        for (int i = 0; i < 8; ++i) g[c][i] = r * (g[c][i] - m1 - x[c][i] * m2);
         store_8<F32>(p.dx + (row * p.n + col) * ELT, left, g[c]);
       }
     }
-    if constexpr (GL > 64) __syncthreads();  // tmp is read
   }
   if (p.part == nullptr && p.dweight == nullptr && p.dbias == nullptr) return;
   // the workgroup's sums: its row groups in order
@@ -274,45 +315,56 @@ __global__ void __launch_bounds__(1024) layer_norm_reduce_kernel(const NormParam
   put_sum(dst, p.w_f32, col, v);
 }
 
-// Lanes of a row and chunks a lane, by the width.
+// Lanes of a row and chunks a lane, by the width.  The forward keeps up to 64 elements a lane, so that a wave has a row of
+// 4096 and waits for no other; the backward, whose sums and weights stay in registers too, 16.
 struct NormShape {
   int gl, ch;
 };
-static NormShape norm_shape(int64_t n) {
+static NormShape norm_shape(int64_t n, bool bwd) {
   if (n <= 512) return {n <= 64 ? 8 : n <= 128 ? 16 : n <= 256 ? 32 : 64, 1};
   if (n <= 1024) return {64, 2};
-  if (n <= 4096) return {256, n <= 2048 ? 1 : 2};
-  return {1024, n <= 8192 ? 1 : 2};
+  if (bwd) return n <= 4096 ? NormShape{256, n <= 2048 ? 1 : 2} : NormShape{1024, n <= 8192 ? 1 : 2};
+  if (n <= 4096) return {64, n <= 2048 ? 4 : 8};
+  return {256, n <= 8192 ? 4 : 8};
 }
 constexpr int64_t kNormMost = 16384;
 // Workgroups of the backward: their sums cost 16 bytes a column, a row's step 6 to 12.
 static int64_t norm_bwd_wgs(int64_t rows, int64_t n) {
-  const int gl = norm_shape(n).gl, rpw = gl > 256 ? 1 : 256 / gl;
+  const int gl = norm_shape(n, true).gl, rpw = gl > 256 ? 1 : 256 / gl;
   const int64_t steps = (rows + rpw - 1) / rpw, most = gl > 256 ? 256 : 512;
   return steps < most ? steps : most;
 }
 
 template <int GL, int CH>
-static void launch_norm(bool bwd, bool f32, const NormParams &p, hipStream_t st) {
+static void launch_fwd(bool f32, const NormParams &p, hipStream_t st) {
   using C = NormGroup<GL>;
-  const dim3 grid((unsigned)(bwd ? p.nwg : (p.rows + C::RPW - 1) / C::RPW)), block(C::NTHR);
-  if (bwd) {
-    if (f32) hipLaunchKernelGGL((layer_norm_bwd_kernel<GL, CH, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((layer_norm_bwd_kernel<GL, CH, false>), grid, block, 0, st, p);
-  } else {
-    if (f32) hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, false>), grid, block, 0, st, p);
-  }
+  const dim3 grid((unsigned)((p.rows + C::RPW - 1) / C::RPW)), block(C::NTHR);
+  if (f32) hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, false>), grid, block, 0, st, p);
+}
+template <int GL, int CH>
+static void launch_bwd(bool f32, const NormParams &p, hipStream_t st) {
+  const dim3 grid((unsigned)p.nwg), block(NormGroup<GL>::NTHR);
+  if (f32) hipLaunchKernelGGL((layer_norm_bwd_kernel<GL, CH, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((layer_norm_bwd_kernel<GL, CH, false>), grid, block, 0, st, p);
 }
 static void launch_norm(bool bwd, bool f32, const NormParams &p, hipStream_t st) {
-  const NormShape s = norm_shape(p.n);
-  switch (s.gl) {
-    case 8: return launch_norm<8, 1>(bwd, f32, p, st);
-    case 16: return launch_norm<16, 1>(bwd, f32, p, st);
-    case 32: return launch_norm<32, 1>(bwd, f32, p, st);
-    case 64: return s.ch == 1 ? launch_norm<64, 1>(bwd, f32, p, st) : launch_norm<64, 2>(bwd, f32, p, st);
-    case 256: return s.ch == 1 ? launch_norm<256, 1>(bwd, f32, p, st) : launch_norm<256, 2>(bwd, f32, p, st);
-    default: return s.ch == 1 ? launch_norm<1024, 1>(bwd, f32, p, st) : launch_norm<1024, 2>(bwd, f32, p, st);
+  const NormShape s = norm_shape(p.n, bwd);
+  const int key = s.gl * 16 + s.ch;
+  switch (key) {
+    case 8 * 16 + 1: return bwd ? launch_bwd<8, 1>(f32, p, st) : launch_fwd<8, 1>(f32, p, st);
+    case 16 * 16 + 1: return bwd ? launch_bwd<16, 1>(f32, p, st) : launch_fwd<16, 1>(f32, p, st);
+    case 32 * 16 + 1: return bwd ? launch_bwd<32, 1>(f32, p, st) : launch_fwd<32, 1>(f32, p, st);
+    case 64 * 16 + 1: return bwd ? launch_bwd<64, 1>(f32, p, st) : launch_fwd<64, 1>(f32, p, st);
+    case 64 * 16 + 2: return bwd ? launch_bwd<64, 2>(f32, p, st) : launch_fwd<64, 2>(f32, p, st);
+    case 64 * 16 + 4: return launch_fwd<64, 4>(f32, p, st);
+    case 64 * 16 + 8: return launch_fwd<64, 8>(f32, p, st);
+    case 256 * 16 + 4: return launch_fwd<256, 4>(f32, p, st);
+    case 256 * 16 + 8: return launch_fwd<256, 8>(f32, p, st);
+    case 256 * 16 + 1: return launch_bwd<256, 1>(f32, p, st);
+    case 256 * 16 + 2: return launch_bwd<256, 2>(f32, p, st);
+    case 1024 * 16 + 1: return launch_bwd<1024, 1>(f32, p, st);
+    default: return launch_bwd<1024, 2>(f32, p, st);
   }
 }
 
