@@ -55,6 +55,7 @@ FILE_FLAGS = {
     "latent_paged_few.hip": _MFMA_VGPR,
     "latent_paged_wide.hip": _MFMA_VGPR,
     "paged_index_scores.hip": _MFMA_VGPR,
+    "paged_sparse_narrow.hip": _MFMA_VGPR,
 }
 
 

@@ -78,6 +78,21 @@ struct Requests {
     }
     return lo;
   }
+  // The same, lane by lane.
+  __device__ __forceinline__ int of_lane(int t) const {
+    if (query_starts == nullptr) return t < R ? t : R - 1;
+    int lo = 0, hi = R - 1;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo + 1) / 2;
+      if (start(mid) <= t) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  }
+  // Positions that token t of request r sees, -1 where it is not one of the request's.
+  __device__ __forceinline__ int keys_of(int t, int r) const {
+    const int at = start(r), n = tokens(r);
+    return t >= at && t < at + n ? max(kv(r) - n + (t - at) + 1, 0) : -1;
+  }
 };
 
 struct IndexScoreParams {

@@ -162,7 +162,7 @@ extern "C" int dsa_paged_sparse_mla_fwd(const void *q, const void *cache, const 
   DSA_REQUIRE(q && cache && indices && block_table && kv_lens && out && lse2 && aligned16(q) && aligned16(cache) && aligned16(out),
               "%s: null or misaligned pointer", who);
   const size_t need = paged_sparse_workspace(T, topk, H, D_qk, D_v);
-  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return set_error(DSA_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", who, need, workspace_bytes);
   PagedParams p{};
   p.q = (const unsigned char *)q;

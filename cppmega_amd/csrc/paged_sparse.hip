@@ -8,6 +8,7 @@
 
 #include "index_keys.hpp"
 #include "latent_paged.hpp"
+#include "paged_sparse.hpp"
 
 namespace dsa {
 
@@ -69,11 +70,31 @@ static size_t slots_at(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t
   return (paged_workspace(T, T, topk, 1, H, d_qk, d_v) + 255) & ~(size_t)255;
 }
 size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t d_v) {
+  if (d_qk == 128) return sparse_narrow_workspace(T, topk, H);
   return slots_at(T, topk, H, d_qk, d_v) + (size_t)T * ((size_t)topk + 1) * 4;
 }
 
 int launch_paged_sparse(const PagedParams &p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4,
                         unsigned char *ws, hipStream_t st) {
+  const Requests req{p.query_starts, p.kv_lens, (int64_t)p.W * p.block, (int)p.T, p.R};
+  if (d_qk == 128) {
+    SparseParams n{};
+    n.q = p.q;
+    n.cache = p.cache;
+    n.indices = indices;
+    n.table = p.table;
+    n.req = req;
+    n.out = p.out;
+    n.lse = p.lse;
+    n.W = p.W;
+    n.H = p.H;
+    n.topk = (int)topk;
+    n.block = p.block;
+    n.block_shift = p.block_shift;
+    n.num_blocks = p.num_blocks;
+    n.sl2 = p.sl2;
+    return launch_sparse_narrow(n, fp4, ws, st);
+  }
   int32_t *slots = (int32_t *)(ws + slots_at(p.T, topk, p.H, d_qk, d_v)), *picks = slots + p.T * topk;
   // every token a request of one token, its keys on pages of one row
   PagedParams a = p;
@@ -89,7 +110,7 @@ int launch_paged_sparse(const PagedParams &p, const int32_t *indices, int64_t to
   SparseSlotParams s{};
   s.indices = indices;
   s.table = p.table;
-  s.req = Requests{p.query_starts, p.kv_lens, (int64_t)p.W * p.block, (int)p.T, p.R};
+  s.req = req;
   s.slots = slots;
   s.picks = picks;
   s.unit0 = a.unit0;

@@ -133,8 +133,10 @@ def test_c_sparse():
         assert f(**k) == INVALID, k
     assert f(D=192, V=128) == UNSUPPORTED
     size = L.dsa_paged_sparse_mla_workspace_size
-    need = size(5, 16, 8, 128, 64)
-    assert need >= 5 * 9 * 4 and f(n=need - 1) == f(ws=None, n=need) == f(ws=P + 16, n=need) == WORKSPACE
+    for D, V in ((128, 64), (576, 512)):
+        a = dict(T=5, H=16, k=2048, D=D, V=V)
+        need = size(5, 16, 2048, D, V)
+        assert need > 0 and f(**a, n=need - 1) == f(**a, ws=None, n=need) == f(**a, ws=P + 16, n=need) == WORKSPACE
     assert f(T=0, R=0, q=None) == f(T=3, R=0, qs=P, q=None) == OK and size(0, 16, 8, 128, 64) == 0
     assert size(5, 16, 8, 192, 128) == size(5, 0, 8, 128, 64) == size(5, 16, 0, 128, 64) == 0
 
