@@ -1,8 +1,9 @@
-// The paged cache of index keys (page format, conversions) and the requests of a paged call.
+// The paged cache of index keys: page format, conversions, parameters of the scores over it.
 #pragma once
 
 #include "dsa_common.hpp"
 #include "latent_cache.hpp"
+#include "requests.hpp"
 
 namespace dsa {
 
@@ -47,53 +48,6 @@ __device__ __forceinline__ i32x4 key_values(i32x4 chunk, int u, uint32_t e) {
     return e == 255u ? i32x4{nan2, nan2, nan2, nan2} : v;
   }
 }
-
-// The requests of a call: tokens query_starts[r] .. query_starts[r + 1] of the batch (null: token r alone) are the last of
-// request r's kv_lens[r] positions.
-struct Requests {
-  const int32_t *query_starts, *kv_lens;
-  int64_t cap;  // W * block: lengths past it are cut
-  int T, R;
-  __device__ __forceinline__ int start(int r) const { return query_starts == nullptr ? r : min(max(query_starts[r], 0), T); }
-  __device__ __forceinline__ int tokens(int r) const {
-    if (query_starts == nullptr) return r < T ? 1 : 0;
-    const int n = start(r + 1) - start(r);
-    return n > 0 ? n : 0;
-  }
-  __device__ __forceinline__ int kv(int r) const {
-    const int k = kv_lens[r];
-    return k < 0 ? 0 : (k < cap ? k : (int)cap);
-  }
-  // The last request that begins at or before token t (the whole wave: 64 of them are looked at in a step).
-  __device__ __forceinline__ int of(int t) const {
-    if (query_starts == nullptr) return t < R ? t : R - 1;
-    const int lane = lane_id();
-    int lo = 0, n = R;
-    while (n > 1) {
-      const int step = (n + 63) / 64, at = lo + lane * step;
-      const uint64_t before = __builtin_amdgcn_ballot_w64(lane * step < n && start(at < R ? at : 0) <= t);
-      const int k = before == 0 ? 0 : 63 - (int)__builtin_clzll(before);
-      n = n - k * step < step ? n - k * step : step;
-      lo += k * step;
-    }
-    return lo;
-  }
-  // The same, lane by lane.
-  __device__ __forceinline__ int of_lane(int t) const {
-    if (query_starts == nullptr) return t < R ? t : R - 1;
-    int lo = 0, hi = R - 1;
-    while (lo < hi) {
-      const int mid = lo + (hi - lo + 1) / 2;
-      if (start(mid) <= t) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-  }
-  // Positions that token t of request r sees, -1 where it is not one of the request's.
-  __device__ __forceinline__ int keys_of(int t, int r) const {
-    const int at = start(r), n = tokens(r);
-    return t >= at && t < at + n ? max(kv(r) - n + (t - at) + 1, 0) : -1;
-  }
-};
 
 struct IndexScoreParams {
   const unsigned char *q;      // [T, H, D] bf16

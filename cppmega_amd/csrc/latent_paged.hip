@@ -411,19 +411,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Paged<
 // workgroup that began it is in range w + 1, some rows of that unit, a row to 64 lanes
 // (64 channels: to 16), one after the other: its pieces brought to their largest maximum
 // and added in order, read AHEAD at a time.
-template <int D_V>
+template <int D_V, bool SPARSE>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p) {
   constexpr int NCH = D_V / 4, LANES = NCH < 64 ? NCH : 64, CPL = NCH / LANES, AT_ONCE = 256 / LANES, AHEAD = 4;
   const int ln = lane_id() % LANES;
-  const int units = uni(p.unit0[p.R]), total = uni(p.unit_at[units]), per = uni(range_blocks(p, total));
+  int units, total;
+  all_units<SPARSE>(p, units, total);
+  const int per = uni(range_blocks(p, total));
   const int64_t cut = ((int64_t)blockIdx.x + 1) * per;
   if (cut >= total) return;
-  const int u = uni(unit_of(p, units, (int)cut)), ub = uni(p.unit_at[u]), ue = uni(p.unit_at[u + 1]);
+  const int u = uni(unit_of<SPARSE>(p, units, (int)cut)), ub = unit_begin<SPARSE>(p, u), ue = unit_begin<SPARSE>(p, u + 1);
   const int w0 = ub / per, pieces = (ue - 1) / per - w0 + 1;
   if (ub == cut || w0 != (int)blockIdx.x) return;  // no unit is cut here, or it was cut before
-  const int req = uni(p.unit_req[u]), first = uni(p.unit_first[u]);
-  const int nrows = min(uni(request_tokens(p, req)) * p.H - first, p.unit_rows);
-  const int64_t row0 = (int64_t)uni(request_start(p, req)) * p.H + first;
+  int at_unit = ub;
+  const PagedPiece x_u = next_piece<SPARSE>(p, u, at_unit, ue);
+  const int nrows = x_u.nrows;
+  const int64_t row0 = x_u.row0;
   const int rows = p.unit_rows / (int)gridDim.y;
   for (int ur = (int)blockIdx.y * rows + (int)threadIdx.x / LANES; ur < min(((int)blockIdx.y + 1) * rows, nrows); ur += AT_ONCE) {
     const int64_t row = row0 + ur;
@@ -549,8 +552,16 @@ static int launch(const PagedParams &p, hipStream_t st) {
   return check_launch("dsa_paged_latent_mla_fwd");
 }
 
-// The fields of p that the sizes decide, and its places in the workspace.
-void paged_setup(PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws) {
+int launch_paged_combine(const PagedParams &p, int64_t d_v, bool sparse, hipStream_t st) {
+  if (p.nwg == 1) return DSA_OK;  // one workgroup: no unit has several pieces
+  const dim3 grid((unsigned)(p.nwg - 1), (unsigned)(p.unit_rows / (p.unit_rows < 64 ? 4 : 16)));
+  if (sparse) hipLaunchKernelGGL((paged_combine_kernel<512, true>), grid, dim3(256), 0, st, p);
+  else if (d_v == 512) hipLaunchKernelGGL((paged_combine_kernel<512, false>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((paged_combine_kernel<64, false>), grid, dim3(256), 0, st, p);
+  return check_launch("dsa_paged_latent_mla_fwd (combine)");
+}
+
+int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st) {
   const PagedSections s = paged_sections(p.T, p.R, p.W, p.block, p.H, d_qk, d_v, fp4);
   const PagedPlan k = paged_plan(p.T, p.R, p.W, p.block, p.H, d_qk, fp4);
   p.unit_rows = k.unit_rows;
@@ -564,26 +575,14 @@ void paged_setup(PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, unsigned c
   p.unit_at = (int32_t *)(ws + s.unit_at);
   p.part_ml = (float *)(ws + s.part_ml);
   p.part_o = (float *)(ws + s.part_o);
-}
-// Attention over the units that stand in p's arrays.
-int launch_paged_units(const PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, hipStream_t st) {
-  const PagedPlan k = paged_plan(p.T, p.R, p.W, p.block, p.H, d_qk, fp4);
-  int rc;
-  if (k.wide) rc = launch_paged_wide(p, k.wide, fp4, st);
+  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, st, p);
+  int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
+  if (rc) return rc;
+  if (k.wide) rc = launch_paged_wide(p, k.wide, fp4, false, st);
   else if (k.few) rc = launch_paged_few(p, fp4, st);
   else if (k.nt == 4) rc = fp4 ? launch<4, true>(p, st) : launch<4, false>(p, st);
   else rc = launch<2, false>(p, st);
-  if (rc || p.nwg == 1) return rc;  // one workgroup: no unit has several pieces
-  const dim3 grid((unsigned)(p.nwg - 1), (unsigned)(p.unit_rows / (p.unit_rows < 64 ? 4 : 16)));
-  if (d_v == 512) hipLaunchKernelGGL(paged_combine_kernel<512>, grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(paged_combine_kernel<64>, grid, dim3(256), 0, st, p);
-  return check_launch("dsa_paged_latent_mla_fwd (combine)");
-}
-int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st) {
-  paged_setup(p, d_qk, d_v, fp4, ws);
-  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, st, p);
-  const int rc = check_launch("dsa_paged_latent_mla_fwd (plan)");
-  return rc ? rc : launch_paged_units(p, d_qk, d_v, fp4, st);
+  return rc ? rc : launch_paged_combine(p, d_v, false, st);
 }
 
 }  // namespace dsa

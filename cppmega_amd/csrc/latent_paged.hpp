@@ -3,6 +3,7 @@
 
 #include "dsa_common.hpp"
 #include "latent_cache.hpp"
+#include "requests.hpp"
 
 namespace dsa {
 
@@ -23,6 +24,9 @@ struct PagedParams {
   int32_t *unit0, *unit_req, *unit_first;
   int32_t *unit_at;
   float *part_ml, *part_o;       // [2 nwg][unit_rows]: (m, l), [d_v]
+  // sparse attention: every token a request of its picks (block 1), in token_units units of unit_blocks blocks
+  Picks picks;
+  int token_units, unit_blocks;
 };
 
 static __device__ const i32x4 kZeroRow[80] = {};  // a masked key's row
@@ -60,33 +64,68 @@ __device__ __forceinline__ int range_blocks(const PagedParams &p, int total) {
 // A wave-uniform value as a scalar.
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// All units and their blocks.
+template <bool SPARSE>
+__device__ __forceinline__ void all_units(const PagedParams &p, int &units, int &total) {
+  if constexpr (SPARSE) {
+    units = (int)p.T * p.token_units;
+    total = units * p.unit_blocks;
+  } else {
+    units = uni(p.unit0[p.R]);
+    total = uni(p.unit_at[units]);
+  }
+}
+// First block of unit u.
+template <bool SPARSE>
+__device__ __forceinline__ int unit_begin(const PagedParams &p, int u) {
+  if constexpr (SPARSE) return u * p.unit_blocks;
+  else return uni(p.unit_at[u]);
+}
+
 // A piece of a unit: blocks [b0, b1) of it, from a workgroup's range of all blocks.
 struct PagedPiece {
   int b0, b1, first, n, kv, nrows, slot;  // first row within the request; partial result's place
   bool whole;                             // the unit entire
   int64_t row0;                           // first row in q, out and lse
   const int32_t *table;
+  int token, req, seen;                   // sparse: the token, its request and the positions that it sees
 };
 // Piece at block `at` of unit u, for a range that ends at `end`; at moves past it.
+template <bool SPARSE = false>
 __device__ __forceinline__ PagedPiece next_piece(const PagedParams &p, int u, int &at, int end) {
-  const int ub = uni(p.unit_at[u]), ue = uni(p.unit_at[u + 1]), req = uni(p.unit_req[u]);
+  const int ub = unit_begin<SPARSE>(p, u), ue = unit_begin<SPARSE>(p, u + 1);
   PagedPiece x;
   x.b0 = at - ub;
   x.b1 = (ue < end ? ue : end) - ub;
   x.whole = x.b0 == 0 && ub + x.b1 == ue;
   x.slot = (int)blockIdx.x * 2 + (x.b0 == 0 ? 1 : 0);
   at = ub + x.b1;
-  x.first = uni(p.unit_first[u]);
-  x.n = uni(request_tokens(p, req));
-  x.kv = uni(request_kv(p, req));
-  x.nrows = min(x.n * p.H - x.first, p.unit_rows);
-  x.row0 = (int64_t)uni(request_start(p, req)) * p.H + x.first;
-  x.table = p.table + (int64_t)req * p.W;
+  if constexpr (SPARSE) {
+    x.token = uni(u / p.token_units);
+    x.req = uni(p.picks.req.of(x.token));
+    x.seen = uni(p.picks.req.keys_of(x.token, x.req));
+    x.first = (u - x.token * p.token_units) * p.unit_rows;
+    x.n = 1;
+    x.kv = x.seen < 0 ? 0 : p.picks.topk;
+    x.nrows = x.seen < 0 ? 0 : min(p.H - x.first, p.unit_rows);  // (a token of no request: no rows)
+    x.row0 = (int64_t)x.token * p.H + x.first;
+    x.table = nullptr;
+  } else {
+    const int req = uni(p.unit_req[u]);
+    x.first = uni(p.unit_first[u]);
+    x.n = uni(request_tokens(p, req));
+    x.kv = uni(request_kv(p, req));
+    x.nrows = min(x.n * p.H - x.first, p.unit_rows);
+    x.row0 = (int64_t)uni(request_start(p, req)) * p.H + x.first;
+    x.table = p.table + (int64_t)req * p.W;
+  }
   return x;
 }
 
 // The last unit that begins at or before block `at` (the whole wave: 64 units are looked at in a step).
+template <bool SPARSE = false>
 __device__ __forceinline__ int unit_of(const PagedParams &p, int units, int at) {
+  if constexpr (SPARSE) return at / p.unit_blocks;
   const int lane = lane_id();
   int lo = 0, n = units;  // it is one of lo .. lo + n - 1
   while (n > 1) {
@@ -123,19 +162,18 @@ constexpr int kWindow = 1024;  // table entries of a request that a workgroup ha
 constexpr int vmcnt_only(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
 
 int paged_wide_keys();  // keys of a step
-int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st);
+int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, bool sparse, hipStream_t st);
 int launch_paged_few(const PagedParams &p, bool fp4, hipStream_t st);
 
 // The blocks of all units can be numbered in 32 bits, whatever the lengths.
 bool paged_countable(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk);
 size_t paged_workspace(int64_t T, int64_t R, int64_t W, int64_t block, int64_t H, int64_t d_qk, int64_t d_v);
-void paged_setup(PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws);
-int launch_paged_units(const PagedParams &p, int64_t d_qk, int64_t d_v, bool fp4, hipStream_t st);
 int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws, hipStream_t st);
+int launch_paged_combine(const PagedParams &p, int64_t d_v, bool sparse, hipStream_t st);
 
 // Attention over the cached rows that indices [T, topk] name by their positions in p.table's requests; p as for launch_paged_fwd.
 size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t d_v);
-int launch_paged_sparse(const PagedParams &p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4,
+int launch_paged_sparse(PagedParams p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4,
                         unsigned char *ws, hipStream_t st);
 
 }  // namespace dsa

@@ -26,7 +26,7 @@ namespace dsa {
 
 constexpr int kWideKeys = 64;  // keys of a step
 
-template <int RG_, bool FP4>
+template <int RG_, bool FP4, bool SPARSE = false>
 struct PagedWide {
   using Row = CacheRow<576, 512, FP4>;
   static constexpr int RG = RG_, ROWS = 16 * RG;
@@ -40,16 +40,17 @@ struct PagedWide {
   static constexpr int KS = 18, NDT = 32;
   static constexpr int TPR = 4, CPT = 16 / TPR, RPT = 8 / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
   static constexpr int OFF_T = 2 * STEP;
-  static constexpr int OFF_ML = OFF_T + kWindow * 4;         // [2][16][2]
+  static constexpr int WINDOW = SPARSE ? 2 * kWindow : kWindow;
+  static constexpr int OFF_ML = OFF_T + WINDOW * 4;          // [2][16][2]
   static constexpr int BYTES = OFF_ML + 2 * 16 * 8;
   static constexpr int O_BYTES = 512 * 16 * 4;
   static_assert(BYTES <= 159 * 1024 && (KG == 1 || RG * O_BYTES <= OFF_T), "LDS");
   static_assert(!FP4 || (ROLES && 64 * LW == kWideKeys * TPR), "MXFP4 rows: by the loading waves");
 };
 
-template <int RG, bool FP4>
+template <int RG, bool FP4, bool SPARSE>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) paged_wide_kernel(const PagedParams p) {
-  using C = PagedWide<RG, FP4>;
+  using C = PagedWide<RG, FP4, SPARSE>;
   using Row = typename C::Row;
   constexpr int KEYS = kWideKeys, KS = C::KS, NDT = C::NDT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -63,15 +64,18 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
   const unsigned char *zero = reinterpret_cast<const unsigned char *>(kZeroRow);
   // MXFP4: chunks are also permuted by their panel, as neighbouring lanes write one row's blocks, a panel to two of them
   auto panel_swz = [](int panel) { return FP4 ? (panel & 7) << 4 : 0; };
-  auto page_of = [&](int key) { return p.block_shift >= 0 ? key >> p.block_shift : (int)((uint32_t)key / (uint32_t)p.block); };
+  // (sparse: a pick is its own page)
+  auto page_of = [&](int key) { return SPARSE ? key : p.block_shift >= 0 ? key >> p.block_shift : (int)((uint32_t)key / (uint32_t)p.block); };
 
-  const int units = uni(p.unit0[p.R]), total = uni(p.unit_at[units]), per = uni(range_blocks(p, total));
+  int units, total;
+  all_units<SPARSE>(p, units, total);
+  const int per = uni(range_blocks(p, total));
   if ((int64_t)blockIdx.x * per >= total) return;
   int at = (int)blockIdx.x * per;
   const int end = per < total - at ? at + per : total;
-  for (int u = uni(unit_of(p, units, at)); at < end; ++u) {
-    const PagedPiece x = next_piece(p, u, at, end);
-    const int tok0 = x.first / p.H, tok1 = (x.first + x.nrows - 1) / p.H;
+  for (int u = uni(unit_of<SPARSE>(p, units, at)); at < end; ++u) {
+    const PagedPiece x = next_piece<SPARSE>(p, u, at, end);
+    const int tok0 = SPARSE ? 0 : x.first / p.H, tok1 = SPARSE ? 0 : (x.first + x.nrows - 1) / p.H;
     auto my_row = [&] { return 16 * rg + (lane_here() & 15); };  // of the unit
     // Tokens [ta, tb] with the keys cut at tb's: all at once, or, where that left something that is not finite, one by
     // one, since a weight of zero does not remove the Inf or NaN of a later token's key.
@@ -79,8 +83,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
     bool probe = tok0 != tok1;
     while (true) {
       const int lim = token_keys(x.kv, x.n, tb), lim_min = token_keys(x.kv, x.n, ta);
-      const int j1 = min(x.b1, (lim + KEYS - 1) / KEYS);  // steps past it hold no key
+      int j1 = min(x.b1, (lim + KEYS - 1) / KEYS);  // steps past it hold no key
       auto row_keys = [&](int row) {
+        if constexpr (SPARSE) return lim;
         const int t = (x.first + row) / p.H;
         return token_keys(x.kv, x.n, t < tb ? t : tb);
       };
@@ -91,6 +96,23 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
         const int pages = lim > 0 ? page_of(lim - 1) + 1 : 0;
         bool ok = true;
         __syncthreads();  // the window's readers are done
+        if constexpr (SPARSE) {
+          // the picks' slots: all positions, then all entries, so that two latencies are waited for
+          constexpr int N = C::WINDOW / 512;
+          int pos[N], e[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) pos[k] = p.picks.position(x.token, base + k * 512 + (int)threadIdx.x, x.seen);
+#pragma unroll
+          for (int k = 0; k < N; ++k) e[k] = p.picks.entry(x.req, pos[k]);
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const int i = k * 512 + (int)threadIdx.x, slot = p.picks.slot(pos[k], e[k]);
+            if (base + i < pages && slot < 0) ok = false;
+            window[i] = slot;
+          }
+          all_there = __syncthreads_and(ok) != 0;
+          return;
+        }
         for (int i = (int)threadIdx.x; i < kWindow; i += 512) {
           int e = -1;
           if (base + i < pages) {
@@ -106,7 +128,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
       };
       auto key_at = [&](int key) -> const unsigned char * {  // row of a key, by the window
         const int pg = page_of(key), e = key < lim ? window[pg - base] : -1;
-        const int64_t slot = (int64_t)e * p.block + (key - pg * p.block);
+        const int64_t slot = SPARSE ? e : (int64_t)e * p.block + (key - pg * p.block);
         return e >= 0 ? p.cache + slot * Row::BYTES : zero;
       };
       // bf16: a step's eight 8-row groups
@@ -164,9 +186,19 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
       // steps that are asked for before they are worked on, and their pages in the window
       constexpr int kAsked = FP4 ? 3 : 1;
       auto window_for = [&](int j) {
-        if (page_of((j + kAsked + 1) * KEYS - 1) >= base + kWindow && page_of(lim - 1) >= base + kWindow) refill(page_of(j * KEYS));
+        if (page_of((j + kAsked + 1) * KEYS - 1) >= base + C::WINDOW && page_of(lim - 1) >= base + C::WINDOW) refill(page_of(j * KEYS));
       };
       refill(page_of(x.b0 * KEYS));
+      if constexpr (SPARSE) {
+        // behind the last pick that is there: no step (a top-k of few keys), where the window shows it
+        if (!all_there && x.b1 * KEYS <= base + C::WINDOW) {
+          int last = 0;
+          for (int i = lane_here(); i < x.b1 * KEYS - base; i += 64)
+            if (window[i] >= 0) last = base + i + 1;
+          for (int k = 32; k >= 1; k >>= 1) last = max(last, __shfl_xor(last, k, 64));
+          j1 = min(j1, uni((last + KEYS - 1) / KEYS));
+        }
+      }
       int buf = 0;
       bool again = false;
       if (computes) {  // (the registers of Q and O are these waves' alone)
@@ -393,20 +425,25 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
   }
 }
 
-template <int RG, bool FP4>
+template <int RG, bool FP4, bool SPARSE>
 static int launch(const PagedParams &p, hipStream_t st) {
-  using C = PagedWide<RG, FP4>;
-  const auto kernel = paged_wide_kernel<RG, FP4>;
+  using C = PagedWide<RG, FP4, SPARSE>;
+  const char *who = SPARSE ? "dsa_paged_sparse_mla_fwd" : "dsa_paged_latent_mla_fwd";
+  const auto kernel = paged_wide_kernel<RG, FP4, SPARSE>;
   const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::BYTES);
-  if (e != hipSuccess) return set_error(DSA_ERR_HIP, "dsa_paged_latent_mla_fwd: LDS attribute: %s", hipGetErrorString(e));
+  if (e != hipSuccess) return set_error(DSA_ERR_HIP, "%s: LDS attribute: %s", who, hipGetErrorString(e));
   hipLaunchKernelGGL(kernel, dim3((unsigned)p.nwg), dim3(512), C::BYTES, st, p);
-  return check_launch("dsa_paged_latent_mla_fwd");
+  return check_launch(who);
 }
 
 int paged_wide_keys() { return kWideKeys; }
-int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, hipStream_t st) {
-  if (fp4) return tiles16 == 2 ? launch<2, true>(p, st) : launch<4, true>(p, st);
-  return tiles16 == 4 ? launch<4, false>(p, st) : launch<8, false>(p, st);
+template <bool SPARSE>
+static int launch_of(const PagedParams &p, int tiles16, bool fp4, hipStream_t st) {
+  if (fp4) return tiles16 == 2 ? launch<2, true, SPARSE>(p, st) : launch<4, true, SPARSE>(p, st);
+  return tiles16 == 4 ? launch<4, false, SPARSE>(p, st) : launch<8, false, SPARSE>(p, st);
+}
+int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, bool sparse, hipStream_t st) {
+  return sparse ? launch_of<true>(p, tiles16, fp4, st) : launch_of<false>(p, tiles16, fp4, st);
 }
 
 }  // namespace dsa

@@ -1,134 +1,69 @@
 // SparseMLA of new tokens over the paged latent cache, on gfx950: each token attends to the cached rows that its top-k
 // names by their positions in its request.
 //
-// Positions become cache slots once a call (sparse_slots_kernel); a token is then a request of one token whose pages are
-// single rows, and the kernels of paged latent attention take it: their workgroups share all tokens' picks evenly, 32 or 64
-// at a time, whatever the number of tokens, and add the pieces of a token that was cut.
-#include <math.h>
-
-#include "index_keys.hpp"
+// Rows of 128 channels: paged_sparse_narrow.hip.  Rows of 576: the kernels of paged latent attention, for which a token is a
+// request of one token whose pages are single rows.  Their workgroups share all tokens' picks evenly, 64 at a time, whatever
+// the number of tokens, and paged_combine_kernel adds the pieces of a token that was cut; the picks' slots are formed as a
+// workgroup fills its window of pages.
 #include "latent_paged.hpp"
 #include "paged_sparse.hpp"
 
 namespace dsa {
 
-struct SparseSlotParams {
-  const int32_t *indices, *table;  // [T, topk] positions, [R, W]
-  Requests req;
-  int32_t *slots, *picks;          // [T, topk]; [T] one past the last valid pick
-  int32_t *unit0, *unit_req, *unit_first, *unit_at;
-  int W, topk, block, block_shift, num_blocks;
-  int H, units, unit_rows, unit_blocks;  // units of a token, their rows and blocks of keys
+// How a call with 576 channels is run.
+struct SparseWidePlan {
+  int wide, unit_rows, token_units, unit_blocks, nwg, min_blocks;
 };
-
-// A workgroup a token: its slots (-1: a position that it does not see, or on no page), and its units for the attention.
-__global__ void __launch_bounds__(256) sparse_slots_kernel(const SparseSlotParams p) {
-  __shared__ int last[4];
-  const int t = (int)blockIdx.x, tid = (int)threadIdx.x, lane = lane_id(), w = wave_id();
-  int r = 0, lim = -1;
-  if (p.req.R > 0) {
-    r = __builtin_amdgcn_readfirstlane(p.req.of(t));
-    const int at = p.req.start(r), n = p.req.tokens(r);
-    if (t >= at && t < at + n) lim = max(p.req.kv(r) - n + (t - at) + 1, 0);
-  }
-  const int32_t *idx = p.indices + (int64_t)t * p.topk, *table = p.table + (int64_t)r * p.W;
-  int32_t *slots = p.slots + (int64_t)t * p.topk;
-  int end = 0;
-#pragma unroll 8
-  for (int i = tid; i < p.topk; i += 256) {
-    const int pos = idx[i];
-    int slot = -1;
-    if (pos >= 0 && pos < lim) {
-      const int pg = p.block_shift >= 0 ? pos >> p.block_shift : (int)((uint32_t)pos / (uint32_t)p.block);
-      const int e = table[pg];
-      if (e >= 0 && e < p.num_blocks) {
-        slot = e * p.block + (pos - pg * p.block);
-        end = i + 1;
-      }
-    }
-    slots[i] = slot;
-  }
-  for (int x = 32; x >= 1; x >>= 1) end = max(end, __shfl_xor(end, x, 64));
-  if (lane == 0) last[w] = end;
-  __syncthreads();
-  end = max(max(last[0], last[1]), max(last[2], last[3]));
-  if (tid == 0) {
-    p.picks[t] = end;
-    if (t == 0) p.unit0[p.req.T] = p.req.T * p.units;
-    if (t + 1 == p.req.T) p.unit_at[p.req.T * p.units] = p.req.T * p.units * p.unit_blocks;
-  }
-  for (int i = tid; i < p.units; i += 256) {
-    const int u = t * p.units + i;
-    p.unit_req[u] = t;
-    // (a token of no request: rows past its last, which are nobody's)
-    p.unit_first[u] = lim < 0 ? p.H : i * p.unit_rows;
-    p.unit_at[u] = u * p.unit_blocks;
-  }
+static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool fp4) {
+  SparseWidePlan r{};
+  r.wide = fp4 ? (H <= 32 ? 2 : 4) : (H <= 64 ? 4 : 8);
+  r.unit_rows = 16 * r.wide;
+  r.token_units = (int)((H + r.unit_rows - 1) / r.unit_rows);
+  r.unit_blocks = (int)((topk + paged_wide_keys() - 1) / paged_wide_keys());
+  r.min_blocks = 256 / paged_wide_keys();  // picks that are worth a piece's beginning and end
+  const int64_t n = (T * r.token_units * r.unit_blocks + r.min_blocks - 1) / r.min_blocks;
+  r.nwg = (int)(n < 256 ? n : 256);
+  return r;
 }
 
-static size_t slots_at(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t d_v) {  // (256-byte aligned)
-  return (paged_workspace(T, T, topk, 1, H, d_qk, d_v) + 255) & ~(size_t)255;
-}
 size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t d_v) {
   if (d_qk == 128) return sparse_narrow_workspace(T, topk, H);
-  return slots_at(T, topk, H, d_qk, d_v) + (size_t)T * ((size_t)topk + 1) * 4;
+  size_t most = 0;  // of the two formats': the query does not know it
+  for (int fp4 = 0; fp4 < 2; ++fp4) {
+    const SparseWidePlan k = sparse_wide_plan(T, topk, H, fp4 != 0);
+    const size_t n = (size_t)k.nwg * 2 * (size_t)k.unit_rows * ((size_t)d_v + 2) * 4;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
-int launch_paged_sparse(const PagedParams &p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4,
-                        unsigned char *ws, hipStream_t st) {
-  const Requests req{p.query_starts, p.kv_lens, (int64_t)p.W * p.block, (int)p.T, p.R};
+int launch_paged_sparse(PagedParams p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws,
+                        hipStream_t st) {
+  const Picks picks{indices, p.table, Requests{p.query_starts, p.kv_lens, (int64_t)p.W * p.block, (int)p.T, p.R}, p.W, (int)topk,
+                    p.block, p.block_shift, p.num_blocks};
   if (d_qk == 128) {
     SparseParams n{};
     n.q = p.q;
     n.cache = p.cache;
-    n.indices = indices;
-    n.table = p.table;
-    n.req = req;
+    n.picks = picks;
     n.out = p.out;
     n.lse = p.lse;
-    n.W = p.W;
     n.H = p.H;
-    n.topk = (int)topk;
-    n.block = p.block;
-    n.block_shift = p.block_shift;
-    n.num_blocks = p.num_blocks;
     n.sl2 = p.sl2;
     return launch_sparse_narrow(n, fp4, ws, st);
   }
-  int32_t *slots = (int32_t *)(ws + slots_at(p.T, topk, p.H, d_qk, d_v)), *picks = slots + p.T * topk;
-  // every token a request of one token, its keys on pages of one row
-  PagedParams a = p;
-  a.table = slots;
-  a.query_starts = nullptr;
-  a.kv_lens = picks;
-  a.R = (int)p.T;
-  a.W = (int)topk;
-  a.block = 1;
-  a.block_shift = 0;
-  a.num_blocks = p.num_blocks * p.block;
-  paged_setup(a, d_qk, d_v, fp4, ws);
-  SparseSlotParams s{};
-  s.indices = indices;
-  s.table = p.table;
-  s.req = req;
-  s.slots = slots;
-  s.picks = picks;
-  s.unit0 = a.unit0;
-  s.unit_req = a.unit_req;
-  s.unit_first = a.unit_first;
-  s.unit_at = a.unit_at;
-  s.W = p.W;
-  s.topk = (int)topk;
-  s.block = p.block;
-  s.block_shift = p.block_shift;
-  s.num_blocks = p.num_blocks;
-  s.H = p.H;
-  s.unit_rows = a.unit_rows;
-  s.units = (p.H + a.unit_rows - 1) / a.unit_rows;
-  s.unit_blocks = ((int)topk + a.step_keys - 1) / a.step_keys;
-  hipLaunchKernelGGL(sparse_slots_kernel, dim3((unsigned)p.T), dim3(256), 0, st, s);
-  const int rc = check_launch("dsa_paged_sparse_mla_fwd (slots)");
-  return rc ? rc : launch_paged_units(a, d_qk, d_v, fp4, st);
+  const SparseWidePlan k = sparse_wide_plan(p.T, topk, p.H, fp4);
+  p.picks = picks;
+  p.unit_rows = k.unit_rows;
+  p.token_units = k.token_units;
+  p.unit_blocks = k.unit_blocks;
+  p.step_keys = paged_wide_keys();
+  p.nwg = k.nwg;
+  p.min_blocks = k.min_blocks;
+  p.part_ml = (float *)ws;
+  p.part_o = p.part_ml + (size_t)k.nwg * 2 * (size_t)k.unit_rows * 2;
+  const int rc = launch_paged_wide(p, k.wide, fp4, true, st);
+  return rc ? rc : launch_paged_combine(p, d_v, true, st);
 }
 
 }  // namespace dsa

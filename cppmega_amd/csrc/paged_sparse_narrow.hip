@@ -6,7 +6,6 @@
 //   S^T[pick][head] = K Q^T, O^T[channel][head] += V^T P^T   on 32x32x16 MFMAs (lane = head)
 // Many tokens: a wave has a unit.  Fewer: the four waves of a workgroup share a unit's picks and are joined through LDS,
 // and workgroups may share them as well, whose fp32 sums sparse_narrow_combine_kernel adds in order.
-#include "index_keys.hpp"
 #include "latent_mla.hpp"
 #include "latent_paged.hpp"
 #include "paged_sparse.hpp"
@@ -25,29 +24,23 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) s
   using Row = CacheRow<128, 64, FP4>;
   __shared__ __attribute__((aligned(16))) unsigned char tiles[4][8192];
   __shared__ float ML[WPU > 1 ? 4 : 1][32][2];
+  constexpr int UPG = 4 / WPU;  // units of a workgroup
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   unsigned char *K = tiles[w];
   const int64_t item = xcd_remap(blockIdx.x, gridDim.x);
-  const int64_t unit = WPU > 1 ? item / p.nsplit : item * 4 + w;
-  if (unit >= (int64_t)p.req.T * p.htiles) return;
-  const int t = __builtin_amdgcn_readfirstlane((int)(unit / p.htiles)), head0 = __builtin_amdgcn_readfirstlane((int)(unit % p.htiles)) * 32;
-  const int r = __builtin_amdgcn_readfirstlane(p.req.of(t)), lim = __builtin_amdgcn_readfirstlane(p.req.keys_of(t, r));
-  if (lim < 0) return;  // a token of no request
-  const int32_t *idx = p.indices + (int64_t)t * p.topk, *table = p.table + (int64_t)r * p.W;
+  const int64_t unit = item / p.nsplit * UPG + w / WPU, units = (int64_t)p.picks.req.T * p.htiles;
+  if (WPU == 1 && unit >= units) return;
+  const int t = __builtin_amdgcn_readfirstlane((int)((unit < units ? unit : units - 1) / p.htiles));
+  const int head0 = __builtin_amdgcn_readfirstlane((int)(unit % p.htiles)) * 32;
+  const int r = __builtin_amdgcn_readfirstlane(p.picks.req.of(t)), lim = __builtin_amdgcn_readfirstlane(p.picks.req.keys_of(t, r));
+  const bool nobody = unit >= units || lim < 0;  // (a token of no request)
+  if (WPU == 1 && nobody) return;
   // this wave's blocks of picks
-  const int nb = (p.topk + 31) / 32, parts = WPU * p.nsplit;
-  const int part = WPU > 1 ? (int)(item % p.nsplit) * WPU + w : 0;
-  const int b0 = (int)((int64_t)nb * part / parts), b1 = (int)((int64_t)nb * (part + 1) / parts);
+  const int nb = (p.picks.topk + 31) / 32, parts = WPU * p.nsplit;
+  const int part = (int)(item % p.nsplit) * WPU + w % WPU;
+  const int b0 = (int)((int64_t)nb * part / parts), b1 = nobody ? b0 : (int)((int64_t)nb * (part + 1) / parts);
 
-  auto pick = [&](int b) {  // position of the lane's pick in block b, -1: none
-    const int i = 32 * b + l32, pos = idx[i < p.topk ? i : p.topk - 1];
-    return i < p.topk && pos >= 0 && pos < lim ? pos : -1;
-  };
-  auto entry = [&](int pos) { return table[pos > 0 ? p.page_of(pos) : 0]; };
-  auto slot_of = [&](int pos, int e) {
-    if (pos < 0 || e < 0 || e >= p.num_blocks) return -1;
-    return e * p.block + (pos - p.page_of(pos) * p.block);
-  };
+  auto pick = [&](int b) { return p.picks.position(t, 32 * b + l32, lim); };  // of the lane in block b
   const unsigned char *zero = reinterpret_cast<const unsigned char *>(kZeroRow);
   auto row_at = [&](int slot) { return slot >= 0 ? p.cache + (int64_t)slot * Row::BYTES : zero; };
   auto load = [&](NarrowRows<FP4> &x, int slot) {
@@ -91,8 +84,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) s
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) q[ks] = ld_row_16(src + 32 * ks);
     }
-    const int slot0 = slot_of(pos0, entry(pos0));
-    int ent1 = entry(pos1);
+    const int slot0 = p.picks.slot(pos0, p.picks.entry(r, pos0));
+    int ent1 = p.picks.entry(r, pos1);
     uint32_t there = (uint32_t)wv::ballot(slot0 >= 0);
     load(rows, slot0);
     const RowRead row_read;
@@ -100,11 +93,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) s
     for (int b = b0; b < b1; ++b) {
       put(rows);
       const uint32_t vm = there;
-      const int slot = slot_of(pos1, ent1);
+      const int slot = p.picks.slot(pos1, ent1);
       there = (uint32_t)wv::ballot(slot >= 0);
       load(rows, slot);  // (past the last block: rows that are not used)
       pos1 = pos2;
-      ent1 = entry(pos1);
+      ent1 = p.picks.entry(r, pos1);
       pos2 = pick(b + 3);
       wave_lds_sync();
       if (vm != 0u) {
@@ -174,31 +167,32 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) s
       ML[w][l32][1] = l_run;
     }
     __syncthreads();
-    float m = kLeastMax, l = 0.0f, a[4];
+    if (nobody || head >= p.H) return;
+    const int w0 = w / WPU * WPU;
+    float m = kLeastMax, l = 0.0f, a[WPU];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (ML[k][l32][1] != 0.0f) m = fmaxf(m, ML[k][l32][0]);
+    for (int k = 0; k < WPU; ++k)
+      if (ML[w0 + k][l32][1] != 0.0f) m = fmaxf(m, ML[w0 + k][l32][0]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float lk = ML[k][l32][1];
-      a[k] = lk == 0.0f ? 0.0f : exp2_fast(ML[k][l32][0] - m);  // (no pick of the wave: its O is 0; a NaN sum joins)
+    for (int k = 0; k < WPU; ++k) {
+      const float lk = ML[w0 + k][l32][1];
+      a[k] = lk == 0.0f ? 0.0f : exp2_fast(ML[w0 + k][l32][0] - m);  // (no pick of the wave: its O is 0; a NaN sum joins)
       l += lk * a[k];
     }
-    if (head >= p.H) return;
     const bool whole = p.nsplit == 1;
-    const int64_t part_row = item * 32 + l32;
+    const int64_t part_row = (unit * p.nsplit + item % p.nsplit) * 32 + l32;
     const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int dm = 2 * w + i, col = acc_col(dm >> 2, 4 * (dm & 3), g32);
+    for (int i = 0; i < 8 / WPU; ++i) {
+      const int dm = 8 / WPU * (w - w0) + i, col = acc_col(dm >> 2, 4 * (dm & 3), g32);
       f32x4 x{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x += a[k] * *reinterpret_cast<const f32x4 *>(tiles[k] + (dm * 64 + lane) * 16);
+      for (int k = 0; k < WPU; ++k) x += a[k] * *reinterpret_cast<const f32x4 *>(tiles[w0 + k] + (dm * 64 + lane) * 16);
       x *= inv;
       if (whole) *reinterpret_cast<i32x2 *>(p.out + row * 64 + col) = i32x2{(int)pack_bf16x2(x[0], x[1]), (int)pack_bf16x2(x[2], x[3])};
       else *reinterpret_cast<f32x4 *>(p.part_o + part_row * 64 + col) = x;
     }
-    if (w == 0 && g32 == 0) {
+    if (w == w0 && g32 == 0) {
       if (whole) {
         p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
       } else {
@@ -212,10 +206,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) s
 // 16 lanes a (token, head): its splits' sums brought to their largest maximum and added in order.
 __global__ void __launch_bounds__(256) sparse_narrow_combine_kernel(const SparseParams p) {
   const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (row >= (int64_t)p.req.T * p.H) return;
+  if (row >= (int64_t)p.picks.req.T * p.H) return;
   const int64_t t = row / p.H;
   const int head = (int)(row - t * p.H), c = (int)(threadIdx.x & 15) * 4;
-  if (p.req.keys_of((int)t, p.req.of_lane((int)t)) < 0) return;
+  if (p.picks.req.keys_of((int)t, p.picks.req.of_lane((int)t)) < 0) return;
   const int64_t at = (t * p.htiles + head / 32) * p.nsplit * 32 + head % 32;
   float m = kLeastMax, l = 0.0f;
   for (int s = 0; s < p.nsplit; ++s)
@@ -238,7 +232,8 @@ struct NarrowPlan {
 };
 static NarrowPlan narrow_plan(int64_t T, int64_t topk, int64_t H) {
   const int64_t units = T * ((H + 31) / 32), nb = (topk + 31) / 32;
-  if (units >= 1536) return {1, 1};
+  if (units >= 3072) return {1, 1};
+  if (units >= 1024) return {2, 1};
   int64_t ns = 768 / units;               // workgroups that fill the card
   if (ns > nb / 8) ns = nb / 8;           // two blocks a wave at least
   return {4, (int)(ns < 1 ? 1 : ns)};
@@ -251,20 +246,21 @@ size_t sparse_narrow_workspace(int64_t T, int64_t topk, int64_t H) {
 template <bool FP4>
 static void launch_as(const SparseParams &p, int wpu, int64_t n, hipStream_t st) {
   if (wpu == 1) hipLaunchKernelGGL((sparse_narrow_kernel<FP4, 1>), dim3((unsigned)n), dim3(256), 0, st, p);
+  else if (wpu == 2) hipLaunchKernelGGL((sparse_narrow_kernel<FP4, 2>), dim3((unsigned)n), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((sparse_narrow_kernel<FP4, 4>), dim3((unsigned)n), dim3(256), 0, st, p);
 }
 int launch_sparse_narrow(SparseParams p, bool fp4, unsigned char *ws, hipStream_t st) {
-  const NarrowPlan k = narrow_plan(p.req.T, p.topk, p.H);
+  const NarrowPlan k = narrow_plan(p.picks.req.T, p.picks.topk, p.H);
   p.htiles = (p.H + 31) / 32;
   p.nsplit = k.nsplit;
-  const int64_t units = (int64_t)p.req.T * p.htiles, n = k.wpu == 1 ? (units + 3) / 4 : units * k.nsplit;
+  const int64_t units = (int64_t)p.picks.req.T * p.htiles, n = (units * k.wpu + 3) / 4 * k.nsplit;
   p.part_o = (float *)ws;
   p.part_ml = p.part_o + units * k.nsplit * 32 * 64;
   if (fp4) launch_as<true>(p, k.wpu, n, st);
   else launch_as<false>(p, k.wpu, n, st);
   const int rc = check_launch("dsa_paged_sparse_mla_fwd");
   if (rc || k.nsplit == 1) return rc;
-  hipLaunchKernelGGL(sparse_narrow_combine_kernel, dim3((unsigned)(((int64_t)p.req.T * p.H + 15) / 16)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(sparse_narrow_combine_kernel, dim3((unsigned)(((int64_t)p.picks.req.T * p.H + 15) / 16)), dim3(256), 0, st, p);
   return check_launch("dsa_paged_sparse_mla_fwd (combine)");
 }
 
