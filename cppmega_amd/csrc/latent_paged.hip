@@ -23,37 +23,6 @@ __device__ __forceinline__ int unit_blocks(const PagedParams &p, int kv, int n, 
   return max((token_keys(kv, n, last / p.H) + p.step_keys - 1) / p.step_keys, 1);
 }
 
-// Sums that stop at 2^32 - 1: starts that do not ascend may count a token many times over.
-__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
-__device__ __forceinline__ uint32_t wave_scan_sat(uint32_t x) {  // wv::wave_incl_scan's steps
-  x = add_sat(x, wv::dpp<0x111, 0xf, true>(x));
-  x = add_sat(x, wv::dpp<0x112, 0xf, true>(x));
-  x = add_sat(x, wv::dpp<0x114, 0xf, true>(x));
-  x = add_sat(x, wv::dpp<0x118, 0xf, true>(x));
-  x = add_sat(x, wv::dpp<0x142, 0xa>(x));
-  x = add_sat(x, wv::dpp<0x143, 0xc>(x));
-  return x;
-}
-// Exclusive prefix over the workgroup of one value below 2^31 per thread; total in every thread.  Exact below 2^32 - 1,
-// at least 2^31 (the stop, less the thread's value) past it.
-template <int NTHR>
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *tmp, uint32_t &total) {
-  const int lane = lane_id(), w = (int)(threadIdx.x >> 6);
-  const uint32_t v = wave_scan_sat(x);
-  __syncthreads();
-  if (lane == 63) tmp[w] = v;
-  __syncthreads();
-  uint32_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < NTHR / 64; ++i) {
-    const uint32_t t = tmp[i];
-    if (i < w) before = add_sat(before, t);
-    total = add_sat(total, t);
-  }
-  return add_sat(before, v) - x;
-}
-
 // The plan, one workgroup: unit_req[u], unit_first[u] (first row), unit_at[u] (first block,
 // unit_at[units] = all), unit0[r] (first unit of request r; unit0[R] = all).
 __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {

@@ -6,17 +6,22 @@
 // matrix instructions that take 8-bit codes keep fewer bits of their sums than 32 (a score was off by 1.5e-5 of the scores'
 // size; this way 1e-7), and every key that is read serves 16 products at least.
 //
-// Two kernels.  Single tokens (index_rows_kernel): a workgroup has one token and a chunk of its keys, whose 32-key tiles
-// its waves take in turn, straight from memory to operand registers (a lane's 16-byte piece of a key is two steps' operands
-// in MXFP8 and four in MXFP4: the order of the channels in a product is free), two tiles ahead, without a barrier.
-// Several tokens of a request (index_tiles_kernel): four waves with the (token, head) rows of 4 * 64 / H tokens share
-// tiles of 64 keys in LDS, widened as they enter it.
+// Two kernels.  Single tokens (index_rows_kernel): a workgroup's waves take the 32-key tiles of a token in turn, straight from
+// memory to operand registers (a lane's 16-byte piece of a key is two steps' operands in MXFP8 and four in MXFP4: the order
+// of the channels in a product is free), two tiles ahead, without a barrier.  Several tokens of a request
+// (index_tiles_kernel): four waves with the (token, head) rows of 4 * 64 / H tokens share tiles of 64 keys in LDS, widened
+// as they enter it.
+//
+// A unit is a token (or tile of tokens) with its request's keys in blocks of 128, and behind them the columns that no token
+// of it sees, in blocks of -inf to write.  All units' blocks, one after the other, are split evenly over the workgroups
+// that the card holds, on the device, from the lengths: the host knows none of them.
 #include "index_keys.hpp"
 #include "wave_ops.hpp"
 
 namespace dsa {
 
-constexpr int kMostChunk = 2048;  // keys of a workgroup, at most: its pages lie in LDS
+constexpr int kWindowPages = 2048;  // pages of a unit that a workgroup has in LDS
+constexpr int kBlockKeys = 128;
 
 static __device__ const i32x4 kNoKey[16] = {};  // the row of a key that is not there
 
@@ -65,8 +70,125 @@ __device__ __forceinline__ KeyAt key_at(const IndexScoreParams &p, const int *wi
   k.expo = k.there ? page + (int64_t)p.block * Row::CODES + (int64_t)off * 4 : none;
   return k;
 }
+// -inf into columns [from, to) of a row.
 __device__ __forceinline__ void fill_none(float *row, int from, int to) {
-  for (int i = from + (int)threadIdx.x; i < to; i += 256) row[i] = -INFINITY;
+  int head = from + (int)((16u - (uint32_t)reinterpret_cast<uintptr_t>(row + from) % 16u) % 16u / 4u);  // 16-byte stores from here
+  head = head < to ? head : to;
+  const int wide = (to - head) / 4;
+  if (from + (int)threadIdx.x < head) row[from + threadIdx.x] = -INFINITY;
+  for (int i = (int)threadIdx.x; i < wide; i += 256)
+    reinterpret_cast<f32x4 *>(row + head)[i] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (head + 4 * wide + (int)threadIdx.x < to) row[head + 4 * wide + threadIdx.x] = -INFINITY;
+}
+
+// The blocks of a request's units: its tokens that are scored by TT, each with nb blocks of keys and fb of columns to fill.
+struct RequestUnits {
+  int ta, n, nb, fb;  // first token, tokens
+};
+template <int TT>
+struct ScoreUnits {
+  static constexpr int FILL = 4096 / TT;  // columns of a block to fill: about the time of a block of keys
+  static __device__ __forceinline__ RequestUnits of(const IndexScoreParams &p, int r) {
+    RequestUnits u;
+    const int at = p.req.start(r), tb = min(at + p.req.tokens(r), p.first + p.tokens);
+    u.ta = max(at, p.first);
+    u.n = max(tb - u.ta, 0);
+    const int keys = min(p.req.kv(r), p.L);
+    u.nb = (keys + kBlockKeys - 1) / kBlockKeys;
+    u.fb = max(p.L - u.nb * kBlockKeys + FILL - 1, 0) / FILL;
+    return u;
+  }
+  static __device__ __forceinline__ uint32_t blocks(const IndexScoreParams &p, int r) {
+    const RequestUnits u = of(p, r);
+    return (uint32_t)((u.n + TT - 1) / TT) * (uint32_t)(u.nb + u.fb);
+  }
+};
+// The workgroup's range [at, end) of all blocks, and the request at `at`: 256 requests' first blocks stand in `begin`.
+struct ScoreWalk {
+  uint32_t at, end;
+  int chunk, i;  // requests 256 chunk .., of which request i is at hand
+};
+struct ScoreLds {
+  uint32_t tmp[4], begin[257];
+};
+template <int TT>
+__device__ __forceinline__ void load_requests(const IndexScoreParams &p, ScoreLds &s, int chunk, uint32_t base) {
+  const int r = 256 * chunk + (int)threadIdx.x;
+  uint32_t total;
+  const uint32_t mine = block_scan<256>(r < p.req.R ? ScoreUnits<TT>::blocks(p, r) : 0u, s.tmp, total);
+  s.begin[threadIdx.x] = add_sat(base, mine);
+  if (threadIdx.x == 0) s.begin[256] = add_sat(base, total);
+  __syncthreads();
+}
+template <int TT>
+__device__ __forceinline__ ScoreWalk start_walk(const IndexScoreParams &p, ScoreLds &s) {
+  const int chunks = (p.req.R + 255) / 256;
+  uint32_t total = 0;
+  for (int c = 0; c < chunks; ++c) {
+    load_requests<TT>(p, s, c, total);
+    total = s.begin[256];
+    __syncthreads();
+  }
+  const uint32_t per = total / gridDim.x + (total % gridDim.x != 0);
+  ScoreWalk k;
+  const uint64_t at = (uint64_t)blockIdx.x * per;
+  k.at = at < total ? (uint32_t)at : total;
+  k.end = per < total - k.at ? k.at + per : total;
+  k.chunk = 0;
+  k.i = 0;
+  if (chunks > 1 && k.at < k.end) {
+    uint32_t base = 0;
+    for (int c = 0; c < chunks; ++c) {
+      load_requests<TT>(p, s, c, base);
+      base = s.begin[256];
+      k.chunk = c;
+      if (base > k.at) break;  // (uniform)
+      __syncthreads();
+    }
+  }
+  return k;
+}
+// The piece at k.at: request, its units' first block, the unit's tokens and its blocks [b0, b1); k.at moves past it.
+struct ScorePiece {
+  int r, ta, tb, nb, b0, b1;
+};
+template <int TT>
+__device__ __forceinline__ ScorePiece next_piece(const IndexScoreParams &p, ScoreLds &s, ScoreWalk &k) {
+  while (true) {
+    if (k.i == 256) {  // (uniform, as are the loop's other values)
+      const uint32_t base = s.begin[256];
+      __syncthreads();
+      load_requests<TT>(p, s, ++k.chunk, base);
+      k.i = 0;
+    }
+    if (s.begin[k.i + 1] > k.at) break;
+    ++k.i;
+  }
+  ScorePiece x;
+  x.r = __builtin_amdgcn_readfirstlane(256 * k.chunk + k.i);
+  const RequestUnits u = ScoreUnits<TT>::of(p, x.r);
+  const uint32_t off = k.at - s.begin[k.i], ub = (uint32_t)(u.nb + u.fb), tile = off / ub, b0 = off - tile * ub;
+  x.ta = __builtin_amdgcn_readfirstlane(u.ta + (int)tile * TT);
+  x.tb = __builtin_amdgcn_readfirstlane(min(x.ta + TT, u.ta + u.n));
+  x.nb = __builtin_amdgcn_readfirstlane(u.nb);
+  x.b0 = __builtin_amdgcn_readfirstlane((int)b0);
+  x.b1 = __builtin_amdgcn_readfirstlane((int)(ub - b0 < k.end - k.at ? ub : b0 + (k.end - k.at)));
+  k.at += (uint32_t)(x.b1 - x.b0);
+  return x;
+}
+// The piece's blocks to fill.
+template <int TT>
+__device__ __forceinline__ void fill_piece(const IndexScoreParams &p, const ScorePiece &x) {
+  constexpr int FILL = ScoreUnits<TT>::FILL;
+  if (x.b1 <= x.nb) return;
+  const int keys = x.nb * kBlockKeys, from = keys + max(x.b0 - x.nb, 0) * FILL;
+  const int64_t to = (int64_t)keys + (int64_t)(x.b1 - x.nb) * FILL;
+  for (int t = x.ta; t < x.tb; ++t) fill_none(p.out + (int64_t)(t - p.first) * p.L, from, to < p.L ? (int)to : p.L);
+}
+__device__ __forceinline__ void write_limits(const IndexScoreParams &p) {
+  if (p.limits == nullptr) return;
+  for (int i = (int)blockIdx.x * 256 + (int)threadIdx.x; i < p.tokens; i += (int)gridDim.x * 256)
+    p.limits[i] = p.req.R > 0 ? min(max(p.req.keys_of(p.first + i, p.req.of_lane(p.first + i)), 0), p.L) : 0;
 }
 
 template <int H, int D, int FMT>
@@ -74,94 +196,93 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
   using Row = KeyRow<D, FMT>;
   constexpr int MT = H > 32 ? H / 32 : 1, ROWS = H < 32 ? H / 2 : 16;  // row tiles; their accumulators with a head in them
   constexpr int NC = Row::CODES / 32, U = Row::CPE / 8;               // pieces of a key in a lane; their steps
-  __shared__ int window[kMostChunk];
+  __shared__ int window[kWindowPages];
+  __shared__ ScoreLds units;
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
-  const int tile = (int)blockIdx.x % p.tiles, k0 = (int)blockIdx.x / p.tiles * p.chunk, t = p.first + tile;
-  int r = 0, lim = -1;  // keys of the token, -1: a token of no request
-  if (p.req.R > 0) {
-    r = __builtin_amdgcn_readfirstlane(p.req.of(t));
-    const int at = p.req.start(r), n = p.req.tokens(r);
-    if (t >= at && t < at + n) lim = max(p.req.kv(r) - n + (t - at) + 1, 0);
-  }
-  lim = __builtin_amdgcn_readfirstlane(lim);
-  if (p.limits != nullptr && k0 == 0 && threadIdx.x == 0) p.limits[tile] = min(max(lim, 0), p.L);
-  if (lim < 0) return;
-  float *out = p.out + (int64_t)tile * p.L;
-  const int k1 = min(k0 + p.chunk, p.L), kend = min(k1, lim);
-  fill_none(out, max(k0, kend), k1);
-  if (kend <= k0) return;
+  const float least = p.relu ? 0.0f : -INFINITY;
+  write_limits(p);
+  ScoreWalk walk = start_walk<1>(p, units);
+  while (walk.at < walk.end) {
+    const ScorePiece x = next_piece<1>(p, units, walk);
+    fill_piece<1>(p, x);
+    if (x.b0 >= x.nb) continue;
+    const int t = x.ta, lim = min(__builtin_amdgcn_readfirstlane(p.req.keys_of(t, x.r)), p.L);
+    const int kb1 = min(min(x.b1, x.nb) * kBlockKeys, p.L);
+    float *out = p.out + (int64_t)(t - p.first) * p.L;
 
-  // operand of step (c, u): channels CPE (2 c + g32) + 8 u ..
-  i32x4 q[MT][NC * U];
-  float wv[MT][ROWS];
+    // operand of step (c, u): channels CPE (2 c + g32) + 8 u ..
+    i32x4 q[MT][NC * U];
+    float wv[MT][ROWS];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int h = 32 * m + l32;
+    for (int m = 0; m < MT; ++m) {
+      const int h = 32 * m + l32;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        q[m][c * U + u] = h < H ? ld_global_16(p.q + (((int64_t)t * H + h) * D + Row::CPE * (2 * c + g32) + 8 * u) * 2) : i32x4{0, 0, 0, 0};
-  }
-  {
+        for (int u = 0; u < U; ++u)
+          q[m][c * U + u] = h < H ? ld_global_16(p.q + (((int64_t)t * H + h) * D + Row::CPE * (2 * c + g32) + 8 * u) * 2) : i32x4{0, 0, 0, 0};
+    }
     const float wl = lane < H ? weight_at(p, (int64_t)t * H + lane) : 0.0f;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int a = 0; a < ROWS; ++a) wv[m][a] = __shfl(wl, 32 * m + score_row(a, g32), 64);
-  }
-  const float least = p.relu ? 0.0f : -INFINITY;
-  fill_window<256>(p, window, r, k0, kend);
-  const int pg0 = page_of(p, k0);
 
-  struct Piece {
-    i32x4 codes[NC];
-    uint32_t expo;
-    bool there;
-  };
-  auto load = [&](Piece &x, int sub) {
-    const KeyAt k = key_at<Row>(p, window, pg0, k0 + 32 * sub + l32, kend);
-    x.there = k.there;
+    for (int k0 = x.b0 * kBlockKeys; k0 < kb1; k0 += p.span) {
+      const int k1 = min(k0 + p.span, kb1), kend = min(k1, lim);  // columns; keys that the token sees
+      __syncthreads();  // the window's readers are done
+      if (kend > k0) fill_window<256>(p, window, x.r, k0, kend);
+      const int pg0 = page_of(p, k0);
+      struct Piece {
+        i32x4 codes[NC];
+        uint32_t expo;
+        bool there;
+      };
+      auto load = [&](Piece &y, int sub) {
+        const KeyAt k = key_at<Row>(p, window, pg0, k0 + 32 * sub + l32, kend);
+        y.there = k.there;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) x.codes[c] = ld_16(k.codes + 16 * (2 * c + g32));
-    x.expo = FMT == KEY_BF16 ? 0u : ld_4(k.expo);
-  };
-  auto score = [&](const Piece &x, int sub) {
-    f32x16 acc[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int a = 0; a < 16; ++a) acc[m][a] = 0.0f;
-    const uint32_t mine = FMT == KEY_MXFP4 ? x.expo >> (8 * g32) : x.expo;  // byte of piece c: 2 c + g32, c
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const uint32_t e = (mine >> (FMT == KEY_MXFP4 ? 16 * c : 8 * c)) & 255u;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const i32x4 k = key_values<FMT>(x.codes[c], u, e);
+        for (int c = 0; c < NC; ++c) y.codes[c] = ld_16(k.codes + 16 * (2 * c + g32));
+        y.expo = FMT == KEY_BF16 ? 0u : ld_4(k.expo);
+      };
+      auto score = [&](const Piece &y, int sub) {
+        f32x16 acc[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(q[m][c * U + u]), as_bf16x8(k), acc[m], 0, 0, 0);
+#pragma unroll
+          for (int a = 0; a < 16; ++a) acc[m][a] = 0.0f;
+        const uint32_t mine = FMT == KEY_MXFP4 ? y.expo >> (8 * g32) : y.expo;  // byte of piece c: 2 c + g32, c
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const uint32_t e = (mine >> (FMT == KEY_MXFP4 ? 16 * c : 8 * c)) & 255u;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const i32x4 k = key_values<FMT>(y.codes[c], u, e);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(q[m][c * U + u]), as_bf16x8(k), acc[m], 0, 0, 0);
+          }
+        }
+        float part = 0.0f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int a = 0; a < ROWS; ++a) part = fmaf(__builtin_elementwise_maximum(acc[m][a], least), wv[m][a], part);
+        part = sum_halves(part);
+        const int key = k0 + 32 * sub + l32;
+        if (g32 == 0 && key < k1) out[key] = y.there ? part : -INFINITY;
+      };
+      const int nsub = (k1 - k0 + 31) / 32;
+      Piece a, b;  // (tiles past the last: kNoKey)
+      load(a, w);
+      load(b, w + 4);
+      for (int sub = w; sub < nsub; sub += 8) {
+        score(a, sub);
+        load(a, sub + 8);
+        if (sub + 4 < nsub) score(b, sub + 4);
+        load(b, sub + 12);
       }
     }
-    float part = 0.0f;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int a = 0; a < ROWS; ++a) part = fmaf(__builtin_elementwise_maximum(acc[m][a], least), wv[m][a], part);
-    part = sum_halves(part);
-    const int key = k0 + 32 * sub + l32;
-    if (g32 == 0 && key < kend) out[key] = x.there ? part : -INFINITY;
-  };
-  const int nsub = (kend - k0 + 31) / 32;
-  Piece a, b;  // (tiles past the last: kNoKey)
-  load(a, w);
-  load(b, w + 4);
-  for (int sub = w; sub < nsub; sub += 8) {
-    score(a, sub);
-    load(a, sub + 8);
-    if (sub + 4 < nsub) score(b, sub + 4);
-    load(b, sub + 12);
   }
 }
 
@@ -182,77 +303,67 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
   using Row = typename C::Row;
   constexpr int TPW = C::TPW, KS = D / 16;
   __shared__ __attribute__((aligned(16))) unsigned char K[2][C::KT * C::RB];
-  __shared__ int window[kMostChunk];
+  __shared__ int window[kWindowPages];
+  __shared__ ScoreLds units;
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
-  const int tile0 = (int)blockIdx.x % p.tiles * C::TT, k0 = (int)blockIdx.x / p.tiles * p.chunk, k1 = min(k0 + p.chunk, p.L);
-  const int t0 = p.first + tile0, t1 = min(t0 + C::TT, p.first + p.tokens), my0 = t0 + w * TPW;  // the wave's first token
+  const float least = p.relu ? 0.0f : -INFINITY;
+  write_limits(p);
+  ScoreWalk walk = start_walk<C::TT>(p, units);
+  while (walk.at < walk.end) {
+    const ScorePiece x = next_piece<C::TT>(p, units, walk);
+    fill_piece<C::TT>(p, x);
+    if (x.b0 >= x.nb) continue;
+    const int my0 = x.ta + w * TPW;  // the wave's first token
+    const int at = __builtin_amdgcn_readfirstlane(p.req.start(x.r)), n = __builtin_amdgcn_readfirstlane(p.req.tokens(x.r));
+    const int kv = __builtin_amdgcn_readfirstlane(p.req.kv(x.r));
+    auto keys_of = [&](int t) { return max(kv - n + (t - at) + 1, 0); };
+    const int kb1 = min(min(x.b1, x.nb) * kBlockKeys, p.L), most = keys_of(x.tb - 1);
 
-  i32x4 q[2][KS];
-  float wv[2][16];
+    i32x4 q[2][KS];
+    float wv[2][16];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int row = 32 * m + l32;
-    const bool ok = my0 + row / H < t1;
+    for (int m = 0; m < 2; ++m) {
+      const int row = 32 * m + l32;
+      const bool ok = my0 + row / H < x.tb;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      q[m][ks] = ok ? ld_global_16(p.q + (((int64_t)my0 * H + row) * D + 16 * ks + 8 * g32) * 2) : i32x4{0, 0, 0, 0};
-  }
-  {
-    const float wl = my0 + lane / H < t1 ? weight_at(p, (int64_t)my0 * H + lane) : 0.0f;
+      for (int ks = 0; ks < KS; ++ks)
+        q[m][ks] = ok ? ld_global_16(p.q + (((int64_t)my0 * H + row) * D + 16 * ks + 8 * g32) * 2) : i32x4{0, 0, 0, 0};
+    }
+    const float wl = my0 + lane / H < x.tb ? weight_at(p, (int64_t)my0 * H + lane) : 0.0f;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int a = 0; a < 16; ++a) wv[m][a] = __shfl(wl, 32 * m + score_row(a, g32), 64);
-  }
-  const float least = p.relu ? 0.0f : -INFINITY;
+    const bool works = my0 < x.tb;  // wave-uniform
 
-  // the tile's tokens, request by request: [ta, tb) are of one
-  for (int ta = t0; ta < t1;) {
-    int r = 0, at = 0, n = 0;
-    if (p.req.R > 0) {
-      r = __builtin_amdgcn_readfirstlane(p.req.of(ta));
-      at = __builtin_amdgcn_readfirstlane(p.req.start(r));
-      n = __builtin_amdgcn_readfirstlane(p.req.tokens(r));
-    }
-    if (ta < at || ta >= at + n) {  // of no request
-      if (p.limits != nullptr && k0 == 0 && threadIdx.x == 0) p.limits[ta - p.first] = 0;
-      ++ta;
-      continue;
-    }
-    const int tb = min(t1, at + n), kv = __builtin_amdgcn_readfirstlane(p.req.kv(r));
-    auto keys_of = [&](int t) { return max(kv - n + (t - at) + 1, 0); };
-    if (p.limits != nullptr && k0 == 0)
-      for (int t = ta + (int)threadIdx.x; t < tb; t += 256) p.limits[t - p.first] = min(keys_of(t), p.L);
-    const int kend = min(k1, keys_of(tb - 1));
-    for (int t = ta; t < tb; ++t) fill_none(p.out + (int64_t)(t - p.first) * p.L, max(k0, kend), k1);
-    if (kend > k0) {
-      __syncthreads();  // the window's readers are done
-      const bool all_there = fill_window<256>(p, window, r, k0, kend);
+    for (int k0 = x.b0 * kBlockKeys; k0 < kb1; k0 += p.span) {
+      const int k1 = min(k0 + p.span, kb1), kend = min(k1, most);  // columns; keys that a token sees
+      __syncthreads();  // the readers of the window and the tiles are done
+      const bool all_there = kend <= k0 || fill_window<256>(p, window, x.r, k0, kend);
       const int pg0 = page_of(p, k0);
-      const bool works = my0 < tb && my0 + TPW > ta;  // wave-uniform
       i32x4 raw[C::NL];
       uint32_t expo[C::NL];
       auto load = [&](int j) {
 #pragma unroll
         for (int i = 0; i < C::NL; ++i) {
-          const int x = (int)threadIdx.x + 256 * i;
-          if (C::N % 256 != 0 && x >= C::N) break;
-          const KeyAt k = key_at<Row>(p, window, pg0, k0 + C::KT * j + x / C::CPR, kend);
-          raw[i] = ld_16(k.codes + 16 * (x % C::CPR));
+          const int y = (int)threadIdx.x + 256 * i;
+          if (C::N % 256 != 0 && y >= C::N) break;
+          const KeyAt k = key_at<Row>(p, window, pg0, k0 + C::KT * j + y / C::CPR, kend);
+          raw[i] = ld_16(k.codes + 16 * (y % C::CPR));
           expo[i] = FMT == KEY_BF16 ? 0u : ld_4(k.expo);
         }
       };
       auto store = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < C::NL; ++i) {
-          const int x = (int)threadIdx.x + 256 * i, row = x / C::CPR, c = x % C::CPR;
-          if (C::N % 256 != 0 && x >= C::N) break;
+          const int y = (int)threadIdx.x + 256 * i, row = y / C::CPR, c = y % C::CPR;
+          if (C::N % 256 != 0 && y >= C::N) break;
           const uint32_t e = (expo[i] >> (8 * (c * Row::CPE / 32))) & 255u;
 #pragma unroll
           for (int u = 0; u < C::U; ++u) *reinterpret_cast<i32x4 *>(K[buf] + C::at(row, c * C::U + u)) = key_values<FMT>(raw[i], u, e);
         }
       };
-      const int nt = (kend - k0 + C::KT - 1) / C::KT;
+      const int nt = (k1 - k0 + C::KT - 1) / C::KT;
       load(0);
       for (int j = 0; j < nt; ++j) {
         store(j & 1);
@@ -285,11 +396,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
             }
         }
         // two sums at a time: the low lanes get the first one's, the high lanes the second's
-        auto put = [&](float x, float y, int t, int key) {
-          const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+        auto put = [&](float y, float z, int t, int key) {
+          const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(z), false, false);
           float v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
           if (key >= keys_of(t) || (!all_there && key < kend && window[page_of(p, key) - pg0] < 0)) v = -INFINITY;
-          if (t >= ta && t < tb && key < kend) p.out[(int64_t)(t - p.first) * p.L + key] = v;
+          if (t < x.tb && key < k1) p.out[(int64_t)(t - p.first) * p.L + key] = v;
         };
         const int key0 = k0 + C::KT * j;
         if constexpr (TPW == 1) {
@@ -301,9 +412,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
             for (int tl = 0; tl < TPW; tl += 2) put(part[sub][tl], part[sub][tl + 1], my0 + tl + g32, key0 + 32 * sub + l32);
         }
       }
-      __syncthreads();  // the tiles' readers are done
     }
-    ta = tb;
   }
 }
 
@@ -312,15 +421,17 @@ static int launch_scores(IndexScoreParams p, hipStream_t st) {
   using C = IndexTile<H, D, FMT>;
   // single tokens: a request has fewer than two on average
   const bool rows = p.req.query_starts == nullptr || p.req.R == 0 || p.req.T < 2 * (int64_t)p.req.R;
-  p.tiles = rows ? p.tokens : (p.tokens + C::TT - 1) / C::TT;
-  // keys of a workgroup: as many as leave four workgroups for every compute unit
-  p.chunk = kMostChunk;
-  const auto chunks = [&] { return p.L > 0 ? ((int64_t)p.L + p.chunk - 1) / p.chunk : 1; };
-  while (p.chunk > 128 && p.tiles * chunks() < 1024) p.chunk /= 2;
-  const int64_t n = p.tiles * chunks();
+  p.span = (int)((int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys < (1 << 30) ? (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys
+                                                                                            : 1 << 30);
+  // blocks, at most: fewer than 2^31 of them, and workgroups that all run at once
+  const int tt = rows ? 1 : C::TT, fill = 4096 / tt;
+  const int64_t units = rows ? p.tokens : (int64_t)p.tokens / tt + (p.tokens < p.req.R ? p.tokens : p.req.R);
+  const int64_t n = units * (((int64_t)p.L + kBlockKeys - 1) / kBlockKeys + ((int64_t)p.L + fill - 1) / fill);
   DSA_REQUIRE(n < (1ll << 31), "dsa_paged_index_scores: too many tokens for one call");
-  if (rows) hipLaunchKernelGGL((index_rows_kernel<H, D, FMT>), dim3((unsigned)n), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((index_tiles_kernel<H, D, FMT>), dim3((unsigned)n), dim3(256), 0, st, p);
+  const int64_t most = 256 * (rows ? (H == 64 ? 2 : 4) : 2);
+  const dim3 grid((unsigned)(n < 1 ? 1 : n < most ? n : most));
+  if (rows) hipLaunchKernelGGL((index_rows_kernel<H, D, FMT>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((index_tiles_kernel<H, D, FMT>), grid, dim3(256), 0, st, p);
   return check_launch("dsa_paged_index_scores");
 }
 template <int H, int D>

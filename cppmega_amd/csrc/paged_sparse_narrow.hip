@@ -226,14 +226,15 @@ __global__ void __launch_bounds__(256) sparse_narrow_combine_kernel(const Sparse
   if (c == 0) p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
 }
 
-// How a call is run: waves of a unit, workgroups that share it.
+// How a call is run: waves of a unit, workgroups that share it.  Replays of n tokens, 32 heads, one and four waves a unit:
+// top-256: n = 512 19 us, 17; 1000 19, 22; 1656 24, 28; 2200 28, 31; top-2048: 64 (four waves of eight workgroups) 76, 25;
+// 1000 82, 62; 1656 100, 103.  (Two waves a unit: between the two, or behind both.)
 struct NarrowPlan {
   int wpu, nsplit;
 };
 static NarrowPlan narrow_plan(int64_t T, int64_t topk, int64_t H) {
   const int64_t units = T * ((H + 31) / 32), nb = (topk + 31) / 32;
-  if (units >= 3072) return {1, 1};
-  if (units >= 1024) return {2, 1};
+  if (units >= 1536) return {1, 1};
   int64_t ns = 768 / units;               // workgroups that fill the card
   if (ns > nb / 8) ns = nb / 8;           // two blocks a wave at least
   return {4, (int)(ns < 1 ? 1 : ns)};
@@ -246,7 +247,6 @@ size_t sparse_narrow_workspace(int64_t T, int64_t topk, int64_t H) {
 template <bool FP4>
 static void launch_as(const SparseParams &p, int wpu, int64_t n, hipStream_t st) {
   if (wpu == 1) hipLaunchKernelGGL((sparse_narrow_kernel<FP4, 1>), dim3((unsigned)n), dim3(256), 0, st, p);
-  else if (wpu == 2) hipLaunchKernelGGL((sparse_narrow_kernel<FP4, 2>), dim3((unsigned)n), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((sparse_narrow_kernel<FP4, 4>), dim3((unsigned)n), dim3(256), 0, st, p);
 }
 int launch_sparse_narrow(SparseParams p, bool fp4, unsigned char *ws, hipStream_t st) {

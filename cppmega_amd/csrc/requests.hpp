@@ -2,8 +2,40 @@
 #pragma once
 
 #include "dsa_common.hpp"
+#include "wave_ops.hpp"
 
 namespace dsa {
+
+// Sums that stop at 2^32 - 1: starts that do not ascend may count a token many times over.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ uint32_t wave_scan_sat(uint32_t x) {  // wv::wave_incl_scan's steps
+  x = add_sat(x, wv::dpp<0x111, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x112, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x114, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x118, 0xf, true>(x));
+  x = add_sat(x, wv::dpp<0x142, 0xa>(x));
+  x = add_sat(x, wv::dpp<0x143, 0xc>(x));
+  return x;
+}
+// Exclusive prefix over the workgroup of one value below 2^31 per thread; total in every thread.  Exact below 2^32 - 1,
+// at least 2^31 (the stop, less the thread's value) past it.
+template <int NTHR>
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *tmp, uint32_t &total) {
+  const int lane = lane_id(), w = (int)(threadIdx.x >> 6);
+  const uint32_t v = wave_scan_sat(x);
+  __syncthreads();
+  if (lane == 63) tmp[w] = v;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < NTHR / 64; ++i) {
+    const uint32_t t = tmp[i];
+    if (i < w) before = add_sat(before, t);
+    total = add_sat(total, t);
+  }
+  return add_sat(before, v) - x;
+}
 
 // The requests of a call: tokens query_starts[r] .. query_starts[r + 1] of the batch (null: token r alone) are the last of
 // request r's kv_lens[r] positions.
