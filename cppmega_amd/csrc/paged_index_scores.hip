@@ -23,6 +23,9 @@ namespace dsa {
 constexpr int kWindowPages = 2048;  // pages of a unit that a workgroup has in LDS
 constexpr int kBlockKeys = 128;
 
+// Keeps a wave-uniform branch a branch.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
 static __device__ const i32x4 kNoKey[16] = {};  // the row of a key that is not there
 
 __device__ __forceinline__ i32x4 ld_16(const unsigned char *x) {
@@ -87,7 +90,7 @@ struct RequestUnits {
 };
 template <int TT>
 struct ScoreUnits {
-  static constexpr int FILL = 4096 / TT;  // columns of a block to fill: about the time of a block of keys
+  static constexpr int FILL = TT == 1 ? 4096 : 16384 / TT;  // columns of a block to fill: about the time of a block of keys
   static __device__ __forceinline__ RequestUnits of(const IndexScoreParams &p, int r) {
     RequestUnits u;
     const int at = p.req.start(r), tb = min(at + p.req.tokens(r), p.first + p.tokens);
@@ -363,6 +366,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
           for (int u = 0; u < C::U; ++u) *reinterpret_cast<i32x4 *>(K[buf] + C::at(row, c * C::U + u)) = key_values<FMT>(raw[i], u, e);
         }
       };
+      // the rows that the lane writes: of tokens 2 i + g32 (one token a wave: its)
+      constexpr int NP = TPW > 1 ? TPW / 2 : 1;
+      float *row[NP];
+      int sees[NP];
+      bool mine[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int t = my0 + (TPW > 1 ? 2 * i + g32 : 0);
+        mine[i] = t < x.tb;
+        sees[i] = keys_of(t);
+        row[i] = p.out + (int64_t)(t - p.first) * p.L + k0;
+      }
+      const int least_keys = min(keys_of(my0), k1);
       const int nt = (k1 - k0 + C::KT - 1) / C::KT;
       load(0);
       for (int j = 0; j < nt; ++j) {
@@ -370,46 +386,64 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
         load(j + 1);  // (past the last: kNoKey)
         __syncthreads();  // tile j is whole; its buffer's readers of two tiles ago passed the barrier before
         if (!works) continue;
+        // Four tiles of 32 rows by 32 keys; a tile's ReLU and weights beside the next one's products, in one stream, since the
+        // SIMD overlaps the two within a wave far more than across waves.
         float part[2][TPW];
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          f32x16 acc[2];
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int a = 0; a < 16; ++a) acc[m][a] = 0.0f;
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const i32x4 k = *reinterpret_cast<const i32x4 *>(K[j & 1] + C::at(32 * sub + l32, 2 * ks + g32));
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-              acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(q[m][ks]), as_bf16x8(k), acc[m], 0, 0, 0);
-          }
+        for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
           for (int tl = 0; tl < TPW; ++tl) part[sub][tl] = 0.0f;
+        f32x16 acc[2];
+        i32x4 k[KS];
+        auto weigh = [&](int tile) {  // tile: 2 sub + m
+          const int sub = tile >> 1, m = tile & 1;
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
+          for (int a = 0; a < 16; ++a) {
+            const int tl = (32 * m + 8 * (a >> 2)) / H;
+            part[sub][tl] = fmaf(__builtin_elementwise_maximum(acc[m][a], least), wv[m][a], part[sub][tl]);
+          }
+        };
 #pragma unroll
-            for (int a = 0; a < 16; ++a) {
-              const int tl = (32 * m + 8 * (a >> 2)) / H;
-              part[sub][tl] = fmaf(__builtin_elementwise_maximum(acc[m][a], least), wv[m][a], part[sub][tl]);
-            }
+        for (int tile = 0; tile < 4; ++tile) {
+          if ((tile & 1) == 0)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) k[ks] = *reinterpret_cast<const i32x4 *>(K[j & 1] + C::at(16 * tile + l32, 2 * ks + g32));
+          const int m = tile & 1;
+#pragma unroll
+          for (int a = 0; a < 16; ++a) acc[m][a] = 0.0f;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(q[m][ks]), as_bf16x8(k[ks]), acc[m], 0, 0, 0);
+          if (tile > 0) weigh(tile - 1);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
+            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);   // and what goes beside it
+          }
         }
+        weigh(3);
         // two sums at a time: the low lanes get the first one's, the high lanes the second's
-        auto put = [&](float y, float z, int t, int key) {
+        const int at_key = C::KT * j;
+        const bool inside = all_there && k0 + at_key + C::KT <= least_keys;  // (wave-uniform) every key is seen by every token
+        auto put = [&](float y, float z, int i, int off) {
           const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(z), false, false);
           float v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-          if (key >= keys_of(t) || (!all_there && key < kend && window[page_of(p, key) - pg0] < 0)) v = -INFINITY;
-          if (t < x.tb && key < k1) p.out[(int64_t)(t - p.first) * p.L + key] = v;
+          off += at_key;
+          if (!inside) {
+            keep_branch();
+            const int key = k0 + off;
+            if (key >= sees[i] || (!all_there && key < kend && window[page_of(p, key) - pg0] < 0)) v = -INFINITY;
+            if (key >= k1) return;
+          }
+          if (mine[i]) row[i][off] = v;
         };
-        const int key0 = k0 + C::KT * j;
         if constexpr (TPW == 1) {
-          put(part[0][0], part[1][0], my0, key0 + lane);
+          put(part[0][0], part[1][0], 0, lane);
         } else {
 #pragma unroll
           for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-            for (int tl = 0; tl < TPW; tl += 2) put(part[sub][tl], part[sub][tl + 1], my0 + tl + g32, key0 + 32 * sub + l32);
+            for (int i = 0; i < NP; ++i) put(part[sub][2 * i], part[sub][2 * i + 1], i, 32 * sub + l32);
         }
       }
     }
@@ -424,7 +458,7 @@ static int launch_scores(IndexScoreParams p, hipStream_t st) {
   p.span = (int)((int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys < (1 << 30) ? (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys
                                                                                             : 1 << 30);
   // blocks, at most: fewer than 2^31 of them, and workgroups that all run at once
-  const int tt = rows ? 1 : C::TT, fill = 4096 / tt;
+  const int tt = rows ? 1 : C::TT, fill = rows ? ScoreUnits<1>::FILL : ScoreUnits<C::TT>::FILL;
   const int64_t units = rows ? p.tokens : (int64_t)p.tokens / tt + (p.tokens < p.req.R ? p.tokens : p.req.R);
   const int64_t n = units * (((int64_t)p.L + kBlockKeys - 1) / kBlockKeys + ((int64_t)p.L + fill - 1) / fill);
   DSA_REQUIRE(n < (1ll << 31), "dsa_paged_index_scores: too many tokens for one call");
