@@ -15,6 +15,8 @@
 // A unit is a token (or tile of tokens) with its request's keys in blocks of 128, and behind them the columns that no token
 // of it sees, in blocks of -inf to write.  All units' blocks, one after the other, are split evenly over the workgroups
 // that the card holds, on the device, from the lengths: the host knows none of them.
+#include <type_traits>
+
 #include "index_keys.hpp"
 #include "wave_ops.hpp"
 
@@ -316,7 +318,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
     const ScorePiece x = next_piece<C::TT>(p, units, walk);
     fill_piece<C::TT>(p, x);
     if (x.b0 >= x.nb) continue;
-    const int my0 = x.ta + w * TPW;  // the wave's first token
+    // Tiles that half of the waves would have: the other half takes the second 32 keys of every 64.
+    const bool halves = x.tb - x.ta <= C::TT / 2;  // (uniform)
+    const int my0 = x.ta + (halves ? w & 1 : w) * TPW;  // the wave's first token
     const int at = __builtin_amdgcn_readfirstlane(p.req.start(x.r)), n = __builtin_amdgcn_readfirstlane(p.req.tokens(x.r));
     const int kv = __builtin_amdgcn_readfirstlane(p.req.kv(x.r));
     auto keys_of = [&](int t) { return max(kv - n + (t - at) + 1, 0); };
@@ -386,8 +390,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
         load(j + 1);  // (past the last: kNoKey)
         __syncthreads();  // tile j is whole; its buffer's readers of two tiles ago passed the barrier before
         if (!works) continue;
-        // Four tiles of 32 rows by 32 keys; a tile's ReLU and weights beside the next one's products, in one stream, since the
-        // SIMD overlaps the two within a wave far more than across waves.
+        // Tiles of 32 rows by 32 keys, two or four; a tile's ReLU and weights beside the next one's products, in one stream,
+        // since the SIMD overlaps the two within a wave far more than across waves.
         float part[2][TPW];
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
@@ -395,39 +399,43 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
           for (int tl = 0; tl < TPW; ++tl) part[sub][tl] = 0.0f;
         f32x16 acc[2];
         i32x4 k[KS];
-        auto weigh = [&](int tile) {  // tile: 2 sub + m
-          const int sub = tile >> 1, m = tile & 1;
+        auto weigh = [&](int sub, int m) {
 #pragma unroll
           for (int a = 0; a < 16; ++a) {
             const int tl = (32 * m + 8 * (a >> 2)) / H;
             part[sub][tl] = fmaf(__builtin_elementwise_maximum(acc[m][a], least), wv[m][a], part[sub][tl]);
           }
         };
+        auto tiles = [&](auto count, const unsigned char *keys) {  // of 32-key tiles from `keys` on
 #pragma unroll
-        for (int tile = 0; tile < 4; ++tile) {
-          if ((tile & 1) == 0)
+          for (int tile = 0; tile < decltype(count)::value; ++tile) {
+            const int m = tile & 1;
+            if (m == 0)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) k[ks] = *reinterpret_cast<const i32x4 *>(K[j & 1] + C::at(16 * tile + l32, 2 * ks + g32));
-          const int m = tile & 1;
+              for (int ks = 0; ks < KS; ++ks) k[ks] = *reinterpret_cast<const i32x4 *>(keys + C::at(16 * tile + l32, 2 * ks + g32));
 #pragma unroll
-          for (int a = 0; a < 16; ++a) acc[m][a] = 0.0f;
+            for (int a = 0; a < 16; ++a) acc[m][a] = 0.0f;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(q[m][ks]), as_bf16x8(k[ks]), acc[m], 0, 0, 0);
-          if (tile > 0) weigh(tile - 1);
+            for (int ks = 0; ks < KS; ++ks)
+              acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(q[m][ks]), as_bf16x8(k[ks]), acc[m], 0, 0, 0);
+            if (tile > 0) weigh((tile - 1) >> 1, (tile - 1) & 1);
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
-            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);   // and what goes beside it
+            for (int ks = 0; ks < KS; ++ks) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+              __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // and what goes beside it
+            }
           }
-        }
-        weigh(3);
+          weigh((decltype(count)::value - 1) >> 1, 1);
+        };
+        if (halves) tiles(std::integral_constant<int, 2>(), K[j & 1] + (w >> 1) * 32 * C::RB);
+        else tiles(std::integral_constant<int, 4>(), K[j & 1]);
         // two sums at a time: the low lanes get the first one's, the high lanes the second's
         const int at_key = C::KT * j;
         const bool inside = all_there && k0 + at_key + C::KT <= least_keys;  // (wave-uniform) every key is seen by every token
         auto put = [&](float y, float z, int i, int off) {
           const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(z), false, false);
           float v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+          if (TPW == 1 && off == C::KT) return;
           off += at_key;
           if (!inside) {
             keep_branch();
@@ -438,12 +446,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
           if (mine[i]) row[i][off] = v;
         };
         if constexpr (TPW == 1) {
-          put(part[0][0], part[1][0], 0, lane);
+          // (halves: both halves of the wave have the one sum's two parts, and the low lanes' result is stored)
+          if (!halves) put(part[0][0], part[1][0], 0, lane);
+          else put(part[0][0], part[0][0], 0, g32 == 0 ? 32 * (w >> 1) + l32 : C::KT);
         } else {
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
+          for (int sub = 0; sub < 2; ++sub) {
+            if (sub == 1 && halves) break;
 #pragma unroll
-            for (int i = 0; i < NP; ++i) put(part[sub][2 * i], part[sub][2 * i + 1], i, 32 * sub + l32);
+            for (int i = 0; i < NP; ++i) put(part[sub][2 * i], part[sub][2 * i + 1], i, 32 * (halves ? w >> 1 : sub) + l32);
+          }
         }
       }
     }
@@ -453,7 +465,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
 template <int H, int D, int FMT>
 static int launch_scores(IndexScoreParams p, hipStream_t st) {
   using C = IndexTile<H, D, FMT>;
-  // single tokens: a request has fewer than two on average
+  // Single tokens: a request has fewer than two on average.  Replays of 32 requests, 8192 .. 32768 MXFP8 keys, us, tiles of tokens
+  // and single ones: 2 tokens, 16 heads 45, 44; 64 heads 48, 46 (bf16 52, 63); 3 tokens 45, 57 and 57, 60; 4 tokens 46, 72 and 61, 77.
   const bool rows = p.req.query_starts == nullptr || p.req.R == 0 || p.req.T < 2 * (int64_t)p.req.R;
   p.span = (int)((int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys < (1 << 30) ? (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys
                                                                                             : 1 << 30);
