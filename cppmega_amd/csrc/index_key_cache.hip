@@ -73,14 +73,11 @@ __global__ void __launch_bounds__(256) index_key_append_kernel(const KeyCachePar
     }
     *reinterpret_cast<i32x2 *>(row + c * 8) = codes;
   } else {
-    uint32_t codes = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(x[e]);
-      // 0 0.5 1 1.5 2 3 4 6 are codes 0 .. 7: a tie goes to the even one
-      const uint32_t code = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-      codes |= (code | (__float_as_uint(x[e]) >> 31) << 3) << (4 * e);
-    }
+    uint32_t codes = 0;  // (the conversion rounds to nearest even and saturates)
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], 1.0f, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], 1.0f, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], 1.0f, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], 1.0f, 3);
     *reinterpret_cast<uint32_t *>(row + c * 4) = codes;
   }
   unsigned char *expo = page + (int64_t)p.block * Row::CODES + (int64_t)off * 4;

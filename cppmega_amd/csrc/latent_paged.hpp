@@ -90,6 +90,12 @@ struct PagedPiece {
   const int32_t *table;
   int token, req, seen;                   // sparse: the token, its request and the positions that it sees
 };
+// The workgroup's place among the ranges of blocks.  Sparse: neighbouring ranges, which may be a token's units and read the
+// same rows, on one XCD.
+template <bool SPARSE>
+__device__ __forceinline__ int range_of() {
+  return SPARSE ? (int)xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
+}
 // Piece at block `at` of unit u, for a range that ends at `end`; at moves past it.
 template <bool SPARSE = false>
 __device__ __forceinline__ PagedPiece next_piece(const PagedParams &p, int u, int &at, int end) {
@@ -98,7 +104,7 @@ __device__ __forceinline__ PagedPiece next_piece(const PagedParams &p, int u, in
   x.b0 = at - ub;
   x.b1 = (ue < end ? ue : end) - ub;
   x.whole = x.b0 == 0 && ub + x.b1 == ue;
-  x.slot = (int)blockIdx.x * 2 + (x.b0 == 0 ? 1 : 0);
+  x.slot = range_of<SPARSE>() * 2 + (x.b0 == 0 ? 1 : 0);
   at = ub + x.b1;
   if constexpr (SPARSE) {
     x.token = uni(u / p.token_units);

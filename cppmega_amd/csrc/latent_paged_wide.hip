@@ -7,7 +7,8 @@
 // Steps of 64 keys (two 32-key tiles), one ahead in LDS, one barrier a step:
 //   RG 8 (128 rows, bf16): all eight waves fetch and compute;
 //   RG 4, 2: four waves compute (RG row groups x KG = 4 / RG key groups), the other four
-//     bring the rows.
+//     bring the rows;
+//   RG 1 (sparse attention): two key groups by two halves of V's channels, both with all of S.
 // bf16 rows come by LDS-DMA loads; MXFP4 rows (a third of the bytes) by registers, two
 // more steps ahead, converted to exact bf16 values as they are written to LDS.  At a
 // piece's end the key groups' O are brought to one maximum and added pairwise through LDS.
@@ -31,20 +32,21 @@ struct PagedWide {
   using Row = CacheRow<576, 512, FP4>;
   static constexpr int RG = RG_, ROWS = 16 * RG;
   static constexpr bool ROLES = RG < 8;                      // waves 4..7 bring the rows
-  static constexpr int CW = ROLES ? 4 : 8, LW = ROLES ? 4 : 8, KG = CW / RG;  // computing, loading waves
+  static constexpr int DG = RG == 1 ? 2 : 1;                 // groups of V's channels
+  static constexpr int CW = ROLES ? 4 : 8, LW = ROLES ? 4 : 8, KG = CW / (RG * DG);  // computing, loading waves; key groups
   static constexpr int SUB = 2 / KG;                         // tiles of a computing wave
   static constexpr int PANELS = 9, TILE = PANELS * 4096, STEP = 2 * TILE;
   // operands read at once (3, 4: registers spill in the step; 2: none does there, MXFP4 with RG 2 spills 21 around a piece's
   // joining and the window's refill)
   static constexpr int GROUP = 2;
-  static constexpr int KS = 18, NDT = 32;
+  static constexpr int KS = 18, NDT = 32 / DG;               // 16-channel tiles of O in a wave
   static constexpr int TPR = 4, CPT = 16 / TPR, RPT = 8 / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
   static constexpr int OFF_T = 2 * STEP;
   static constexpr int WINDOW = SPARSE ? 2 * kWindow : kWindow;
   static constexpr int OFF_ML = OFF_T + WINDOW * 4;          // [2][16][2]
   static constexpr int BYTES = OFF_ML + 2 * 16 * 8;
-  static constexpr int O_BYTES = 512 * 16 * 4;
-  static_assert(BYTES <= 159 * 1024 && (KG == 1 || RG * O_BYTES <= OFF_T), "LDS");
+  static constexpr int O_BYTES = NDT * 16 * 16 * 4;
+  static_assert(BYTES <= 159 * 1024 && (KG == 1 || RG * DG * O_BYTES <= OFF_T), "LDS");
   static_assert(!FP4 || (ROLES && 64 * LW == kWideKeys * TPR), "MXFP4 rows: by the loading waves");
 };
 
@@ -55,7 +57,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
   constexpr int KEYS = kWideKeys, KS = C::KS, NDT = C::NDT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int w = wave_id();
-  const int rg = w % RG, kg = C::ROLES ? (w & 3) / RG : 0;
+  const int rg = w % RG, kg = C::ROLES ? (w & 3) / RG % C::KG : 0, dg = C::DG > 1 ? (w & 3) / (RG * C::KG) : 0;
   const bool computes = !C::ROLES || w < 4;  // wave-uniform
   const int lw = C::ROLES ? w - 4 : w;       // loading wave
   int *window = reinterpret_cast<int *>(smem + C::OFF_T);
@@ -70,8 +72,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
   int units, total;
   all_units<SPARSE>(p, units, total);
   const int per = uni(range_blocks(p, total));
-  if ((int64_t)blockIdx.x * per >= total) return;
-  int at = (int)blockIdx.x * per;
+  const int range = range_of<SPARSE>();
+  if ((int64_t)range * per >= total) return;
+  int at = range * per;
   const int end = per < total - at ? at + per : total;
   for (int u = uni(unit_of<SPARSE>(p, units, at)); at < end; ++u) {
     const PagedPiece x = next_piece<SPARSE>(p, u, at, end);
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             return *reinterpret_cast<const i32x4 *>(K + (ka[h][ks & 1] ^ panel_swz(ks >> 1)) + (ks >> 1) * 4096);
           };
           auto cols = [&](int dt) {
-            const unsigned char *b = K + (dt >> 2) * 4096;
+            const unsigned char *b = K + dg * (NDT / 4 * 4096) + (dt >> 2) * 4096;
             const i32x2 r0 = ds_read_tr16(b + (va[0][dt & 3] ^ panel_swz(dt >> 2)));
             const i32x2 r1 = ds_read_tr16(b + (va[1][dt & 3] ^ panel_swz(dt >> 2)));
             return i32x4{r0[0], r0[1], r1[0], r1[1]};
@@ -245,7 +248,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) va[h][u] = tile_byte(8 * g16 + 4 * h + (l16 >> 2), 2 * u + ((l16 & 3) >> 1)) + (l16 & 1) * 8;
+            for (int u = 0; u < 4; ++u)
+              va[h][u] = (tile_byte(8 * g16 + 4 * h + (l16 >> 2), 2 * u + ((l16 & 3) >> 1)) + (l16 & 1) * 8) ^ panel_swz(dg * (NDT / 4));
           load_group<NDT>(a0, 0, cols);
           __builtin_amdgcn_sched_barrier(0);
           if (!all_there || key0 + 32 > lim_min) {
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             __syncthreads();
             const int lane = lane_here(), g16 = lane >> 4, l16 = lane & 15;
             if (kg >= half && kg < 2 * half) {
-              const int slot = (kg - half) * RG + rg;
+              const int slot = ((kg - half) * RG + rg) * C::DG + dg;
               unsigned char *dst = smem + slot * C::O_BYTES;
 #pragma unroll
               for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4 *>(dst + (dt * 64 + lane) * 16) = o[dt];
@@ -337,7 +341,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             }
             __syncthreads();
             if (kg < half) {
-              const int slot = kg * RG + rg;
+              const int slot = (kg * RG + rg) * C::DG + dg;
               const unsigned char *src = smem + slot * C::O_BYTES;
               const float m2 = ML[(slot * 16 + l16) * 2], l2 = ML[(slot * 16 + l16) * 2 + 1];
               // (a group without a key of the row has l = 0 and O = 0; a NaN sum joins)
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             const bool none = row_keys(row) <= x.b0 * KEYS || l_run == 0.0f;  // no key of this piece
             const float inv = none ? 0.0f : 1.0f / l_run;
             const int64_t part = (int64_t)x.slot * C::ROWS + row;
-            if (g16 == 0) {
+            if (g16 == 0 && dg == 0) {
               if (x.whole) {
                 p.lse[x.row0 + row] = none ? -INFINITY : log2f(l_run) + m_run;
               } else {
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             }
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
-              const int col = 16 * dt + 4 * g16;
+              const int col = 16 * (dg * NDT + dt) + 4 * g16;
               if (x.whole) {
                 // a row without keys: 0, whatever its neighbours' keys left
                 *reinterpret_cast<i32x2 *>(p.out + (x.row0 + row) * 512 + col) =
@@ -437,13 +441,15 @@ static int launch(const PagedParams &p, hipStream_t st) {
 }
 
 int paged_wide_keys() { return kWideKeys; }
-template <bool SPARSE>
-static int launch_of(const PagedParams &p, int tiles16, bool fp4, hipStream_t st) {
-  if (fp4) return tiles16 == 2 ? launch<2, true, SPARSE>(p, st) : launch<4, true, SPARSE>(p, st);
-  return tiles16 == 4 ? launch<4, false, SPARSE>(p, st) : launch<8, false, SPARSE>(p, st);
-}
 int launch_paged_wide(const PagedParams &p, int tiles16, bool fp4, bool sparse, hipStream_t st) {
-  return sparse ? launch_of<true>(p, tiles16, fp4, st) : launch_of<false>(p, tiles16, fp4, st);
+  if (sparse) {
+    if (tiles16 == 1) return fp4 ? launch<1, true, true>(p, st) : launch<1, false, true>(p, st);
+    if (tiles16 == 2) return fp4 ? launch<2, true, true>(p, st) : launch<2, false, true>(p, st);
+    if (tiles16 == 4) return fp4 ? launch<4, true, true>(p, st) : launch<4, false, true>(p, st);
+    return launch<8, false, true>(p, st);
+  }
+  if (fp4) return tiles16 == 2 ? launch<2, true, false>(p, st) : launch<4, true, false>(p, st);
+  return tiles16 == 4 ? launch<4, false, false>(p, st) : launch<8, false, false>(p, st);
 }
 
 }  // namespace dsa

@@ -10,19 +10,33 @@
 
 namespace dsa {
 
-// How a call with 576 channels is run.
+// How a call with 576 channels is run: the rows of a unit.  A row that a unit reads serves all of its rows; fewer rows mean
+// more units, of which fewer are cut, and their neighbours' reads of the same rows meet in an XCD's L2.  Replays of T tokens
+// of as many requests (where marked *, of one), top-2048, us, fewer rows a unit and more:
+//   bf16, 128 heads   of 32 and 64: T = 8* 34, 41; 32* 47, 48; 48 64, 73; 56 67, 79; of 64 and 128: 64 70, 80; 96 117, 120;
+//                     192* 146, 155; 256* (no unit of 128 is cut) 174, 153; 400* 284, 275
+//         64 heads    of 32 and 64: T = 2* 25, 34; 32* 37, 43; 64* 47, 48; 96 81, 77; 128 96, 91; of 64 and 128: 64* 48, 61
+//         32 heads    of 32 and 64: T = 8* 27, 34; 64* 37, 44; 400* 112, 147
+//         16 heads    of 16 (their waves share keys and channels) and 64: T = 8* 23, 32; 64* 31, 41; 400* 97, 150
+//   MXFP4, 128 heads  of 32 and 64: T = 8* 36, 46; 32* 54, 53; 56 77, 83; 96* 115, 111; 256* 258, 213
+//         64 heads    of 32 and 64: T = 16* 36, 45; 64* 54, 53; 128* 73, 76; 256* 135, 111
+//         16 heads    of 16 and 32: T = 8* 26, 27; 96 49, 57; 400* 110, 122
 struct SparseWidePlan {
   int wide, unit_rows, token_units, unit_blocks, nwg, min_blocks;
 };
+static bool nearly_all(int64_t units) { return units >= 192 && units <= 256; }
 static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool fp4) {
   SparseWidePlan r{};
-  r.wide = fp4 ? (H <= 32 ? 2 : 4) : (H <= 64 ? 4 : 8);
+  if (H <= 16) r.wide = 1;
+  else if (H <= 32 || T * H <= 4096 || (H > 64 && nearly_all(T * ((H + 31) / 32)))) r.wide = 2;
+  else r.wide = fp4 || H <= 64 || T * ((H + 127) / 128) < 256 ? 4 : 8;
   r.unit_rows = 16 * r.wide;
   r.token_units = (int)((H + r.unit_rows - 1) / r.unit_rows);
   r.unit_blocks = (int)((topk + paged_wide_keys() - 1) / paged_wide_keys());
   r.min_blocks = 256 / paged_wide_keys();  // picks that are worth a piece's beginning and end
-  const int64_t n = (T * r.token_units * r.unit_blocks + r.min_blocks - 1) / r.min_blocks;
-  r.nwg = (int)(n < 256 ? n : 256);
+  const int64_t units = T * r.token_units, n = (units * r.unit_blocks + r.min_blocks - 1) / r.min_blocks;
+  // units that nearly fill the card are left whole (224 tokens, 64 heads, bf16: 152 us cut, 136 whole; 112, 128 heads: 131, 107)
+  r.nwg = (int)(n < 256 ? n : nearly_all(units) ? units : 256);
   return r;
 }
 

@@ -191,6 +191,12 @@ SPARSE = [
     (4, [3, 0, 50], [7, 2, 4], 16, 64),
     (64, [900, 400], [11, 6], 64, 512),
     (32, [5000], [1], 64, 2048),
+    (33, [700], [40], 16, 96),                  # two units of 32 rows a token
+    (128, [1500], [60], 16, 128),               # many tokens: units that nearly fill the card, none of them cut
+    (128, [700], [70], 16, 192),
+    (80, [600], [130], 16, 96),
+    (64, [600], [200], 16, 96),
+    (16, [900], [300], 16, 160),
 ]
 
 
