@@ -23,6 +23,7 @@ namespace dsa {
 //         16 heads    of 16 and 32: T = 8* 26, 27; 96 49, 57; 400* 110, 122
 struct SparseWidePlan {
   int wide, unit_rows, token_units, unit_blocks, nwg, min_blocks;
+  int64_t per;  // blocks of a workgroup
 };
 static bool nearly_all(int64_t units) { return units >= 192 && units <= 256; }
 static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool fp4) {
@@ -34,9 +35,21 @@ static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool 
   r.token_units = (int)((H + r.unit_rows - 1) / r.unit_rows);
   r.unit_blocks = (int)((topk + paged_wide_keys() - 1) / paged_wide_keys());
   r.min_blocks = 256 / paged_wide_keys();  // picks that are worth a piece's beginning and end
-  const int64_t units = T * r.token_units, n = (units * r.unit_blocks + r.min_blocks - 1) / r.min_blocks;
-  // units that nearly fill the card are left whole (224 tokens, 64 heads, bf16: 152 us cut, 136 whole; 112, 128 heads: 131, 107)
-  r.nwg = (int)(n < 256 ? n : nearly_all(units) ? units : 256);
+  // Workgroups: a whole number of equal pieces of a unit each, so that none has the end of one unit and the beginning of the
+  // next (112 tokens, 16 heads, bf16 64 us by even ranges of all blocks, 61 so; 96, 64 heads 77, 67; 224 units left whole 152,
+  // 136), or, where that leaves much of the card idle, even ranges.
+  const int64_t units = T * r.token_units;
+  if (units <= 128 || nearly_all(units)) {
+    const int most = 256 / (int)units, even = (r.unit_blocks + most - 1) / most, per = even > r.min_blocks ? even : r.min_blocks;
+    const int pieces = (r.unit_blocks + per - 1) / per;
+    r.per = per;
+    r.unit_blocks = pieces * per;  // (blocks past the last pick hold none)
+    r.nwg = (int)units * pieces;
+  } else {
+    r.nwg = 256;
+    const int64_t per = (units * r.unit_blocks + 255) / 256;
+    r.per = per > r.min_blocks ? per : r.min_blocks;
+  }
   return r;
 }
 
@@ -77,7 +90,8 @@ int launch_paged_sparse(PagedParams p, const int32_t *indices, int64_t topk, int
   p.part_ml = (float *)ws;
   p.part_o = p.part_ml + (size_t)k.nwg * 2 * (size_t)k.unit_rows * 2;
   const int rc = launch_paged_wide(p, k.wide, fp4, true, st);
-  return rc ? rc : launch_paged_combine(p, d_v, true, st);
+  if (rc || k.per % k.unit_blocks == 0) return rc;  // ranges of whole units: nothing to join
+  return launch_paged_combine(p, d_v, true, st);
 }
 
 }  // namespace dsa
