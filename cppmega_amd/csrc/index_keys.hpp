@@ -62,6 +62,7 @@ struct IndexScoreParams {
   int W, L, block, block_shift, num_blocks;
   int span;                    // keys whose pages lie in the window, whole blocks
   int w_f32, relu;
+  int whole_tiles;             // 64 keys from a multiple of 64 on lie on one page
 };
 int launch_index_scores(IndexScoreParams p, int64_t H, int64_t D, int fmt, hipStream_t st);
 
