@@ -164,7 +164,7 @@ extern "C" int dsa_index_key_append(void *cache, const void *k, int64_t k_stride
   const char *who = "dsa_index_key_append";
   const int rc = check_keys(who, num_blocks, block_size, D, dtype);
   if (rc) return rc;
-  DSA_REQUIRE(T >= 0 && T < (1ll << 31), "%s: T=%lld out of range", who, (long long)T);
+  DSA_REQUIRE(T >= 0 && T < (1ll << 28), "%s: T=%lld must be in [0, 2^28)", who, (long long)T);
   if (T == 0) return DSA_OK;
   DSA_REQUIRE(cache && k && slots && aligned16(cache) && aligned16(k), "%s: null or misaligned pointer", who);
   DSA_REQUIRE(k_stride >= 0 && k_stride % 8 == 0, "%s: the row stride must be a non-negative multiple of 8 elements", who);
@@ -182,7 +182,7 @@ extern "C" int dsa_index_key_gather(const void *cache, const int64_t *slots, voi
   const char *who = "dsa_index_key_gather";
   const int rc = check_keys(who, num_blocks, block_size, D, dtype);
   if (rc) return rc;
-  DSA_REQUIRE(T >= 0 && T < (1ll << 31), "%s: T=%lld out of range", who, (long long)T);
+  DSA_REQUIRE(T >= 0 && T < (1ll << 28), "%s: T=%lld must be in [0, 2^28)", who, (long long)T);
   if (T == 0) return DSA_OK;
   DSA_REQUIRE(cache && slots && out && aligned16(cache) && aligned16(out), "%s: null or misaligned pointer", who);
   KeyCacheParams p{};

@@ -178,6 +178,7 @@ int launch_paged_fwd(PagedParams p, int64_t d_qk, int64_t d_v, bool fp4, unsigne
 int launch_paged_combine(const PagedParams &p, int64_t d_v, bool sparse, hipStream_t st);
 
 // Attention over the cached rows that indices [T, topk] name by their positions in p.table's requests; p as for launch_paged_fwd.
+bool paged_sparse_countable(int64_t T, int64_t topk, int64_t H, int64_t d_qk);
 size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t d_v);
 int launch_paged_sparse(PagedParams p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4,
                         unsigned char *ws, hipStream_t st);

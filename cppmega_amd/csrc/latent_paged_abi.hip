@@ -131,10 +131,10 @@ extern "C" int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const 
 
 static int check_sparse(const char *who, int64_t T, int64_t H, int64_t topk, int64_t d_qk) {
   DSA_REQUIRE(T >= 0 && H > 0 && topk > 0, "%s: bad sizes T=%lld H=%lld topk=%lld", who, (long long)T, (long long)H, (long long)topk);
-  DSA_REQUIRE(H <= 4096 && T < (1ll << 30) && T * H < (1ll << 31) - 1024 && topk < (1ll << 31) - 1024,
-              "%s: sizes out of range (H <= 4096, T * H and topk below 2^31 - 1024)", who);
-  DSA_REQUIRE(T == 0 || paged_countable(T, T, topk, 1, H, d_qk), "%s: sizes out of range (row groups times blocks of picks must stay below 2^31)",
-              who);
+  DSA_REQUIRE(H <= 4096 && T < (1ll << 30) && T * H < (1ll << 31) - 1024 && topk <= (1ll << 27),
+              "%s: sizes out of range (H <= 4096, T * H below 2^31 - 1024, topk at most 2^27)", who);
+  DSA_REQUIRE(T == 0 || paged_sparse_countable(T, topk, H, d_qk),
+              "%s: sizes out of range (T times groups of 32 heads must stay below 2^26, for 576 channels times blocks of 64 picks below 2^31)", who);
   return DSA_OK;
 }
 

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(c
   constexpr int ELT = F32 ? 4 : 2;
   __shared__ float tmp[2][GL > 64 ? C::NW : 1];
   const int gl = (int)threadIdx.x % GL;
-  const int64_t row = (int64_t)blockIdx.x * C::RPW + (int)threadIdx.x / GL;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * C::RPW + (int)threadIdx.x / GL;
   const bool there = row < p.rows;  // (whole rows of lanes)
   float v[CH][8], sum = 0.0f;
 #pragma unroll
@@ -338,7 +338,8 @@ static int64_t norm_bwd_wgs(int64_t rows, int64_t n) {
 template <int GL, int CH>
 static void launch_fwd(bool f32, const NormParams &p, hipStream_t st) {
   using C = NormGroup<GL>;
-  const dim3 grid((unsigned)((p.rows + C::RPW - 1) / C::RPW)), block(C::NTHR);
+  const int64_t n = (p.rows + C::RPW - 1) / C::RPW, most = 1 << 20;  // (2^32 threads and more: not along one axis)
+  const dim3 grid((unsigned)(n < most ? n : most), (unsigned)((n + most - 1) / most)), block(C::NTHR);
   if (f32) hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, true>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((layer_norm_fwd_kernel<GL, CH, false>), grid, block, 0, st, p);
 }

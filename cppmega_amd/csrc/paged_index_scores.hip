@@ -24,6 +24,7 @@ namespace dsa {
 
 constexpr int kWindowPages = 2048;  // pages of a unit that a workgroup has in LDS
 constexpr int kBlockKeys = 128;
+constexpr int kMostSpan = 65536 - kBlockKeys;  // past a column, below 2^31 - 65536, it stays below 2^31
 
 // Keeps a wave-uniform branch a branch.
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
@@ -352,8 +353,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
       uint32_t expo[C::NL];
       auto load = [&](int j) {
         if (p.whole_tiles) {
-          // The tile lies on one page, its codes and its exponents in a row each: one address a wave (2048 tokens over 16384 MXFP8
-          // keys 254 -> 241 us).  Keys past kend are masked below, as are those of a page that is not there, for which page 0 stands.
+          // The tile lies on one page, its codes and its exponents in a row each: one address a wave (2048 tokens over 8192 MXFP8
+          // keys 254 -> 243 us).  Keys past kend are masked below, as are those of a page that is not there, for which page 0 stands.
           const int key = min(k0 + C::KT * j, kend - 1) & ~(C::KT - 1), pg = page_of(p, key), off = key - pg * p.block;
           const int e = max(__builtin_amdgcn_readfirstlane(window[pg - pg0]), 0);
           const unsigned char *page = p.cache + (int64_t)e * p.page_bytes;
@@ -489,8 +490,8 @@ static int launch_scores(IndexScoreParams p, hipStream_t st) {
   // and single ones: 2 tokens, 16 heads 45, 44; 64 heads 48, 46 (bf16 52, 63); 3 tokens 45, 57 and 57, 60; 4 tokens 46, 72 and 61, 77.
   const bool rows = p.req.query_starts == nullptr || p.req.R == 0 || p.req.T < 2 * (int64_t)p.req.R;
   p.whole_tiles = p.block % C::KT == 0;
-  p.span = (int)((int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys < (1 << 30) ? (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys
-                                                                                            : 1 << 30);
+  const int64_t span = (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys;
+  p.span = (int)(span < kMostSpan ? span : kMostSpan);
   // blocks, at most: fewer than 2^31 of them, and workgroups that all run at once
   const int tt = rows ? 1 : C::TT, fill = rows ? ScoreUnits<1>::FILL : ScoreUnits<C::TT>::FILL;
   const int64_t units = rows ? p.tokens : (int64_t)p.tokens / tt + (p.tokens < p.req.R ? p.tokens : p.req.R);

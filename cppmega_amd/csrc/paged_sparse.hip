@@ -53,6 +53,17 @@ static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool 
   return r;
 }
 
+// Workgroups and blocks can be numbered.
+bool paged_sparse_countable(int64_t T, int64_t topk, int64_t H, int64_t d_qk) {
+  if (T * ((H + 31) / 32) >= (1ll << 26)) return false;
+  bool ok = true;
+  for (int fp4 = 0; d_qk == 576 && fp4 < 2; ++fp4) {
+    const SparseWidePlan k = sparse_wide_plan(T, topk, H, fp4 != 0);
+    ok = ok && T * k.token_units * (int64_t)k.unit_blocks < (1ll << 31);
+  }
+  return ok;
+}
+
 size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, int64_t d_v) {
   if (d_qk == 128) return sparse_narrow_workspace(T, topk, H);
   size_t most = 0;  // of the two formats': the query does not know it

@@ -96,6 +96,26 @@ def test_shapes_strides_and_alignment(dev):
                ("y", "dx", "dweight", "dbias"))
 
 
+def test_rows_past_a_grid_and_past_four_gigabytes(dev):
+    """The last rows of a call with more than 2^32 threads, and of one whose rows lie past 2^32 bytes: those of a call on them alone."""
+    w, b = torch.tensor([1.0, 2.0, -0.5], device=dev), torch.tensor([0.0, 1.0, 0.25], device=dev)
+    x = torch.randn((1 << 29) + 77, 3, dtype=BF, device=dev)
+    y, mean, rstd = layer_norm(x, w, b, return_stats=True)
+    for part in (slice(0, 50), slice((1 << 29) - 40, None)):
+        assert torch.equal(y[part], layer_norm(x[part], w, b))
+    dx, _, _ = layer_norm_backward(y, x, w, mean, rstd, (True, False, False))
+    part = slice((1 << 29) - 40, None)
+    assert torch.equal(dx[part], layer_norm_backward(y[part], x[part], w, mean[part], rstd[part], (True, False, False))[0])
+    del x, y, mean, rstd, dx
+    x = torch.zeros((1 << 22) + 9, 1024, dtype=BF, device=dev)[:, 5:69]
+    x[-40:] = torch.randn(40, 64, device=dev).to(BF)
+    y, mean, rstd = layer_norm(x, return_stats=True)
+    assert (y[:-40] == 0).all() and torch.equal(y[-40:], layer_norm(x[-40:].contiguous()))
+    dw = layer_norm_backward(x, x, None, mean, rstd)[1]                # (rows of zeros add nothing)
+    ref = orc.layer_norm(x[-40:].cpu(), None, None, 1e-5, x[-40:].cpu(), BF, F32)
+    assert ((dw.double().cpu() - ref["dweight"]).abs() <= ref["e_dweight"]).all()
+
+
 def test_no_rows(dev):
     x = torch.zeros(0, 96, dtype=BF, device=dev)
     w, b = torch.ones(96, device=dev), torch.ones(96, device=dev)

@@ -141,6 +141,19 @@ def test_c_sparse():
     assert size(5, 16, 8, 192, 128) == size(5, 0, 8, 128, 64) == size(5, 16, 0, 128, 64) == 0
 
 
+def test_c_calls_too_large_for_their_numbering():
+    L = _lib.load()
+    keys = lambda T: L.dsa_index_key_append(P, P, 64, P, T, 2, 16, 64, DTYPE_BF16, None)  # noqa: E731
+    assert keys(1 << 28) == INVALID
+    size = L.dsa_paged_sparse_mla_workspace_size
+    assert size(5, 16, 1 << 27, 128, 64) > 0 and size(5, 16, 1 << 27, 576, 512) > 0
+    for D, V in ((128, 64), (576, 512)):
+        for T, H, topk in ((5, 16, (1 << 27) + 1), (1 << 26, 1, 8), (1 << 19, 4095, 8)):
+            assert size(T, H, topk, D, V) == 0
+            assert L.dsa_paged_sparse_mla_fwd(P, P, P, P, P, P, P, P, P, 1 << 60, T, 3, 4, H, topk, D, V, 2, 16, DTYPE_BF16, 0.1, None) == INVALID
+    assert size(1 << 20, 64, 1 << 18, 576, 512) == 0                # blocks of picks past 2^31
+
+
 def test_c_layer_norm():
     L = _lib.load()
     fwd = lambda **k: L.dsa_layer_norm_fwd(*({**dict(x=P, w=P, b=P, y=P, m=P, r=P, rows=4, n=64, xs=64, eps=1e-5, dt=DTYPE_BF16, wd=DTYPE_F32,  # noqa: E731
