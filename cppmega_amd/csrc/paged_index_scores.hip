@@ -14,7 +14,13 @@
 //
 // A unit is a token (or tile of tokens) with its request's keys in blocks of 128, and behind them the columns that no token
 // of it sees, in blocks of -inf to write.  All units' blocks, one after the other, are split evenly over the workgroups
-// that the card holds, on the device, from the lengths: the host knows none of them.
+// that the card holds, on the device, from the lengths: the host knows none of them (64 single tokens 99 -> 67 us, prompts 127 ->
+// 109).
+//
+// Single tokens are bound by the keys' bytes: 64 tokens over 301 .. 65536 MXFP8 keys, 64 heads of 128 channels, 65 us, 4.5 TB/s.
+// Several tokens are bound by the MFMAs and the ReLU and weights beside them, which the SIMD overlaps in part: 5 prompts of 33
+// .. 512 tokens on 1024 .. 16384 MXFP4 keys, 32 heads, 78 us, 740 TFLOP/s (MFMA busy 45 % of it, VALU 50 %); without the
+// weights' work it would be 69, without the conversion and the keys' loads 63.
 #include <type_traits>
 
 #include "index_keys.hpp"

@@ -6,6 +6,10 @@
 //   S^T[pick][head] = K Q^T, O^T[channel][head] += V^T P^T   on 32x32x16 MFMAs (lane = head)
 // Many tokens: a wave has a unit.  Fewer: the four waves of a workgroup share a unit's picks and are joined through LDS,
 // and workgroups may share them as well, whose fp32 sums sparse_narrow_combine_kernel adds in order.
+//
+// Bound by the chain of a block (LDS, S, softmax, P V) at three waves a SIMD, nothing saturated: 6 prompts of 40 .. 512 tokens,
+// 32 heads, top-256, MXFP4 21 us (VALU busy 40 %, MFMA 16 %, LDS 25 %); bf16 the same.  Rows two blocks ahead 27, four waves a
+// SIMD (registers spill) 44, S in two accumulators 26, operands read in groups 28.  One token of 777 keys: 6.4.
 #include "latent_mla.hpp"
 #include "latent_paged.hpp"
 #include "paged_sparse.hpp"
