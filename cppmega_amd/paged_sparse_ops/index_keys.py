@@ -157,7 +157,8 @@ def paged_indexer_topk(q, weights, cache, block_table, kv_lens, topk, query_star
     ``paged_index_scores``: equal scores prefer the lower position, NaN ranks as +inf): what ``paged_sparse_mla_fwd``
     takes.  The scores go through a scratch of at most ``max_scratch_bytes`` (one token's at least), tokens in chunks.
     A token with fewer than topk keys gets all of them (those on no page too, which the attention masks), a token of
-    no request -1 alone.
+    no request -1 alone.  num_keys, and topk with it, have ``topk_indices``' limits: a caller with room for more in
+    its block_table passes the longest request's length.
     """
     T, H, R, W, L = _check_scores(q, weights, cache, block_table, kv_lens, query_starts, num_keys)
     assert topk > 0, f"topk must be positive, got {topk}"
