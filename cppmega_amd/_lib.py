@@ -205,7 +205,7 @@ _SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
-_checked_devices: set[int] = set()
+checked_devices: set[int] = set()
 
 
 class DSAError(RuntimeError):
@@ -249,9 +249,9 @@ def ensure_device(t: torch.Tensor) -> int:
             f"cppmega_amd kernels need tensors on a gfx950 GPU (got device {t.device}); "
             "there is no CPU path")
     dev = t.device.index if t.device.index is not None else torch.cuda.current_device()
-    if dev not in _checked_devices:
+    if dev not in checked_devices:
         check(load().dsa_device_check(dev), "dsa_device_check")
-        _checked_devices.add(dev)
+        checked_devices.add(dev)
     return dev
 
 

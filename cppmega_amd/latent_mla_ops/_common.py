@@ -28,6 +28,8 @@ def dense(t: torch.Tensor) -> torch.Tensor:
 def launch_on(t: torch.Tensor):
     """(stream pointer, context) for a launch on ``t``'s device: the context makes that device current
     where another one is, as a launch on a stream of its own needs."""
-    dev = _lib.ensure_device(t)
-    here = _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    dev = t.get_device()
+    if dev not in _lib.checked_devices:  # (-1 for one that is on no GPU)
+        dev = _lib.ensure_device(t)
+    here = _HERE if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
     return torch._C._cuda_getCurrentRawStream(dev), here  # (a Stream object of it would take a microsecond)

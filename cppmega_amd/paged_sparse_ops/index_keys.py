@@ -89,7 +89,7 @@ def index_key_gather(cache, slots):
     same_device(cache.data, slots)
     stream, here = launch_on(cache.data)
     with here:
-        out = torch.empty((T, cache.d), dtype=torch.bfloat16, device=slots.device)
+        out = slots.new_empty((T, cache.d), dtype=torch.bfloat16)
         rc = _lib.load().dsa_index_key_gather(cache.data.data_ptr(), slots.data_ptr(), out.data_ptr(), T, cache.num_blocks,
                                               cache.block_size, cache.d, cache.dtype_code, stream)
     _lib.check(rc, "dsa_index_key_gather")
@@ -106,7 +106,7 @@ def check_requests(T, block_table, kv_lens, query_starts):
     if query_starts is None:
         assert T == R, f"without query_starts every request has one token: {T} tokens, {R} requests"
     else:
-        assert tuple(query_starts.shape) == (R + 1,), f"query_starts must be [{R + 1}], got {tuple(query_starts.shape)}"
+        assert query_starts.shape == (R + 1,), f"query_starts must be [{R + 1}], got {tuple(query_starts.shape)}"
     return R, block_table.shape[1]
 
 
@@ -140,8 +140,8 @@ def paged_index_scores(q, weights, cache, block_table, kv_lens, query_starts=Non
     stream, here = launch_on(q)
     with here:
         if out is None:
-            out = torch.empty((T, L), dtype=torch.float32, device=q.device)
-        assert tuple(out.shape) == (T, L) and out.dtype == torch.float32 and out.is_contiguous(), \
+            out = q.new_empty((T, L), dtype=torch.float32)
+        assert out.shape == (T, L) and out.dtype == torch.float32 and out.is_contiguous(), \
             f"out must be contiguous float32 [{T}, {L}], got {out.dtype} {tuple(out.shape)}"
         rc = _lib.load().dsa_paged_index_scores(
             q.data_ptr(), weights.data_ptr(), cache.data.data_ptr(), block_table.data_ptr(), _lib.ptr(query_starts),

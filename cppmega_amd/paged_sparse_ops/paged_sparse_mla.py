@@ -36,16 +36,16 @@ def paged_sparse_mla_fwd(q, cache, indices, block_table, kv_lens, query_starts=N
     L = _lib.load()
     with here:
         if out is None:
-            out = torch.empty((T, H, cache.d_v), dtype=torch.bfloat16, device=q.device)
+            out = q.new_empty((T, H, cache.d_v))
         if lse is None:
-            lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
-        assert tuple(out.shape) == (T, H, cache.d_v) and tuple(lse.shape) == (T, H) and lse.dtype == torch.float32
+            lse = q.new_empty((T, H), dtype=torch.float32)
+        assert out.shape == (T, H, cache.d_v) and lse.shape == (T, H) and lse.dtype == torch.float32
         _check_bf16(out=out)
         _check_dense(out=out, lse=lse)
         n = int(L.dsa_paged_sparse_mla_workspace_size(T, H, topk, D, cache.d_v))
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty((n,), dtype=torch.uint8) if n else None
         rc = L.dsa_paged_sparse_mla_fwd(q.data_ptr(), cache.data.data_ptr(), indices.data_ptr(), block_table.data_ptr(),
-                                        _lib.ptr(query_starts), kv_lens.data_ptr(), out.data_ptr(), lse.data_ptr(), ws.data_ptr(),
+                                        _lib.ptr(query_starts), kv_lens.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(ws),
                                         n, T, R, W, H, topk, D, cache.d_v, cache.num_blocks, cache.block_size, cache.dtype_code,
                                         scale, stream)
     _lib.check(rc, "dsa_paged_sparse_mla_fwd")
