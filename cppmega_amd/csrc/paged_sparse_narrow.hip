@@ -9,7 +9,9 @@
 //
 // Bound by the chain of a block (LDS, S, softmax, P V) at three waves a SIMD, nothing saturated: 6 prompts of 40 .. 512 tokens,
 // 32 heads, top-256, MXFP4 21 us (VALU busy 40 %, MFMA 16 %, LDS 25 %); bf16 the same.  Rows two blocks ahead 27, four waves a
-// SIMD (registers spill) 44, S in two accumulators 26, operands read in groups 28.  One token of 777 keys: 6.4.
+// SIMD (registers spill) 44, S in two accumulators 26, operands read in groups 28.  With a long top-k the rows' way through the
+// L2s bounds it: 1537 tokens, 32 heads, top-1000 49 us, 8 TB/s (a row of MXFP4 is two or three of their lines, as one of bf16 is
+// two); up to 16 heads on 16x16x32 MFMAs at four waves a SIMD took 43 us against 46 here.  One token of 777 keys: 6.4.
 #include "latent_mla.hpp"
 #include "latent_paged.hpp"
 #include "paged_sparse.hpp"
