@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             }
             if (x.whole && !FP4) {
               // Two channel tiles at a time, neighbouring lane groups' halves swapped, so that a lane has eight channels of one: 1537
-              // tokens, 128 heads, top-64 151 -> 141 us, 32 heads 90 -> 83 (MXFP4: 180 -> 165, but 70 -> 73 and 102 -> 105 with 2048).
+              // tokens, 128 heads, top-64 151 -> 139 us, 32 heads 90 -> 84 (MXFP4: 180 -> 165, but 70 -> 73 and 102 -> 105 with 2048).
               unsigned char *dst = reinterpret_cast<unsigned char *>(p.out + (x.row0 + row) * 512 + 16 * dg * NDT + 16 * (g16 & 1) + 8 * (g16 >> 1));
 #pragma unroll
               for (int dt = 0; dt < NDT; dt += 2) {
