@@ -56,12 +56,13 @@ struct IndexScoreParams {
   const int32_t *table;        // [R, W]
   Requests req;
   float *out;                  // [tokens, L] scores of tokens first ..
-  int32_t *limits;             // [tokens] columns that a token sees (0: a token of no request), or null
+  int32_t *limits;             // [tokens] columns that a token sees (0: a token of no request); null: every column is written
   int64_t page_bytes;
   int first, tokens;           // tokens of the batch that are scored
   int W, L, block, block_shift, num_blocks;
   int span;                    // keys whose pages lie in the window, whole blocks
   int w_f32, relu;
+  int fill;                    // columns that no token of a request sees are written
   int whole_tiles;             // 64 keys from a multiple of 64 on lie on one page
 };
 int launch_index_scores(IndexScoreParams p, int64_t H, int64_t D, int fmt, hipStream_t st);

@@ -107,7 +107,7 @@ struct ScoreUnits {
     u.n = max(tb - u.ta, 0);
     const int keys = min(p.req.kv(r), p.L);
     u.nb = (keys + kBlockKeys - 1) / kBlockKeys;
-    u.fb = max(p.L - u.nb * kBlockKeys + FILL - 1, 0) / FILL;
+    u.fb = p.fill ? max(p.L - u.nb * kBlockKeys + FILL - 1, 0) / FILL : 0;
     return u;
   }
   static __device__ __forceinline__ uint32_t blocks(const IndexScoreParams &p, int r) {
@@ -496,6 +496,10 @@ static int launch_scores(IndexScoreParams p, hipStream_t st) {
   // and single ones: 2 tokens, 16 heads 45, 44; 64 heads 48, 46 (bf16 52, 63); 3 tokens 45, 57 and 57, 60; 4 tokens 46, 72 and 61, 77.
   const bool rows = p.req.query_starts == nullptr || p.req.R == 0 || p.req.T < 2 * (int64_t)p.req.R;
   p.whole_tiles = p.block % C::KT == 0;
+  // With limits nobody needs the columns that no token sees.  A top-k that reads whole rows finds those of a small call in the caches
+  // all the same where they were written: 64 tokens of up to 8192 keys in 32768 columns, top-2048, us, written and not 39, 43; of
+  // 65536 keys in 65536, top-256 97, 97, in 131072 101, 95; 1361 tokens of 16384 keys in 32768, top-2048 124, 113.
+  p.fill = p.limits == nullptr || (int64_t)p.tokens * p.L <= (4 << 20);
   const int64_t span = (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys;
   p.span = (int)(span < kMostSpan ? span : kMostSpan);
   // blocks, at most: fewer than 2^31 of them, and workgroups that all run at once

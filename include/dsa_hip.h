@@ -753,7 +753,8 @@ int dsa_index_key_gather(const void *cache, const int64_t *slots, void *out, int
  * and kv_lens as in dsa_paged_latent_mla_fwd.  A NaN or Inf of a key, a query or a weight
  * reaches the scores of that key, token and no other.  Rows of tokens of no request are not
  * written.  limits [tokens] int32 (or NULL): the columns that each token sees, 0 for a token
- * of no request: with 0 as the starts, the windows of a top-k over the scores.
+ * of no request: with 0 as the starts, the windows of a top-k over the scores.  With limits,
+ * columns at and past a token's limit may be left as they were: the windows leave them out.
  */
 int dsa_paged_index_scores(const void *q, const void *w, const void *cache, const int32_t *block_table,
                            const int32_t *query_starts, const int32_t *kv_lens, float *scores, int32_t *limits,

@@ -5,6 +5,7 @@ import torch
 
 from cppmega_amd import latent_mla_ops as lat
 from cppmega_amd import paged_sparse_ops as ops
+from cppmega_amd import topk_indices
 from oracle import index_keys as orc
 from tests.test_gpu_latent_paged import DIMS, _cache_rows, _check, _normal, _paged_case
 from tests.test_gpu_paged_sparse import FMTS, INF, _compare, _lims, _picks, _score_case
@@ -81,6 +82,25 @@ def test_missing_pages_of_64_keys(dev, news):
     ref, tol, _ = orc.scores(q, w, orc.unpack_pages(cache.data.cpu(), 128), table, starts, kv, 64, 512)
     assert (ref[0, 128:192] == -INF).all() and not ref.isnan().any()
     _compare(ops.paged_index_scores(q.to(dev), w.to(dev), cache, table.to(dev), kv.to(dev), starts.to(dev), num_keys=512), ref, tol)
+
+
+@pytest.mark.parametrize("lens,news", [([700, 20, 0, 512] * 5, [1] * 20), ([700, 20, 30, 512], [30, 2, 0, 11])])
+def test_topk_over_a_scratch_that_held_anything(dev, lens, news):
+    """Columns that no token sees are not written for the top-k, and not read."""
+    args, starts, L, (_, _, limits) = _scores(dev, "mxfp8", 16, 64, lens, news, 64, L=4096 * 64)
+    q, w, cache, table, kv = args
+    table = torch.cat([table, torch.full((len(lens), 4096 - table.shape[1]), -1, dtype=I32, device=dev)], 1)
+    T = len(q)
+    s = ops.paged_index_scores(q, w, cache, table, kv, starts, num_keys=1024)
+    want = topk_indices(s, 40, causal=False, starts=torch.zeros(T, dtype=I32, device=dev), ends=limits.to(dev))
+    for value in (float("nan"), INF):
+        for num_keys in (None, 1024, 40_000):
+            n = T * (num_keys or L)
+            held = torch.full((n,), value, device=dev)
+            del held                                                   # its memory is the scratch's
+            assert torch.equal(ops.paged_indexer_topk(q, w, cache, table, kv, 40, starts, num_keys=num_keys), want)
+    assert torch.equal(ops.paged_indexer_topk(q, w, cache, table, kv, 300, starts, num_keys=128) >= 0,
+                       torch.arange(300, device=dev)[None] < limits.clamp(max=128).to(dev)[:, None])   # more picks than columns
 
 
 def test_nothing_to_score(dev):
