@@ -195,7 +195,7 @@ extern "C" int dsa_index_key_gather(const void *cache, const int64_t *slots, voi
 }
 
 extern "C" int dsa_paged_index_scores(const void *q, const void *w, const void *cache, const int32_t *block_table,
-                                      const int32_t *query_starts, const int32_t *kv_lens, float *scores, int32_t *limits, int64_t T,
+                                      const int32_t *query_starts, const int32_t *kv_lens, float *scores, int32_t *windows, int64_t T,
                                       int64_t R, int64_t W, int64_t first, int64_t tokens, int64_t L, int64_t H, int64_t D,
                                       int64_t num_blocks, int64_t block_size, int dtype, int w_dtype, int use_relu, void *stream) {
   const char *who = "dsa_paged_index_scores";
@@ -211,7 +211,7 @@ extern "C" int dsa_paged_index_scores(const void *q, const void *w, const void *
     return set_error(DSA_ERR_UNSUPPORTED, "%s: no kernel for %lld index heads (16, 32, 64)", who, (long long)H);
   DSA_REQUIRE(query_starts != nullptr || T == R, "%s: without query_starts every request has one token: %lld tokens, %lld requests", who,
               (long long)T, (long long)R);
-  if (tokens == 0 || (L == 0 && limits == nullptr)) return DSA_OK;
+  if (tokens == 0 || (L == 0 && windows == nullptr)) return DSA_OK;
   DSA_REQUIRE(q && w && cache && (L == 0 || scores) && (R == 0 || (block_table && kv_lens)) && aligned16(q) && aligned16(cache),
               "%s: null or misaligned pointer", who);
   IndexScoreParams p{};
@@ -221,7 +221,7 @@ extern "C" int dsa_paged_index_scores(const void *q, const void *w, const void *
   p.table = block_table;
   p.req = Requests{query_starts, kv_lens, W * block_size, (int)T, (int)R};
   p.out = scores;
-  p.limits = limits;
+  p.windows = windows;
   p.first = (int)first;
   p.tokens = (int)tokens;
   p.W = (int)W;

@@ -56,7 +56,7 @@ struct IndexScoreParams {
   const int32_t *table;        // [R, W]
   Requests req;
   float *out;                  // [tokens, L] scores of tokens first ..
-  int32_t *limits;             // [tokens] columns that a token sees (0: a token of no request); null: every column is written
+  int32_t *windows;            // [2, tokens] 0 and the columns that a token sees (0: of no request); null: every column is written
   int64_t page_bytes;
   int first, tokens;           // tokens of the batch that are scored
   int W, L, block, block_shift, num_blocks;

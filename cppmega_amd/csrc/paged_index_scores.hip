@@ -197,10 +197,12 @@ __device__ __forceinline__ void fill_piece(const IndexScoreParams &p, const Scor
   const int64_t to = (int64_t)keys + (int64_t)(x.b1 - x.nb) * FILL;
   for (int t = x.ta; t < x.tb; ++t) fill_none(p.out + (int64_t)(t - p.first) * p.L, from, to < p.L ? (int)to : p.L);
 }
-__device__ __forceinline__ void write_limits(const IndexScoreParams &p) {
-  if (p.limits == nullptr) return;
-  for (int i = (int)blockIdx.x * 256 + (int)threadIdx.x; i < p.tokens; i += (int)gridDim.x * 256)
-    p.limits[i] = p.req.R > 0 ? min(max(p.req.keys_of(p.first + i, p.req.of_lane(p.first + i)), 0), p.L) : 0;
+__device__ __forceinline__ void write_windows(const IndexScoreParams &p) {
+  if (p.windows == nullptr) return;
+  for (int i = (int)blockIdx.x * 256 + (int)threadIdx.x; i < p.tokens; i += (int)gridDim.x * 256) {
+    p.windows[i] = 0;
+    p.windows[p.tokens + i] = p.req.R > 0 ? min(max(p.req.keys_of(p.first + i, p.req.of_lane(p.first + i)), 0), p.L) : 0;
+  }
 }
 
 template <int H, int D, int FMT>
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
   __shared__ ScoreLds units;
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const float least = p.relu ? 0.0f : -INFINITY;
-  write_limits(p);
+  write_windows(p);
   ScoreWalk walk = start_walk<1>(p, units);
   while (walk.at < walk.end) {
     const ScorePiece x = next_piece<1>(p, units, walk);
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
   __shared__ ScoreLds units;
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const float least = p.relu ? 0.0f : -INFINITY;
-  write_limits(p);
+  write_windows(p);
   ScoreWalk walk = start_walk<C::TT>(p, units);
   while (walk.at < walk.end) {
     const ScorePiece x = next_piece<C::TT>(p, units, walk);
@@ -496,10 +498,10 @@ static int launch_scores(IndexScoreParams p, hipStream_t st) {
   // and single ones: 2 tokens, 16 heads 45, 44; 64 heads 48, 46 (bf16 52, 63); 3 tokens 45, 57 and 57, 60; 4 tokens 46, 72 and 61, 77.
   const bool rows = p.req.query_starts == nullptr || p.req.R == 0 || p.req.T < 2 * (int64_t)p.req.R;
   p.whole_tiles = p.block % C::KT == 0;
-  // With limits nobody needs the columns that no token sees.  A top-k that reads whole rows finds those of a small call in the caches
+  // With windows nobody needs the columns that no token sees.  A top-k that reads whole rows finds those of a small call in the caches
   // all the same where they were written: 64 tokens of up to 8192 keys in 32768 columns, top-2048, us, written and not 39, 43; of
   // 65536 keys in 65536, top-256 97, 97, in 131072 101, 95; 1361 tokens of 16384 keys in 32768, top-2048 124, 113.
-  p.fill = p.limits == nullptr || (int64_t)p.tokens * p.L <= (4 << 20);
+  p.fill = p.windows == nullptr || (int64_t)p.tokens * p.L <= (4 << 20);
   const int64_t span = (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys;
   p.span = (int)(span < kMostSpan ? span : kMostSpan);
   // blocks, at most: fewer than 2^31 of them, and workgroups that all run at once

@@ -169,16 +169,16 @@ def paged_indexer_topk(q, weights, cache, block_table, kv_lens, topk, query_star
         if T == 0 or L == 0:
             return torch.full((T, topk), -1, dtype=torch.int32, device=q.device)
         step = max(1, min(T, max_scratch_bytes // (4 * L)))
-        scores = torch.empty((step, L), dtype=torch.float32, device=q.device)
-        starts, ends = torch.zeros(step, dtype=torch.int32, device=q.device), torch.empty(step, dtype=torch.int32, device=q.device)
+        scores = q.new_empty((step, L), dtype=torch.float32)
         parts = []
         for first in range(0, T, step):
             n = min(step, T - first)
+            windows = q.new_empty((2, n), dtype=torch.int32)
             rc = lib.dsa_paged_index_scores(
                 q.data_ptr(), weights.data_ptr(), cache.data.data_ptr(), block_table.data_ptr(), _lib.ptr(query_starts),
-                kv_lens.data_ptr(), scores.data_ptr(), ends.data_ptr(), T, R, W, first, n, L, H, cache.d, cache.num_blocks,
+                kv_lens.data_ptr(), scores.data_ptr(), windows.data_ptr(), T, R, W, first, n, L, H, cache.d, cache.num_blocks,
                 cache.block_size, cache.dtype_code, _lib.DTYPE_F32 if weights.dtype == torch.float32 else _lib.DTYPE_BF16,
                 1 if use_relu else 0, stream)
             _lib.check(rc, "dsa_paged_index_scores")
-            parts.append(topk_indices(scores[:n], topk, causal=False, starts=starts[:n], ends=ends[:n]))
+            parts.append(topk_indices(scores[:n], topk, causal=False, starts=windows[0], ends=windows[1]))
         return parts[0] if len(parts) == 1 else torch.cat(parts)

@@ -752,12 +752,12 @@ int dsa_index_key_gather(const void *cache, const int64_t *slots, void *out, int
  * [T, H] bf16 or f32 (w_dtype), H in {16, 32, 64}; requests, block_table [R, W], query_starts
  * and kv_lens as in dsa_paged_latent_mla_fwd.  A NaN or Inf of a key, a query or a weight
  * reaches the scores of that key, token and no other.  Rows of tokens of no request are not
- * written.  limits [tokens] int32 (or NULL): the columns that each token sees, 0 for a token
- * of no request: with 0 as the starts, the windows of a top-k over the scores.  With limits,
- * columns at and past a token's limit may be left as they were: the windows leave them out.
+ * written.  windows [2, tokens] int32 (or NULL): the starts and ends of a top-k over the scores,
+ * 0 and the columns that each token sees (0 for a token of no request).  With windows, columns
+ * past a token's own may be left as they were.
  */
 int dsa_paged_index_scores(const void *q, const void *w, const void *cache, const int32_t *block_table,
-                           const int32_t *query_starts, const int32_t *kv_lens, float *scores, int32_t *limits,
+                           const int32_t *query_starts, const int32_t *kv_lens, float *scores, int32_t *windows,
                            int64_t T, int64_t R, int64_t W, int64_t first, int64_t tokens, int64_t L, int64_t H,
                            int64_t D, int64_t num_blocks, int64_t block_size, int dtype, int w_dtype, int use_relu,
                            void *stream);
