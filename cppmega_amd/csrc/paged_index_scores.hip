@@ -6,11 +6,11 @@
 // matrix instructions that take 8-bit codes keep fewer bits of their sums than 32 (a score was off by 1.5e-5 of the scores'
 // size; this way 1e-7), and every key that is read serves 16 products at least.
 //
-// Two kernels.  Single tokens (index_rows_kernel): a workgroup's waves take the 32-key tiles of a token in turn, straight from
-// memory to operand registers (a lane's 16-byte piece of a key is two steps' operands in MXFP8 and four in MXFP4: the order
-// of the channels in a product is free), two tiles ahead, without a barrier.  Several tokens of a request
-// (index_tiles_kernel): four waves with the (token, head) rows of 4 * 64 / H tokens share tiles of 64 keys in LDS, widened
-// as they enter it.
+// Two kernels.  Single tokens, or the few of a request that fill 64 (token, head) rows (index_rows_kernel): a workgroup's waves
+// take the 32-key tiles of a unit in turn, straight from memory to operand registers (a lane's 16-byte piece of a key is two
+// steps' operands in MXFP8 and four in MXFP4: the order of the channels in a product is free), two tiles ahead, without a
+// barrier.  Several tokens of a request (index_tiles_kernel): four waves with the (token, head) rows of 4 * 64 / H tokens share
+// tiles of 64 keys in LDS, widened as they enter it.
 //
 // A unit is a token (or tile of tokens) with its request's keys in blocks of 128, and behind them the columns that no token
 // of it sees, in blocks of -inf to write.  All units' blocks, one after the other, are split evenly over the workgroups
@@ -205,26 +205,38 @@ __device__ __forceinline__ void write_windows(const IndexScoreParams &p) {
   }
 }
 
-template <int H, int D, int FMT>
+// NT tokens of a request at a time: one, or the 64 / H that fill two row tiles.
+template <int H, int D, int FMT, int NT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) index_rows_kernel(const IndexScoreParams p) {
   using Row = KeyRow<D, FMT>;
-  constexpr int MT = H > 32 ? H / 32 : 1, ROWS = H < 32 ? H / 2 : 16;  // row tiles; their accumulators with a head in them
-  constexpr int NC = Row::CODES / 32, U = Row::CPE / 8;               // pieces of a key in a lane; their steps
+  constexpr int RT = NT * H;                                              // rows
+  constexpr int MT = RT > 32 ? RT / 32 : 1, ROWS = RT < 32 ? RT / 2 : 16;  // row tiles; their accumulators with a head in them
+  constexpr int NC = Row::CODES / 32, U = Row::CPE / 8;                   // pieces of a key in a lane; their steps
   __shared__ int window[kWindowPages];
   __shared__ ScoreLds units;
   const int lane = lane_id(), w = wave_id(), g32 = lane >> 5, l32 = lane & 31;
   const float least = p.relu ? 0.0f : -INFINITY;
   write_windows(p);
-  ScoreWalk walk = start_walk<1>(p, units);
+  ScoreWalk walk = start_walk<NT>(p, units);
   while (walk.at < walk.end) {
-    const ScorePiece x = next_piece<1>(p, units, walk);
-    fill_piece<1>(p, x);
+    const ScorePiece x = next_piece<NT>(p, units, walk);
+    fill_piece<NT>(p, x);
     if (x.b0 >= x.nb) continue;
-    const int t = x.ta, lim = min(__builtin_amdgcn_readfirstlane(p.req.keys_of(t, x.r)), p.L);
-    const int kb1 = min(min(x.b1, x.nb) * kBlockKeys, p.L);
-    float *out = p.out + (int64_t)(t - p.first) * p.L;
+    const int t = x.ta, kb1 = min(min(x.b1, x.nb) * kBlockKeys, p.L);
+    const int most = __builtin_amdgcn_readfirstlane(p.req.keys_of(x.tb - 1, x.r));  // keys that the last token sees
+    // the rows that the lane writes: of tokens 2 i + g32 (one token: its)
+    constexpr int NP = NT > 1 ? NT / 2 : 1;
+    float *out[NP];
+    int sees[NP];  // (of a token that is not there: -1)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int tl = t + (NT > 1 ? 2 * i + g32 : 0);
+      sees[i] = tl < x.tb ? max(most - (x.tb - 1 - tl), 0) : -1;
+      out[i] = p.out + (int64_t)(tl - p.first) * p.L;
+    }
 
     // operand of step (c, u): channels CPE (2 c + g32) + 8 u ..
+    const int rows = (x.tb - t) * H;
     i32x4 q[MT][NC * U];
     float wv[MT][ROWS];
 #pragma unroll
@@ -234,16 +246,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          q[m][c * U + u] = h < H ? ld_global_16(p.q + (((int64_t)t * H + h) * D + Row::CPE * (2 * c + g32) + 8 * u) * 2) : i32x4{0, 0, 0, 0};
+          q[m][c * U + u] = h < rows ? ld_global_16(p.q + (((int64_t)t * H + h) * D + Row::CPE * (2 * c + g32) + 8 * u) * 2) : i32x4{0, 0, 0, 0};
     }
-    const float wl = lane < H ? weight_at(p, (int64_t)t * H + lane) : 0.0f;
+    const float wl = lane < rows ? weight_at(p, (int64_t)t * H + lane) : 0.0f;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int a = 0; a < ROWS; ++a) wv[m][a] = __shfl(wl, 32 * m + score_row(a, g32), 64);
 
     for (int k0 = x.b0 * kBlockKeys; k0 < kb1; k0 += p.span) {
-      const int k1 = min(k0 + p.span, kb1), kend = min(k1, lim);  // columns; keys that the token sees
+      const int k1 = min(k0 + p.span, kb1), kend = min(k1, most);  // columns; keys that a token sees
       __syncthreads();  // the window's readers are done
       if (kend > k0) fill_window<256>(p, window, x.r, k0, kend);
       const int pg0 = page_of(p, k0);
@@ -277,14 +289,29 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
               acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(q[m][c * U + u]), as_bf16x8(k), acc[m], 0, 0, 0);
           }
         }
-        float part = 0.0f;
+        float part[NT];
+#pragma unroll
+        for (int tl = 0; tl < NT; ++tl) part[tl] = 0.0f;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int a = 0; a < ROWS; ++a) part = fmaf(__builtin_elementwise_maximum(acc[m][a], least), wv[m][a], part);
-        part = sum_halves(part);
+          for (int a = 0; a < ROWS; ++a) {
+            const int tl = (32 * m + 8 * (a >> 2)) / H;
+            part[tl] = fmaf(__builtin_elementwise_maximum(acc[m][a], least), wv[m][a], part[tl]);
+          }
         const int key = k0 + 32 * sub + l32;
-        if (g32 == 0 && key < k1) out[key] = y.there ? part : -INFINITY;
+        if constexpr (NT == 1) {
+          part[0] = sum_halves(part[0]);
+          if (g32 == 0 && key < k1) out[0][key] = y.there ? part[0] : -INFINITY;
+        } else {
+          // two sums at a time: the low lanes get the first one's, the high lanes the second's
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(part[2 * i]), __float_as_uint(part[2 * i + 1]), false, false);
+            const float v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+            if (sees[i] >= 0 && key < k1) out[i][key] = y.there && key < sees[i] ? v : -INFINITY;
+          }
+        }
       };
       const int nsub = (k1 - k0 + 31) / 32;
       Piece a, b;  // (tiles past the last: kNoKey)
@@ -494,9 +521,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
 template <int H, int D, int FMT>
 static int launch_scores(IndexScoreParams p, hipStream_t st) {
   using C = IndexTile<H, D, FMT>;
-  // Single tokens: a request has fewer than two on average.  Replays of 32 requests, 8192 .. 32768 MXFP8 keys, us, tiles of tokens
-  // and single ones: 2 tokens, 16 heads 45, 44; 64 heads 48, 46 (bf16 52, 63); 3 tokens 45, 57 and 57, 60; 4 tokens 46, 72 and 61, 77.
-  const bool rows = p.req.query_starts == nullptr || p.req.R == 0 || p.req.T < 2 * (int64_t)p.req.R;
+  // Tokens of a unit, by those that a request has on average.  Replays of 32 requests, 8192 .. 32768 keys, us, tiles of tokens in LDS
+  // and 64 rows from memory:
+  //   16 heads  2 tokens MXFP8 42, 32, MXFP4 41, 28, bf16 42, 39; 4 tokens 43, 35; 43, 32; 44, 43; 6 tokens 47, 46; 48, 41; 47, 63
+  //   32 heads  2 tokens MXFP8 41, 35, MXFP4 41, 32, bf16 40, 42; 4 tokens 48, 48; 48, 44; 45, 62; 6 tokens 58, 62; 57, 54; 55, 84
+  //   64 heads  2 tokens MXFP8 48, 46, MXFP4 48, 41, bf16 52, 63; 3 tokens MXFP8 57, 60
+  // and of 64 requests, 301 .. 65536 keys: 2 tokens, 32 heads MXFP8 110, 83, MXFP4 90, 58; 4 tokens, 16 heads MXFP4 98, 61.
+  const int64_t T = p.req.T, R = p.req.R;
+  const int nt = p.req.query_starts == nullptr || R == 0 || T < 2 * R ? 1 : T <= (FMT == KEY_MXFP4 ? 2 : 1) * C::TPW * R ? C::TPW : C::TT;  // tokens of a unit
+  const bool rows = nt < C::TT;
   p.whole_tiles = p.block % C::KT == 0;
   // With windows nobody needs the columns that no token sees.  A top-k that reads whole rows finds those of a small call in the caches
   // all the same where they were written: 64 tokens of up to 8192 keys in 32768 columns, top-2048, us, written and not 39, 43; of
@@ -505,13 +538,14 @@ static int launch_scores(IndexScoreParams p, hipStream_t st) {
   const int64_t span = (int64_t)(kWindowPages - 2) * p.block / kBlockKeys * kBlockKeys;
   p.span = (int)(span < kMostSpan ? span : kMostSpan);
   // blocks, at most: fewer than 2^31 of them, and workgroups that all run at once
-  const int tt = rows ? 1 : C::TT, fill = rows ? ScoreUnits<1>::FILL : ScoreUnits<C::TT>::FILL;
-  const int64_t units = rows ? p.tokens : (int64_t)p.tokens / tt + (p.tokens < p.req.R ? p.tokens : p.req.R);
+  const int fill = nt == 1 ? ScoreUnits<1>::FILL : nt == C::TPW ? ScoreUnits<C::TPW>::FILL : ScoreUnits<C::TT>::FILL;
+  const int64_t units = nt == 1 ? p.tokens : (int64_t)p.tokens / nt + (p.tokens < p.req.R ? p.tokens : p.req.R);
   const int64_t n = units * (((int64_t)p.L + kBlockKeys - 1) / kBlockKeys + ((int64_t)p.L + fill - 1) / fill);
   DSA_REQUIRE(n < (1ll << 31), "dsa_paged_index_scores: too many tokens for one call");
-  const int64_t most = 256 * (rows ? (H == 64 ? 2 : 4) : 2);
+  const int64_t most = 256 * (nt * H < 64 ? 4 : 2);
   const dim3 grid((unsigned)(n < 1 ? 1 : n < most ? n : most));
-  if (rows) hipLaunchKernelGGL((index_rows_kernel<H, D, FMT>), grid, dim3(256), 0, st, p);
+  if (rows && nt == 1) hipLaunchKernelGGL((index_rows_kernel<H, D, FMT, 1>), grid, dim3(256), 0, st, p);
+  else if (rows) hipLaunchKernelGGL((index_rows_kernel<H, D, FMT, C::TPW>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((index_tiles_kernel<H, D, FMT>), grid, dim3(256), 0, st, p);
   return check_launch("dsa_paged_index_scores");
 }

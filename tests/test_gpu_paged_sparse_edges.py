@@ -58,6 +58,39 @@ def test_one_long_request(dev, news):
     _compare(ops.paged_index_scores(*args, starts), ref, tol)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("H,d", [(16, 64), (16, 128), (32, 64), (32, 128), (64, 128)])
+@pytest.mark.parametrize("lens,news,bs", [([300, 77, 2100], [2, 2, 2], 16), ([90, 64, 0, 700, 33], [3, 1, 2, 0, 4], 64), ([50, 5], [4, 4], 4), ([1000], [2], 128),
+                                          ([129, 4500, 3], [1, 7, 4], 16)])
+def test_few_tokens(dev, fmt, H, d, lens, news, bs):
+    """A few tokens of each request: units that they fill, or not."""
+    args, starts, L, (ref, tol, limits) = _scores(dev, fmt, H, d, lens, news, bs)
+    _compare(ops.paged_index_scores(*args, starts), ref, tol)
+    part = max(1, max(lens) - 5)
+    _compare(ops.paged_index_scores(*args, starts, num_keys=part), ref[:, :part], tol[:, :part])
+    picks = ops.paged_indexer_topk(*args, 16, starts, max_scratch_bytes=4 * L * 3)     # chunks of three tokens
+    assert torch.equal(picks, ops.paged_indexer_topk(*args, 16, starts))
+    assert torch.equal((picks >= 0).sum(1).cpu().to(I32), limits.clamp(max=16))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("H", [16, 32])
+def test_few_tokens_and_keys_that_are_not_seen(dev, fmt, H):
+    """NaN behind a token's own position, of a later token's key, reaches nothing; pages that are not there hide their keys."""
+    gen = torch.Generator().manual_seed(15)
+    lens, news, bs, d = [100, 66, 50], [3, 1, 2], 16, 128
+    cache, table, kv, starts, q, w = _score_case(dev, gen, fmt, H, d, lens, news, bs)
+    bad = torch.full((1, d), float("nan"), dtype=BF, device=dev)
+    flat = torch.arange(cache.num_blocks * bs, device=dev)
+    for r, pos in ((0, 99), (0, 40), (2, 49)):
+        s = int(table[r, pos // bs]) * bs + pos % bs
+        ops.index_key_append(cache, bad, flat[s:s + 1])
+    table[0, 1], table[1, 0] = cache.num_blocks + 1, -3
+    ref, tol, _ = orc.scores(q, w, orc.unpack_pages(cache.data.cpu(), d), table, starts, kv, bs, table.shape[1] * bs)
+    assert ref[0, 40].isnan() and (ref[0, 98:] == -INF).all() and ref[2, 99].isnan() and (ref[1, 16:32] == -INF).all()
+    _compare(ops.paged_index_scores(q.to(dev), w.to(dev), cache, table.to(dev), kv.to(dev), starts.to(dev)), ref, tol)
+
+
 @pytest.mark.parametrize("L", [1, 2, 5, 63, 65, 127, 129, 321])
 def test_odd_columns(dev, L):
     for news in ([1, 1, 1], [30, 8, 2]):
