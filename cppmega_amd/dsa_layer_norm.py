@@ -7,6 +7,8 @@ other rows of up to 16384 elements.
 x [..., n] bf16 or f32; weight and bias [n], bf16 or f32, or None (ones, zeros); statistics
 and sums in 32 bits, gradients bit-identical between runs.  A small step is bound by the host, half of it by the hand-off
 between autograd's two threads: ``torch.autograd.set_multithreading_enabled(False)`` saves that, a captured graph both.
+Capture a backward on leaves of its own (``x.detach().requires_grad_()``) while an eager graph of the same leaves is alive:
+torch runs a leaf's accumulation on the stream of that graph, which a capture cannot join.
 """
 from __future__ import annotations
 

@@ -189,6 +189,24 @@ def test_on_another_stream_and_in_a_graph(dev):
         assert all(torch.equal(held[k], eager[k]) for k in eager), i
 
 
+def test_capture_beside_a_living_graph(dev):
+    """Captured on leaves of its own while an eager graph of the same tensors waits for its backward."""
+    gen = torch.Generator().manual_seed(16)
+    x, dy, w, b = (t.to(dev) for t in _inputs(gen, 200, 64, BF, F32))
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    living = LayerNorm.apply(*leaves, 1e-5)
+    _step(dev, leaves[0], dy, leaves[1], leaves[2], 1e-5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _step(dev, leaves[0], dy, leaves[1], leaves[2], 1e-5)
+    graph.replay()
+    living.backward(dy)
+    torch.cuda.synchronize()
+    for name, t in zip(("dx", "dweight", "dbias"), leaves):
+        assert torch.equal(held[name], t.grad)
+
+
 def test_second_gradients_are_refused(dev):
     x = torch.randn(4, 64, device=dev, requires_grad=True)
     (g,) = torch.autograd.grad(LayerNorm.apply(x).sum(), x, create_graph=True)
