@@ -217,14 +217,20 @@ __global__ void __launch_bounds__(256) sparse_narrow_combine_kernel(const Sparse
   const int head = (int)(row - t * p.H), c = (int)(threadIdx.x & 15) * 4;
   if (p.picks.req.keys_of((int)t, p.picks.req.of_lane((int)t)) < 0) return;
   const int64_t at = (t * p.htiles + head / 32) * p.nsplit * 32 + head % 32;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 *ml = reinterpret_cast<const f32x2 *>(p.part_ml) + at;
   float m = kLeastMax, l = 0.0f;
-  for (int s = 0; s < p.nsplit; ++s)
-    if (p.part_ml[(at + 32 * s) * 2 + 1] != 0.0f) m = fmaxf(m, p.part_ml[(at + 32 * s) * 2]);
-  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < p.nsplit; ++s) {
-    const float ls = p.part_ml[(at + 32 * s) * 2 + 1], a = ls == 0.0f ? 0.0f : exp2_fast(p.part_ml[(at + 32 * s) * 2] - m);
-    l += ls * a;
+    const f32x2 x = ml[32 * s];
+    m = x[1] != 0.0f ? fmaxf(m, x[0]) : m;
+  }
+  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int s = 0; s < p.nsplit; ++s) {
+    const f32x2 x = ml[32 * s];
+    const float a = x[1] == 0.0f ? 0.0f : exp2_fast(x[0] - m);
+    l += x[1] * a;
     o += a * *reinterpret_cast<const f32x4 *>(p.part_o + (at + 32 * s) * 64 + c);
   }
   o *= l == 0.0f ? 0.0f : 1.0f / l;
@@ -233,7 +239,7 @@ __global__ void __launch_bounds__(256) sparse_narrow_combine_kernel(const Sparse
 }
 
 // How a call is run: waves of a unit, workgroups that share it.  Replays of n tokens, 32 heads, one and four waves a unit:
-// top-256: n = 512 19 us, 17; 1000 19, 22; 1656 24, 28; 2200 28, 31; top-2048: 64 (four waves of eight workgroups) 76, 25;
+// top-256: n = 512 19 us, 17; 1000 19, 22; 1656 24, 28; 2200 28, 31; top-2048: 64 (four waves of eight workgroups) 76, 21;
 // 1000 82, 62; 1656 100, 103.  (Two waves a unit: between the two, or behind both.)
 struct NarrowPlan {
   int wpu, nsplit;
@@ -241,7 +247,7 @@ struct NarrowPlan {
 static NarrowPlan narrow_plan(int64_t T, int64_t topk, int64_t H) {
   const int64_t units = T * ((H + 31) / 32), nb = (topk + 31) / 32;
   if (units >= 1536) return {1, 1};
-  int64_t ns = 768 / units;               // workgroups that fill the card
+  int64_t ns = 512 / units;               // two workgroups a CU (three, top-2048: 128 tokens 28 us, two 25; 320 44, 39)
   if (ns > nb / 8) ns = nb / 8;           // two blocks a wave at least
   return {4, (int)(ns < 1 ? 1 : ns)};
 }
