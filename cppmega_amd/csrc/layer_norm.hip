@@ -12,7 +12,9 @@
 // row in flight while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
 //
 // Bound by the bytes moved, or by a launch's own time: 16384 rows of 4096 bf16, forward, backward, sums: 57 us (4.7 TB/s),
-// 86 (4.7), 4.6; 2051 rows of 1001 f32: 6.6, 9.8, 5.2; 8192 rows of 64 bf16: 3.8, 4.7, 3.0.
+// 86 (4.7), 4.6; 2051 rows of 1001 f32: 6.4, 9.6, 4.0; 8192 rows of 64 bf16: 3.3, 4.7, 2.9.  Results stored past the caches
+// make these calls shorter and what reads the results longer: 16384 rows of 4096, both directions 147 -> 128 us, but the forward
+// and a kernel that reads y 98 -> 106 (of 32768 rows 195 -> 199).
 #include <math.h>
 
 #include "dsa_common.hpp"
