@@ -238,15 +238,16 @@ __global__ void __launch_bounds__(256) sparse_narrow_combine_kernel(const Sparse
   if (c == 0) p.lse[row] = l == 0.0f ? -INFINITY : log2f(l) + m;
 }
 
-// How a call is run: waves of a unit, workgroups that share it.  Replays of n tokens, 32 heads, one and four waves a unit:
-// top-256: n = 512 19 us, 17; 1000 19, 22; 1656 24, 28; 2200 28, 31; top-2048: 64 (four waves of eight workgroups) 76, 21;
-// 1000 82, 62; 1656 100, 103.  (Two waves a unit: between the two, or behind both.)
+// How a call is run: waves of a unit, workgroups that share it.  Replays of n tokens, 32 heads, one and four waves a unit, us:
+// top-128: n = 768 17, 16; 1000 17, 20; 1300 19, 25; top-256: 768 20, 18; 1000 21, 23; 1300 25, 29; top-512: 1000 31, 28;
+// 1300 37, 36; top-1000: 1300 60, 50; top-2048: 64 (four waves of eight workgroups) 76, 21; 1000 82, 62; 1656 100, 103.
+// (Two waves a unit: between the two, or behind both.)
 struct NarrowPlan {
   int wpu, nsplit;
 };
 static NarrowPlan narrow_plan(int64_t T, int64_t topk, int64_t H) {
   const int64_t units = T * ((H + 31) / 32), nb = (topk + 31) / 32;
-  if (units >= 1536) return {1, 1};
+  if (units >= (nb <= 8 ? 900 : 1536)) return {1, 1};
   int64_t ns = 512 / units;               // two workgroups a CU (three, top-2048: 128 tokens 28 us, two 25; 320 44, 39)
   if (ns > nb / 8) ns = nb / 8;           // two blocks a wave at least
   return {4, (int)(ns < 1 ? 1 : ns)};
