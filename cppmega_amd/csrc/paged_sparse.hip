@@ -38,7 +38,8 @@ static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool 
   r.unit_rows = 16 * r.wide;
   r.token_units = (int)((H + r.unit_rows - 1) / r.unit_rows);
   r.unit_blocks = (int)((topk + paged_wide_keys() - 1) / paged_wide_keys());
-  r.min_blocks = 256 / paged_wide_keys();  // picks that are worth a piece's beginning and end
+  r.min_blocks = 256 / paged_wide_keys();  // picks that are worth a piece's beginning and end: a unit of fewer is not cut
+  const bool short_units = r.unit_blocks <= r.min_blocks;
   // Workgroups: a whole number of equal pieces of a unit each, so that none has the end of one unit and the beginning of the
   // next (112 tokens, 16 heads, bf16 64 us by even ranges of all blocks, 61 so; 96, 64 heads 77, 67; 224 units left whole 152,
   // 136), or, where that leaves much of the card idle, even ranges.
@@ -51,8 +52,11 @@ static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool 
     r.nwg = (int)units * pieces;
   } else {
     r.nwg = 256;
-    const int64_t per = (units * r.unit_blocks + 255) / 256;
-    r.per = per > r.min_blocks ? per : r.min_blocks;
+    // (short units, whole and by even ranges of four blocks at least: 160 tokens, 16 heads, top-64, MXFP4 17 us, 43; 300 26, 43; 300, 32
+    // heads, top-128 36, 36; 400, top-200, MXFP4 45, 61)
+    const int64_t per = short_units ? (units + 255) / 256 * r.unit_blocks : (units * r.unit_blocks + 255) / 256;
+    r.per = short_units || per > r.min_blocks ? per : r.min_blocks;
+    if (short_units) r.min_blocks = (int)per;
   }
   return r;
 }
