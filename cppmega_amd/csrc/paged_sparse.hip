@@ -38,26 +38,28 @@ static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool 
   r.unit_rows = 16 * r.wide;
   r.token_units = (int)((H + r.unit_rows - 1) / r.unit_rows);
   r.unit_blocks = (int)((topk + paged_wide_keys() - 1) / paged_wide_keys());
-  r.min_blocks = 256 / paged_wide_keys();  // picks that are worth a piece's beginning and end: a unit of fewer is not cut
-  const bool short_units = r.unit_blocks <= r.min_blocks;
+  r.min_blocks = 256 / paged_wide_keys();  // picks that are worth a piece's beginning and end
   // Workgroups: a whole number of equal pieces of a unit each, so that none has the end of one unit and the beginning of the
   // next (112 tokens, 16 heads, bf16 64 us by even ranges of all blocks, 61 so; 96, 64 heads 77, 67; 224 units left whole 152,
   // 136), or, where that leaves much of the card idle, even ranges.
   const int64_t units = T * r.token_units;
   if (units <= 128 || nearly_all(units)) {
-    const int most = 256 / (int)units, even = (r.unit_blocks + most - 1) / most, per = even > r.min_blocks ? even : r.min_blocks;
+    const int most = 256 / (int)units, even = (r.unit_blocks + most - 1) / most, least = even > r.min_blocks ? even : r.min_blocks;
+    const int per = r.unit_blocks - even <= 4 ? r.unit_blocks : least;  // (128 tokens, 32 heads, top-512 in two pieces 34, whole 28)
     const int pieces = (r.unit_blocks + per - 1) / per;
     r.per = per;
     r.unit_blocks = pieces * per;  // (blocks past the last pick hold none)
     r.nwg = (int)units * pieces;
   } else {
+    // Units left whole, if that costs a workgroup no more than ten blocks: a cut one has two beginnings and ends and is joined
+    // (even ranges and whole units, us: 160 tokens, 16 heads, top-64, MXFP4 43, 17; 400, 32 heads, top-200 61, 45; 424, 16 heads, top-512
+    // 57, 47; 400, 32 heads, top-1000, bf16 85, 71; 500, 16 heads, top-2048, bf16 120, 98; not so: 400, 16 heads, top-2048, MXFP4, 14 more
+    // 110, 118; 1537, 8 heads, top-1000, bf16, 15 more 178, 184).
     r.nwg = 256;
-    // (short units, whole and by even ranges of four blocks at least: 160 tokens, 16 heads, top-64, MXFP4 17 us, 43; 300 26, 43; 300, 32
-    // heads, top-128 36, 36; 400, top-200, MXFP4 45, 61)
-    const int64_t per = short_units ? (units + 255) / 256 * r.unit_blocks : (units * r.unit_blocks + 255) / 256;
-    r.per = short_units || per > r.min_blocks ? per : r.min_blocks;
-    if (short_units) r.min_blocks = (int)per;
+    const int64_t even = (units * r.unit_blocks + 255) / 256, whole = (units + 255) / 256 * r.unit_blocks;
+    r.per = whole - even <= 10 ? whole : even > r.min_blocks ? even : r.min_blocks;
   }
+  r.min_blocks = (int)r.per;  // (what range_blocks has on the device)
   return r;
 }
 

@@ -201,6 +201,15 @@ def test_head_counts(dev, d_qk, d_v, H):
 
 
 @pytest.mark.parametrize("d_qk,d_v", DIMS)
+@pytest.mark.parametrize("T,H,topk", [(5, 128, 320), (100, 20, 512), (128, 16, 192), (140, 16, 64), (140, 16, 200), (160, 16, 1000), (150, 32, 1900), (300, 16, 130),
+                                      (300, 32, 700), (290, 33, 129), (520, 8, 200)])
+def test_units_cut_and_whole(dev, d_qk, d_v, T, H, topk):
+    """Numbers of tokens and picks at which units are cut, in equal pieces or by ranges of several, or left whole."""
+    args, ref = _sparse(dev, "mxfp4" if T % 20 else "bf16", d_qk, d_v, H, [T + 50], [T], 16, topk)
+    _check(ops.paged_sparse_mla_fwd(*args), ref)
+
+
+@pytest.mark.parametrize("d_qk,d_v", DIMS)
 @pytest.mark.parametrize("H,T", [(16, 5), (16, 280), (64, 90), (128, 40), (128, 270)])
 def test_tokens_without_picks(dev, d_qk, d_v, H, T):
     """Every other token picks nothing, or keys past its own alone; in cut units, whole ones and ranges of several."""
