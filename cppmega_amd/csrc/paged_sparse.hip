@@ -2,9 +2,9 @@
 // names by their positions in its request.
 //
 // Rows of 128 channels: paged_sparse_narrow.hip.  Rows of 576: the kernels of paged latent attention, for which a token is a
-// request of one token whose pages are single rows.  Their workgroups share all tokens' picks evenly, 64 at a time, whatever
-// the number of tokens, and paged_combine_kernel adds the pieces of a token that was cut; the picks' slots are formed as a
-// workgroup fills its window of pages.
+// request of one token whose pages are single rows.  Their workgroups have whole tokens, equal pieces of one, or even ranges of
+// all tokens' picks, 64 at a time, and paged_combine_kernel adds the pieces of a token that was cut; the picks' slots are formed as
+// a workgroup fills its window of pages.
 //
 // 64 tokens, 128 heads, top-2048, bf16: 69 us, 530 TFLOP/s; its units of 32 rows read 600 MB through the L2s, 8.8 TB/s, which
 // bounds it (rows by registers, two more steps in flight: 80).  96 tokens, 16 heads, MXFP4: 36 us and 4.3 for the joining, bound by
