@@ -5,8 +5,8 @@
 //   dx = rstd (g - mean(g) - xhat mean(g xhat)),  dweight = sum dy xhat,  dbias = sum dy  (over rows)
 //
 // GL lanes have a row, 8 neighbouring elements a lane and chunk (CH chunks), all in registers, so the variance is that of
-// the differences from the mean and the row is read once; the index keys' 64 channels take 8 lanes, a hidden state's 4096
-// a workgroup.  Rows need no alignment beyond their elements': the loads and stores are 16 bytes wide wherever a row begins.
+// the differences from the mean, the mean's own rounding is taken out of them, and the row is read once; the index keys' 64
+// channels take 8 lanes, a hidden state's 4096 a wave forward and a workgroup backward.  Rows need no alignment beyond their elements': the loads and stores are 16 bytes wide wherever a row begins.
 // The backward adds a lane's columns over the rows that it meets, then its workgroup's lanes in order through LDS, and
 // layer_norm_reduce_kernel the workgroups' sums: no atomics, the order depends on the sizes alone.  The backward has its next
 // row in flight while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
@@ -153,9 +153,10 @@ struct NormGroup {
 
 template <int GL, int CH, bool F32>
 __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(const NormParams p) {
+#pragma clang fp contract(off)  // (the first mean is a rounded one: fused into the differences it would be another there)
   using C = NormGroup<GL>;
   constexpr int ELT = F32 ? 4 : 2;
-  __shared__ float tmp[2][GL > 64 ? C::NW : 1];
+  __shared__ float tmp[3][GL > 64 ? C::NW : 1];
   const int gl = (int)threadIdx.x % GL;
   const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * C::RPW + (int)threadIdx.x / GL;
   const bool there = row < p.rows;  // (whole rows of lanes)
@@ -169,17 +170,30 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(c
   }
   float total[1] = {sum};
   row_sums<GL>(total, tmp[0]);
-  const float mean = total[0] * p.inv_n;
+  const float mean0 = total[0] * p.inv_n;
+  // mean0's error, some steps of its last bit, would stand in every difference: it is the differences' own mean
+  float rest = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[c][i] = 8 * (gl + GL * c) + i < p.n ? v[c][i] - mean0 : 0.0f;
+      rest += v[c][i];
+    }
+  total[0] = rest;
+  row_sums<GL>(total, tmp[1]);
+  rest = total[0] * p.inv_n;
+  const float mean = mean0 + rest;
   float sq = 0.0f;
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[c][i] = 8 * (gl + GL * c) + i < p.n ? v[c][i] - mean : 0.0f;
+      v[c][i] = 8 * (gl + GL * c) + i < p.n ? v[c][i] - rest : 0.0f;
       sq = fmaf(v[c][i], v[c][i], sq);
     }
   total[0] = sq;
-  row_sums<GL>(total, tmp[1]);
+  row_sums<GL>(total, tmp[2]);
   const float rstd = 1.0f / sqrtf(total[0] * p.inv_n + p.eps);
   if (!there) return;
 #pragma unroll

@@ -5,7 +5,9 @@ TEST INFRASTRUCTURE ONLY (see oracle/__init__.py).
 y = xhat w + b, xhat = (x - mean) r, r = (var + eps)^-1/2;  g = dy w, dx = r (g - mean(g) - xhat mean(g xhat)),
 dw = sum dy xhat, db = sum dy.  Bounds, with v = 2^-24 and u half a step of the result's type (bf16 2^-8, fp32 v), each widened
 by 1/16 for second-order terms: a lane adds up to 16 values one after the other and the lanes are joined in up to 20 steps, so a
-row's sum is off by 36 v of the sum of the magnitudes; a column's sum over rows takes at most ROWS steps.
+row's sum is off by 36 v of the sum of the magnitudes, and its 1/n by 2 more; a column's sum over rows takes at most ROWS steps.
+The mean is a first one, m0, and the mean of the differences from it, which is as exact as those are small; the forward takes both
+from x one after the other, the backward their rounded sum.
 """
 from __future__ import annotations
 
@@ -13,6 +15,7 @@ import torch
 
 V = 2.0 ** -24
 SUM = 36 * V
+MEAN = SUM + 2 * V
 ROWS = 256 * V
 WIDEN = 1 + 1 / 16
 
@@ -36,9 +39,11 @@ def layer_norm(x, weight, bias, eps, dy=None, dtype=torch.bfloat16, param_dtype=
     r = (var + eps) ** -0.5
     xhat = xc * r
     y = xhat * w + b
-    e_mean = SUM * x.abs().mean(1, keepdim=True) + V * mean.abs()
-    e_xc = e_mean + V * xc.abs()
-    rel_r = (SUM + 2 * (xc.abs() * e_xc).mean(1, keepdim=True) / (var + eps)) / 2 + 4 * V
+    e_m0 = MEAN * x.abs().mean(1, keepdim=True)
+    e_rest = (MEAN + V) * (xc.abs().mean(1, keepdim=True) + e_m0)
+    e_mean = e_rest + V * mean.abs()
+    e_xc = e_rest + V * (2 * xc.abs() + e_m0)
+    rel_r = (MEAN + 2 * (xc.abs() * e_xc).mean(1, keepdim=True) / (var + eps)) / 2 + 4 * V
     e_xhat = r * e_xc + xhat.abs() * (rel_r + 2 * V)
     res = dict(y=y, mean=mean[:, 0], rstd=r[:, 0], e_mean=WIDEN * e_mean[:, 0], e_rstd=WIDEN * (rel_r * r)[:, 0],
                e_y=WIDEN * (w.abs() * e_xhat + 3 * V * ((w * xhat).abs() + b.abs()) + u * y.abs()))
@@ -46,6 +51,7 @@ def layer_norm(x, weight, bias, eps, dy=None, dtype=torch.bfloat16, param_dtype=
         return res
     dy = dy.double()
     g = dy * w
+    e_xhat = r * (e_mean + V * (xc.abs() + e_mean)) + xhat.abs() * (rel_r + 2 * V)  # by the rounded mean
     s1, s2 = g.mean(1, keepdim=True), (g * xhat).mean(1, keepdim=True)
     e_s1 = SUM * g.abs().mean(1, keepdim=True)
     e_s2 = SUM * (g * xhat).abs().mean(1, keepdim=True) + (g.abs() * e_xhat).mean(1, keepdim=True)

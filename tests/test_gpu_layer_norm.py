@@ -140,6 +140,32 @@ def test_constant_rows(dev):
     assert (got["y"] == 0.5).all() and (got["dx"] == 0).all() and (got["dweight"] == 0).all() and (got["dbias"] == 9).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n", [14, 28, 56, 97, 1001, 3584, 7168, 16383])
+def test_constant_rows_at_any_width(dev, n, dtype):
+    """1 / n is no binary number: the mean is the rows' value all the same, and the differences from it vanish.  The first mean is
+    off by MEAN of the value c, what is left of that by MEAN again, and eps = 1e-6 makes 1000 times that of it."""
+    value = torch.tensor([3.0, 50.0, 100.0, 1000.0, -0.0078125, 0.0]).to(dtype)
+    x = value[:, None].expand(6, n).contiguous().to(dev)
+    y, mean, rstd = layer_norm(x, eps=1e-6, return_stats=True)
+    assert torch.equal(mean.cpu(), value.float())
+    assert (y.double().cpu().abs() <= orc.WIDEN * 1000 * orc.MEAN ** 2 * value.double().abs()[:, None]).all()
+    gen = torch.Generator().manual_seed(n)
+    dy = torch.randn(6, n, generator=gen).to(dtype)
+    dx, dw, _ = layer_norm_backward(dy.to(dev), x, None, mean, rstd)
+    assert (dw == 0).all()
+    _check(dict(dx=dx), orc.layer_norm(x.cpu(), None, None, 1e-6, dy, dtype), ("dx",))
+
+
+@pytest.mark.parametrize("n", [97, 1001, 3584, 7168, 16383])
+def test_a_far_mean_and_a_small_spread(dev, n):
+    """Rows of 1000 +- 0.05: the forward holds their mean to more than 32 bits, the backward to those."""
+    gen = torch.Generator().manual_seed(n)
+    x, dy = 1000.0 + 0.05 * torch.randn(12, n, generator=gen), torch.randn(12, n, generator=gen)
+    w, b = (1 + 0.3 * torch.randn(n, generator=gen)), torch.randn(n, generator=gen)
+    _run(dev, x, dy, w, b, eps=1e-6)
+
+
 @pytest.mark.parametrize("what", [float("nan"), float("inf")])
 @pytest.mark.parametrize("n", [64, 640, 3000])
 def test_a_row_that_is_not_finite(dev, n, what):
