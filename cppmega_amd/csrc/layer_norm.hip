@@ -6,7 +6,8 @@
 //
 // GL lanes have a row, 8 neighbouring elements a lane and chunk (CH chunks), all in registers, so the variance is that of
 // the differences from the mean, the mean's own rounding is taken out of them, and the row is read once; the index keys' 64
-// channels take 8 lanes, a hidden state's 4096 a wave forward and a workgroup backward.  Rows need no alignment beyond their elements': the loads and stores are 16 bytes wide wherever a row begins.
+// channels take 8 lanes, a hidden state's 4096 a wave forward and a workgroup backward.  Rows need no alignment beyond their
+// elements': the loads and stores are 16 bytes wide wherever a row begins.
 // The backward adds a lane's columns over the rows that it meets, then its workgroup's lanes in order through LDS, and
 // layer_norm_reduce_kernel the workgroups' sums: no atomics, the order depends on the sizes alone.  The backward has its next
 // row in flight while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
@@ -165,8 +166,10 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(c
   for (int c = 0; c < CH; ++c) {
     const int col = 8 * (gl + GL * c);
     load_8<F32>(p.x + ((there ? row : 0) * p.x_stride + col) * ELT, p.n - col, v[c]);
+    float part = 0.0f;  // (chunk by chunk: 64 elements one after the other would lose up to as many steps of the sum)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += v[c][i];
+    for (int i = 0; i < 8; ++i) part += v[c][i];
+    sum += part;
   }
   float total[1] = {sum};
   row_sums<GL>(total, tmp[0]);
@@ -174,24 +177,30 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_fwd_kernel(c
   // mean0's error, some steps of its last bit, would stand in every difference: it is the differences' own mean
   float rest = 0.0f;
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c) {
+    float part = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[c][i] = 8 * (gl + GL * c) + i < p.n ? v[c][i] - mean0 : 0.0f;
-      rest += v[c][i];
+      part += v[c][i];
     }
+    rest += part;
+  }
   total[0] = rest;
   row_sums<GL>(total, tmp[1]);
   rest = total[0] * p.inv_n;
   const float mean = mean0 + rest;
   float sq = 0.0f;
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c) {
+    float part = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[c][i] = 8 * (gl + GL * c) + i < p.n ? v[c][i] - rest : 0.0f;
-      sq = fmaf(v[c][i], v[c][i], sq);
+      part = fmaf(v[c][i], v[c][i], part);
     }
+    sq += part;
+  }
   total[0] = sq;
   row_sums<GL>(total, tmp[2]);
   const float rstd = 1.0f / sqrtf(total[0] * p.inv_n + p.eps);

@@ -166,6 +166,17 @@ def test_a_far_mean_and_a_small_spread(dev, n):
     _run(dev, x, dy, w, b, eps=1e-6)
 
 
+@pytest.mark.parametrize("n", [4096, 16384])
+def test_small_elements_behind_a_large_one(dev, n):
+    """Rows with 64 elements a lane: one of them 1, whose square swallows each of 63 squares of just below half its last step where
+    they are added to it one by one."""
+    col = torch.arange(n)
+    x = torch.where((col < n // 8) & (col % 8 == 0), 1.0, (0.99 * 2.0 ** -24) ** 0.5) * torch.where((col // 8) % 2 == 0, 1.0, -1.0)
+    x = x.repeat(5, 1)
+    y, mean, rstd = layer_norm(x.to(dev), eps=1e-9, return_stats=True)
+    _check(dict(y=y, mean=mean, rstd=rstd), orc.layer_norm(x, None, None, 1e-9, dtype=F32), ("y", "mean", "rstd"))
+
+
 @pytest.mark.parametrize("what", [float("nan"), float("inf")])
 @pytest.mark.parametrize("n", [64, 640, 3000])
 def test_a_row_that_is_not_finite(dev, n, what):
