@@ -9,8 +9,9 @@
 // channels take 8 lanes, a hidden state's 4096 a wave forward and a workgroup backward.  Rows need no alignment beyond their
 // elements': the loads and stores are 16 bytes wide wherever a row begins.
 // The backward adds a lane's columns over the rows that it meets, then its workgroup's lanes in order through LDS, and
-// layer_norm_reduce_kernel the workgroups' sums: no atomics, the order depends on the sizes alone.  The backward has its next
-// row in flight while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
+// layer_norm_reduce_kernel the workgroups' sums: no atomics, the order depends on the sizes alone.  A lane adds kNormRun rows at
+// most before its sum joins the workgroup's, whose roundings are kept beside it: a column of any length is off by 256 steps of
+// the sum of its magnitudes at most (128 rows, 32 lanes, 32 and 16 workgroups' sums).  The backward has its next row in flight while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
 //
 // Bound by the bytes moved, or by a launch's own time: 16384 rows of 4096 bf16, forward, backward, sums: 57 us (4.7 TB/s),
 // 86 (4.7), 4.6; 2051 rows of 1001 f32: 6.4, 9.6, 4.0; 8192 rows of 64 bf16: 3.3, 4.7, 2.9.  Results stored past the caches
@@ -29,6 +30,7 @@ struct NormParams {
   unsigned char *y, *dx;     // dense
   float *mean, *rstd;        // [rows]
   float *part;               // [nwg][2][n] sums of dy xhat and dy, or null
+  float *low;                // the same of what their additions rounded away, or null
   void *dweight, *dbias;     // nwg == 1: written at once
   int64_t rows, x_stride, dy_stride;  // strides in elements
   int n, w_f32, nwg;
@@ -227,12 +229,14 @@ __device__ __forceinline__ void put_sum(void *dst, int f32, int col, float v) {
   else static_cast<uint16_t *>(dst)[col] = (uint16_t)pack_bf16x2(v, 0.0f);
 }
 
+constexpr int kNormRun = 128;  // rows that a lane of the backward adds one after the other
+
 template <int GL, int CH, bool F32>
 __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_bwd_kernel(const NormParams p) {
   using C = NormGroup<GL>;
   constexpr int ELT = F32 ? 4 : 2;
   __shared__ float tmp[2][GL > 64 ? 2 * C::NW : 1];
-  __shared__ float sums[C::RPW > 1 ? C::RPW * GL * CH * 8 : 1];
+  __shared__ float sums[C::RPW * GL * CH * 8];
   const int gl = (int)threadIdx.x % GL, grp = (int)threadIdx.x / GL;
   const int64_t step = (int64_t)p.nwg * C::RPW;
   // a row, fetched while the one before it is worked on
@@ -252,76 +256,94 @@ __global__ void __launch_bounds__((NormGroup<GL>::NTHR)) layer_norm_bwd_kernel(c
   };
   int64_t row = (int64_t)blockIdx.x * C::RPW + grp;
   fetch(row);
-  float w[CH][8], dw[CH][8], db[CH][8];
+  float w[CH][8];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int col = 8 * (gl + GL * c);
     load_param(p.weight, p.w_f32, col, p.n - col, 1.0f, w[c]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dw[c][i] = db[c][i] = 0.0f;
   }
-  for (int turn = 0; row - grp < p.rows; row += step, turn ^= 1) {
-    const bool there = row < p.rows;
-    const float r = rstd;
-    float x[CH][8], g[CH][8], s[2] = {0.0f, 0.0f};
+  const bool sums_wanted = p.part != nullptr || p.dweight != nullptr || p.dbias != nullptr;
+  int turn = 0;
+  for (bool first = true;; first = false) {
+    float dw[CH][8], db[CH][8];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      widen<F32>(rx[c], x[c]);
-      widen<F32>(rg[c], g[c]);
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[c][i] = there && 8 * (gl + GL * c) + i < p.n ? (x[c][i] - mean) * r : 0.0f;
-        dw[c][i] = fmaf(g[c][i], x[c][i], dw[c][i]);
-        db[c][i] += g[c][i];
-        g[c][i] *= w[c][i];
-        s[0] += g[c][i];
-        s[1] = fmaf(g[c][i], x[c][i], s[1]);
-      }
-    }
-    fetch(row + step);
-    if (p.dx == nullptr) continue;  // (uniform)
-    row_sums<GL>(s, tmp[turn]);     // (two places in turn: no wait for the readers)
-    const float m1 = s[0] * p.inv_n, m2 = s[1] * p.inv_n;
-    if (there) {
+      for (int i = 0; i < 8; ++i) dw[c][i] = db[c][i] = 0.0f;
+    for (int run = 0; run < kNormRun && row - grp < p.rows; ++run, row += step, turn ^= 1) {
+      const bool there = row < p.rows;
+      const float r = rstd;
+      float x[CH][8], g[CH][8], s[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const int col = 8 * (gl + GL * c), left = p.n - col;
-        if (left <= 0) continue;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[c][i] = r * (g[c][i] - m1 - x[c][i] * m2);
-        store_8<F32>(p.dx + (row * p.n + col) * ELT, left, g[c]);
-      }
-    }
-  }
-  if (p.part == nullptr && p.dweight == nullptr && p.dbias == nullptr) return;
-  // the workgroup's sums: its row groups in order
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    auto put = [&](int col, float v) {
-      if (p.nwg > 1) p.part[((int64_t)blockIdx.x * 2 + which) * p.n + col] = v;
-      else if (void *dst = which ? p.dbias : p.dweight) put_sum(dst, p.w_f32, col, v);
-    };
-    if constexpr (C::RPW == 1) {
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
+        widen<F32>(rx[c], x[c]);
+        widen<F32>(rg[c], g[c]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int col = 8 * (gl + GL * c) + i;
-          if (col < p.n) put(col, which ? db[c][i] : dw[c][i]);
+          x[c][i] = there && 8 * (gl + GL * c) + i < p.n ? (x[c][i] - mean) * r : 0.0f;
+          dw[c][i] = fmaf(g[c][i], x[c][i], dw[c][i]);
+          db[c][i] += g[c][i];
+          g[c][i] *= w[c][i];
+          s[0] += g[c][i];
+          s[1] = fmaf(g[c][i], x[c][i], s[1]);
         }
-    } else {
+      }
+      fetch(row + step);
+      if (p.dx == nullptr) continue;  // (uniform)
+      row_sums<GL>(s, tmp[turn]);     // (two places in turn: no wait for the readers)
+      const float m1 = s[0] * p.inv_n, m2 = s[1] * p.inv_n;
+      if (there) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int col = 8 * (gl + GL * c), left = p.n - col;
+          if (left <= 0) continue;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[c][i] = r * (g[c][i] - m1 - x[c][i] * m2);
+          store_8<F32>(p.dx + (row * p.n + col) * ELT, left, g[c]);
+        }
+      }
+    }
+    const bool last = row - grp >= p.rows;  // (uniform)
+    if (!sums_wanted) {
+      if (last) return;
+      continue;
+    }
+    // the workgroup's sums: its row groups in order
+    int th = (int)threadIdx.x;
+    asm("" : "+v"(th));  // (its addresses are made here, not held in registers through the rows)
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[grp * GL * CH * 8 + 8 * (gl + GL * c) + i] = which ? db[c][i] : dw[c][i];
+        for (int i = 0; i < 8; ++i) sums[th / GL * GL * CH * 8 + 8 * (th % GL + GL * c) + i] = which ? db[c][i] : dw[c][i];
       __syncthreads();
-      for (int col = (int)threadIdx.x; col < p.n; col += C::NTHR) {
+      auto column = [&](int col) {
         float v = 0.0f;
         for (int k = 0; k < C::RPW; ++k) v += sums[k * GL * CH * 8 + col];
-        put(col, v);
+        return v;
+      };
+      const int64_t at = ((int64_t)blockIdx.x * 2 + which) * p.n;
+      if (p.nwg == 1) {
+        if (void *dst = which ? p.dbias : p.dweight)
+          for (int col = th; col < p.n; col += C::NTHR) put_sum(dst, p.w_f32, col, column(col));
+      } else if (p.low == nullptr) {
+        for (int col = th; col < p.n; col += C::NTHR) p.part[at + col] = column(col);
+      } else {
+        for (int col = th; col < p.n; col += C::NTHR) {  // (a column is one thread's in every run)
+          float v = column(col), low = 0.0f;
+          if (!first) {
+            const float had = p.part[at + col], sum = had + v, grown = sum - had;
+            low = p.low[at + col] + ((had - (sum - grown)) + (v - grown));  // what the addition rounded away, exactly
+            v = sum;
+          }
+          p.part[at + col] = v;
+          p.low[at + col] = low;
+        }
       }
     }
+    if (last) return;
   }
 }
 
@@ -335,6 +357,11 @@ __global__ void __launch_bounds__(1024) layer_norm_reduce_kernel(const NormParam
   if (col < p.n) {
 #pragma unroll 8
     for (int k = w; k < p.nwg; k += 16) v += p.part[((int64_t)k * 2 + which) * p.n + col];
+    if (p.low != nullptr) {
+      float low = 0.0f;
+      for (int k = w; k < p.nwg; k += 16) low += p.low[((int64_t)k * 2 + which) * p.n + col];
+      v += low;
+    }
   }
   sums[w][lane] = v;
   __syncthreads();
@@ -359,11 +386,20 @@ constexpr int64_t kNormMost = 16384;
 // Workgroups of the backward, whose sums cost 16 bytes a column, a row's step 6 to 12: as few as take no more turns than the most
 // would (replays of forward and backward, the most and so, us: 2051 rows of 1001 f32 24.4, 23.0; 600 of 2048 f32 26.4, 24.4; 9000
 // of 1001 f32 44.3, 45.1).
-static int64_t norm_bwd_wgs(int64_t rows, int64_t n) {
+struct NormBwdPlan {
+  int64_t nwg;
+  bool runs;  // lanes add more rows than a run
+  size_t bytes;
+};
+static NormBwdPlan norm_bwd_plan(int64_t rows, int64_t n) {
   const int gl = norm_shape(n, true).gl, rpw = gl > 256 ? 1 : 256 / gl;
   const int64_t steps = (rows + rpw - 1) / rpw, most = gl > 256 ? 256 : 512;
   const int64_t turns = (steps + most - 1) / most;
-  return steps <= most ? steps : (steps + turns - 1) / turns;
+  NormBwdPlan k;
+  k.nwg = steps <= most ? steps : (steps + turns - 1) / turns;
+  k.runs = turns > kNormRun;
+  k.bytes = k.nwg > 1 ? (size_t)k.nwg * 2 * (size_t)n * 4 * (k.runs ? 2 : 1) : 0;
+  return k;
 }
 
 template <int GL, int CH>
@@ -445,8 +481,7 @@ extern "C" int dsa_layer_norm_fwd(const void *x, const void *weight, const void 
 
 extern "C" size_t dsa_layer_norm_bwd_workspace_size(int64_t rows, int64_t n) {
   if (check_norm("dsa_layer_norm_bwd_workspace_size", rows, n, DSA_DTYPE_F32, DSA_DTYPE_F32)) return 0;
-  const int64_t nwg = norm_bwd_wgs(rows, n);
-  return nwg > 1 ? (size_t)nwg * 2 * (size_t)n * 4 : 0;
+  return norm_bwd_plan(rows, n).bytes;
 }
 
 extern "C" int dsa_layer_norm_bwd(const void *dy, const void *x, const void *weight, const float *mean, const float *rstd, void *dx,
@@ -476,13 +511,14 @@ extern "C" int dsa_layer_norm_bwd(const void *dy, const void *x, const void *wei
   p.n = (int)n;
   p.w_f32 = w_dtype == DSA_DTYPE_F32;
   p.inv_n = 1.0f / (float)n;
-  p.nwg = (int)norm_bwd_wgs(rows, n);
+  const NormBwdPlan k = norm_bwd_plan(rows, n);
+  p.nwg = (int)k.nwg;
   const bool sums = dweight != nullptr || dbias != nullptr;
   if (sums && p.nwg > 1) {
-    const size_t need = (size_t)p.nwg * 2 * (size_t)n * 4;
-    if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 4))
-      return set_error(DSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace_bytes);
+    if (workspace == nullptr || workspace_bytes < k.bytes || !aligned_to(workspace, 4))
+      return set_error(DSA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, k.bytes, workspace_bytes);
     p.part = (float *)workspace;
+    if (k.runs) p.low = p.part + k.nwg * 2 * n;
   }
   if (rows > 0 && (sums || dx != nullptr)) {
     launch_norm(true, dtype == DSA_DTYPE_F32, p, (hipStream_t)stream);

@@ -74,6 +74,39 @@ def test_without_parameters(dev, weight, bias, n):
     _run(dev, *_inputs(gen, 50, n, BF, F32, weight, bias))
 
 
+def test_a_column_of_very_many_equal_values(dev):
+    """2^26 rows, whose value rounds down by almost half a step of the sum where a lane's 4096 are added one after the other."""
+    rows, n = 1 << 26, 8
+    c = 1 + 2.0 ** -13 - 2.0 ** -23
+    x, dy = torch.ones(1, n, device=dev).expand(rows, n), torch.full((1, n), c, device=dev).expand(rows, n)
+    mean, rstd = torch.zeros(rows, device=dev), torch.ones(rows, device=dev)
+    _, dw, db = layer_norm_backward(dy, x, None, mean, rstd, (False, True, True))
+    for got in (dw, db):
+        assert ((got.double().cpu() - rows * c).abs() <= orc.WIDEN * (orc.ROWS + orc.V) * rows * c).all()
+
+
+@pytest.mark.parametrize("rows,n", [(2_200_003, 3), (270_001, 300), (70_001, 1100), (33_001, 9000)])
+def test_columns_over_very_many_rows(dev, rows, n):
+    """More rows than a lane adds in a run, in every form of the workgroup; the sums in 64 bits beside them."""
+    gen = torch.Generator(device=dev).manual_seed(n)
+    x, dy = (torch.randn(rows, n, generator=gen, device=dev, dtype=F32).to(BF) for _ in range(2))
+    mean, rstd = 0.1 * torch.randn(rows, generator=gen, device=dev), 0.5 + torch.rand(rows, generator=gen, device=dev)
+    got = layer_norm_backward(dy, x, None, mean, rstd)
+    again = layer_norm_backward(dy, x, None, mean, rstd)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    part = slice(rows - 40, None)
+    assert torch.equal(got[0][part], layer_norm_backward(dy[part], x[part], None, mean[part], rstd[part], (True, False, False))[0])
+    sums = torch.zeros(4, n, dtype=torch.float64, device=dev)
+    for at in range(0, rows, 1 << 14):
+        a, g = x[at:at + (1 << 14)].double(), dy[at:at + (1 << 14)].double()
+        t = g * ((a - mean[at:at + (1 << 14), None].double()) * rstd[at:at + (1 << 14), None].double())
+        sums += torch.stack([t.sum(0), g.sum(0), t.abs().sum(0), g.abs().sum(0)])
+    sums = sums.cpu()                                                  # (xhat: two roundings)
+    _check(dict(dweight=got[1], dbias=got[2]),
+           dict(dweight=sums[0], dbias=sums[1], e_dweight=orc.WIDEN * ((orc.ROWS + 2 * orc.V) * sums[2] + orc.V * sums[0].abs()),
+                e_dbias=orc.WIDEN * (orc.ROWS * sums[3] + orc.V * sums[1].abs())), ("dweight", "dbias"))
+
+
 def test_shapes_strides_and_alignment(dev):
     """Leading axes, rows inside a wider tensor at any element, broadcast and transposed gradients."""
     gen = torch.Generator().manual_seed(4)
