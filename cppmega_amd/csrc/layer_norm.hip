@@ -11,7 +11,8 @@
 // The backward adds a lane's columns over the rows that it meets, then its workgroup's lanes in order through LDS, and
 // layer_norm_reduce_kernel the workgroups' sums: no atomics, the order depends on the sizes alone.  A lane adds kNormRun rows at
 // most before its sum joins the workgroup's, whose roundings are kept beside it: a column of any length is off by 256 steps of
-// the sum of its magnitudes at most (128 rows, 32 lanes, 32 and 16 workgroups' sums).  The backward has its next row in flight while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
+// the sum of its magnitudes at most (128 rows, 32 lanes, 32 and 16 workgroups' sums).  The backward has its next row in flight
+// while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
 //
 // Bound by the bytes moved, or by a launch's own time: 16384 rows of 4096 bf16, forward, backward, sums: 57 us (4.7 TB/s),
 // 86 (4.7), 4.6; 2051 rows of 1001 f32: 6.4, 9.6, 4.0; 8192 rows of 64 bf16: 3.3, 4.7, 2.9.  Results stored past the caches
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(1024) layer_norm_reduce_kernel(const NormParam
     if (p.low != nullptr) {
       float low = 0.0f;
       for (int k = w; k < p.nwg; k += 16) low += p.low[((int64_t)k * 2 + which) * p.n + col];
-      v += low;
+      if (fabsf(low) < INFINITY) v += low;  // (not of a sum that is not finite)
     }
   }
   sums[w][lane] = v;

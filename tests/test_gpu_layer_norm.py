@@ -85,6 +85,16 @@ def test_a_column_of_very_many_equal_values(dev):
         assert ((got.double().cpu() - rows * c).abs() <= orc.WIDEN * (orc.ROWS + orc.V) * rows * c).all()
 
 
+def test_an_infinite_gradient_among_very_many(dev):
+    """It stays in its column, and a sum of one sign of infinity is that infinity."""
+    rows, n = 2_200_003, 4
+    x, dy = torch.ones(rows, n, device=dev), torch.ones(rows, n, device=dev)
+    dy[77, 1], dy[1_900_000, 2], dy[2_000_000, 2] = float("inf"), float("inf"), -float("inf")
+    _, dw, db = layer_norm_backward(dy, x, None, torch.zeros(rows, device=dev), torch.ones(rows, device=dev), (False, True, True))
+    for got in (dw, db):
+        assert got[0] == got[3] == rows and got[1] == float("inf") and got[2].isnan()
+
+
 @pytest.mark.parametrize("rows,n", [(2_200_003, 3), (270_001, 300), (70_001, 1100), (33_001, 9000)])
 def test_columns_over_very_many_rows(dev, rows, n):
     """More rows than a lane adds in a run, in every form of the workgroup; the sums in 64 bits beside them."""
