@@ -13,7 +13,6 @@ torch runs a leaf's accumulation on the stream of that graph, which a capture ca
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .latent_mla_ops._common import launch_on, same_device
@@ -93,7 +92,8 @@ def _backward(dy, x, weight, mean, rstd, need, param_dtype):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, return_stats=False):
-    """y of x's shape and type; with ``return_stats`` (y, mean, rstd), f32 of x's leading shape, for the backward."""
+    """y of x's shape and type, without a gradient (``LayerNorm.apply`` has one); with ``return_stats`` (y, mean, rstd), f32 of
+    x's leading shape, for ``layer_norm_backward``."""
     y, stats = _forward(x, weight, bias, eps, return_stats)
     return (y, *stats.view(2, *x.shape[:-1])) if return_stats else y
 
@@ -114,7 +114,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, need=(True, True, True), para
 
 
 class LayerNorm(torch.autograd.Function):
-    """apply(x, weight=None, bias=None, eps=1e-5) -> y, with gradients to x, weight and bias."""
+    """apply(x, weight=None, bias=None, eps=1e-5) -> y, with gradients to x, weight and bias; second ones are refused."""
 
     @staticmethod
     def forward(ctx, x, weight=None, bias=None, eps=1e-5):
@@ -125,16 +125,25 @@ class LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _once(ctx, dy) if torch.is_grad_enabled() else _gradients(ctx, dy)
+        x, weight, stats = ctx.saved_tensors
+        given = ctx.needs_input_grad  # (arguments left to their defaults have no place in it)
+        need = (*given, False, False)[:3]
+        gradients = _Gradients.apply if torch.is_grad_enabled() else _gradients
+        return (*gradients(dy, x, weight, stats, need, ctx.param_dtype), None)[:len(given)]
 
 
-def _gradients(ctx, dy):
-    x, weight, stats = ctx.saved_tensors
-    given = ctx.needs_input_grad  # (arguments left to their defaults have no place in it)
-    need = (*given, False, False)[:3]
+def _gradients(dy, x, weight, stats, need, param_dtype):
     mean = stats.data_ptr()
-    grads = _backward(dy, x, weight, mean, mean + 4 * stats.shape[1], need, ctx.param_dtype)
-    return (*grads, None)[:len(given)]
+    return _backward(dy, x, weight, mean, mean + 4 * stats.shape[1], need, param_dtype)
 
 
-_once = once_differentiable(_gradients)  # under create_graph; its wrapping costs time on the host
+class _Gradients(torch.autograd.Function):
+    """The gradients under create_graph: they hang on dy, x and weight, so that whatever asks for theirs is refused."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _gradients(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("LayerNorm has no second gradients: detach what its first are used for")

@@ -294,6 +294,25 @@ def test_second_gradients_are_refused(dev):
         torch.autograd.grad(g.sum(), x)
 
 
+@pytest.mark.parametrize("of", ["x", "weight", "bias"])
+def test_a_penalty_on_a_gradient_is_refused_not_dropped(dev, of):
+    """The gradient hangs on x and weight though the upstream one hangs on nothing; its values are those without create_graph."""
+    x, w, b = torch.randn(4, 64, device=dev, requires_grad=True), torch.ones(64, device=dev, requires_grad=True), torch.zeros(64, device=dev, requires_grad=True)
+    leaf = dict(x=x, weight=w, bias=b)[of]
+    up = torch.randn(4, 64, device=dev)
+    (plain,) = torch.autograd.grad(LayerNorm.apply(x, w, b), leaf, up)
+    assert not plain.requires_grad
+    (g,) = torch.autograd.grad(LayerNorm.apply(x, w, b), leaf, up, create_graph=True)
+    assert torch.equal(g, plain) and g.requires_grad
+    with pytest.raises(RuntimeError, match="second gradients"):
+        (g.square().sum() + x.square().sum()).backward()
+    fixed = x.detach()
+    (g,) = torch.autograd.grad(LayerNorm.apply(fixed, None, b), b, up, create_graph=True)
+    assert not g.requires_grad                                        # of nothing that asks for a gradient
+    (g.square().sum() + b.square().sum()).backward()
+    assert (b.grad == 0).all()
+
+
 def test_in_front_of_the_indexer(dev):
     """Normed keys through the indexer's scores and loss: the gradient reaches the norm's weight and its input."""
     gen = torch.Generator().manual_seed(11)
