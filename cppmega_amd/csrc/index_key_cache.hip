@@ -126,6 +126,8 @@ static int launch_of(const char *who, bool append, int fmt, const KeyCacheParams
   return fmt == KEY_MXFP8 ? launch_as<D, KEY_MXFP8>(who, append, p, st) : launch_as<D, KEY_MXFP4>(who, append, p, st);
 }
 
+// A grid's threads along an axis stay below 2^32, its last workgroup's among them.
+static bool countable(int64_t T, int64_t d) { return T >= 0 && T < (1ll << 28) && (T * (d / 8) + 255) / 256 < (1ll << 24); }
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static int check_keys(const char *who, int64_t num_blocks, int64_t block, int64_t d, int dtype) {
@@ -165,7 +167,7 @@ extern "C" int dsa_index_key_append(void *cache, const void *k, int64_t k_stride
   const char *who = "dsa_index_key_append";
   const int rc = check_keys(who, num_blocks, block_size, D, dtype);
   if (rc) return rc;
-  DSA_REQUIRE(T >= 0 && T < (1ll << 28), "%s: T=%lld must be in [0, 2^28)", who, (long long)T);
+  DSA_REQUIRE(countable(T, D), "%s: T=%lld must be in [0, 2^28), for 128 channels at most 2^28 - 16", who, (long long)T);
   if (T == 0) return DSA_OK;
   DSA_REQUIRE(cache && k && slots && aligned16(cache) && aligned16(k), "%s: null or misaligned pointer", who);
   DSA_REQUIRE(k_stride >= 0 && k_stride % 8 == 0, "%s: the row stride must be a non-negative multiple of 8 elements", who);
@@ -183,7 +185,7 @@ extern "C" int dsa_index_key_gather(const void *cache, const int64_t *slots, voi
   const char *who = "dsa_index_key_gather";
   const int rc = check_keys(who, num_blocks, block_size, D, dtype);
   if (rc) return rc;
-  DSA_REQUIRE(T >= 0 && T < (1ll << 28), "%s: T=%lld must be in [0, 2^28)", who, (long long)T);
+  DSA_REQUIRE(countable(T, D), "%s: T=%lld must be in [0, 2^28), for 128 channels at most 2^28 - 16", who, (long long)T);
   if (T == 0) return DSA_OK;
   DSA_REQUIRE(cache && slots && out && aligned16(cache) && aligned16(out), "%s: null or misaligned pointer", who);
   KeyCacheParams p{};

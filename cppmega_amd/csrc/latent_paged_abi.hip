@@ -134,7 +134,7 @@ static int check_sparse(const char *who, int64_t T, int64_t H, int64_t topk, int
   DSA_REQUIRE(H <= 4096 && T < (1ll << 30) && T * H < (1ll << 31) - 1024 && topk <= (1ll << 27),
               "%s: sizes out of range (H <= 4096, T * H below 2^31 - 1024, topk at most 2^27)", who);
   DSA_REQUIRE(T == 0 || paged_sparse_countable(T, topk, H, d_qk),
-              "%s: sizes out of range (T times groups of 32 heads must stay below 2^26, for 576 channels times blocks of 64 picks below 2^31)", who);
+              "%s: sizes out of range (T times groups of 32 heads must stay below 2^26 - 3, for 576 channels below 2^26 and times blocks of 64 picks below 2^31)", who);
   return DSA_OK;
 }
 

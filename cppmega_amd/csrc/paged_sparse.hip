@@ -65,7 +65,8 @@ static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool 
 
 // Workgroups and blocks can be numbered.
 bool paged_sparse_countable(int64_t T, int64_t topk, int64_t H, int64_t d_qk) {
-  if (T * ((H + 31) / 32) >= (1ll << 26)) return false;
+  const int64_t units = T * ((H + 31) / 32);
+  if (units >= (1ll << 26) || (d_qk == 128 && (units + 3) / 4 >= (1ll << 24))) return false;  // (four waves each, below 2^32 threads)
   bool ok = true;
   for (int fp4 = 0; d_qk == 576 && fp4 < 2; ++fp4) {
     const SparseWidePlan k = sparse_wide_plan(T, topk, H, fp4 != 0);

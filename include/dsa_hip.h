@@ -735,7 +735,7 @@ int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const int32_t *bl
  *   119 (all zeros: 2^0); MXFP4: 2^(floor(log2 amax) - 2), held to +-125; codes to nearest
  *   even, saturating; a block with Inf or NaN gets 255.
  * gather: out [T, D] bf16 of slots (zeros outside the cache), exact.
- * Pointers of rows are 16-byte aligned, k_stride a multiple of 8; T < 2^28.
+ * Pointers of rows are 16-byte aligned, k_stride a multiple of 8; T < 2^28 (128 channels: T <= 2^28 - 16).
  */
 int64_t dsa_index_key_row_bytes(int64_t D, int dtype);
 int dsa_index_key_append(void *cache, const void *k, int64_t k_stride, const int64_t *slots, int64_t T,
@@ -767,7 +767,7 @@ int dsa_paged_index_scores(const void *q, const void *w, const void *cache, cons
  * (int32 [T, topk], positions in its request, any order; a position outside the token's own
  * ones, in particular -1, is masked; a repeated one counts every time).  Everything else as
  * in dsa_paged_latent_mla_fwd, whose results for the same rows it gives; num_blocks *
- * block_size < 2^31, topk <= 2^27, T * ceil(H / 32) < 2^26.  workspace:
+ * block_size < 2^31, topk <= 2^27, T * ceil(H / 32) < 2^26 (128 channels: at most 2^26 - 4).  workspace:
  * dsa_paged_sparse_mla_workspace_size() bytes, 256-byte aligned.
  */
 size_t dsa_paged_sparse_mla_workspace_size(int64_t T, int64_t H, int64_t topk, int64_t D_qk, int64_t D_v);

@@ -154,6 +154,20 @@ def test_c_calls_too_large_for_their_numbering():
     assert size(1 << 20, 64, 1 << 18, 576, 512) == 0                # blocks of picks past 2^31
 
 
+def test_c_the_last_call_of_a_grid():
+    """A grid's axis has fewer than 2^32 threads, its last workgroup's among them.  Admitted calls end at a later check."""
+    L = _lib.load()
+    why = lambda: L.dsa_last_error().decode()  # noqa: E731
+    for D, most in ((128, (1 << 28) - 16), (64, (1 << 28) - 1)):
+        for f, a in ((L.dsa_index_key_append, (P, None, 128, P)), (L.dsa_index_key_gather, (P, P, None))):
+            assert f(*a, most, 2, 16, D, DTYPE_BF16, None) == INVALID and "pointer" in why()
+            assert f(*a, most + 1, 2, 16, D, DTYPE_BF16, None) == INVALID and "T=" in why()
+    sparse = lambda T, H, D, V: L.dsa_paged_sparse_mla_fwd(P, P, P, P, P, P, P, P, P, 1 << 60, T, 0, 4, H, 8, D, V, 2, 16, DTYPE_BF16, 0.1, None)  # noqa: E731
+    for D, V, most in ((128, 64, (1 << 26) - 4), (576, 512, (1 << 26) - 1)):
+        assert sparse(most, 1, D, V) == sparse(most // 2, 33, D, V) == OK                    # (no requests: nothing to do)
+        assert sparse(most + 1, 1, D, V) == sparse(most // 2 + 1, 33, D, V) == INVALID and "out of range" in why()
+
+
 def test_c_layer_norm():
     L = _lib.load()
     fwd = lambda **k: L.dsa_layer_norm_fwd(*({**dict(x=P, w=P, b=P, y=P, m=P, r=P, rows=4, n=64, xs=64, eps=1e-5, dt=DTYPE_BF16, wd=DTYPE_F32,  # noqa: E731
