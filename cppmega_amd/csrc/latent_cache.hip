@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256) latent_cache_gather_kernel(const unsigned
 template <int D_QK, int D_V, bool FP4>
 static int append_as(const AppendParams &p, hipStream_t st) {
   const int64_t n = (p.T * (D_QK / 8) + 255) / 256;
-  DSA_REQUIRE(n < (1ll << 31), "dsa_latent_cache_append: too many rows");
+  DSA_REQUIRE(n < (1ll << 24), "dsa_latent_cache_append: too many rows");  // (a grid's axis: fewer than 2^32 threads)
   hipLaunchKernelGGL((latent_cache_append_kernel<D_QK, D_V, FP4>), dim3((unsigned)n), dim3(256), 0, st, p);
   return check_launch("dsa_latent_cache_append");
 }
@@ -109,7 +109,7 @@ int launch_cache_append(void *cache, const void *latent, int64_t latent_t, const
 template <int D_QK, int D_V, bool FP4>
 static int gather_as(const void *cache, const int64_t *slots, void *out, int64_t T, int64_t num_slots, hipStream_t st) {
   const int64_t n = (T * (D_QK / 8) + 255) / 256;
-  DSA_REQUIRE(n < (1ll << 31), "dsa_latent_cache_gather: too many rows");
+  DSA_REQUIRE(n < (1ll << 24), "dsa_latent_cache_gather: too many rows");
   hipLaunchKernelGGL((latent_cache_gather_kernel<D_QK, D_V, FP4>), dim3((unsigned)n), dim3(256), 0, st,
                      (const unsigned char *)cache, slots, (uint16_t *)out, T, num_slots);
   return check_launch("dsa_latent_cache_gather");

@@ -667,7 +667,8 @@ int dsa_latent_mla_expanded_bwd(const void *q, const void *k_nope, const void *k
  *   2^(floor(log2 amax) - 2) of each 32 channels, its exponent held to +-125 (all zeros:
  *   2^0), codes to nearest even, saturating at 6; a block with Inf or NaN gets 255.
  * gather: out [T, D_qk] bf16 of slots (zeros outside the cache), exact.
- * Pointers of rows are 16-byte aligned, row strides multiples of 8 elements.
+ * Pointers of rows are 16-byte aligned, row strides multiples of 8 elements; T * D_qk / 8 at
+ * most 2^32 - 256.
  */
 int64_t dsa_latent_cache_row_bytes(int64_t D_qk, int64_t D_v, int dtype);
 int dsa_latent_cache_append(void *cache, const void *latent, int64_t latent_stride, const void *rope,

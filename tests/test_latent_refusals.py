@@ -178,6 +178,15 @@ def test_c_cache():
     assert f(T=0, q=None) == OK and f(R=0, kv=None) == OK
 
 
+def test_c_cache_rows_past_a_grid():
+    """A grid's axis has fewer than 2^32 threads."""
+    L = _lib.load()
+    for D, V, T in ((128, 64, (1 << 28) - 15), (576, 512, 59652321), (576, 512, (1 << 31) - 1)):
+        for dt in (DTYPE_BF16, DTYPE_MXFP4):
+            assert L.dsa_latent_cache_append(P, P, V, P, 64, P, T, 2, 16, D, V, dt, None) == INVALID
+            assert L.dsa_latent_cache_gather(P, P, P, T, 2, 16, D, V, dt, None) == INVALID
+
+
 def test_c_plan():
     L = _lib.load()
     names = "ctx new table free count t_out slots pos starts kv ctx_out granted f_out c_out".split()
