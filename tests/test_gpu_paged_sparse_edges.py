@@ -209,6 +209,14 @@ def test_units_cut_and_whole(dev, d_qk, d_v, T, H, topk):
     _check(ops.paged_sparse_mla_fwd(*args), ref)
 
 
+@pytest.mark.parametrize("T,H", [(270, 100), (270, 65), (140, 200), (262, 127)])
+@pytest.mark.parametrize("topk", [100, 1000])
+def test_units_of_128_rows_with_fewer(dev, T, H, topk):
+    """Many tokens, more than 64 heads, bf16: units of 128 rows of which some are no head's, whole and cut."""
+    args, ref = _sparse(dev, "bf16", 576, 512, H, [T + 900], [T], 16, topk)
+    _check(ops.paged_sparse_mla_fwd(*args), ref)
+
+
 @pytest.mark.parametrize("d_qk,d_v", DIMS)
 @pytest.mark.parametrize("H,T", [(16, 5), (16, 280), (64, 90), (128, 40), (128, 270)])
 def test_tokens_without_picks(dev, d_qk, d_v, H, T):
