@@ -29,6 +29,8 @@ struct SparseWidePlan {
   int wide, unit_rows, token_units, unit_blocks, nwg, min_blocks;
   int64_t per;  // blocks of a workgroup
 };
+// Ranges of whole units: nothing is cut, and nothing to join.
+static bool all_whole(const SparseWidePlan &k) { return k.per % k.unit_blocks == 0; }
 static bool nearly_all(int64_t units) { return units >= 192 && units <= 256; }
 static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool fp4) {
   SparseWidePlan r{};
@@ -80,7 +82,7 @@ size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, 
   size_t most = 0;  // of the two formats': the query does not know it
   for (int fp4 = 0; fp4 < 2; ++fp4) {
     const SparseWidePlan k = sparse_wide_plan(T, topk, H, fp4 != 0);
-    const size_t n = (size_t)k.nwg * 2 * (size_t)k.unit_rows * ((size_t)d_v + 2) * 4;
+    const size_t n = all_whole(k) ? 0 : (size_t)k.nwg * 2 * (size_t)k.unit_rows * ((size_t)d_v + 2) * 4;
     most = n > most ? n : most;
   }
   return most;
@@ -112,7 +114,7 @@ int launch_paged_sparse(PagedParams p, const int32_t *indices, int64_t topk, int
   p.part_ml = (float *)ws;
   p.part_o = p.part_ml + (size_t)k.nwg * 2 * (size_t)k.unit_rows * 2;
   const int rc = launch_paged_wide(p, k.wide, fp4, true, st);
-  if (rc || k.per % k.unit_blocks == 0) return rc;  // ranges of whole units: nothing to join
+  if (rc || all_whole(k)) return rc;
   return launch_paged_combine(p, d_v, true, st);
 }
 

@@ -168,6 +168,17 @@ def test_c_the_last_call_of_a_grid():
         assert sparse(most + 1, 1, D, V) == sparse(most // 2 + 1, 33, D, V) == INVALID and "out of range" in why()
 
 
+def test_c_workspace_of_whole_units():
+    """No workspace where no unit is cut: it would be two 32-bit pieces a workgroup that nobody writes."""
+    L = _lib.load()
+    size = lambda T, H, topk: L.dsa_paged_sparse_mla_workspace_size(T, H, topk, 576, 512)  # noqa: E731
+    for whole in ((1537, 128, 64), (64, 128, 2048), (160, 16, 64), (1, 16, 64), (256, 16, 2048)):
+        assert size(*whole) == 0, whole
+    for cut in ((96, 16, 2048), (1, 128, 2048), (400, 16, 2048)):
+        assert size(*cut) > 0, cut
+    assert L.dsa_paged_sparse_mla_fwd(P, P, P, P, P, P, P, P, None, 0, 160, 0, 4, 16, 64, 576, 512, 2, 16, DTYPE_BF16, 0.1, None) == OK
+
+
 def test_c_layer_norm():
     L = _lib.load()
     fwd = lambda **k: L.dsa_layer_norm_fwd(*({**dict(x=P, w=P, b=P, y=P, m=P, r=P, rows=4, n=64, xs=64, eps=1e-5, dt=DTYPE_BF16, wd=DTYPE_F32,  # noqa: E731
