@@ -53,13 +53,19 @@ static SparseWidePlan sparse_wide_plan(int64_t T, int64_t topk, int64_t H, bool 
     r.unit_blocks = pieces * per;  // (blocks past the last pick hold none)
     r.nwg = (int)units * pieces;
   } else {
-    // Units left whole, if that costs a workgroup no more than ten blocks: a cut one has two beginnings and ends and is joined
-    // (even ranges and whole units, us: 160 tokens, 16 heads, top-64, MXFP4 43, 17; 400, 32 heads, top-200 61, 45; 424, 16 heads, top-512
-    // 57, 47; 400, 32 heads, top-1000, bf16 85, 71; 500, 16 heads, top-2048, bf16 120, 98; not so: 400, 16 heads, top-2048, MXFP4, 14 more
-    // 110, 118; 1537, 8 heads, top-1000, bf16, 15 more 178, 184).
+    // Units left whole, if that costs a workgroup no more than `most` blocks: a cut one has two beginnings and ends and is joined.
+    // Even ranges and whole units, us, by the blocks that whole ones cost more (replays of one request's prompt):
+    //   bf16, 16 rows   4: 257 tokens 37, 35; 420 59, 50;  7: 257 41, 41; 700 122, 112 (6);  10: 350 63, 58;  11: 257 46, 50
+    //         32        4: 257 49, 43;  9: 257 56, 54;  10: 350 79, 68;  11: 257 58, 58;  15: 257 65, 68; 350 92, 89
+    //         64        4: 257 57, 49;  8: 300 72, 72; 560 103, 104;  9: 257 70, 72;  10: 350 102, 99;  11: 257 75, 80; 420 175, 169
+    //         128       4: 257 85, 72;  8: 300 111, 109; 560 167, 161;  9: 257 108, 109;  10: 350 161, 156;  11: 257 115, 124
+    //   MXFP4, 16       4: 257 39, 38;  6: 560 65, 66;  7: 257 44, 46; 350 63, 58;  8: 300 49, 53; 700 169, 170;  9: 257 47, 52
+    //         32        4: 257 50, 46;  7: 257 56, 56; 350 78, 70;  8: 300 60, 62; 700 198, 194;  9: 257 60, 63;  11: 257 63, 70
+    //         64        4: 257 61, 59;  5: 350 86, 77;  6: 300 72, 77; 700 257, 256;  7: 257 72, 77; 350 104, 100;  9: 257 77, 88
     r.nwg = 256;
     const int64_t even = (units * r.unit_blocks + 255) / 256, whole = (units + 255) / 256 * r.unit_blocks;
-    r.per = whole - even <= 10 ? whole : even > r.min_blocks ? even : r.min_blocks;
+    const int64_t most = !fp4 ? 10 : r.wide == 4 ? 5 : 7;
+    r.per = whole - even <= most ? whole : even > r.min_blocks ? even : r.min_blocks;
   }
   r.min_blocks = (int)r.per;  // (what range_blocks has on the device)
   return r;

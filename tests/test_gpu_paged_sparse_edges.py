@@ -209,6 +209,14 @@ def test_units_cut_and_whole(dev, d_qk, d_v, T, H, topk):
     _check(ops.paged_sparse_mla_fwd(*args), ref)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("T,H,topk", [(257, 64, 320), (257, 64, 640), (257, 40, 1000), (130, 128, 640), (257, 16, 512), (300, 32, 640)])
+def test_units_by_the_blocks_that_whole_ones_cost(dev, fmt, T, H, topk):
+    """Both sides of the rule that leaves units whole, which differs by type and rows."""
+    args, ref = _sparse(dev, fmt, 576, 512, H, [T + 700], [T], 16, topk)
+    _check(ops.paged_sparse_mla_fwd(*args), ref)
+
+
 @pytest.mark.parametrize("T,H", [(270, 100), (270, 65), (140, 200), (262, 127)])
 @pytest.mark.parametrize("topk", [100, 1000])
 def test_units_of_128_rows_with_fewer(dev, T, H, topk):

@@ -174,7 +174,7 @@ def test_c_workspace_of_whole_units():
     size = lambda T, H, topk: L.dsa_paged_sparse_mla_workspace_size(T, H, topk, 576, 512)  # noqa: E731
     for whole in ((1537, 128, 64), (64, 128, 2048), (160, 16, 64), (1, 16, 64), (256, 16, 2048)):
         assert size(*whole) == 0, whole
-    for cut in ((96, 16, 2048), (1, 128, 2048), (400, 16, 2048)):
+    for cut in ((96, 16, 2048), (1, 128, 2048), (400, 16, 2048), (257, 64, 640)):            # (the last: MXFP4's)
         assert size(*cut) > 0, cut
     assert L.dsa_paged_sparse_mla_fwd(P, P, P, P, P, P, P, P, None, 0, 160, 0, 4, 16, 64, 576, 512, 2, 16, DTYPE_BF16, 0.1, None) == OK
 
