@@ -329,6 +329,9 @@ __device__ __forceinline__ void lds_dma_16(uint32_t lds, uint32_t voffset, i32x4
                : "memory", "m0");
 }
 
+// Keeps a wave-uniform branch a branch: what it holds is then not computed, and selected from, where it is not taken.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
 // Remap a linear block id so that consecutive logical blocks land on the
 // same XCD (blocks are dispatched round-robin over the 8 XCDs of MI355X).
 __device__ __forceinline__ int64_t xcd_remap(int64_t bid, int64_t nblocks) {
@@ -343,6 +346,9 @@ __device__ __forceinline__ int64_t xcd_remap(int64_t bid, int64_t nblocks) {
 // Host-side status helpers (defined in dsa_abi.hip)
 // ---------------------------------------------------------------------------
 namespace dsa {
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// log2 of a page's rows, -1: no power of two
+inline int shift_of(int64_t block) { return (block & (block - 1)) == 0 ? __builtin_ctzll((unsigned long long)block) : -1; }
 int set_error(int code, const char *fmt, ...);
 int check_launch(const char *what);
 // Top-k over nbatch batches of rows in one launch (defined in topk_select.hip).

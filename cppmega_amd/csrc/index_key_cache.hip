@@ -128,7 +128,6 @@ static int launch_of(const char *who, bool append, int fmt, const KeyCacheParams
 
 // A grid's threads along an axis stay below 2^32, its last workgroup's among them.
 static bool countable(int64_t T, int64_t d) { return T >= 0 && T < (1ll << 28) && (T * (d / 8) + 255) / 256 < (1ll << 24); }
-static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static int check_keys(const char *who, int64_t num_blocks, int64_t block, int64_t d, int dtype) {
   DSA_REQUIRE(num_blocks > 0 && num_blocks < (1ll << 31) && block > 0 && block <= 65536,
@@ -142,7 +141,6 @@ static int check_keys(const char *who, int64_t num_blocks, int64_t block, int64_
   return DSA_OK;
 }
 static int key_format(int dtype) { return dtype == DSA_DTYPE_BF16 ? KEY_BF16 : dtype == DSA_DTYPE_MXFP8 ? KEY_MXFP8 : KEY_MXFP4; }
-static int shift_of(int64_t block) { return (block & (block - 1)) == 0 ? __builtin_ctzll((unsigned long long)block) : -1; }
 
 static int run_keys(const char *who, bool append, KeyCacheParams p, int64_t num_blocks, int64_t block, int64_t d, int dtype, hipStream_t st) {
   const int fmt = key_format(dtype);

@@ -161,9 +161,6 @@ __device__ __forceinline__ void pack_operand(const f32x16 &x, i32x4 (&b)[2]) {
                  (int)pack_bf16x2(x[8 * u + 4], x[8 * u + 5]), (int)pack_bf16x2(x[8 * u + 6], x[8 * u + 7])};
 }
 
-// Keeps a wave-uniform branch a branch: what it holds is then not computed, and selected from, where it is not taken.
-__device__ __forceinline__ void keep_branch() { asm volatile(""); }
-
 // The operands of N products read from LDS, kGroup at a time, a group ahead of its use:
 // use(i, operand) for i in order.  The first group was loaded by the caller (while
 // something else ran); the barriers keep the compiler from sinking a load to its use.

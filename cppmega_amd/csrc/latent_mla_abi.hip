@@ -5,7 +5,6 @@
 
 namespace dsa {
 
-static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 // Tensors may be empty (no tokens): their pointers are then not looked at.
 static bool given(const void *p, int64_t n) { return n == 0 || (p != nullptr && aligned16(p)); }
 

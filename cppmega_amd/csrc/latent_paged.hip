@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
   for (int r0 = 0; r0 < p.R; r0 += 1024) {
     const int r = r0 + (int)threadIdx.x;
     // (starts that do not ascend may ask for more units than there are: cut)
-    const int n = r < p.R ? min((request_tokens(p, r) * p.H + p.unit_rows - 1) / p.unit_rows, p.max_units) : 0;
+    const int n = r < p.R ? min((p.req.tokens(r) * p.H + p.unit_rows - 1) / p.unit_rows, p.max_units) : 0;
     const uint32_t x = add_sat(at, block_scan<1024>((uint32_t)n, tmp, total));
     if (r < p.R) p.unit0[r] = (int)min(x, most);
     at = min(add_sat(at, total), most);
@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(const PagedParams p) {
         const int mid = (lo + hi + 1) >> 1;
         if (p.unit0[mid] <= u) lo = mid; else hi = mid - 1;
       }
-      const int first = (u - p.unit0[lo]) * p.unit_rows, n = request_tokens(p, lo);
-      nb = unit_blocks(p, request_kv(p, lo), n, first, n * p.H, p.unit_rows);
+      const int first = (u - p.unit0[lo]) * p.unit_rows, n = p.req.tokens(lo);
+      nb = unit_blocks(p, p.req.kv(lo), n, first, n * p.H, p.unit_rows);
       p.unit_req[u] = lo;
       p.unit_first[u] = first;
     }

@@ -11,8 +11,7 @@ struct PagedParams {
   const unsigned char *q;        // [T, H, d_qk] bf16
   const unsigned char *cache;    // [num_blocks][block] rows
   const int32_t *table;          // [R, W] pages, others mask their keys
-  const int32_t *query_starts;   // [R + 1] first token of every request, or null: one token each
-  const int32_t *kv_lens;        // [R] keys of a request, its new tokens' among them
+  Requests req;                  // starts [R + 1] or null (one token each), lengths [R], a request's new tokens' keys among them
   uint16_t *out;                 // [T, H, d_v]
   float *lse;                    // [T, H]
   int64_t T;
@@ -38,23 +37,6 @@ __device__ __forceinline__ i32x4 ld_row_16(const unsigned char *x) {
 __device__ __forceinline__ uint32_t ld_row_1(const unsigned char *x) {
   return *reinterpret_cast<const __attribute__((address_space(1))) unsigned char *>(reinterpret_cast<uint64_t>(x));
 }
-
-__device__ __forceinline__ int request_start(const PagedParams &p, int r) {
-  return p.query_starts == nullptr ? r : min(max(p.query_starts[r], 0), (int)p.T);
-}
-// new tokens of request r (within q's rows)
-__device__ __forceinline__ int request_tokens(const PagedParams &p, int r) {
-  if (p.query_starts == nullptr) return r < p.T ? 1 : 0;
-  const int n = request_start(p, r + 1) - request_start(p, r);
-  return n > 0 ? n : 0;
-}
-__device__ __forceinline__ int request_kv(const PagedParams &p, int r) {
-  const int kv = p.kv_lens[r];
-  const int64_t cap = (int64_t)p.W * p.block;
-  return kv < 0 ? 0 : (kv < cap ? kv : (int)cap);
-}
-// keys that token t of n new ones sees
-__device__ __forceinline__ int token_keys(int kv, int n, int t) { return max(kv - n + t + 1, 0); }
 
 // Blocks of a workgroup's range: at least min_blocks, so that a piece is worth its prologue.
 __device__ __forceinline__ int range_blocks(const PagedParams &p, int total) {
@@ -119,10 +101,10 @@ __device__ __forceinline__ PagedPiece next_piece(const PagedParams &p, int u, in
   } else {
     const int req = uni(p.unit_req[u]);
     x.first = uni(p.unit_first[u]);
-    x.n = uni(request_tokens(p, req));
-    x.kv = uni(request_kv(p, req));
+    x.n = uni(p.req.tokens(req));
+    x.kv = uni(p.req.kv(req));
     x.nrows = min(x.n * p.H - x.first, p.unit_rows);
-    x.row0 = (int64_t)uni(request_start(p, req)) * p.H + x.first;
+    x.row0 = (int64_t)uni(p.req.start(req)) * p.H + x.first;
     x.table = p.table + (int64_t)req * p.W;
   }
   return x;

@@ -6,8 +6,6 @@
 
 using namespace dsa;
 
-static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 static int check_cache(const char *who, int64_t num_blocks, int64_t block, int64_t d_qk, int64_t d_v, int dtype) {
   DSA_REQUIRE(num_blocks > 0 && num_blocks < (1ll << 31) && block > 0 && block <= 65536,
               "%s: num_blocks=%lld must be in [1, 2^31), block_size=%lld in [1, 65536]", who, (long long)num_blocks, (long long)block);
@@ -114,8 +112,7 @@ extern "C" int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const 
   p.q = (const unsigned char *)q;
   p.cache = (const unsigned char *)cache;
   p.table = block_table;
-  p.query_starts = query_starts;
-  p.kv_lens = kv_lens;
+  p.req = Requests{query_starts, kv_lens, W * block_size, (int)T, (int)R};
   p.out = (uint16_t *)out;
   p.lse = lse2;
   p.T = T;
@@ -123,7 +120,7 @@ extern "C" int dsa_paged_latent_mla_fwd(const void *q, const void *cache, const 
   p.W = (int)W;
   p.H = (int)H;
   p.block = (int)block_size;
-  p.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)block_size) : -1;
+  p.block_shift = shift_of(block_size);
   p.num_blocks = (int)num_blocks;
   p.sl2 = sm_scale * kLog2e;
   return launch_paged_fwd(p, D_qk, D_v, dtype == DSA_DTYPE_MXFP4, (unsigned char *)workspace, (hipStream_t)stream);
@@ -168,8 +165,7 @@ extern "C" int dsa_paged_sparse_mla_fwd(const void *q, const void *cache, const 
   p.q = (const unsigned char *)q;
   p.cache = (const unsigned char *)cache;
   p.table = block_table;
-  p.query_starts = query_starts;
-  p.kv_lens = kv_lens;
+  p.req = Requests{query_starts, kv_lens, W * block_size, (int)T, (int)R};
   p.out = (uint16_t *)out;
   p.lse = lse2;
   p.T = T;
@@ -177,7 +173,7 @@ extern "C" int dsa_paged_sparse_mla_fwd(const void *q, const void *cache, const 
   p.W = (int)W;
   p.H = (int)H;
   p.block = (int)block_size;
-  p.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)block_size) : -1;
+  p.block_shift = shift_of(block_size);
   p.num_blocks = (int)num_blocks;
   p.sl2 = sm_scale * kLog2e;
   return launch_paged_sparse(p, indices, topk, D_qk, D_v, dtype == DSA_DTYPE_MXFP4, (unsigned char *)workspace, (hipStream_t)stream);

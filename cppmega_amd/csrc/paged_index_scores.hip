@@ -32,9 +32,6 @@ constexpr int kWindowPages = 2048;  // pages of a unit that a workgroup has in L
 constexpr int kBlockKeys = 128;
 constexpr int kMostSpan = 65536 - kBlockKeys;  // past a column, below 2^31 - 65536, it stays below 2^31
 
-// Keeps a wave-uniform branch a branch.
-__device__ __forceinline__ void keep_branch() { asm volatile(""); }
-
 static __device__ const i32x4 kNoKey[16] = {};  // the row of a key that is not there
 
 __device__ __forceinline__ i32x4 ld_16(const unsigned char *x) {
@@ -359,7 +356,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) i
     const int my0 = x.ta + (halves ? w & 1 : w) * TPW;  // the wave's first token
     const int at = __builtin_amdgcn_readfirstlane(p.req.start(x.r)), n = __builtin_amdgcn_readfirstlane(p.req.tokens(x.r));
     const int kv = __builtin_amdgcn_readfirstlane(p.req.kv(x.r));
-    auto keys_of = [&](int t) { return max(kv - n + (t - at) + 1, 0); };
+    auto keys_of = [&](int t) { return token_keys(kv, n, t - at); };
     const int kb1 = min(min(x.b1, x.nb) * kBlockKeys, p.L), most = keys_of(x.tb - 1);
 
     i32x4 q[2][KS];

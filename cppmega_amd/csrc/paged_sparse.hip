@@ -96,8 +96,7 @@ size_t paged_sparse_workspace(int64_t T, int64_t topk, int64_t H, int64_t d_qk, 
 
 int launch_paged_sparse(PagedParams p, const int32_t *indices, int64_t topk, int64_t d_qk, int64_t d_v, bool fp4, unsigned char *ws,
                         hipStream_t st) {
-  const Picks picks{indices, p.table, Requests{p.query_starts, p.kv_lens, (int64_t)p.W * p.block, (int)p.T, p.R}, p.W, (int)topk,
-                    p.block, p.block_shift, p.num_blocks};
+  const Picks picks{indices, p.table, p.req, p.W, (int)topk, p.block, p.block_shift, p.num_blocks};
   if (d_qk == 128) {
     SparseParams n{};
     n.q = p.q;

@@ -37,6 +37,9 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *tmp, uint32
   return add_sat(before, v) - x;
 }
 
+// Keys that token t of n new ones sees.
+__device__ __forceinline__ int token_keys(int kv, int n, int t) { return max(kv - n + t + 1, 0); }
+
 // The requests of a call: tokens query_starts[r] .. query_starts[r + 1] of the batch (null: token r alone) are the last of
 // request r's kv_lens[r] positions.
 struct Requests {
@@ -80,7 +83,7 @@ struct Requests {
   // Positions that token t of request r sees, -1 where it is not one of the request's.
   __device__ __forceinline__ int keys_of(int t, int r) const {
     const int at = start(r), n = tokens(r);
-    return t >= at && t < at + n ? max(kv(r) - n + (t - at) + 1, 0) : -1;
+    return t >= at && t < at + n ? token_keys(kv(r), n, t - at) : -1;
   }
 };
 
