@@ -1,9 +1,10 @@
 // Index keys into and out of their paged cache, on gfx950: one thread per 8 channels (16
 // bytes of bf16), bound by the bytes moved.  The four neighbouring lanes of a 32-channel
 // block share its largest magnitude.  MXFP8: the scale is the least power of two under
-// which that is at most 448, e4m3's largest value, so nothing saturates; MXFP4: as the
-// latent cache's.  65536 keys of 128 channels in MXFP4: append 7.0 us (3.1 TB/s, slots and
-// rows one latency behind the other), gather 6.3; 64 keys 2.2 and 2.1, the launch.
+// which that is at most 448, e4m3's largest value, so nothing saturates (but magnitudes
+// past 1.75 2^127, as the exponent is held to 119); MXFP4: as the latent cache's.
+// 65536 keys of 128 channels in MXFP4: append 7.0 us (3.1 TB/s, slots and rows one
+// latency behind the other), gather 6.3; 64 keys 2.3 and 2.2, the launch.
 #include "index_keys.hpp"
 
 namespace dsa {

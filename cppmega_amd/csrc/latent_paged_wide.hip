@@ -36,8 +36,9 @@ struct PagedWide {
   static constexpr int CW = ROLES ? 4 : 8, LW = ROLES ? 4 : 8, KG = CW / (RG * DG);  // computing, loading waves; key groups
   static constexpr int SUB = 2 / KG;                         // tiles of a computing wave
   static constexpr int PANELS = 9, TILE = PANELS * 4096, STEP = 2 * TILE;
-  // operands read at once (3, 4: registers spill in the step; 2: none does there, MXFP4 with RG 2 spills 21 around a piece's
-  // joining and the window's refill)
+  // Operands read at once (3, 4: registers spill among a step's products).  2: none does there; around a piece's joining, the
+  // window's refill and a step with masked keys, MXFP4 with RG 2 spills 22, sparse 28, sparse bf16 with RG 2 22, sparse MXFP4 with
+  // RG 4 and sparse bf16 with RG 8 2.
   static constexpr int GROUP = 2;
   static constexpr int KS = 18, NDT = 32 / DG;               // 16-channel tiles of O in a wave
   static constexpr int TPR = 4, CPT = 16 / TPR, RPT = 8 / TPR;  // MXFP4: threads of a row; their code pieces, rope chunks
@@ -280,6 +281,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             e2[e] = exp2_fast(fmaf(s[e >> 2][e & 3], p.sl2, -m_run));
             l_run += e2[e];
           }
+          // the weights in bf16, the product's operand: each off by 2^-8 of itself at most, their sum is of the 32-bit ones (results
+          // are 0.0020 of their size from those in 64 bits, whose own rounding to bf16 is 0.0017)
           const i32x4 pb{(int)pack_bf16x2(e2[0], e2[1]), (int)pack_bf16x2(e2[2], e2[3]), (int)pack_bf16x2(e2[4], e2[5]),
                          (int)pack_bf16x2(e2[6], e2[7])};
           stream_operands<NDT>(a0, cols, [&](int dt, i32x4 a) {
@@ -370,6 +373,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) p
             if (x.whole && !FP4) {
               // Two channel tiles at a time, neighbouring lane groups' halves swapped, so that a lane has eight channels of one: 1537
               // tokens, 128 heads, top-64 151 -> 139 us, 32 heads 90 -> 84 (MXFP4: 180 -> 165, but 70 -> 73 and 102 -> 105 with 2048).
+              // Dense: 6 prompts of 40 .. 512 tokens on 600 .. 4096 keys, 128 heads 1373 -> 1241, 16 heads 216 -> 202; 32 of 16 .. 64 tokens
+              // on 64 .. 200 keys 227 -> 208; 64 single tokens of 301 .. 16384 keys, 16 heads 148, 147.
               unsigned char *dst = reinterpret_cast<unsigned char *>(p.out + (x.row0 + row) * 512 + 16 * dg * NDT + 16 * (g16 & 1) + 8 * (g16 >> 1));
 #pragma unroll
               for (int dt = 0; dt < NDT; dt += 2) {

@@ -14,10 +14,12 @@
 // the sum of its magnitudes at most (128 rows, 32 lanes, 32 and 16 workgroups' sums).  The backward has its next row in flight
 // while it works on one, and one exchange between a row's lanes for both of its sums (135 -> 86 us at 4096).
 //
-// Bound by the bytes moved, or by a launch's own time: 16384 rows of 4096 bf16, forward, backward, sums: 57 us (4.7 TB/s),
-// 86 (4.7), 4.6; 2051 rows of 1001 f32: 6.4, 9.6, 4.0; 8192 rows of 64 bf16: 3.3, 4.7, 2.9.  Results stored past the caches
-// make these calls shorter and what reads the results longer: 16384 rows of 4096, both directions 147 -> 128 us, but the forward
-// and a kernel that reads y 98 -> 106 (of 32768 rows 195 -> 199).
+// Bound by the bytes moved, or by a launch's own time: 16384 rows of 4096 bf16, forward, backward, sums: 60 us (4.5 TB/s),
+// 83 (4.9), 5.6; 2051 rows of 1001 f32: 6.4, 10.7, 4.0; 8192 rows of 64 bf16: 3.2, 4.7, 3.1.  The backward of more than 8192 columns
+// spills 119 (bf16) and 171 (f32) registers, part of them read in each row (weights, sums and two rows of 16 elements a lane do not
+// fit into 128): 4096 rows of 16384 135 us (3.0 TB/s) and 265 (3.0), of 12288 124 and 230, of 8192 48 (4.2) and 83 (4.9).  Results
+// stored past the caches make these calls shorter and what reads the results longer: 16384 rows of 4096, both directions 147 -> 128
+// us, but the forward and a kernel that reads y 98 -> 106 (of 32768 rows 195 -> 199).
 #include <math.h>
 
 #include "dsa_common.hpp"

@@ -19,8 +19,10 @@
 //
 // Single tokens are bound by the keys' bytes: 64 tokens over 301 .. 65536 MXFP8 keys, 64 heads of 128 channels, 65 us, 4.5 TB/s.
 // Several tokens are bound by the MFMAs and the ReLU and weights beside them, which the SIMD overlaps in part: 5 prompts of 33
-// .. 512 tokens on 1024 .. 16384 MXFP4 keys, 32 heads, 78 us, 740 TFLOP/s (MFMA busy 45 % of it, VALU 50 %); without the
-// weights' work it would be 69, without the conversion and the keys' loads 63.
+// .. 512 tokens on 1024 .. 16384 MXFP4 keys, 32 heads, 77 to 81 us, 730 TFLOP/s (of a CU's busy time MFMA 41 %, VALU 41 %); without the
+// weights' work it would be 69, without the conversion and the keys' loads 63.  At 64 channels a tile is half the products between the
+// same two barriers: 3 prompts of 100 .. 700 tokens on 1024 .. 8192 keys, 16 heads, 24 to 26 us in each type, 430 TFLOP/s.
+// Most of index_tiles_kernel's forms of 128 channels spill 2 to 9 registers, read once a piece, none among a tile's products.
 #include <type_traits>
 
 #include "index_keys.hpp"

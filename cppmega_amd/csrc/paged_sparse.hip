@@ -6,9 +6,11 @@
 // all tokens' picks, 64 at a time, and paged_combine_kernel adds the pieces of a token that was cut; the picks' slots are formed as
 // a workgroup fills its window of pages.
 //
-// 64 tokens, 128 heads, top-2048, bf16: 69 us, 530 TFLOP/s; its units of 32 rows read 600 MB through the L2s, 8.8 TB/s, which
-// bounds it (rows by registers, two more steps in flight: 80).  96 tokens, 16 heads, MXFP4: 36 us and 4.3 for the joining, bound by
-// the rows' loads and widening, one workgroup a CU.
+// 64 tokens, 128 heads, top-2048, bf16: 67 us, 540 TFLOP/s, in units of 32 rows.  Its four computing waves, one a SIMD, bound it: of a
+// replay of 74 us the products alone take 64, the rows' loads alone 54 (by registers, two more steps in flight, the whole took 80).
+// The rows come through the L2s, 600 MB at 9 TB/s; those are not the limit, as 500 tokens of 16 heads, 1.2 GB, get 12 of them (99 us:
+// loads alone 86, products alone 82, which overlap in part).  1024 tokens, 128 heads: of 581 us the products 520, the loads 167.
+// 96 tokens, 16 heads, MXFP4: 37 us and 4.4 for the joining; of a replay of 46 the products alone 41, loads and widening alone 34.
 #include "latent_paged.hpp"
 #include "paged_sparse.hpp"
 

@@ -8,10 +8,11 @@
 // and workgroups may share them as well, whose fp32 sums sparse_narrow_combine_kernel adds in order.
 //
 // Bound by the chain of a block (LDS, S, softmax, P V) at three waves a SIMD, nothing saturated: 6 prompts of 40 .. 512 tokens,
-// 32 heads, top-256, MXFP4 21 us (VALU busy 40 %, MFMA 16 %, LDS 25 %); bf16 the same.  Rows two blocks ahead 27, four waves a
-// SIMD (registers spill) 44, S in two accumulators 26, operands read in groups 28.  With a long top-k the rows' way through the
-// L2s bounds it: 1537 tokens, 32 heads, top-1000 49 us, 8 TB/s (a row of MXFP4 is two or three of their lines, as one of bf16 is
-// two); up to 16 heads on 16x16x32 MFMAs at four waves a SIMD took 43 us against 46 here.  One token of 777 keys: 6.4.
+// 32 heads, top-256, MXFP4 21 us (of a CU's busy time VALU 31 %, MFMA 12 %, LDS 21 %); bf16 the same.  Rows two blocks ahead 27, four
+// waves a SIMD (registers spill) 44, S in two accumulators 26, operands read in groups 28.  With a long top-k the same: 1537 tokens,
+// 32 heads, top-1000, bf16 55 us; of a replay of 58, the rows' loads and their way into LDS alone 46, all but the loads 47 (VALU
+// 35 %, MFMA 15 %, LDS 27 %; of 390 MB of rows 220 come from the L2s); up to 16 heads on 16x16x32 MFMAs at four waves a SIMD took 43 us against 46 here.  One
+// token of 777 keys: 6.5.
 #include "latent_mla.hpp"
 #include "latent_paged.hpp"
 #include "paged_sparse.hpp"
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) s
           l_run += acc[i];
         }
         i32x4 pb[2];
-        pack_operand(acc, pb);
+        pack_operand(acc, pb);  // (weights in bf16, the product's operand: off by 2^-8 of themselves at most; their sum is of the 32-bit ones)
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
