@@ -769,7 +769,7 @@ int dsa_paged_index_scores(const void *q, const void *w, const void *cache, cons
  * ones, in particular -1, is masked; a repeated one counts every time).  Everything else as
  * in dsa_paged_latent_mla_fwd, whose results for the same rows it gives; num_blocks *
  * block_size < 2^31, topk <= 2^27, T * ceil(H / 32) < 2^26 (128 channels: at most 2^26 - 4).  workspace:
- * dsa_paged_sparse_mla_workspace_size() bytes, 256-byte aligned.
+ * dsa_paged_sparse_mla_workspace_size() bytes, 256-byte aligned (0: none, may be NULL).
  */
 size_t dsa_paged_sparse_mla_workspace_size(int64_t T, int64_t H, int64_t topk, int64_t D_qk, int64_t D_v);
 int dsa_paged_sparse_mla_fwd(const void *q, const void *cache, const int32_t *indices, const int32_t *block_table,
